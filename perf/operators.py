@@ -86,9 +86,9 @@ def draw(rng):
     dtype = rng.choice(("bf16", "bf16", "f32"))
     if kind in ("lookup", "embed"):
         es = 2 if dtype == "bf16" else 4
-        h = spread(64, min(8192, (1 << 30) // (v * es)))
+        h = spread(64, min(8192, (3 << 28) // (v * es)))
         h = h if rng.random() < 0.3 else max(64, h // 64 * 64)
-        n = spread(1, 1024) if kind == "lookup" else spread(1, min(131072, (1 << 27) // h))
+        n = spread(1, 1024) if kind == "lookup" else spread(1, min(131072, (1 << 27) * 2 // (h * es)))
         start = rng.choice((0, 0, v))
         odtype = rng.choice(("bf16", dtype))
         return dict(kind=kind, wdtype=dtype, odtype=odtype, n=n, h=h, v=v, start=start)
