@@ -498,6 +498,36 @@ int nmce_lmhead_ce_fused_chunk_grads(const void* hidden, const void* weight, int
                                      void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * Embedding lookup over a vocabulary shard (tp_layers.py:91-132):
+ *   out[i, :] = scale * weight[tokens[i] - vocab_start, :]   (in fp32, rounded once)
+ * for ids in [vocab_start, vocab_start + vocab_local), and zeros for others
+ * (any int64; nothing is read out of bounds). weight [vocab_local, ldw] and
+ * out [n_tokens, ldo] are NMCE_F32 or NMCE_BF16 each, aligned to their
+ * element; rows on the 16-byte grid go by 16-byte vectors. n_tokens and
+ * vocab_local below 2^31.
+ */
+int nmce_embedding_fwd(const int64_t* tokens, int64_t n_tokens, const void* weight,
+                       int weight_dtype, int64_t vocab_local, int64_t hidden, int64_t ldw,
+                       int64_t vocab_start, float scale, void* out, int out_dtype, int64_t ldo,
+                       void* stream);
+
+/* Workspace of nmce_embedding_bwd in bytes (-1: sizes it does not take). */
+int64_t nmce_embedding_bwd_workspace_bytes(int64_t n_tokens, int64_t vocab_local, int64_t hidden);
+
+/*
+ * The weight's gradient of nmce_embedding_fwd, written whole:
+ *   grad_weight[v, :] = scale * sum of grad_out[i, :] over tokens[i] = vocab_start + v
+ * (fp32 sums in an order that the tokens alone decide, rounded once; zeros
+ * where no token is). grad_weight is [vocab_local, hidden] contiguous, 16-byte
+ * aligned; grad_out [n_tokens, ldg] aligned to its element. The workspace
+ * (16-byte aligned) belongs to this call until it is done on the stream.
+ */
+int nmce_embedding_bwd(const int64_t* tokens, int64_t n_tokens, const void* grad_out,
+                       int grad_dtype, int64_t ldg, int64_t vocab_local, int64_t hidden,
+                       int64_t vocab_start, float scale, void* grad_weight, int weight_dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * The GEMM core of the fused path, exposed for testing and measurement (no
  * counterpart in the reference): c[i, j] = sum_l a[i, l] * b[j, l] for
  * i < m, j < n, l < k, with bf16 a [m, lda] and b [n, ldb], fp32

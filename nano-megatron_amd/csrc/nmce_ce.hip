@@ -1002,11 +1002,6 @@ inline unsigned grid_for_rows(int64_t n_rows) {
   return static_cast<unsigned>(n_rows < cap ? n_rows : cap);
 }
 
-inline int launch_status() {
-  hipError_t e = hipGetLastError();
-  return e == hipSuccess ? NMCE_OK : static_cast<int>(e);
-}
-
 }  // namespace
 }  // namespace nmce
 

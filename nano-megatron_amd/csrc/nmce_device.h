@@ -39,6 +39,18 @@ inline int device_cus() {
   return n > 0 ? n : 256;
 }
 
+// Host: the status of the launch just made: 0 or a hipError_t.
+inline int launch_status() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : static_cast<int>(e);
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+inline int64_t align256(int64_t x) { return round_up(x, 256); }
+
 constexpr float kLog2e = 1.4426950408889634f;  // exp(x) = exp2(x * kLog2e)
 constexpr float kNegHuge = -3.402823466e+38f;  // finite floor for running maxima
 

@@ -1492,15 +1492,6 @@ __global__ __launch_bounds__(256) void transpose_bf16_kernel(const uint16_t* __r
                  static_cast<int64_t>(blockIdx.x) * kTrTile);
 }
 
-inline int launch_status() {
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? NMCE_OK : static_cast<int>(e);
-}
-
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
-
 int configure_lds() {
   static std::atomic<bool> done[4];
   const void* kernels[] = {
@@ -1627,7 +1618,6 @@ struct BwdLayout {
   int64_t off_xt, off_wt, off_dzt, off_dz, off_acc, total;
 };
 
-inline int64_t align256(int64_t x) { return round_up(x, 256); }
 
 BwdLayout bwd_layout(int64_t n, int64_t h, int64_t v, int64_t chunk) {
   BwdLayout L{};

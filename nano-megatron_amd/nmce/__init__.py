@@ -11,9 +11,13 @@ Public API (mirrors nano_megatron/cross_entropy.py and parallel.py):
   and weight gradients.
 * ``FusedParallelLMHead(config, ctx)`` -- drop-in for model.py's
   ``ParallelLMHead`` whose ``forward(x, labels)`` returns that fused loss.
+* ``vocab_parallel_embedding(tokens, weight, vocab_start, vocab_end, ctx)`` /
+  ``VocabParallelEmbedding(config, ctx)`` -- the scaled lookup over the same
+  shard (tp_layers.py:91-132), with the weight's dense gradient.
 * ``copy_to_tensor_parallel_region`` / ``gather_from_sequence_parallel_region``
   / ``gather_tokens_rank_major`` -- the collectives on the LM head's input side
-  (mappings.py:83-94, :109-120).
+  (mappings.py:83-94, :109-120); ``reduce_from_tensor_parallel_region`` /
+  ``reduce_scatter_to_sequence_parallel_region`` -- on the embedding's output.
 * ``ParallelContext`` / ``vocab_range`` / ``divide`` -- the topology fields and
   shard rule the loss reads.
 
@@ -26,6 +30,11 @@ from .cross_entropy import (
     validate_targets,
     vocab_parallel_cross_entropy,
 )
+from .embedding import (
+    VocabParallelEmbedding,
+    _VocabParallelEmbedding,
+    vocab_parallel_embedding,
+)
 from .lmhead import (
     FusedParallelLMHead,
     _LMHeadVocabParallelCrossEntropy,
@@ -35,6 +44,8 @@ from .mappings import (
     copy_to_tensor_parallel_region,
     gather_from_sequence_parallel_region,
     gather_tokens_rank_major,
+    reduce_from_tensor_parallel_region,
+    reduce_scatter_to_sequence_parallel_region,
     targets_rank_major,
 )
 from .parallel import ParallelContext, divide, vocab_range
@@ -43,14 +54,19 @@ __all__ = [
     "FusedParallelLMHead",
     "_LMHeadVocabParallelCrossEntropy",
     "_VocabParallelCrossEntropy",
+    "_VocabParallelEmbedding",
     "ParallelContext",
+    "VocabParallelEmbedding",
     "copy_to_tensor_parallel_region",
     "divide",
     "gather_from_sequence_parallel_region",
     "gather_tokens_rank_major",
     "lmhead_vocab_parallel_cross_entropy",
+    "reduce_from_tensor_parallel_region",
+    "reduce_scatter_to_sequence_parallel_region",
     "targets_rank_major",
     "validate_targets",
     "vocab_parallel_cross_entropy",
+    "vocab_parallel_embedding",
     "vocab_range",
 ]

@@ -69,6 +69,11 @@ SIGNATURES: dict[str, tuple] = {
     "nmce_lmhead_ce_fused_chunk_grads": (_c_int, [_p, _p, _c_int, _i64, _i64, _i64, _p, _i64,
                                                   _i64, _i64, _p, _p, _p, _p, _i64,
                                                   ctypes.c_float, _p, _p, _p, _i64, _p]),
+    "nmce_embedding_fwd": (_c_int, [_p, _i64, _p, _c_int, _i64, _i64, _i64, _i64, ctypes.c_float,
+                                    _p, _c_int, _i64, _p]),
+    "nmce_embedding_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "nmce_embedding_bwd": (_c_int, [_p, _i64, _p, _c_int, _i64, _i64, _i64, _i64, ctypes.c_float,
+                                    _p, _c_int, _p, _i64, _p]),
     "nmce_gemm_nt_bf16": (_c_int, [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _c_int, _i64, _p]),
     "nmce_gemm_mn_bf16": (_c_int, [_c_int, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "nmce_lmhead_ce_bwd_layout": (_c_int, [_i64, _i64, _i64, _i64, _p]),

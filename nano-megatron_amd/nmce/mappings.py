@@ -1,4 +1,5 @@
-"""The collectives on the LM head's input side, as autograd Functions.
+"""The collectives on the LM head's input side and the embedding's output side,
+as autograd Functions.
 
 Before the projection ``x @ W.t()`` the reference maps the hidden state into
 the tensor-parallel region (model.py:188-191):
@@ -17,6 +18,10 @@ that is the layout ``all_gather_into_tensor`` produces and
 mappings.py:43-79). The targets are permuted to the same order, which is an
 int64 copy of one value per token. The natural-order gather stays available
 for callers that want the logits themselves.
+
+The embedding's rows, nonzero on one rank each, go the other way: ``g``
+(all-reduce forward, identity backward) or, under sequence parallelism, the
+reduce-scatter along the sequence, whose backward all-gathers.
 
 A gloo group gets host copies of device tensors: gloo collectives are only
 run on CPU tensors here.
@@ -131,6 +136,44 @@ class _GatherTokensRankMajor(torch.autograd.Function):
                 None, None)
 
 
+class _ReduceFromTensorParallelRegion(torch.autograd.Function):
+    """``g``: all-reduce forward, identity backward (mappings.py:101-102)."""
+
+    @staticmethod
+    def forward(ctx, x, group, world_size):
+        if world_size == 1:
+            return x.view_as(x)
+        return _all_reduce(x.clone(), group, world_size)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return grad, None, None
+
+
+class _ReduceScatterToSequenceParallelRegion(torch.autograd.Function):
+    """``[B, S, ...]`` -> ``[B, S/tp, ...]``: the SUM over ranks, this rank's
+    part of dim 1 (mappings.py:61-80); backward all-gathers dim 1."""
+
+    @staticmethod
+    def forward(ctx, x, group, world_size):
+        _check_sequence_tensor(x)
+        ctx.group, ctx.world_size = group, world_size
+        if world_size == 1:
+            return x.view_as(x)
+        if x.shape[1] % world_size:
+            raise ValueError(f"sequence length {x.shape[1]} is not divisible by TP size "
+                             f"{world_size}")
+        r = _reduce_scatter_rows(x.transpose(0, 1), group, world_size)
+        return r.transpose(0, 1).contiguous()
+
+    @staticmethod
+    def backward(ctx, grad):
+        if ctx.world_size == 1:
+            return grad, None, None
+        g = _all_gather_rows(grad.transpose(0, 1), ctx.group, ctx.world_size)
+        return g.transpose(0, 1).contiguous(), None, None
+
+
 def copy_to_tensor_parallel_region(x: torch.Tensor, ctx) -> torch.Tensor:
     """``f`` of mappings.py:83-94 for the group in ``ctx``."""
     return _CopyToTensorParallelRegion.apply(x, ctx.tp_group, ctx.tp_size)
@@ -139,6 +182,16 @@ def copy_to_tensor_parallel_region(x: torch.Tensor, ctx) -> torch.Tensor:
 def gather_from_sequence_parallel_region(x: torch.Tensor, ctx) -> torch.Tensor:
     """The sequence all-gather of mappings.py:109-120, in the reference's order."""
     return _GatherFromSequenceParallelRegion.apply(x, ctx.tp_group, ctx.tp_size)
+
+
+def reduce_from_tensor_parallel_region(x: torch.Tensor, ctx) -> torch.Tensor:
+    """``g`` (mappings.py:101-102): the sum of ``x`` over the group in ``ctx``."""
+    return _ReduceFromTensorParallelRegion.apply(x, ctx.tp_group, ctx.tp_size)
+
+
+def reduce_scatter_to_sequence_parallel_region(x: torch.Tensor, ctx) -> torch.Tensor:
+    """The sum over the group, scattered along the sequence (mappings.py:61-80)."""
+    return _ReduceScatterToSequenceParallelRegion.apply(x, ctx.tp_group, ctx.tp_size)
 
 
 def gather_tokens_rank_major(x: torch.Tensor, ctx) -> torch.Tensor:
