@@ -528,6 +528,34 @@ int nmce_embedding_bwd(const int64_t* tokens, int64_t n_tokens, const void* grad
                        void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * 8-bit rows: scale[r] = max |x[r, :]| / 127 and q[r, k] = x[r, k] / scale[r]
+ * to the nearest integer, halves to even (formed from 127 x / max |x|, whose
+ * halves are exact). x [n_rows, ldx] NMCE_F32 or NMCE_BF16, aligned to its
+ * element; q [n_rows, ldq] gets zeros in columns .. ldq - 1. A row of zeros
+ * gets the scale 0; one with an infinity or a NaN the scale NaN and zeros.
+ */
+int nmce_quantize_rows(const void* x, int dtype, int64_t n_rows, int64_t columns, int64_t ldx,
+                       int8_t* q, int64_t ldq, float* scale, void* stream);
+
+/* Workspace of nmce_int8_linear in bytes (-1: sizes it does not take). */
+int64_t nmce_int8_linear_workspace_bytes(int64_t n_rows, int64_t columns);
+
+/*
+ * Logits from an 8-bit weight: x quantised as nmce_quantize_rows does, then
+ *   out[n, v] = (sum_k qx[n, k] * weight[v, k]) * sx[n] * w_scale[v]
+ * with the sum exact in 32-bit integers (columns <= 131072), the rest in fp32,
+ * rounded once to out_dtype. weight [vocab_local, ldw]: 16-byte aligned, ldw a
+ * multiple of 16 below 2^23, each row allocated to a whole 16 bytes (what they
+ * hold past `columns` does not matter). x and out are aligned to their
+ * elements. The workspace (16-byte aligned) belongs to this call until it is
+ * done on the stream.
+ */
+int nmce_int8_linear(const void* x, int dtype, int64_t n_rows, int64_t columns, int64_t ldx,
+                     const int8_t* weight, int64_t vocab_local, int64_t ldw, const float* w_scale,
+                     void* out, int out_dtype, int64_t ldo, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/*
  * The GEMM core of the fused path, exposed for testing and measurement (no
  * counterpart in the reference): c[i, j] = sum_l a[i, l] * b[j, l] for
  * i < m, j < n, l < k, with bf16 a [m, lda] and b [n, ldb], fp32

@@ -91,6 +91,16 @@ __device__ __forceinline__ void mfma_16x16x32(f32x4_t& c, const bf16x8_t& a, con
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
+// The same on 8-bit integers, K = 64: its fragments are the same 16 bytes a
+// lane (row l % 16, bytes 16 (l / 16) .. + 15 of 64), its accumulators 32-bit
+// integers in the same places, and it takes the same 16 cycles. So the whole
+// core runs on bytes: an operand of 8-bit elements is one of half as many
+// 16-bit ones, and c holds the integers' bits.
+__device__ __forceinline__ void mfma_i8_16x16x64(f32x4_t& c, const bf16x8_t& a,
+                                                 const bf16x8_t& b) {
+  asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+
 // Tile index for workgroup b. The dispatcher deals workgroups to the 8 XCDs
 // round-robin (block b runs on XCD b % 8); give each XCD a contiguous band of
 // tile ids, and inside the band walk groups of kGroupM tile rows column by
@@ -122,7 +132,11 @@ __device__ __forceinline__ void tile_coords(int b, int tiles_m, int tiles_n, int
 //
 // The buffer resource has no stride and no range limit (every offset is
 // clamped in bounds) and gfx9's data format word.
-template <bool kMN>
+//
+// kTail (K-contiguous): a row's 16-byte chunks may end inside the last stage;
+// those past the last are read as the last, and the other operand holds zeros
+// there.
+template <bool kMN, bool kTail = false>
 struct StageLoads {
   i32x4_t rsrc;
   const char* base;
@@ -142,7 +156,8 @@ struct StageLoads {
     return chunk * 16;
   }
   // first: the operand's element at the tile's first row (column), k = 0;
-  // rows: the operand's rows (columns) from there on; krows_: its k-rows (kMN).
+  // rows: the operand's rows (columns) from there on; krows_: its k-rows (kMN)
+  // or a row's 16-byte chunks (kTail).
   __device__ __forceinline__ void init(const uint16_t* first, int64_t ld, int64_t rows,
                                        int64_t krows_, int wave, int lane_) {
     lane = lane_;
@@ -151,6 +166,7 @@ struct StageLoads {
     krows = krows_;
     soff = 0;
     const int blk0 = wave * kBlocksPerWave;
+    if constexpr (kTail) row0 = blk0 * 8 + (lane >> 3);
     if constexpr (kMN) {
       row0 = 2 * blk0 + (lane >> 5);
       const int64_t last = (rows + 7) / 8 - 1;  // >= 0
@@ -173,8 +189,8 @@ struct StageLoads {
   }
   // The number of leading stages whose k-rows all exist.
   __device__ __forceinline__ int full_stages(int stages) const {
-    if constexpr (!kMN) return stages;
-    const int64_t f = krows / kBK;
+    if constexpr (!kMN && !kTail) return stages;
+    const int64_t f = krows / (kMN ? kBK : kBK / 8);
     return f < stages ? static_cast<int>(f) : stages;
   }
   // Stage kt (all of its k-rows exist) is the next one to be loaded.
@@ -203,6 +219,19 @@ struct StageLoads {
                             static_cast<int>((row - b0) * row_bytes) + chunk_bytes(j), 0, 0, 0);
       }
       return;
+    }
+    if constexpr (kTail) {
+      if ((kt + 1) * static_cast<int64_t>(kBK / 8) > krows) {
+#pragma unroll
+        for (int j = 0; j < kBlocksPerWave; ++j) {
+          const int chunk = (lane & 7) ^ (((row0 + 8 * j) >> 1) & 7);
+          int64_t c = static_cast<int64_t>(kt) * (kBK / 8) + chunk;
+          if (c > krows - 1) c = krows - 1;
+          raw_buffer_load_lds(rsrc, (lds_void_t*)(dst + j * 1024), 16,
+                              static_cast<int>(off[j] + (c - chunk) * 16), 0, 0, 0);
+        }
+        return;
+      }
     }
     at(kt);
 #pragma unroll
@@ -282,7 +311,10 @@ struct Frags {
 // kRows hands the MFMA its operands the other way round, which gives the lane
 // four columns of one row instead of four rows of one column (the same sums):
 // what an epilogue wants that stores rows.
-template <bool kAMN, bool kBMN, bool kRows = false>
+//
+// kI8: 8-bit integers, two to a 16-bit element (lda, ldb and K count pairs);
+// ka_rows and kb_rows are then the 16-byte chunks that each operand's rows hold.
+template <bool kAMN, bool kBMN, bool kRows = false, bool kI8 = false>
 __device__ __forceinline__ void gemm_mainloop(const uint16_t* __restrict__ A, int64_t lda,
                                               int64_t M, const uint16_t* __restrict__ B,
                                               int64_t ldb, int64_t N, int64_t K, int64_t m0,
@@ -294,8 +326,8 @@ __device__ __forceinline__ void gemm_mainloop(const uint16_t* __restrict__ A, in
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / kWavesN, wn = wave % kWavesN;
 
-  StageLoads<kAMN> la;
-  StageLoads<kBMN> lb;
+  StageLoads<kAMN, kI8> la;
+  StageLoads<kBMN, kI8> lb;
   la.init(kAMN ? A + m0 : A + m0 * lda, lda, M - m0, ka_rows, wave, lane);
   lb.init(kBMN ? B + n0 : B + n0 * ldb, ldb, N - n0, kb_rows, wave, lane);
   Frags<kAMN> fa;
@@ -365,10 +397,14 @@ __device__ __forceinline__ void gemm_mainloop(const uint16_t* __restrict__ A, in
   // instructions.
   constexpr int kLoadGap = 6;
   auto mma = [&](int i, int j, const Set& f) {
-    if constexpr (kRows)
+    if constexpr (kI8) {
+      static_assert(kRows || !kI8, "8-bit products are stored");
+      mfma_i8_16x16x64(acc.c[i][j], f.b[j], f.a[i]);
+    } else if constexpr (kRows) {
       mfma_16x16x32(acc.c[i][j], f.b[j], f.a[i]);
-    else
+    } else {
       mfma_16x16x32(acc.c[i][j], f.a[i], f.b[j]);
+    }
   };
   auto step = [&](const char* pa, const char* pb, int s, Set& next, const Set& cur, auto loads,
                   auto&& load) {

@@ -14,6 +14,9 @@ Public API (mirrors nano_megatron/cross_entropy.py and parallel.py):
 * ``vocab_parallel_embedding(tokens, weight, vocab_start, vocab_end, ctx)`` /
   ``VocabParallelEmbedding(config, ctx)`` -- the scaled lookup over the same
   shard (tp_layers.py:91-132), with the weight's dense gradient.
+* ``quantize_rows(x)`` / ``int8_linear(x, weight, weight_scale)`` /
+  ``Int8ParallelLMHead`` -- 8-bit rows, their product, and the serving head made
+  of it (``FusedParallelLMHead.quantized()``).
 * ``copy_to_tensor_parallel_region`` / ``gather_from_sequence_parallel_region``
   / ``gather_tokens_rank_major`` -- the collectives on the LM head's input side
   (mappings.py:83-94, :109-120); ``reduce_from_tensor_parallel_region`` /
@@ -35,6 +38,7 @@ from .embedding import (
     _VocabParallelEmbedding,
     vocab_parallel_embedding,
 )
+from .int8 import Int8ParallelLMHead, int8_linear, quantize_rows
 from .lmhead import (
     FusedParallelLMHead,
     _LMHeadVocabParallelCrossEntropy,
@@ -52,6 +56,7 @@ from .parallel import ParallelContext, divide, vocab_range
 
 __all__ = [
     "FusedParallelLMHead",
+    "Int8ParallelLMHead",
     "_LMHeadVocabParallelCrossEntropy",
     "_VocabParallelCrossEntropy",
     "_VocabParallelEmbedding",
@@ -61,7 +66,9 @@ __all__ = [
     "divide",
     "gather_from_sequence_parallel_region",
     "gather_tokens_rank_major",
+    "int8_linear",
     "lmhead_vocab_parallel_cross_entropy",
+    "quantize_rows",
     "reduce_from_tensor_parallel_region",
     "reduce_scatter_to_sequence_parallel_region",
     "targets_rank_major",

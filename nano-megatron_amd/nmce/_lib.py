@@ -74,6 +74,10 @@ SIGNATURES: dict[str, tuple] = {
     "nmce_embedding_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "nmce_embedding_bwd": (_c_int, [_p, _i64, _p, _c_int, _i64, _i64, _i64, _i64, ctypes.c_float,
                                     _p, _c_int, _p, _i64, _p]),
+    "nmce_quantize_rows": (_c_int, [_p, _c_int, _i64, _i64, _i64, _p, _i64, _p, _p]),
+    "nmce_int8_linear_workspace_bytes": (_i64, [_i64, _i64]),
+    "nmce_int8_linear": (_c_int, [_p, _c_int, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _c_int,
+                                  _i64, _p, _i64, _p]),
     "nmce_gemm_nt_bf16": (_c_int, [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _c_int, _i64, _p]),
     "nmce_gemm_mn_bf16": (_c_int, [_c_int, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "nmce_lmhead_ce_bwd_layout": (_c_int, [_i64, _i64, _i64, _i64, _p]),

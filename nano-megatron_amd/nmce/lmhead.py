@@ -44,6 +44,7 @@ Both ``x`` and ``W`` must be bf16 on a ROCm device; there is no CPU path.
 from __future__ import annotations
 
 import sys
+from types import SimpleNamespace
 
 import torch
 
@@ -518,6 +519,17 @@ class FusedParallelLMHead(torch.nn.Module):
         """This rank's global id range (model.py:242-245)."""
         per = self.weight.shape[0]
         return self.ctx.tp_rank * per, (self.ctx.tp_rank + 1) * per
+
+    @torch.no_grad()
+    def quantized(self):
+        """An ``Int8ParallelLMHead`` of this head's present weight, for serving."""
+        from .int8 import Int8ParallelLMHead
+        config = SimpleNamespace(vocab_size=self.weight.shape[0] * self.ctx.tp_size,
+                                 n_embd=self.weight.shape[1],
+                                 sequence_parallel=self.sequence_parallel)
+        head = Int8ParallelLMHead(config, self.ctx).to(self.weight.device)
+        head.load_weight(self.weight)
+        return head
 
     def forward(self, x: torch.Tensor, labels: torch.Tensor | None = None) -> torch.Tensor:
         if labels is None:

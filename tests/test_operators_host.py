@@ -101,3 +101,72 @@ def test_embedding_refuses_shapes_and_types():
     for shape in ((10,), (10, 0), (2, 5, 8)):
         with pytest.raises(ValueError, match="must be"):
             check(t, Fake(shape, f32), 0, 10, f32)
+
+
+def test_int8_argument_errors_before_launch(lib):
+    p = 4096
+    quant = lib.nmce_quantize_rows
+    assert quant(p, 2, 4, 8, 8, p, 16, p, None) == -1
+    assert quant(p, 0, -1, 8, 8, p, 16, p, None) == -2
+    assert quant(p, 0, 4, 0, 8, p, 16, p, None) == -2
+    assert quant(p, 0, 4, 8, 7, p, 16, p, None) == -2
+    assert quant(p, 0, 4, 8, 8, p, 7, p, None) == -2
+    assert quant(p + 2, 0, 4, 8, 8, p, 16, p, None) == -3
+    assert quant(p, 0, 4, 8, 8, p, 16, p + 2, None) == -3
+    assert quant(p, 0, 4, 8, 8, None, 16, p, None) == -4
+    assert quant(None, 0, 0, 8, 8, None, 16, None, None) == 0
+    size, lin = lib.nmce_int8_linear_workspace_bytes, lib.nmce_int8_linear
+    assert size(-1, 8) == size(4, 0) == size(4, 131073) == -1 and size(0, 8) >= 0
+    ws = size(4, 32)
+    assert lin(p, 9, 4, 32, 32, p, 10, 32, p, p, 0, 10, p, ws, None) == -1
+    assert lin(p, 0, 4, 32, 32, p, 10, 32, p, p, 9, 10, p, ws, None) == -1
+    assert lin(p, 0, 4, 32, 31, p, 10, 32, p, p, 0, 10, p, ws, None) == -2
+    assert lin(p, 0, 4, 32, 32, p, 0, 32, p, p, 0, 10, p, ws, None) == -2
+    assert lin(p, 0, 4, 32, 32, p, 10, 16, p, p, 0, 10, p, ws, None) == -2
+    assert lin(p, 0, 4, 32, 32, p, 10, 1 << 23, p, p, 0, 10, p, ws, None) == -2
+    assert lin(p, 0, 4, 32, 32, p, 10, 32, p, p, 0, 9, p, ws, None) == -2
+    assert lin(p, 0, 4, 131073, 131073, p, 10, 131088, p, p, 0, 10, p, 1 << 40, None) == -2
+    assert lin(p, 0, 4, 32, 32, p + 8, 10, 32, p, p, 0, 10, p, ws, None) == -3
+    assert lin(p, 0, 4, 32, 32, p, 10, 40, p, p, 0, 10, p, ws, None) == -3
+    assert lin(p, 0, 4, 32, 32, p, 10, 32, p, p + 2, 0, 10, p, ws, None) == -3
+    assert lin(p, 0, 4, 32, 32, None, 10, 32, p, p, 0, 10, p, ws, None) == -4
+    assert lin(p, 0, 4, 32, 32, p, 10, 32, p, p, 0, 10, p, ws - 1, None) == -6
+    assert lin(p, 0, 4, 32, 32, p, 10, 32, p, p, 0, 10, None, ws, None) == -6
+    assert lin(None, 0, 0, 32, 32, None, 10, 32, None, None, 0, 10, None, 0, None) == 0
+
+
+def test_int8_refusals_without_a_gpu():
+    import nmce
+    x = torch.randn(4, 32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nmce.quantize_rows(x)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nmce.int8_linear(x, torch.zeros(3, 32, dtype=torch.int8), torch.ones(3))
+    cfg = types.SimpleNamespace(vocab_size=1000, n_embd=30, sequence_parallel=False)
+    two = nmce.ParallelContext(rank=1, world_size=2, tp_size=2, tp_rank=1, pp_size=1, pp_rank=0,
+                               dp_size=1, dp_rank=0)
+    head = nmce.Int8ParallelLMHead(cfg, two)
+    assert head.weight_q.shape == (500, 32) and head.vocab_range() == (500, 1000)
+    assert sorted(head.state_dict()) == ["weight_q", "weight_scale"]
+    assert not list(head.parameters())
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        head(torch.randn(2, 30))
+
+
+def test_int8_weight_rows():
+    """Which weights the product reads as they lie (no device needed)."""
+    from nmce.int8 import _weight_rows
+    base = torch.randint(-128, 128, (10, 48), dtype=torch.int8)
+    pad = (-base.data_ptr()) % 16
+    assert pad == 0
+    for w, same in ((base, True), (base[:, :33], True), (base[:, 16:40], True),
+                    (base[:, 8:40], False), (base[:, 32:47], True), (base.t(), False),
+                    (base[:1, :33], True), (base[:1].expand(10, 48), False),
+                    (base[:, :40].contiguous(), False), (base[3:7:2], True)):
+        got, ld = _weight_rows(w)
+        assert (got is w) == same, (w.shape, w.stride())
+        assert ld % 16 == 0 and ld >= w.shape[1]
+        assert torch.equal(got[:, :w.shape[1]], w)
+    # the last row ends with the storage, inside 16 bytes
+    tight = torch.zeros(9 * 48 + 33, dtype=torch.int8).as_strided((10, 33), (48, 1))
+    assert _weight_rows(tight)[0] is not tight
