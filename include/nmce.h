@@ -556,6 +556,70 @@ int nmce_int8_linear(const void* x, int dtype, int64_t n_rows, int64_t columns, 
                      int64_t workspace_bytes, void* stream);
 
 /*
+ * Verification of drafted tokens over a vocabulary shard, from given uniform
+ * numbers. With p = softmax(target / T), q = softmax(draft / T) at position i
+ * (all in 64 bits), the drafted token d stands while accept_u q(d) < p(d). At
+ * the first that does not, the next token is the first id whose running sum of
+ * max(p - q, 0) passes sample_u times all of it; after the last draft, of p.
+ *   - T not above 0 (or NaN): a draft stands where it is the lowest id of the
+ *     largest logit, which is also the next token.
+ *   - draft NULL: q is one at the drafted token.
+ *   - A drafted token outside [0, vocab_total) ends its sequence's drafts (the
+ *     padding of shorter ones); the next token comes from p there.
+ *   - A draft row that is no distribution (all -inf, or an infinity or NaN in
+ *     it) lets nothing stand; the next token comes from p. Such a target row
+ *     gives the token -1.
+ *   - Where max(p - q, 0) is nothing (adds up to 1e-14 or less, what rounding
+ *     leaves of equal distributions), the next token comes from p.
+ *   - Uniform numbers outside [0, 1) are taken as the nearest inside, NaN as 0.
+ * Shapes: target [batch, drafts + 1, vocab_local], draft [batch, drafts,
+ * vocab_local] with the given strides (elements; the vocabulary's is 1),
+ * aligned to their elements; draft_tokens and accept_u [batch, drafts] and
+ * sample_u [batch] contiguous; temperature [batch], or NULL: temperature_all.
+ */
+typedef struct nmce_verify_batch {
+  const void* target;
+  const void* draft;
+  const int64_t* draft_tokens;
+  const float* accept_u;
+  const float* sample_u;
+  const float* temperature;
+  int64_t target_batch_stride, target_row_stride;
+  int64_t draft_batch_stride, draft_row_stride;
+  int64_t batch, drafts;
+  int64_t vocab_local, vocab_start, vocab_total;
+  float temperature_all;
+  int dtype;
+} nmce_verify_batch;
+
+/* Slabs that a shard's rows are cut into, and the decisions' workspace. */
+int64_t nmce_verify_slabs(int64_t vocab_local);
+int64_t nmce_verify_workspace_bytes(int64_t batch);
+
+/*
+ * The steps, in order. stats: doubles [rows][slabs][4] of this shard's rows
+ * (batch x (drafts + 1) of the target, then batch x drafts of the draft). With
+ * several ranks gather them to [ranks][rows][slabs][4] for the next step, and
+ * its masses [batch][slabs][2] to [ranks][batch][slabs][2] for the one after.
+ * nmce_verify_masses writes accepted [batch] (how many drafts stand) and
+ * tokens, logprobs [batch][drafts + 1] but for the next token, whose place
+ * holds -1 and 0 until nmce_verify_pick writes it (one rank, picked NULL), or
+ * writes picked [batch][2], of which nmce_verify_finish takes the ranks'
+ * elementwise maximum. Places behind the next token hold -1 and 0. logprobs
+ * are log p of the tokens (of T = 1 where T is 0).
+ */
+int nmce_verify_stats(const nmce_verify_batch* batch, double* stats, void* stream);
+int nmce_verify_masses(const nmce_verify_batch* batch, const double* stats, int ranks,
+                       double* masses, int64_t* tokens, int64_t* accepted, float* logprobs,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+int nmce_verify_pick(const nmce_verify_batch* batch, const double* masses, int ranks, int rank,
+                     const void* workspace, int64_t workspace_bytes, int64_t* tokens,
+                     float* logprobs, double* picked, void* stream);
+int nmce_verify_finish(const double* picked, const void* workspace, int64_t workspace_bytes,
+                       int64_t batch, int64_t drafts, int64_t* tokens, float* logprobs,
+                       void* stream);
+
+/*
  * The GEMM core of the fused path, exposed for testing and measurement (no
  * counterpart in the reference): c[i, j] = sum_l a[i, l] * b[j, l] for
  * i < m, j < n, l < k, with bf16 a [m, lda] and b [n, ldb], fp32

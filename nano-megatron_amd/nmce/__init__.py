@@ -17,6 +17,8 @@ Public API (mirrors nano_megatron/cross_entropy.py and parallel.py):
 * ``quantize_rows(x)`` / ``int8_linear(x, weight, weight_scale)`` /
   ``Int8ParallelLMHead`` -- 8-bit rows, their product, and the serving head made
   of it (``FusedParallelLMHead.quantized()``).
+* ``vocab_parallel_verify_drafts(...)`` -- drafted tokens against the target's
+  sharded logits, from given uniform numbers; with no drafts, sampling.
 * ``copy_to_tensor_parallel_region`` / ``gather_from_sequence_parallel_region``
   / ``gather_tokens_rank_major`` -- the collectives on the LM head's input side
   (mappings.py:83-94, :109-120); ``reduce_from_tensor_parallel_region`` /
@@ -53,6 +55,7 @@ from .mappings import (
     targets_rank_major,
 )
 from .parallel import ParallelContext, divide, vocab_range
+from .verify import vocab_parallel_verify_drafts
 
 __all__ = [
     "FusedParallelLMHead",
@@ -75,5 +78,6 @@ __all__ = [
     "validate_targets",
     "vocab_parallel_cross_entropy",
     "vocab_parallel_embedding",
+    "vocab_parallel_verify_drafts",
     "vocab_range",
 ]

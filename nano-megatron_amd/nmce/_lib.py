@@ -78,6 +78,12 @@ SIGNATURES: dict[str, tuple] = {
     "nmce_int8_linear_workspace_bytes": (_i64, [_i64, _i64]),
     "nmce_int8_linear": (_c_int, [_p, _c_int, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _c_int,
                                   _i64, _p, _i64, _p]),
+    "nmce_verify_slabs": (_i64, [_i64]),
+    "nmce_verify_workspace_bytes": (_i64, [_i64]),
+    "nmce_verify_stats": (_c_int, [_p, _p, _p]),
+    "nmce_verify_masses": (_c_int, [_p, _p, _c_int, _p, _p, _p, _p, _p, _i64, _p]),
+    "nmce_verify_pick": (_c_int, [_p, _p, _c_int, _c_int, _p, _i64, _p, _p, _p, _p]),
+    "nmce_verify_finish": (_c_int, [_p, _p, _i64, _i64, _i64, _p, _p, _p]),
     "nmce_gemm_nt_bf16": (_c_int, [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _c_int, _i64, _p]),
     "nmce_gemm_mn_bf16": (_c_int, [_c_int, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "nmce_lmhead_ce_bwd_layout": (_c_int, [_i64, _i64, _i64, _i64, _p]),
@@ -85,6 +91,19 @@ SIGNATURES: dict[str, tuple] = {
     "nmce_lmhead_ce_bwd_dz": (_c_int, [_p, _p, _c_int, _i64, _i64, _i64, _p, _i64, _p, _p, _p,
                                        _i64, _i64, _i64, _p, _i64, _p]),
 }
+
+
+class VerifyBatch(ctypes.Structure):
+    """``nmce_verify_batch`` of include/nmce.h."""
+
+    _fields_ = ([(name, _p) for name in ("target", "draft", "draft_tokens", "accept_u", "sample_u",
+                                         "temperature")]
+                + [(name, _i64) for name in ("target_batch_stride", "target_row_stride",
+                                             "draft_batch_stride", "draft_row_stride", "batch",
+                                             "drafts", "vocab_local", "vocab_start",
+                                             "vocab_total")]
+                + [("temperature_all", ctypes.c_float), ("dtype", _c_int)])
+
 
 NMCE_LMHEAD_LAYOUT_FIELDS = 10
 NMCE_LMHEAD_FUSED_LAYOUT_FIELDS = 12

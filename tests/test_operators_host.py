@@ -170,3 +170,57 @@ def test_int8_weight_rows():
     # the last row ends with the storage, inside 16 bytes
     tight = torch.zeros(9 * 48 + 33, dtype=torch.int8).as_strided((10, 33), (48, 1))
     assert _weight_rows(tight)[0] is not tight
+
+
+def test_verify_argument_errors_before_launch(lib):
+    import ctypes
+    from nmce import _lib as L
+    p = 4096
+
+    def batch(**kwargs):
+        fields = dict(target=p, draft=p, draft_tokens=p, accept_u=p, sample_u=p, temperature=None,
+                      target_batch_stride=40, target_row_stride=10, draft_batch_stride=30,
+                      draft_row_stride=10, batch=2, drafts=3, vocab_local=10, vocab_start=0,
+                      vocab_total=10, temperature_all=1.0, dtype=0)
+        fields.update(kwargs)
+        return L.VerifyBatch(**fields)
+
+    def stats(out=p, **kwargs):
+        b = batch(**kwargs)
+        return lib.nmce_verify_stats(ctypes.addressof(b), out, None)
+
+    assert lib.nmce_verify_slabs(0) == -1 and lib.nmce_verify_slabs(1) == 1
+    assert lib.nmce_verify_slabs(8192) == 1 and lib.nmce_verify_slabs(8193) == 2
+    assert lib.nmce_verify_workspace_bytes(-1) == -1 and lib.nmce_verify_workspace_bytes(0) == 0
+    assert lib.nmce_verify_stats(None, p, None) == -4
+    assert stats(dtype=2) == -1
+    for bad in (dict(batch=-1), dict(drafts=-1), dict(vocab_local=0), dict(vocab_start=-1),
+                dict(vocab_start=1), dict(vocab_total=9), dict(batch=1 << 22, drafts=1),
+                dict(batch=1 << 20, vocab_local=80000, vocab_total=80000),
+                dict(vocab_local=1 << 31, vocab_total=1 << 31)):
+        assert stats(**bad) == -2, bad
+    assert stats(target=None) == stats(draft_tokens=None) == stats(accept_u=None) == -4
+    assert stats(sample_u=None) == stats(out=None) == -4
+    assert stats(target=p + 2) == stats(draft=p + 1) == stats(dtype=1, target=p + 1) == -3
+    assert stats(batch=0, target=None) == 0
+    b = batch()
+    at, ws = ctypes.addressof(b), lib.nmce_verify_workspace_bytes(2)
+    assert lib.nmce_verify_masses(at, p, 0, p, p, p, p, p, ws, None) == -5
+    assert lib.nmce_verify_masses(at, None, 1, p, p, p, p, p, ws, None) == -4
+    assert lib.nmce_verify_masses(at, p, 1, p, p, p, None, p, ws, None) == -4
+    assert lib.nmce_verify_masses(at, p, 1, p, p, p, p, p, ws - 1, None) == -6
+    assert lib.nmce_verify_pick(at, p, 2, 2, p, ws, p, p, p, None) == -5
+    assert lib.nmce_verify_pick(at, p, 2, 1, p, ws, p, p, None, None) == -4  # ranks need picked
+    assert lib.nmce_verify_pick(at, p, 1, 0, p, 0, p, p, None, None) == -6
+    assert lib.nmce_verify_finish(None, p, ws, 2, 3, p, p, None) == -4
+    assert lib.nmce_verify_finish(p, p, ws, -1, 3, p, p, None) == -2
+    assert lib.nmce_verify_finish(p, p, 0, 2, 3, p, p, None) == -6
+    assert lib.nmce_verify_finish(None, None, 0, 0, 3, None, None, None) == 0
+
+
+def test_verify_has_no_cpu_path():
+    import nmce
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nmce.vocab_parallel_verify_drafts(
+            torch.zeros(1, 2, 5), torch.zeros(1, 1, dtype=torch.int64), None, torch.zeros(1, 1),
+            torch.zeros(1), 0, 5, nmce.ParallelContext.single())
