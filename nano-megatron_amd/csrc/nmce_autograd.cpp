@@ -1,4 +1,5 @@
-// The drop-in loss's one-pass path at TP = 1 as a C++ autograd node.
+// The drop-in loss's one-pass path at TP = 1, and the embedding lookup, as C++
+// autograd nodes.
 //
 // Forward and backward of cross_entropy.py:16-65 followed by the wrapper's
 // .mean() (:85), for the rows the one-pass kernel takes: one launch of
@@ -18,6 +19,7 @@
 // (one_pass_mean_checked).
 #include <torch/extension.h>
 #include <torch/csrc/autograd/variable.h>
+#include <ATen/TensorUtils.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -411,6 +413,128 @@ at::Tensor assumed_of(const at::Tensor& loss) {
   return saved[node->ctx_.saved_data.at("inplace").toBool() ? 2 : 4];
 }
 
+// ---- the embedding -----------------------------------------------------------
+// One shard's lookup (nmce_embedding_fwd) and the weight's dense gradient
+// (nmce_embedding_bwd). The gradient is linear in the output's, so its own
+// derivative is the lookup again: a backward under create_graph goes through
+// EmbeddingGrad and can be differentiated further.
+
+// [..., h] as rows of contiguous elements: a view where they lie so, else a copy.
+at::Tensor rows_of(const at::Tensor& t, int64_t* ld) {
+  const int64_t h = t.size(-1), n = h ? t.numel() / h : 0;
+  at::Tensor rows;
+  if (t.stride(-1) == 1 || h == 1) {
+    const std::vector<int64_t> shape = {n, h};
+    const auto strides = at::detail::computeStride(t.sizes(), t.strides(), shape);
+    if (strides && (n <= 1 || (*strides)[0] >= h)) rows = t.view(shape);
+  }
+  if (!rows.defined()) rows = t.contiguous().view({n, h});
+  *ld = n > 1 ? rows.stride(0) : h;
+  return rows;
+}
+
+at::Tensor lookup(const at::Tensor& weight, const at::Tensor& flat, at::IntArrayRef lead,
+                  int64_t vocab_start, double scale, at::ScalarType out_type) {
+  const c10::DeviceGuard device_guard(weight.device());
+  const at::Tensor w = weight.detach();
+  int64_t ld;
+  const at::Tensor rows = rows_of(w, &ld);
+  const int64_t v = rows.size(0), h = rows.size(1);
+  std::vector<int64_t> shape = lead.vec();
+  shape.push_back(h);
+  at::Tensor out = at::empty(shape, w.options().dtype(out_type));
+  hipStream_t st = stream_of(w);
+  timed("nmce_embedding_fwd", st, [&] {
+    return nmce_embedding_fwd(flat.data_ptr<int64_t>(), flat.numel(), rows.data_ptr(),
+                              dtype_code(rows), v, h, ld, vocab_start, static_cast<float>(scale),
+                              out.data_ptr(), dtype_code(out), h, st);
+  });
+  return out;
+}
+
+at::Tensor lookup_grad(const at::Tensor& grad, const at::Tensor& flat, int64_t v,
+                       int64_t vocab_start, double scale, at::ScalarType weight_type) {
+  const c10::DeviceGuard device_guard(grad.device());
+  const at::Tensor g = grad.detach();
+  int64_t ld;
+  const at::Tensor dy = rows_of(g, &ld);
+  const int64_t n = flat.numel(), h = dy.size(1);
+  at::Tensor dw = at::empty({v, h}, g.options().dtype(weight_type));
+  const int64_t need = nmce_embedding_bwd_workspace_bytes(n, v, h);
+  at::Tensor ws = at::empty({need > 16 ? need : 16}, g.options().dtype(at::kByte));
+  hipStream_t st = stream_of(g);
+  timed("nmce_embedding_bwd", st, [&] {
+    return nmce_embedding_bwd(flat.data_ptr<int64_t>(), n, dy.data_ptr(), dtype_code(dy), ld, v, h,
+                              vocab_start, static_cast<float>(scale), dw.data_ptr(),
+                              dtype_code(dw), ws.data_ptr(), ws.numel(), st);
+  });
+  return dw;
+}
+
+at::Tensor embedding(const at::Tensor& weight, const at::Tensor& tokens, int64_t vocab_start,
+                     double scale, at::ScalarType out_type);
+
+struct EmbeddingGrad : public torch::autograd::Function<EmbeddingGrad> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& grad,
+                            const at::Tensor& tokens, int64_t v, int64_t vocab_start, double scale,
+                            at::ScalarType weight_type) {
+    ctx->saved_data["start"] = vocab_start;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["type"] = grad.scalar_type();
+    ctx->save_for_backward({tokens});
+    return lookup_grad(grad, tokens.reshape({-1}).contiguous(), v, vocab_start, scale,
+                       weight_type);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(6);
+    out[0] = embedding(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["start"].toInt(),
+                       ctx->saved_data["scale"].toDouble(),
+                       ctx->saved_data["type"].toScalarType());
+    return out;
+  }
+};
+
+struct Embedding : public torch::autograd::Function<Embedding> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& weight,
+                            const at::Tensor& tokens, int64_t vocab_start, double scale,
+                            at::ScalarType out_type) {
+    ctx->saved_data["start"] = vocab_start;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["type"] = weight.scalar_type();
+    ctx->saved_data["rows"] = weight.size(0);
+    ctx->save_for_backward({tokens});
+    return lookup(weight, tokens.reshape({-1}).contiguous(), tokens.sizes(), vocab_start, scale,
+                  out_type);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const at::Tensor tokens = ctx->get_saved_variables()[0];
+    const int64_t start = ctx->saved_data["start"].toInt(), v = ctx->saved_data["rows"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const at::ScalarType type = ctx->saved_data["type"].toScalarType();
+    variable_list out(5);
+    out[0] = at::GradMode::is_enabled() && grads[0].requires_grad()
+                 ? EmbeddingGrad::apply(grads[0], tokens, v, start, scale, type)
+                 : lookup_grad(grads[0], tokens.reshape({-1}).contiguous(), v, start, scale, type);
+    return out;
+  }
+};
+
+at::Tensor embedding(const at::Tensor& weight, const at::Tensor& tokens, int64_t vocab_start,
+                     double scale, at::ScalarType out_type) {
+  return Embedding::apply(weight, tokens, vocab_start, scale, out_type);
+}
+
+// The entry from Python. It reads device addresses: what would hand it another
+// kind of tensor is refused here too (the wrapper has checked the rest).
+at::Tensor embedding_entry(const at::Tensor& weight, const at::Tensor& tokens,
+                           int64_t vocab_start, double scale, bool f32_out) {
+  TORCH_CHECK(weight.is_cuda() && tokens.device() == weight.device() && weight.dim() == 2 &&
+                  tokens.scalar_type() == at::kLong,
+              "nmce: the embedding takes a [vocabulary, hidden] weight and int64 tokens on one "
+              "ROCm device (there is no CPU path)");
+  return embedding(weight, tokens, vocab_start, scale, f32_out ? at::kFloat : at::kBFloat16);
+}
+
 void set_timing(bool on) { g_timing = on; }
 
 // (name, milliseconds) of every launch timed since the last call, in launch
@@ -461,7 +585,8 @@ at::Tensor head_output(const at::Tensor& logits, const at::Tensor& anchor) {
 }  // namespace
 
 PYBIND11_MODULE(_nmce_autograd, m) {
-  m.doc() = "The one-pass loss at TP = 1 as a C++ autograd node over libnmce's C ABI.";
+  m.doc() = "The one-pass loss at TP = 1 and the embedding as C++ autograd nodes over libnmce's "
+            "C ABI.";
   m.def("one_pass_mean", &one_pass_mean, "mean one-pass loss (forward + backward in C++)");
   m.def("one_pass_mean_checked", &one_pass_mean_checked,
         "one_pass_mean after the target check; ValueError on a target outside the vocabulary");
@@ -471,6 +596,8 @@ PYBIND11_MODULE(_nmce_autograd, m) {
       .def("query", &TargetCheck::query, "whether the check is over")
       .def("wait", &TargetCheck::wait, "wait for it; the count of bad targets");
   m.def("assumed_of", &assumed_of, "the assumed upstream value saved by a one-pass loss");
+  m.def("embedding", &embedding_entry,
+        "a vocabulary shard's scaled lookup, with the weight's dense gradient");
   m.def("set_timing", &set_timing, "time every launch with HIP events while on");
   m.def("take_timeline", &take_timeline, "(name, ms) of the launches timed since the last call");
   m.def("head_output", &head_output,

@@ -35,11 +35,7 @@ from .cross_entropy import (
     validate_targets,
     vocab_parallel_cross_entropy,
 )
-from .embedding import (
-    VocabParallelEmbedding,
-    _VocabParallelEmbedding,
-    vocab_parallel_embedding,
-)
+from .embedding import VocabParallelEmbedding, vocab_parallel_embedding
 from .int8 import Int8ParallelLMHead, int8_linear, quantize_rows
 from .lmhead import (
     FusedParallelLMHead,
@@ -62,7 +58,6 @@ __all__ = [
     "Int8ParallelLMHead",
     "_LMHeadVocabParallelCrossEntropy",
     "_VocabParallelCrossEntropy",
-    "_VocabParallelEmbedding",
     "ParallelContext",
     "VocabParallelEmbedding",
     "copy_to_tensor_parallel_region",

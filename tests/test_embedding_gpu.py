@@ -249,6 +249,46 @@ def test_graph_replays():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_second_derivatives():
+    """The weight's gradient is linear in the output's: its derivative is the
+    lookup of the second gradient, and that one's the scatter again."""
+    import nmce
+    ctx = nmce.ParallelContext.single()
+    g = torch.Generator().manual_seed(11)
+    weight = torch.randn(30, 16, generator=g).to(DEV).requires_grad_(True)
+    tokens = torch.randint(-5, 35, (4, 9), generator=g).to(DEV)
+    dy = torch.randn(4, 9, 16, generator=g).to(DEV).requires_grad_(True)
+    out = nmce.vocab_parallel_embedding(tokens, weight, 0, 30, ctx, scale=3.0, validate=False)
+    dw, = torch.autograd.grad(out, weight, dy, create_graph=True)
+    _check(out, dw.detach(), tokens, weight, dy.detach(), 0, 3.0)
+    second = torch.randn(30, 16, generator=g).to(DEV).requires_grad_(True)
+    ddy, = torch.autograd.grad(dw, dy, second, create_graph=True)
+    back, = torch.autograd.grad(ddy, second, dy.detach())
+    _check(ddy, back, tokens, second, dy.detach(), 0, 3.0)
+
+
+def test_gradient_by_differences():
+    """(f(W + e D) - f(W - e D)) / 2 e = <dW, D> for f = <out, dY>: f is linear, so
+    the difference is exact up to fp32's rounding of the sums (2^-24 of their
+    magnitudes, divided by e)."""
+    import nmce
+    ctx = nmce.ParallelContext.single()
+    g = torch.Generator().manual_seed(12)
+    tokens = torch.randint(0, 40, (200,), generator=g).to(DEV)
+    w0, d = (torch.randn(40, 24, generator=g).to(DEV) for _ in range(2))
+    dy = torch.randn(200, 24, generator=g).to(DEV)
+    w = w0.clone().requires_grad_(True)
+    out = nmce.vocab_parallel_embedding(tokens, w, 0, 40, ctx, scale=2.0)
+    dw, = torch.autograd.grad(out, w, dy)
+    step = 2.0 ** -3
+    f = [nmce.vocab_parallel_embedding(tokens, w0 + s * step * d, 0, 40, ctx, scale=2.0).double()
+         for s in (1, -1)]
+    got = ((f[0] - f[1]) * dy.double()).sum() / (2 * step)
+    want = (dw.double() * d.double()).sum()
+    slack = ((f[0].abs() + f[1].abs()) * dy.double().abs()).sum() * 2.0 ** -23 / step
+    assert abs(float(got - want)) <= float(slack)
+
+
 def test_tied_with_the_fused_head():
     """One training step through both ends of a tied weight: the embedding's
     rows go straight into the fused head + loss. The gradient is the sum of

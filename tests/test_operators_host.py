@@ -47,14 +47,15 @@ def test_embedding_argument_errors_before_launch(lib):
     assert bwd(p, 4, p, 0, 8, 8, 8, 0, 1.0, p, 0, p + 8, ws, None) == -6
 
 
-def test_embedding_refusals():
+def test_embedding_refusals(lib):
     import nmce
+    from nmce import _lib as L
     ctx = nmce.ParallelContext.single()
     w, t = torch.randn(10, 8), torch.zeros(3, dtype=torch.int64)
     with pytest.raises(RuntimeError, match="no CPU path"):
         nmce.vocab_parallel_embedding(t, w, 0, 10, ctx)
     with pytest.raises(RuntimeError, match="no CPU path"):
-        nmce._VocabParallelEmbedding.apply(w, t, 0, 10, 1.0, torch.float32)
+        L.autograd_ext().embedding(w, t, 0, 1.0, True)
     cfg = types.SimpleNamespace(vocab_size=1001, n_embd=8)
     two = nmce.ParallelContext(rank=1, world_size=2, tp_size=2, tp_rank=1, pp_size=1, pp_rank=0,
                                dp_size=1, dp_rank=0)
