@@ -504,7 +504,7 @@ int nmce_lmhead_ce_fused_chunk_grads(const void* hidden, const void* weight, int
  * (any int64; nothing is read out of bounds). weight [vocab_local, ldw] and
  * out [n_tokens, ldo] are NMCE_F32 or NMCE_BF16 each, aligned to their
  * element; rows on the 16-byte grid go by 16-byte vectors. n_tokens and
- * vocab_local below 2^31.
+ * vocab_local below 2^31, hidden at most 2^24.
  */
 int nmce_embedding_fwd(const int64_t* tokens, int64_t n_tokens, const void* weight,
                        int weight_dtype, int64_t vocab_local, int64_t hidden, int64_t ldw,

@@ -30,6 +30,7 @@ constexpr int kSlab = 512;         // columns of a wave: 8 a lane
 constexpr int kPerLane = kSlab / 64;
 constexpr int kBlock = 256;        // four waves, each on its own
 constexpr int64_t kMaxBlocks = 1 << 22;  // grid-stride past this many
+constexpr int64_t kMaxHidden = 1 << 24;
 
 // The 8 columns of `slab` that a lane holds: kVec: 8 in a row (16-byte
 // accesses); otherwise every 64th (any alignment; coalesced).
@@ -38,31 +39,64 @@ __device__ __forceinline__ int64_t column(int64_t slab, int lane, int e) {
   return slab * kSlab + (kVec ? lane * kPerLane + e : lane + 64 * e);
 }
 
-template <typename T, bool kVec>
-__device__ __forceinline__ void load_row(const T* __restrict__ row, int64_t slab, int lane,
-                                         int64_t h, float* f) {
-  if (kVec && column<true>(slab, lane, kPerLane - 1) < h) {
-    const T* p = row + column<true>(slab, lane, 0);
-#pragma unroll
-    for (int v = 0; v < kPerLane; v += Elem<T>::kPerVec)
-      Elem<T>::unpack(*reinterpret_cast<const u32x4*>(p + v), f + v);
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < kPerLane; ++e) {
-    const int64_t c = column<kVec>(slab, lane, e);
-    f[e] = c < h ? Elem<T>::load1(row + c) : 0.0f;
-  }
-}
+// A lane's 8 columns of one row as they were loaded, so that several rows' loads
+// are in flight before the first is unpacked.
+template <typename T, bool kVec, bool kStream = false>
+struct Row {
+  static constexpr int kVecs = kPerLane / Elem<T>::kPerVec;
+  u32x4 v[kVec ? kVecs : 1];
+  T e[kVec ? 1 : kPerLane];
 
-template <typename T, bool kVec>
+  __device__ __forceinline__ void load(const T* __restrict__ row, int64_t slab, int lane,
+                                       int64_t h) {
+    if constexpr (kVec) {
+      const int64_t c0 = column<true>(slab, lane, 0);
+      if (c0 + kPerLane <= h) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          const u32x4* p = reinterpret_cast<const u32x4*>(row + c0 + i * Elem<T>::kPerVec);
+          v[i] = kStream ? load_stream(p) : *p;
+        }
+      } else {  // the row's last columns, fewer than 8
+        float f[kPerLane];
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+          f[i] = c0 + i < h ? Elem<T>::load1(row + c0 + i) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) v[i] = Elem<T>::pack(f + i * Elem<T>::kPerVec);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const int64_t c = column<false>(slab, lane, i);
+        e[i] = c < h ? row[c] : T(0);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    if constexpr (kVec) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) Elem<T>::unpack(v[i], f + i * Elem<T>::kPerVec);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) f[i] = Elem<T>::load1(&e[i]);
+    }
+  }
+};
+
+template <typename T, bool kVec, bool kStream = false>
 __device__ __forceinline__ void store_row(T* __restrict__ row, int64_t slab, int lane, int64_t h,
                                           const float* f) {
   if (kVec && column<true>(slab, lane, kPerLane - 1) < h) {
     T* p = row + column<true>(slab, lane, 0);
 #pragma unroll
-    for (int v = 0; v < kPerLane; v += Elem<T>::kPerVec)
-      *reinterpret_cast<u32x4*>(p + v) = Elem<T>::pack(f + v);
+    for (int v = 0; v < kPerLane; v += Elem<T>::kPerVec) {
+      u32x4* q = reinterpret_cast<u32x4*>(p + v);
+      if (kStream)
+        store_stream(q, Elem<T>::pack(f + v));
+      else
+        *q = Elem<T>::pack(f + v);
+    }
     return;
   }
 #pragma unroll
@@ -80,26 +114,41 @@ __device__ __forceinline__ uint32_t local_row(int64_t t, int64_t start, int64_t 
                                                                 : static_cast<uint64_t>(vocab));
 }
 
-// A wave copies 512 columns of one token's row.
-template <typename W, typename O, bool kVec>
+// A wave copies 512 columns (blockIdx.y's) of kRows tokens' rows, whose loads are
+// in flight together. With one row a wave, its three dependent accesses (id, row,
+// output) and nothing beside them, 131072 rows of 1024 took 87 us; with eight 51.
+// Fewer tokens than fill the chip that way take one each.
+template <typename W, typename O, bool kVec, int kRows>
 __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(
     const int64_t* __restrict__ tokens, int64_t n, const W* __restrict__ weight, int64_t vocab,
-    int64_t h, int64_t ldw, int64_t start, float scale, O* __restrict__ out, int64_t ldo,
-    int64_t slabs) {
+    int64_t h, int64_t ldw, int64_t start, float scale, O* __restrict__ out, int64_t ldo) {
   const int lane = threadIdx.x & 63;
-  const int64_t total = n * slabs;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kBlock / 64);
-  for (int64_t id = static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + (threadIdx.x >> 6);
-       id < total; id += step) {
-    const int64_t i = id / slabs, slab = id - i * slabs;
-    const uint32_t r = local_row(tokens[i], start, vocab);
-    float f[kPerLane] = {};
-    if (r < vocab) {
-      load_row<W, kVec>(weight + r * ldw, slab, lane, h, f);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t slab = blockIdx.y;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kBlock / 64) * kRows;
+  for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * (kBlock / 64) + wave) * kRows; i0 < n;
+       i0 += step) {
+    const int mine = lane % kRows;
+    const uint32_t my_row =
+        local_row(tokens[i0 + mine < n ? i0 + mine : n - 1], start, vocab);
+    Row<W, kVec> rows[kRows];
+    uint32_t at[kRows];
 #pragma unroll
-      for (int e = 0; e < kPerLane; ++e) f[e] *= scale;
+    for (int r = 0; r < kRows; ++r) {
+      at[r] = __builtin_amdgcn_readlane(my_row, r);
+      if (at[r] < vocab) rows[r].load(weight + at[r] * ldw, slab, lane, h);
     }
-    store_row<O, kVec>(out + i * ldo, slab, lane, h, f);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (i0 + r >= n) break;
+      float f[kPerLane] = {};
+      if (at[r] < vocab) {
+        rows[r].get(f);
+#pragma unroll
+        for (int e = 0; e < kPerLane; ++e) f[e] *= scale;
+      }
+      store_row<O, kVec, (kRows > 1)>(out + (i0 + r) * ldo, slab, lane, h, f);
+    }
   }
 }
 
@@ -118,6 +167,26 @@ static_assert(kBins == kSortBlock, "a thread per bin");
 constexpr int kMaxTiles = 64;
 constexpr int kMinTile = 4096;
 
+// dW's zeros, written by the workgroups of a sort launch that have no tile: 16
+// bytes a thread (again a launch further on where dW is larger than that), dW's
+// last bytes, fewer than 16, one by one. The sort keeps 64 compute units at most,
+// and waits for memory more than it reads: under the fill it costs nothing. More
+// stores a thread leave the launch's writes further apart: 1.05 GB beside the sort
+// of 16384 ids 164 us with one, 181 with two, 215 with four.
+struct Fill {
+  char* to;
+  int64_t bytes;
+};
+constexpr int64_t kMaxFillThreads = int64_t{1} << 31;
+
+__device__ __forceinline__ void fill_zeros(const Fill& f, int64_t block) {
+  const int64_t vecs = f.bytes / 16;
+  const int64_t first = block * blockDim.x + threadIdx.x;
+  for (int64_t i = first; i < vecs; i += kMaxFillThreads)
+    store_stream(reinterpret_cast<u32x4*>(f.to) + i, u32x4{0, 0, 0, 0});
+  if (first < f.bytes - vecs * 16) f.to[vecs * 16 + first] = 0;
+}
+
 struct SortArgs {
   const int64_t* tokens;  // first pass: the ids; later: keys and positions
   const uint32_t* keys;
@@ -125,9 +194,17 @@ struct SortArgs {
   uint32_t* keys_out;
   uint32_t* pos_out;
   uint32_t* hist;         // [tiles][kBins]
+  Fill fill;              // this launch's share of dW
   int64_t n, start, vocab, tile;
   int tiles, shift, bits;
 };
+
+// A sort launch's workgroups behind the tiles fill; true for those.
+__device__ __forceinline__ bool filled(const SortArgs& a) {
+  if (static_cast<int>(blockIdx.x) < a.tiles) return false;
+  fill_zeros(a.fill, static_cast<int>(blockIdx.x) - a.tiles);
+  return true;
+}
 
 template <bool kFirst>
 __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int64_t i) {
@@ -160,6 +237,7 @@ __device__ __forceinline__ void count_digits(const SortArgs& a, uint32_t (*cnt)[
 template <bool kFirst>
 __global__ __launch_bounds__(kSortBlock) void sort_count_kernel(SortArgs a) {
   __shared__ uint32_t cnt[kSortWaves][kBins];
+  if (filled(a)) return;
   count_digits<kFirst>(a, cnt, threadIdx.x >> 6, threadIdx.x & 63);
   uint32_t sum = 0;
   for (int w = 0; w < kSortWaves; ++w) sum += cnt[w][threadIdx.x];
@@ -170,6 +248,7 @@ template <bool kFirst>
 __global__ __launch_bounds__(kSortBlock) void sort_move_kernel(SortArgs a) {
   __shared__ uint32_t cnt[kSortWaves][kBins];
   __shared__ uint32_t scan[kBins];
+  if (filled(a)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = threadIdx.x;
   count_digits<kFirst>(a, cnt, wave, lane);
   // Keys of smaller digits, of the same digit in earlier tiles, and in this
@@ -226,15 +305,124 @@ __global__ __launch_bounds__(kSortBlock) void sort_move_kernel(SortArgs a) {
   }
 }
 
+// The whole sort in one workgroup, for lists of at most kSmallSort positions: a
+// key and its position share 32 bits (position in the low bits), a thread holds
+// up to 16 of them in registers, and each pass ranks them as above and scatters
+// them through LDS. The counts and the list share the LDS: one is dead where the
+// other is written. One launch, most of it the fill, where the passes above are
+// four and more; 16384 positions take 29 us in it, less than the fill beside it
+// once dW is a few hundred megabytes.
+constexpr int kSmallBlock = 1024;
+constexpr int kSmallWaves = kSmallBlock / 64;
+constexpr int kSmallEach = 16;
+constexpr int kSmallSort = kSmallBlock * kSmallEach;
+constexpr int kSmallCounts = kSmallWaves * kBins * 2 + kBins * 4;  // bytes
+
+struct SmallSortArgs {
+  const int64_t* tokens;
+  uint32_t* keys_out;
+  uint32_t* pos_out;
+  Fill fill;
+  int64_t start, vocab;
+  int n, pos_bits, passes, bits;
+};
+
+__global__ __launch_bounds__(kSmallBlock) void sort_small_kernel(SmallSortArgs a) {
+  extern __shared__ __align__(16) char lds[];
+  if (blockIdx.x > 0) {
+    fill_zeros(a.fill, static_cast<int>(blockIdx.x) - 1);
+    return;
+  }
+  uint32_t* list = reinterpret_cast<uint32_t*>(lds);
+  uint16_t* counts = reinterpret_cast<uint16_t*>(lds);  // [kSmallWaves][kBins]
+  uint32_t* scan = reinterpret_cast<uint32_t*>(lds + kSmallWaves * kBins * 2);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int rounds = (a.n + kSmallBlock - 1) / kSmallBlock;
+  const int first = wave * rounds * 64 + lane;  // this thread's positions: every 64th
+  uint32_t key[kSmallEach], to[kSmallEach];
+#pragma unroll
+  for (int i = 0; i < kSmallEach; ++i) {
+    const int at = first + 64 * i;
+    if (i < rounds && at < a.n)
+      key[i] = local_row(a.tokens[at], a.start, a.vocab) << a.pos_bits | at;
+  }
+  const uint32_t mask = (1u << a.bits) - 1;
+  for (int p = 0; p < a.passes; ++p) {
+    const int shift = a.pos_bits + p * a.bits;
+    if (p > 0) {
+#pragma unroll
+      for (int i = 0; i < kSmallEach; ++i)
+        if (i < rounds && first + 64 * i < a.n) key[i] = list[first + 64 * i];
+      __syncthreads();
+    }
+    for (int d = tid; d < kSmallWaves * kBins / 2; d += kSmallBlock)
+      reinterpret_cast<uint32_t*>(counts)[d] = 0;
+    __syncthreads();
+    // Ranks within the wave; counts[wave][d] ends as its keys of digit d.
+    volatile uint16_t* mine = counts + wave * kBins;
+#pragma unroll
+    for (int i = 0; i < kSmallEach; ++i) {
+      if (i < rounds) {
+        const bool valid = first + 64 * i < a.n;
+        const uint32_t digit = (key[i] >> shift) & mask;
+        uint64_t same = __ballot(valid);
+        for (int b = 0; b < a.bits; ++b) {
+          const uint64_t set = __ballot((digit >> b) & 1u);
+          same &= (digit >> b) & 1u ? set : ~set;
+        }
+        const uint32_t rank = __builtin_amdgcn_mbcnt_hi(
+            static_cast<uint32_t>(same >> 32),
+            __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(same), 0u));
+        const uint32_t before = valid ? mine[digit] : 0u;
+        to[i] = before + rank;
+        __builtin_amdgcn_wave_barrier();
+        if (valid && rank == 0)
+          mine[digit] = static_cast<uint16_t>(before + static_cast<uint32_t>(__popcll(same)));
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    __syncthreads();
+    // Where each wave's first key of each digit goes.
+    uint32_t total = 0;
+    if (tid < kBins) {
+      for (int w = 0; w < kSmallWaves; ++w) total += counts[w * kBins + tid];
+      scan[tid] = total;
+    }
+    __syncthreads();
+    for (int s = 1; s < kBins; s <<= 1) {
+      const uint32_t v = tid >= s && tid < kBins ? scan[tid - s] : 0u;
+      __syncthreads();
+      if (tid < kBins) scan[tid] += v;
+      __syncthreads();
+    }
+    if (tid < kBins) {
+      uint32_t at = scan[tid] - total;
+      for (int w = 0; w < kSmallWaves; ++w) {
+        const uint32_t c = counts[w * kBins + tid];
+        counts[w * kBins + tid] = static_cast<uint16_t>(at);  // below kSmallSort
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSmallEach; ++i)
+      if (i < rounds && first + 64 * i < a.n)
+        to[i] += counts[wave * kBins + ((key[i] >> shift) & mask)];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSmallEach; ++i)
+      if (i < rounds && first + 64 * i < a.n) list[to[i]] = key[i];
+    __syncthreads();
+  }
+  for (int i = tid; i < a.n; i += kSmallBlock) {
+    a.keys_out[i] = list[i] >> a.pos_bits;
+    a.pos_out[i] = list[i] & ((1u << a.pos_bits) - 1);
+  }
+}
+
 // ---- dW ---------------------------------------------------------------------
-// 16 zero bytes a thread; dW's last bytes, fewer than 16, one by one.
-__global__ __launch_bounds__(kBlock) void zero_kernel(char* __restrict__ p, int64_t bytes) {
-  const int64_t vecs = bytes / 16;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kBlock;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
-  for (int64_t i = first; i < vecs; i += step)
-    store_stream(reinterpret_cast<u32x4*>(p) + i, u32x4{0, 0, 0, 0});
-  if (first < bytes - vecs * 16) p[vecs * 16 + first] = 0;
+__global__ __launch_bounds__(kBlock) void zero_kernel(Fill f) {
+  fill_zeros(f, blockIdx.x);
 }
 
 struct SumArgs {
@@ -261,9 +449,15 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const G* __restrict__
     const int64_t c = id / a.slabs, slab = id - c * a.slabs;
     const int64_t first = c * a.chunk;
     const int64_t end = first + a.chunk < a.n ? first + a.chunk : a.n;
-    uint32_t cur = a.keys[first];
+    // The keys around the chunk and its first 64 positions, asked for together.
+    const uint32_t prev_key = c > 0 ? a.keys[first - 1] : 0u;
+    const uint32_t next_key = a.keys[end < a.n ? end : a.n - 1];
+    int count = static_cast<int>(end - first < 64 ? end - first : 64);
+    uint32_t my_key = a.keys[first + (lane < count ? lane : 0)];
+    uint32_t my_pos = a.pos[first + (lane < count ? lane : 0)];
+    uint32_t cur = __builtin_amdgcn_readfirstlane(my_key);
     if (cur >= a.vocab) continue;  // so are all behind it
-    bool from_before = c > 0 && a.keys[first - 1] == cur;
+    bool from_before = c > 0 && prev_key == cur;
     float sum[kPerLane] = {};
     // The current id's sum is complete unless it began before this chunk.
     auto finish = [&](bool goes_on) {
@@ -279,18 +473,21 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const G* __restrict__
     };
     bool others = false;  // the rest of the list is other shards'
     for (int64_t batch = first; batch < end && !others; batch += 64) {
-      const int count = static_cast<int>(end - batch < 64 ? end - batch : 64);
-      const uint32_t my_key = lane < count ? a.keys[batch + lane] : 0u;
-      const uint32_t my_pos = lane < count ? a.pos[batch + lane] : 0u;
-      for (int j0 = 0; j0 < count && !others; j0 += kAhead) {
-        float row[kAhead][kPerLane];
+      if (batch > first) {
+        count = static_cast<int>(end - batch < 64 ? end - batch : 64);
+        my_key = a.keys[batch + (lane < count ? lane : 0)];
+        my_pos = a.pos[batch + (lane < count ? lane : 0)];
+      }
+      // Rows past the count repeat the last one: loads without branches.
+      auto load = [&](Row<G, kVec, true>* rows, int j0) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-          if (j0 + j < count) {
-            const uint32_t p = __builtin_amdgcn_readlane(my_pos, j0 + j);
-            load_row<G, kVec>(dy + p * a.ldy, slab, lane, a.h, row[j]);
-          }
+          const int at = j0 + j < count ? j0 + j : count - 1;
+          const uint32_t p = __builtin_amdgcn_readlane(my_pos, at);
+          rows[j].load(dy + p * a.ldy, slab, lane, a.h);
         }
+      };
+      auto add = [&](const Row<G, kVec, true>* rows, int j0) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
           if (j0 + j >= count || others) continue;
@@ -305,12 +502,22 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const G* __restrict__
               continue;
             }
           }
+          float f[kPerLane];
+          rows[j].get(f);
 #pragma unroll
-          for (int e = 0; e < kPerLane; ++e) sum[e] += row[j][e];
+          for (int e = 0; e < kPerLane; ++e) sum[e] += f[e];
         }
+      };
+      Row<G, kVec, true> r0[kAhead], r1[kAhead];
+      load(r0, 0);
+      for (int j0 = 0; j0 < count && !others; j0 += 2 * kAhead) {
+        if (j0 + kAhead < count) load(r1, j0 + kAhead);
+        add(r0, j0);
+        if (j0 + 2 * kAhead < count) load(r0, j0 + 2 * kAhead);
+        add(r1, j0 + kAhead);
       }
     }
-    if (!others) finish(end < a.n && a.keys[end] == cur);
+    if (!others) finish(end < a.n && next_key == cur);
   }
 }
 
@@ -328,26 +535,40 @@ __global__ __launch_bounds__(kBlock) void embed_join_kernel(W* __restrict__ dw, 
     const int64_t c = id / a.slabs, slab = id - c * a.slabs;
     const int64_t first = c * a.chunk, next = first + a.chunk;
     if (next >= a.n) continue;
-    const uint32_t key = a.keys[next];
-    if (key >= a.vocab || a.keys[next - 1] != key) continue;   // nothing goes on
-    if (a.keys[first] == key && c > 0 && a.keys[first - 1] == key) continue;  // began earlier
-    int64_t lo = next, hi = a.n;  // the first position past the id's
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (a.keys[mid] > key) hi = mid;
-      else lo = mid + 1;
+    const uint32_t key = a.keys[next], in_last = a.keys[next - 1], in_first = a.keys[first];
+    const uint32_t before = c > 0 ? a.keys[first - 1] : key;
+    if (key >= a.vocab || in_last != key) continue;             // nothing goes on
+    if (c > 0 && in_first == key && before == key) continue;    // it began earlier
+    // The last chunk that begins with the id, 64 chunks looked at together.
+    int64_t last = c + 1;
+    for (;; last += 64) {
+      const int64_t at = (last + lane) * a.chunk;
+      const uint64_t same = __ballot(at < a.n && a.keys[at < a.n ? at : next] == key);
+      if (~same) {
+        last += __builtin_ctzll(~same) - 1;
+        break;
+      }
     }
-    const int64_t last = (lo - 1) / a.chunk;  // the chunk in which it ends
     const int64_t parts = last - c + 1, share = (parts + kWaves - 1) / kWaves;
     const int64_t from = wave * share;
     const int64_t to = from + share < parts ? from + share : parts;
     float sum[kPerLane] = {};
-    for (int64_t p = from; p < to; ++p) {
-      float f[kPerLane];
-      load_row<float, kVec>(a.part + (p == 0 ? 2 * c + 1 : 2 * (c + p)) * a.h, slab, lane, a.h,
-                            f);
+    constexpr int kAhead = 8;  // partials whose loads are in flight together
+    for (int64_t p0 = from; p0 < to; p0 += kAhead) {
+      Row<float, kVec> row[kAhead];
 #pragma unroll
-      for (int e = 0; e < kPerLane; ++e) sum[e] += f[e];
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t p = p0 + j < to ? p0 + j : to - 1;
+        row[j].load(a.part + (p == 0 ? 2 * c + 1 : 2 * (c + p)) * a.h, slab, lane, a.h);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (p0 + j >= to) continue;
+        float f[kPerLane];
+        row[j].get(f);
+#pragma unroll
+        for (int e = 0; e < kPerLane; ++e) sum[e] += f[e];
+      }
     }
 #pragma unroll
     for (int e = 0; e < kPerLane; ++e) part[wave][e][lane] = sum[e];
@@ -372,6 +593,12 @@ inline unsigned blocks_for(int64_t blocks) {
   return static_cast<unsigned>(blocks < kMaxBlocks ? blocks : kMaxBlocks);
 }
 
+// Workgroups that fill `bytes`.
+inline int64_t fill_blocks(int64_t bytes, int threads) {
+  const int64_t most = kMaxFillThreads / threads, want = bytes / 16 / threads + 1;
+  return want < most ? want : most;
+}
+
 // Sorted positions per chunk: a power of two that leaves about 4096 waves (16
 // for each compute unit's four SIMDs to switch between), at least 8, so that a
 // wave has rows to keep in flight, and at most 256.
@@ -383,13 +610,14 @@ inline int chunk_of(int64_t n, int64_t h) {
 
 struct BwdLayout {
   int64_t tile, hist, keys[2], pos[2], part, total;
-  int tiles, passes, bits, chunk;
+  int tiles, passes, bits, chunk, key_bits;
 };
 
 BwdLayout embed_layout(int64_t n, int64_t vocab, int64_t h) {
   BwdLayout L{};
   int key_bits = 1;  // rows 0 .. vocab
   while ((vocab >> key_bits) != 0) ++key_bits;
+  L.key_bits = key_bits;
   L.passes = (key_bits + kMaxDigit - 1) / kMaxDigit;
   L.bits = (key_bits + L.passes - 1) / L.passes;
   L.tile = round_up(n > kMaxTiles ? (n + kMaxTiles - 1) / kMaxTiles : 1, kMinTile);
@@ -422,25 +650,91 @@ inline bool rows_aligned(const void* p, int dtype, int64_t ld) {
 int check_sizes(int64_t n, int64_t vocab, int64_t h) {
   // Rows and positions are held in 32 bits.
   const int64_t most = (int64_t{1} << 31) - 1;
-  if (n < 0 || n > most || vocab < 1 || vocab > most || h < 1 || h > most)
+  if (n < 0 || n > most || vocab < 1 || vocab > most || h < 1 || h > kMaxHidden)
     return NMCE_EINVAL_SHAPE;
   return NMCE_OK;
+}
+
+template <typename W, typename O, bool kVec, int kRows>
+int launch_fwd_rows(const int64_t* tokens, int64_t n, const void* weight, int64_t vocab, int64_t h,
+                    int64_t ldw, int64_t start, float scale, void* out, int64_t ldo,
+                    hipStream_t s) {
+  const int64_t slabs = slabs_of(h), per = (kBlock / 64) * kRows;
+  const int64_t want = (n + per - 1) / per, most = (int64_t{1} << 22) / slabs + 1;
+  const dim3 grid(static_cast<unsigned>(want < most ? want : most), static_cast<unsigned>(slabs));
+  hipLaunchKernelGGL((embed_fwd_kernel<W, O, kVec, kRows>), grid, dim3(kBlock), 0, s, tokens, n,
+                     static_cast<const W*>(weight), vocab, h, ldw, start, scale,
+                     static_cast<O*>(out), ldo);
+  return launch_status();
 }
 
 template <typename W, typename O>
 int launch_fwd(const int64_t* tokens, int64_t n, const void* weight, int64_t vocab, int64_t h,
                int64_t ldw, int64_t start, float scale, void* out, int64_t ldo, bool vec,
                hipStream_t s) {
-  const int64_t slabs = slabs_of(h);
-  const dim3 grid(blocks_for((n * slabs + 3) / 4)), block(kBlock);
-  const W* w = static_cast<const W*>(weight);
-  O* o = static_cast<O*>(out);
-  if (vec)
-    hipLaunchKernelGGL((embed_fwd_kernel<W, O, true>), grid, block, 0, s, tokens, n, w, vocab, h,
-                       ldw, start, scale, o, ldo, slabs);
-  else
-    hipLaunchKernelGGL((embed_fwd_kernel<W, O, false>), grid, block, 0, s, tokens, n, w, vocab, h,
-                       ldw, start, scale, o, ldo, slabs);
+  // Eight rows a wave where they still make eight waves for every SIMD.
+  const bool many = n * slabs_of(h) >= 8 * 4 * 8 * 256;
+#define NMCE_FWD(VEC, ROWS)                                                                      \
+  launch_fwd_rows<W, O, VEC, ROWS>(tokens, n, weight, vocab, h, ldw, start, scale, out, ldo, s)
+  if (vec) return many ? NMCE_FWD(true, 8) : NMCE_FWD(true, 1);
+  return many ? NMCE_FWD(false, 8) : NMCE_FWD(false, 1);
+#undef NMCE_FWD
+}
+
+// The sort in passes over tiles, with the fill spread over its launches; the
+// last pass writes list (passes - 1) & 1.
+int launch_sort(const int64_t* tokens, int64_t n, int64_t vocab, int64_t start, const BwdLayout& L,
+                char* ws, const Fill& fill, hipStream_t s) {
+  SortArgs a{};
+  a.tokens = tokens;
+  a.hist = reinterpret_cast<uint32_t*>(ws + L.hist);
+  a.n = n;
+  a.start = start;
+  a.vocab = vocab;
+  a.tile = L.tile;
+  a.tiles = L.tiles;
+  a.bits = L.bits;
+  // Each of the sort's launches takes an equal share of the fill.
+  const int64_t share = round_up((fill.bytes + 2 * L.passes - 1) / (2 * L.passes), 16);
+  int64_t done = 0;
+  auto next_fill = [&] {
+    a.fill = Fill{fill.to + done, fill.bytes - done < share ? fill.bytes - done : share};
+    done += a.fill.bytes;
+    return dim3(static_cast<unsigned>(L.tiles + fill_blocks(a.fill.bytes, kSortBlock)));
+  };
+  for (int p = 0; p < L.passes; ++p) {
+    a.shift = p * L.bits;
+    a.keys = reinterpret_cast<const uint32_t*>(ws + L.keys[(p + 1) & 1]);
+    a.pos = reinterpret_cast<const uint32_t*>(ws + L.pos[(p + 1) & 1]);
+    a.keys_out = reinterpret_cast<uint32_t*>(ws + L.keys[p & 1]);
+    a.pos_out = reinterpret_cast<uint32_t*>(ws + L.pos[p & 1]);
+    const dim3 block(kSortBlock);
+    dim3 grid = next_fill();
+    if (p == 0) {
+      hipLaunchKernelGGL(sort_count_kernel<true>, grid, block, 0, s, a);
+      if (const int st = launch_status()) return st;
+      grid = next_fill();
+      hipLaunchKernelGGL(sort_move_kernel<true>, grid, block, 0, s, a);
+    } else {
+      hipLaunchKernelGGL(sort_count_kernel<false>, grid, block, 0, s, a);
+      if (const int st = launch_status()) return st;
+      grid = next_fill();
+      hipLaunchKernelGGL(sort_move_kernel<false>, grid, block, 0, s, a);
+    }
+    if (const int st = launch_status()) return st;
+  }
+  return NMCE_OK;
+}
+
+// sort_small_kernel's list and the fill of the whole of dW.
+int launch_small_sort(SmallSortArgs a, hipStream_t s) {
+  static std::atomic<bool> lds_set{false};
+  if (const int rc = allow_lds(reinterpret_cast<const void*>(&sort_small_kernel),
+                               kSmallSort * 4, lds_set))
+    return rc;
+  const int list = a.n * 4, lds = list > kSmallCounts ? list : kSmallCounts;
+  const dim3 grid(static_cast<unsigned>(1 + fill_blocks(a.fill.bytes, kSmallBlock)));
+  hipLaunchKernelGGL(sort_small_kernel, grid, dim3(kSmallBlock), lds, s, a);
   return launch_status();
 }
 
@@ -513,42 +807,40 @@ int nmce_embedding_bwd(const int64_t* tokens, int64_t n_tokens, const void* grad
     return NMCE_EINVAL_WORKSPACE;
 
   const int64_t bytes = vocab_local * hidden * size_of(weight_dtype);
-  hipLaunchKernelGGL(zero_kernel, dim3(blocks_for(bytes / (16 * kBlock) + 1)), dim3(kBlock), 0, s,
-                     static_cast<char*>(grad_weight), bytes);
-  if (const int st = launch_status()) return st;
-  if (n_tokens == 0) return NMCE_OK;
+  char* dw = static_cast<char*>(grad_weight);
+  if (n_tokens == 0) {
+    const dim3 grid(static_cast<unsigned>(fill_blocks(bytes, kBlock)));
+    hipLaunchKernelGGL(zero_kernel, grid, dim3(kBlock), 0, s,
+                       Fill{dw, bytes});
+    return launch_status();
+  }
 
-  SortArgs a{};
-  a.tokens = tokens;
-  a.hist = reinterpret_cast<uint32_t*>(ws + L.hist);
-  a.n = n_tokens;
-  a.start = vocab_start;
-  a.vocab = vocab_local;
-  a.tile = L.tile;
-  a.tiles = L.tiles;
-  a.bits = L.bits;
-  for (int p = 0; p < L.passes; ++p) {
-    a.shift = p * L.bits;
-    a.keys = reinterpret_cast<const uint32_t*>(ws + L.keys[(p + 1) & 1]);
-    a.pos = reinterpret_cast<const uint32_t*>(ws + L.pos[(p + 1) & 1]);
-    a.keys_out = reinterpret_cast<uint32_t*>(ws + L.keys[p & 1]);
-    a.pos_out = reinterpret_cast<uint32_t*>(ws + L.pos[p & 1]);
-    const dim3 grid(static_cast<unsigned>(L.tiles)), block(kSortBlock);
-    if (p == 0) {
-      hipLaunchKernelGGL(sort_count_kernel<true>, grid, block, 0, s, a);
-      if (const int st = launch_status()) return st;
-      hipLaunchKernelGGL(sort_move_kernel<true>, grid, block, 0, s, a);
-    } else {
-      hipLaunchKernelGGL(sort_count_kernel<false>, grid, block, 0, s, a);
-      if (const int st = launch_status()) return st;
-      hipLaunchKernelGGL(sort_move_kernel<false>, grid, block, 0, s, a);
-    }
-    if (const int st = launch_status()) return st;
+  int pos_bits = 0;
+  while (((n_tokens - 1) >> pos_bits) != 0) ++pos_bits;
+  int sorted = 0;  // which of the two lists holds the result
+  if (n_tokens <= kSmallSort && L.key_bits + pos_bits <= 32) {
+    SmallSortArgs a{};
+    a.tokens = tokens;
+    a.keys_out = reinterpret_cast<uint32_t*>(ws + L.keys[0]);
+    a.pos_out = reinterpret_cast<uint32_t*>(ws + L.pos[0]);
+    a.fill = Fill{dw, bytes};
+    a.start = vocab_start;
+    a.vocab = vocab_local;
+    a.n = static_cast<int>(n_tokens);
+    a.pos_bits = pos_bits;
+    a.passes = L.passes;
+    a.bits = L.bits;
+    if (const int st = launch_small_sort(a, s)) return st;
+  } else {
+    if (const int st = launch_sort(tokens, n_tokens, vocab_local, vocab_start, L, ws,
+                                   Fill{dw, bytes}, s))
+      return st;
+    sorted = (L.passes - 1) & 1;
   }
 
   SumArgs m{};
-  m.keys = a.keys_out;
-  m.pos = a.pos_out;
+  m.keys = reinterpret_cast<const uint32_t*>(ws + L.keys[sorted]);
+  m.pos = reinterpret_cast<const uint32_t*>(ws + L.pos[sorted]);
   m.part = reinterpret_cast<float*>(ws + L.part);
   m.n = n_tokens;
   m.vocab = vocab_local;
