@@ -14,6 +14,7 @@
 // are 16 bytes a lane whatever they hold, at twice the rate.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <string.h>
 
 #include <type_traits>
 
@@ -25,55 +26,159 @@ namespace nmce {
 namespace {
 
 constexpr int64_t kMaxK = 131072;
-constexpr int kQuantBlock = 256;
-constexpr int kPadK = 128;  // bytes of a stage: tokens' rows are padded to it with zeros
+constexpr int kFewTokens = 128;  // up to here the weight streams through registers
+constexpr int kPadK = 256;  // the tokens' rows are padded to it with zeros: whole steps of K
 
-// x * (127 / top) to the nearest integer, halves to even, as the exact quotient
-// 127 x / top rounds. The fp32 product is off by less than 2e-5 (three roundings of
-// at most 127): only where it lies that near to a half (or 127 / top is not
-// finite) the quotient is formed, in fp64, where 127 x is exact and the quotient
-// of a 31-bit and a 24-bit number is a half only if it is one exactly.
-__device__ __forceinline__ int quantised(float x, float top, float inv) {
-  const float t = x * inv;
-  const float r = rintf(t);
-  if (fabsf(fabsf(t - r) - 0.5f) >= 1e-4f) return static_cast<int>(r);
-  return static_cast<int>(rint(127.0 * static_cast<double>(x) / static_cast<double>(top)));
+// kVec elements as x * 127 / top to the nearest integer, halves to even, as the
+// exact quotient rounds. The fp32 product with inv = 127 / top is off by at most
+// 127 * 2^-23 = 1.6e-5; only where one of the elements lies that near to a half its
+// side of it is settled: 127 |x| against h top for the half h, as the fp32 sum of
+// 127 |x| - hi (hi its rounding) and hi - h top, both exact (the second cancels at
+// least 16 bits of a 32-bit product), whose sign is therefore exact. `slow` rows,
+// where those would leave fp32's range, take the quotient in fp64: 127 x is exact
+// there, and a 31-bit over a 24-bit number is a half only if it is one exactly.
+template <int kVec>
+__device__ __forceinline__ void quantise(const float* x, float top, float inv, bool slow, int* q) {
+  constexpr float kNear = 2e-5f;
+  float near = 1.0f;
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    const float t = x[e] * inv, r = rintf(t);
+    near = fminf(near, fabsf(fabsf(t - r) - 0.5f));
+    q[e] = static_cast<int>(r);
+  }
+  if (slow) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e)
+      q[e] = static_cast<int>(rint(127.0 * static_cast<double>(x[e]) / static_cast<double>(top)));
+  } else if (near < kNear) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const float a = fabsf(x[e]), t = a * inv, k = floorf(t), h = k + 0.5f;
+      if (fabsf(t - h) < kNear) {
+        const float hi = 127.0f * a, lo = fmaf(127.0f, a, -hi);
+        const float s = fmaf(-h, top, hi) + lo;
+        const int below = static_cast<int>(k);
+        const int mag = below + (s > 0.0f || (s == 0.0f && (below & 1)) ? 1 : 0);
+        q[e] = x[e] < 0.0f ? -mag : mag;
+      }
+    }
+  }
 }
 
-// A workgroup quantises one row: its largest magnitude, then the elements, read
-// again. Magnitudes are compared as the integers of their bits, which put
-// infinities and NaNs above every number: such a row gets the scale NaN and
-// zeros, so its products are NaN. A row of zeros gets the scale 0.
-template <typename T, bool kVec>
-__global__ __launch_bounds__(kQuantBlock) void quantize_rows_kernel(
+// 16 bytes of elements at any element's alignment, not kept in the caches
+// (kStream: rows that are read once).
+template <bool kStream, typename T>
+__device__ __forceinline__ void load_vec(const T* p, float* f) {
+  typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+  const u32x4_any* q = reinterpret_cast<const u32x4_any*>(p);
+  const u32x4_any v = kStream ? __builtin_nontemporal_load(q) : *q;
+  Elem<T>::unpack(u32x4{v.x, v.y, v.z, v.w}, f);
+}
+
+// kWaves waves quantise a row: its largest magnitude, then the elements, which a
+// thread holds in registers (32 of them; kHeld = false: longer rows, read twice).
+// Magnitudes are compared as the integers of their bits, which put infinities and
+// NaNs above every number: such a row gets the scale NaN and zeros, so its
+// products are NaN. A row of zeros gets the scale 0. One wave a row needs no
+// barrier: 50257 rows of 1600 take 46 us (5.3 TB/s) where a workgroup a row, an
+// element at a time and twice, took 136; a few rows go faster with four.
+constexpr int kQuantEach = 32;
+
+template <typename T, int kWaves, bool kHeld>
+__global__ __launch_bounds__(64 * (kWaves < 4 ? 4 : kWaves)) void quantize_rows_kernel(
     const T* __restrict__ x, int64_t n, int64_t k, int64_t ldx, int8_t* __restrict__ q,
-    int64_t ldq, float* __restrict__ scale) {
-  __shared__ uint32_t wave_top[kQuantBlock / 64];
-  for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+    int64_t ldq, float* __restrict__ scale, bool whole_stores) {
+  constexpr int kVec = Elem<T>::kPerVec;
+  constexpr int kBlock = 64 * (kWaves < 4 ? 4 : kWaves);
+  constexpr int kRow = 64 * kWaves;            // threads of a row
+  constexpr int kRowsAtOnce = kBlock / kRow;
+  constexpr int kSpan = kRow * kVec;           // columns a round of vectors covers
+  __shared__ uint32_t wave_top[kWaves];
+  const int t = threadIdx.x % kRow;
+  auto get = [&](const T* row, int64_t c, float* f) {
+    if (c + kVec <= k) {
+      load_vec<(kWaves == 1)>(row + c, f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) f[e] = c + e < k ? Elem<T>::load1(row + c + e) : 0.0f;
+    }
+  };
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRowsAtOnce + threadIdx.x / kRow; r < n;
+       r += static_cast<int64_t>(gridDim.x) * kRowsAtOnce) {
     const T* row = x + r * ldx;
+    float f[kQuantEach];
     uint32_t top = 0;
-    for (int64_t c = threadIdx.x; c < k; c += kQuantBlock) {
-      const uint32_t b = __float_as_uint(Elem<T>::load1(row + c)) & 0x7fffffffu;
-      top = b > top ? b : top;
+    auto look = [&](const float* v, int count) {
+#pragma unroll
+      for (int e = 0; e < count; ++e) {
+        const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
+        top = b > top ? b : top;
+      }
+    };
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int i = 0; i < kQuantEach / kVec; ++i) get(row, i * kSpan + t * kVec, f + i * kVec);
+      look(f, kQuantEach);
+    } else {
+      for (int64_t c = t * kVec; c < k; c += kSpan) {
+        get(row, c, f);
+        look(f, kVec);
+      }
     }
     for (int s = 32; s > 0; s >>= 1) {
       const uint32_t o = __shfl_xor(top, s);
       top = o > top ? o : top;
     }
-    if ((threadIdx.x & 63) == 0) wave_top[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (int w = 0; w < kQuantBlock / 64; ++w) top = wave_top[w] > top ? wave_top[w] : top;
-    __syncthreads();
+    if constexpr (kWaves > 1) {
+      if ((t & 63) == 0) wave_top[t >> 6] = top;
+      __syncthreads();
+      for (int w = 0; w < kWaves; ++w) top = wave_top[w] > top ? wave_top[w] : top;
+      __syncthreads();
+    }
     const bool finite = top < 0x7f800000u;
     const float most = __uint_as_float(top);
-    if (threadIdx.x == 0)
+    if (t == 0)
       scale[r] = finite ? static_cast<float>(static_cast<double>(most) / 127.0)
                         : __uint_as_float(0x7fc00000u);
     const bool any = finite && top != 0;
     const float inv = 127.0f / most;
-    for (int64_t c = threadIdx.x; c < ldq; c += kQuantBlock)
-      q[r * ldq + c] = static_cast<int8_t>(
-          any && c < k ? quantised(Elem<T>::load1(row + c), most, inv) : 0);
+    const bool slow = !(most > 1e-30f && most < 1e36f);
+    int8_t* out = q + r * ldq;
+    // kVec columns from c on, zeros past the row's.
+    auto put = [&](int64_t c, const float* v) {
+      uint32_t word[kVec / 4] = {};
+      if (any) {
+        int i8[kVec];
+        quantise<kVec>(v, most, inv, slow, i8);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          word[e / 4] |= static_cast<uint32_t>(i8[e] & 0xff) << (8 * (e % 4));
+      }
+      if (whole_stores && c + kVec <= ldq) {
+        typedef uint32_t word_t __attribute__((ext_vector_type(kVec / 4)));
+        word_t w;
+        memcpy(&w, word, kVec);
+        if (kWaves == 1)
+          __builtin_nontemporal_store(w, reinterpret_cast<word_t*>(out + c));
+        else
+          *reinterpret_cast<word_t*>(out + c) = w;
+      } else {
+        for (int e = 0; e < kVec && c + e < ldq; ++e)
+          out[c + e] = static_cast<int8_t>(word[e / 4] >> (8 * (e % 4)));
+      }
+    };
+    if constexpr (kHeld) {
+#pragma unroll
+      for (int i = 0; i < kQuantEach / kVec; ++i) {
+        const int64_t c = i * kSpan + t * kVec;
+        if (c < ldq) put(c, f + i * kVec);
+      }
+    }
+    for (int64_t c = (kHeld ? int64_t{kQuantEach} * kRow : 0) + t * kVec; c < ldq; c += kSpan) {
+      get(row, c, f);
+      put(c, f);
+    }
   }
 }
 
@@ -131,20 +236,196 @@ __global__ __launch_bounds__(kThreads, 1) void int8_linear_kernel(LinearArgs a) 
     store_bf16_tile(acc, lds, static_cast<uint16_t*>(a.out), a.ldo, a.n, a.v, m0, n0);
 }
 
+// ---- few tokens -------------------------------------------------------------
+// Up to kFewTokens tokens the weight's read is the time: every wave takes 16
+// vocabulary rows of it straight into registers, 256-byte steps of K ahead, and
+// all eight share the tokens' steps in LDS, loaded there directly, kDepth of them.
+// A compute unit so has 64 to 128 KiB of the weight in flight. [128256, 4096], one
+// token 98 us (5.4 TB/s; 104 with the quantisation), 16 108, 64 124. The waves
+// splitting K instead, each with its tokens from L2, took 102, 124 and 212 in all,
+// the 256 x 256 tiles of the core 136 for any; 32 rows a wave 116, 118, 183.
+//
+// Fragments as in the core: A is 16 vocabulary rows, B 16 tokens, lane l holds row
+// (token) l % 16, bytes 16 (l / 16) .. of each 64; the result's lane l has token
+// l % 16, rows 4 (l / 16) + e. A token's step is 16 chunks of 16 bytes, chunk c of
+// token t at c ^ (t % 16): the 16 tokens that 16 lanes read are on distinct bank
+// groups.
+constexpr int kStepK = 256;
+constexpr int kFewWavesWg = 8;
+typedef int i32x4v __attribute__((ext_vector_type(4)));
+
+template <typename O, int kTokFrags, int kDepth>
+__global__ __launch_bounds__(64 * kFewWavesWg, 4) void int8_few_kernel(LinearArgs a) {
+  constexpr int kStage = 16 * kTokFrags * kStepK;
+  constexpr int kBlocks = kStage / 1024;       // 1 KiB: four tokens' steps
+  constexpr int kSlices = kStepK / 64;
+  // A resource's size, past every offset here; a step past the last reads at it,
+  // which is out of range: no memory access, and the loads in flight stay counted.
+  constexpr uint32_t kPast = 1u << 31;
+  __shared__ __align__(16) char lds[kDepth][kStage];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  const int64_t v0 = (static_cast<int64_t>(blockIdx.x) * kFewWavesWg + wave) * 16;
+  const int64_t base = v0 < a.v ? v0 : a.v - 1;  // waves past the last row repeat it
+  const int64_t more = a.v - 1 - base;           // and so do rows
+  const uint32_t w_off = static_cast<uint32_t>((c < more ? c : more) * a.ldw);
+  const auto w_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<int8_t*>(a.w) + base * a.ldw, 0, static_cast<int>(kPast), 0x00020000);
+  i32x4_t q_rsrc;
+  {
+    const uint64_t p = reinterpret_cast<uint64_t>(a.q);
+    q_rsrc = i32x4_t{static_cast<int>(p & 0xffffffffu), static_cast<int>(p >> 32),
+                     static_cast<int>(kPast), 0x00020000};
+  }
+  // Blocks `wave`, + 8, ... of the tokens' step (where there are four, two waves
+  // load each: no branch, and every wave has the same loads in flight): lane p fills
+  // token 4 b + p / 16, physical chunk p % 16.
+  constexpr int kMine = (kBlocks + kFewWavesWg - 1) / kFewWavesWg;
+  static_assert(kBlocks == kMine * kFewWavesWg || kBlocks == kFewWavesWg / 2, "whole rounds");
+  const int block0 = wave % (kBlocks < kFewWavesWg ? kBlocks : kFewWavesWg);
+  uint32_t q_off[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int64_t t = 4 * (block0 + kFewWavesWg * j) + (lane >> 4);
+    const int chunk = (lane & 15) ^ static_cast<int>(t & 15);
+    q_off[j] = static_cast<uint32_t>((t < a.n ? t : a.n - 1) * a.kp) + 16 * chunk;
+  }
+  const int steps = static_cast<int>(a.kp / kStepK);
+  const int last_chunk = static_cast<int>(a.w_chunks) - 1;
+
+  struct Weights {
+    i32x4v w[kSlices];
+  };
+  // Workgroups begin at different steps: rows 4096 bytes apart, all read at the same
+  // columns, would keep to a few of the memory's channels.
+  const int first = static_cast<int>(blockIdx.x % static_cast<unsigned>(steps));
+  auto load = [&](Weights& s, int buf, int i) {
+    int k = first + i;
+    if (k >= steps) k -= steps;
+    const uint32_t past = i < steps ? 0u : kPast;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j)
+      raw_buffer_load_lds(q_rsrc,
+                          (lds_void_t*)(lds[buf] + (block0 + kFewWavesWg * j) * 1024), 16,
+                          static_cast<int>(q_off[j] + k * kStepK + past), 0, 0, 0);
+#pragma unroll
+    for (int h = 0; h < kSlices; ++h) {
+      // Chunks past a row's last read that one: the tokens hold zeros there.
+      int chunk = 16 * k + 4 * h + g;
+      chunk = chunk < last_chunk ? chunk : last_chunk;
+      s.w[h] = __builtin_bit_cast(
+          i32x4v, __builtin_amdgcn_raw_buffer_load_b128(w_rsrc, w_off + 16 * chunk + past, 0, 0));
+    }
+  };
+  i32x4v acc[kTokFrags];
+#pragma unroll
+  for (int t = 0; t < kTokFrags; ++t) acc[t] = i32x4v{0, 0, 0, 0};
+  auto mul = [&](const Weights& s, int buf) {
+    const char* st = lds[buf] + c * kStepK;
+#pragma unroll
+    for (int h = 0; h < kSlices; ++h)
+#pragma unroll
+      for (int t = 0; t < kTokFrags; ++t) {
+        const i32x4v q = *reinterpret_cast<const i32x4v*>(st + t * 16 * kStepK +
+                                                          (((4 * h + g) ^ c) << 4));
+        acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.w[h], q, acc[t], 0, 0, 0);
+      }
+  };
+  // Step k: its loads have landed (all but the newer steps' are waited for), in
+  // every wave, and every wave is done with the step whose buffer step k +
+  // kDepth - 1 takes.
+  constexpr int kNewer = (kDepth - 2) * (kSlices + kMine);
+  auto arrive = [&] {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kNewer) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  Weights s[kDepth];
+#pragma unroll
+  for (int d = 0; d + 1 < kDepth; ++d) load(s[d], d, d);
+  int k = 0;
+  for (; k + kDepth <= steps; k += kDepth) {  // no branch inside: the loads stay counted
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      arrive();
+      constexpr int kLast = kDepth - 1;
+      load(s[(d + kLast) % kDepth], (d + kLast) % kDepth, k + d + kLast);
+      __builtin_amdgcn_sched_barrier(0);
+      mul(s[d], d);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int d = 0; d + 1 < kDepth; ++d)
+    if (k + d < steps) mul(s[d], d);
+  // Four consecutive logits a lane.
+  O* out = static_cast<O*>(a.out);
+  const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(O) - 1)) == 0;
+  const int64_t v = v0 + 4 * g;
+  if (v >= a.v) return;
+  float sw[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sw[e] = a.sw[v + e < a.v ? v + e : v];
+#pragma unroll
+  for (int t = 0; t < kTokFrags; ++t) {
+    const int64_t tok = 16 * t + c;
+    if (tok >= a.n) continue;
+    const float sx = a.sx[tok];
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = static_cast<float>(acc[t][e]) * sx * sw[e];
+    O* dst = out + tok * a.ldo + v;
+    if (vec && v + 4 <= a.v) {
+      if constexpr (std::is_same<O, float>::value) {
+        *reinterpret_cast<u32x4*>(dst) = Elem<float>::pack(y);
+      } else {
+        typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+        *reinterpret_cast<u32x2v*>(dst) = u32x2v{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+      }
+    } else {
+      for (int e = 0; e < 4 && v + e < a.v; ++e) Elem<O>::store1(dst + e, y[e]);
+    }
+  }
+}
+
 inline bool dtype_ok(int d) { return d == NMCE_F32 || d == NMCE_BF16; }
 inline int64_t size_of(int d) { return d == NMCE_F32 ? 4 : 2; }
 
+template <typename T, int kWaves, bool kHeld>
+int launch_quantize_as(const void* x, int64_t n, int64_t k, int64_t ldx, int8_t* q, int64_t ldq,
+                       float* scale, hipStream_t s) {
+  constexpr int kBlock = 64 * (kWaves < 4 ? 4 : kWaves), kRows = kBlock / (64 * kWaves);
+  const int64_t most = 1 << 21, want = (n + kRows - 1) / kRows;
+  // A vector's bytes leave in one store where every row starts on such a boundary.
+  constexpr int kVec = Elem<T>::kPerVec;
+  const bool whole = reinterpret_cast<uintptr_t>(q) % kVec == 0 && ldq % kVec == 0;
+  hipLaunchKernelGGL((quantize_rows_kernel<T, kWaves, kHeld>),
+                     dim3(static_cast<unsigned>(want < most ? want : most)), dim3(kBlock), 0, s,
+                     static_cast<const T*>(x), n, k, ldx, q, ldq, scale, whole);
+  return launch_status();
+}
+
+template <typename T>
+int launch_quantize_of(const void* x, int64_t n, int64_t k, int64_t ldx, int8_t* q, int64_t ldq,
+                       float* scale, hipStream_t s) {
+  // A wave a row where its registers hold the row and there are rows for two
+  // waves on every SIMD; else four, sixteen, or sixteen that read twice.
+  if (k <= 64 * kQuantEach && n >= 2048)
+    return launch_quantize_as<T, 1, true>(x, n, k, ldx, q, ldq, scale, s);
+  if (k <= 256 * kQuantEach)
+    return launch_quantize_as<T, 4, true>(x, n, k, ldx, q, ldq, scale, s);
+  if (k <= 1024 * kQuantEach)
+    return launch_quantize_as<T, 16, true>(x, n, k, ldx, q, ldq, scale, s);
+  return launch_quantize_as<T, 16, false>(x, n, k, ldx, q, ldq, scale, s);
+}
+
 int launch_quantize(const void* x, int dtype, int64_t n, int64_t k, int64_t ldx, int8_t* q,
                     int64_t ldq, float* scale, hipStream_t s) {
-  const int64_t most = 1 << 20;
-  const dim3 grid(static_cast<unsigned>(n < most ? n : most)), block(kQuantBlock);
-  if (dtype == NMCE_F32)
-    hipLaunchKernelGGL((quantize_rows_kernel<float, false>), grid, block, 0, s,
-                       static_cast<const float*>(x), n, k, ldx, q, ldq, scale);
-  else
-    hipLaunchKernelGGL((quantize_rows_kernel<uint16_t, false>), grid, block, 0, s,
-                       static_cast<const uint16_t*>(x), n, k, ldx, q, ldq, scale);
-  return launch_status();
+  return dtype == NMCE_F32 ? launch_quantize_of<float>(x, n, k, ldx, q, ldq, scale, s)
+                           : launch_quantize_of<uint16_t>(x, n, k, ldx, q, ldq, scale, s);
 }
 
 template <typename O, bool kVec>
@@ -168,6 +449,31 @@ int launch_tiles(const LinearArgs& a, hipStream_t s) {
     if (const int st = launch_status()) return st;
   }
   return NMCE_OK;
+}
+
+// Three steps of up to 32 tokens at a time; of more, whose steps take more LDS, two
+// (three leave fewer workgroups a compute unit: 64 tokens the same, 128 6% slower).
+template <typename O, int kTokFrags>
+int launch_few(const LinearArgs& a, hipStream_t s) {
+  constexpr int kDepth = kTokFrags <= 2 ? 3 : 2;
+  constexpr int kRows = 16 * kFewWavesWg;
+  const dim3 grid(static_cast<unsigned>((a.v + kRows - 1) / kRows));
+  hipLaunchKernelGGL((int8_few_kernel<O, kTokFrags, kDepth>), grid, dim3(64 * kFewWavesWg), 0, s,
+                     a);
+  return launch_status();
+}
+
+template <typename O>
+int launch_linear(const LinearArgs& a, bool vec, hipStream_t s) {
+  if (a.n <= kFewTokens) {
+    if (a.n <= 16) return launch_few<O, 1>(a, s);
+    if (a.n <= 32) return launch_few<O, 2>(a, s);
+    if (a.n <= 64) return launch_few<O, 4>(a, s);
+    return launch_few<O, 8>(a, s);
+  }
+  if constexpr (std::is_same<O, float>::value)
+    if (!vec) return launch_tiles<O, false>(a, s);
+  return launch_tiles<O, true>(a, s);
 }
 
 int64_t linear_workspace(int64_t n, int64_t k) {
@@ -235,11 +541,12 @@ int nmce_int8_linear(const void* x, int dtype, int64_t n_rows, int64_t columns, 
   a.ldw = ldw;
   a.ldo = ldo;
   a.w_chunks = (columns + 15) / 16;
-  if (out_dtype == NMCE_BF16) return launch_tiles<uint16_t, true>(a, s);
-  // store_f32_tile's conditions for 16-byte stores.
+  // store_bf16_tile tests its own alignment; store_f32_tile's conditions for
+  // 16-byte stores.
+  if (out_dtype == NMCE_BF16) return launch_linear<uint16_t>(a, true, s);
   const bool vec = vocab_local % 4 == 0 && ldo % 4 == 0 && aligned16(out) &&
                    ldo * 4 * 512 < (int64_t{1} << 32);
-  return vec ? launch_tiles<float, true>(a, s) : launch_tiles<float, false>(a, s);
+  return launch_linear<float>(a, vec, s);
 }
 
 }  // extern "C"
