@@ -29,60 +29,110 @@ constexpr int64_t kMaxK = 131072;
 constexpr int kFewTokens = 128;  // up to here the weight streams through registers
 constexpr int kPadK = 256;  // the tokens' rows are padded to it with zeros: whole steps of K
 
-// kVec elements as x * 127 / top to the nearest integer, halves to even, as the
-// exact quotient rounds. The fp32 product with inv = 127 / top is off by at most
-// 127 * 2^-23 = 1.6e-5; only where one of the elements lies that near to a half its
-// side of it is settled: 127 |x| against h top for the half h, as the fp32 sum of
-// 127 |x| - hi (hi its rounding) and hi - h top, both exact (the second cancels at
-// least 16 bits of a 32-bit product), whose sign is therefore exact. `slow` rows,
-// where those would leave fp32's range, take the quotient in fp64: 127 x is exact
-// there, and a 31-bit over a 24-bit number is a half only if it is one exactly.
-template <int kVec>
-__device__ __forceinline__ void quantise(const float* x, float top, float inv, bool slow, int* q) {
+// A vector's elements as x * 127 / top to the nearest integer, halves to even, as
+// the exact quotient rounds; the result is one byte an element. Adding 1.5 * 2^23
+// rounds to the integers, whose low byte then lies in the sum's own.
+constexpr float kRound = 12582912.0f;
+
+__device__ __forceinline__ uint32_t bytes_of(float a, float b, float c, float d) {
+  // v_perm_b32: bytes 0-3 are the second operand's, 4-7 the first's
+  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x04000c0cu);
+  return lo | hi;
+}
+
+// fp32: the product with inv = 127 / top is off by at most 127 * 2^-23 = 1.6e-5.
+// Only where one of the elements lies that near to a half its side of it is settled:
+// 127 |x| against h top for the half h, as the fp32 sum of 127 |x| - hi (hi its
+// rounding) and hi - h top, both exact (the second cancels at least 16 bits of a
+// 32-bit product), whose sign is therefore exact.
+__device__ __forceinline__ void quantise(const float (&x)[4], float top, uint32_t* q) {
   constexpr float kNear = 2e-5f;
-  float near = 1.0f;
+  const float inv = 127.0f / top;
+  float u[4], off = 0.0f;
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    const float t = x[e] * inv, r = rintf(t);
-    near = fminf(near, fabsf(fabsf(t - r) - 0.5f));
-    q[e] = static_cast<int>(r);
+  for (int e = 0; e < 4; ++e) {
+    const float t = x[e] * inv;
+    u[e] = t + kRound;
+    off = fmaxf(off, fabsf(t - (u[e] - kRound)));
   }
-  if (slow) {
+  if (off > 0.5f - kNear) {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e)
-      q[e] = static_cast<int>(rint(127.0 * static_cast<double>(x[e]) / static_cast<double>(top)));
-  } else if (near < kNear) {
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
+    for (int e = 0; e < 4; ++e) {
       const float a = fabsf(x[e]), t = a * inv, k = floorf(t), h = k + 0.5f;
       if (fabsf(t - h) < kNear) {
         const float hi = 127.0f * a, lo = fmaf(127.0f, a, -hi);
         const float s = fmaf(-h, top, hi) + lo;
-        const int below = static_cast<int>(k);
-        const int mag = below + (s > 0.0f || (s == 0.0f && (below & 1)) ? 1 : 0);
-        q[e] = x[e] < 0.0f ? -mag : mag;
+        const bool up = s > 0.0f || (s == 0.0f && (static_cast<int>(k) & 1));
+        u[e] = (x[e] < 0.0f ? -(up ? k + 1.0f : k) : (up ? k + 1.0f : k)) + kRound;
       }
     }
   }
+  q[0] = bytes_of(u[0], u[1], u[2], u[3]);
 }
 
-// 16 bytes of elements at any element's alignment, not kept in the caches
-// (kStream: rows that are read once).
-template <bool kStream, typename T>
-__device__ __forceinline__ void load_vec(const T* p, float* f) {
-  typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-  const u32x4_any* q = reinterpret_cast<const u32x4_any*>(p);
-  const u32x4_any v = kStream ? __builtin_nontemporal_load(q) : *q;
-  Elem<T>::unpack(u32x4{v.x, v.y, v.z, v.w}, f);
+// bf16: halves are common (every element of half the largest magnitude), and 127 x
+// is exact in fp32. t = 127 x / top is formed by its reciprocal and corrected by its
+// exact remainder, which gives every quotient that fp32 holds, halves among them;
+// others are a 510th part or more away from a half.
+__device__ __forceinline__ void quantise(const float (&x)[8], float top, uint32_t* q) {
+  const float inv = 1.0f / top;
+  float u[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float p = 127.0f * x[e], t = p * inv;
+    u[e] = fmaf(fmaf(-t, top, p), inv, t) + kRound;
+  }
+  q[0] = bytes_of(u[0], u[1], u[2], u[3]);
+  q[1] = bytes_of(u[4], u[5], u[6], u[7]);
+}
+
+// Where those would leave fp32's range: the quotient in fp64, where 127 x is exact
+// and a 31-bit over a 24-bit number is a half only if it is one exactly.
+template <int kVec>
+__device__ __forceinline__ void quantise_wide(const float (&x)[kVec], float top, uint32_t* q) {
+  float u[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e)
+    u[e] = static_cast<float>(
+               rint(127.0 * static_cast<double>(x[e]) / static_cast<double>(top))) + kRound;
+#pragma unroll
+  for (int w = 0; w < kVec / 4; ++w)
+    q[w] = bytes_of(u[4 * w], u[4 * w + 1], u[4 * w + 2], u[4 * w + 3]);
+}
+
+// The largest magnitude as the integer of its bits, which puts infinities and NaNs
+// above every number: running maxima of a vector's elements (bf16: of its even and
+// odd ones), and the fp32 bits of the largest of them.
+__device__ __forceinline__ void raise(uint32_t& top, const u32x4& v, float) {
+  const u32x4 m = v & 0x7fffffffu;
+  const uint32_t a = m.x > m.y ? m.x : m.y, b = m.z > m.w ? m.z : m.w;
+  const uint32_t c = a > b ? a : b;
+  top = c > top ? c : top;
+}
+__device__ __forceinline__ void raise(uint32_t& top, const u32x4& v, uint16_t) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  // (By value: of a vector's element itself the cast takes the first one's bits.)
+  auto pair = [](uint32_t w) { return __builtin_bit_cast(u16x2, w & 0x7fff7fffu); };
+  u16x2 t = __builtin_bit_cast(u16x2, top);
+  t = __builtin_elementwise_max(t, pair(v.x));
+  t = __builtin_elementwise_max(t, pair(v.y));
+  t = __builtin_elementwise_max(t, pair(v.z));
+  t = __builtin_elementwise_max(t, pair(v.w));
+  top = __builtin_bit_cast(uint32_t, t);
+}
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, float) { return top; }
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, uint16_t) {
+  const uint32_t lo = top << 16, hi = top & 0xffff0000u;
+  return lo > hi ? lo : hi;
 }
 
 // kWaves waves quantise a row: its largest magnitude, then the elements, which a
-// thread holds in registers (32 of them; kHeld = false: longer rows, read twice).
-// Magnitudes are compared as the integers of their bits, which put infinities and
-// NaNs above every number: such a row gets the scale NaN and zeros, so its
-// products are NaN. A row of zeros gets the scale 0. One wave a row needs no
-// barrier: 50257 rows of 1600 take 46 us (5.3 TB/s) where a workgroup a row, an
-// element at a time and twice, took 136; a few rows go faster with four.
+// thread holds in registers (32 of them; kHeld = false: longer rows, read twice). A
+// row with an infinity or a NaN gets the scale NaN and zeros, so its products are
+// NaN; a row of zeros gets the scale 0. One wave a row needs no barrier, and four
+// are faster for few rows. 50257 rows of 1600 bf16 take 47 us (5.2 TB/s), of fp32 73
+// (5.5); read twice an element at a time by a workgroup each, 136.
 constexpr int kQuantEach = 32;
 
 template <typename T, int kWaves, bool kHeld>
@@ -94,38 +144,37 @@ __global__ __launch_bounds__(64 * (kWaves < 4 ? 4 : kWaves)) void quantize_rows_
   constexpr int kRow = 64 * kWaves;            // threads of a row
   constexpr int kRowsAtOnce = kBlock / kRow;
   constexpr int kSpan = kRow * kVec;           // columns a round of vectors covers
+  constexpr int kVecs = kQuantEach / kVec;
+  // 16 bytes of elements at any element's alignment.
+  typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+  typedef typename std::conditional<kHeld, int, int64_t>::type col_t;
   __shared__ uint32_t wave_top[kWaves];
   const int t = threadIdx.x % kRow;
-  auto get = [&](const T* row, int64_t c, float* f) {
-    if (c + kVec <= k) {
-      load_vec<(kWaves == 1)>(row + c, f);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) f[e] = c + e < k ? Elem<T>::load1(row + c + e) : 0.0f;
+  const col_t cols = static_cast<col_t>(k);
+  auto get = [&](const T* row, col_t c) {
+    if (c + kVec <= cols) {
+      const u32x4_any v = *reinterpret_cast<const u32x4_any*>(row + c);
+      return u32x4{v.x, v.y, v.z, v.w};
     }
+    float f[kVec];
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) f[e] = c + e < cols ? Elem<T>::load1(row + c + e) : 0.0f;
+    return Elem<T>::pack(f);
   };
   for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRowsAtOnce + threadIdx.x / kRow; r < n;
        r += static_cast<int64_t>(gridDim.x) * kRowsAtOnce) {
     const T* row = x + r * ldx;
-    float f[kQuantEach];
+    u32x4 held[kHeld ? kVecs : 1];
     uint32_t top = 0;
-    auto look = [&](const float* v, int count) {
-#pragma unroll
-      for (int e = 0; e < count; ++e) {
-        const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
-        top = b > top ? b : top;
-      }
-    };
     if constexpr (kHeld) {
 #pragma unroll
-      for (int i = 0; i < kQuantEach / kVec; ++i) get(row, i * kSpan + t * kVec, f + i * kVec);
-      look(f, kQuantEach);
+      for (int i = 0; i < kVecs; ++i) held[i] = get(row, i * kSpan + t * kVec);
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) raise(top, held[i], T());
     } else {
-      for (int64_t c = t * kVec; c < k; c += kSpan) {
-        get(row, c, f);
-        look(f, kVec);
-      }
+      for (int64_t c = t * kVec; c < k; c += kSpan) raise(top, get(row, c), T());
     }
+    top = top_bits(top, T());
     for (int s = 32; s > 0; s >>= 1) {
       const uint32_t o = __shfl_xor(top, s);
       top = o > top ? o : top;
@@ -142,27 +191,24 @@ __global__ __launch_bounds__(64 * (kWaves < 4 ? 4 : kWaves)) void quantize_rows_
       scale[r] = finite ? static_cast<float>(static_cast<double>(most) / 127.0)
                         : __uint_as_float(0x7fc00000u);
     const bool any = finite && top != 0;
-    const float inv = 127.0f / most;
-    const bool slow = !(most > 1e-30f && most < 1e36f);
+    const bool wide = !(most > 1e-25f && most < 1e36f);
     int8_t* out = q + r * ldq;
     // kVec columns from c on, zeros past the row's.
-    auto put = [&](int64_t c, const float* v) {
+    auto put = [&](int64_t c, const u32x4& v) {
       uint32_t word[kVec / 4] = {};
       if (any) {
-        int i8[kVec];
-        quantise<kVec>(v, most, inv, slow, i8);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          word[e / 4] |= static_cast<uint32_t>(i8[e] & 0xff) << (8 * (e % 4));
+        float f[kVec];
+        Elem<T>::unpack(v, f);
+        if (wide)
+          quantise_wide<kVec>(f, most, word);
+        else
+          quantise(f, most, word);
       }
       if (whole_stores && c + kVec <= ldq) {
         typedef uint32_t word_t __attribute__((ext_vector_type(kVec / 4)));
         word_t w;
         memcpy(&w, word, kVec);
-        if (kWaves == 1)
-          __builtin_nontemporal_store(w, reinterpret_cast<word_t*>(out + c));
-        else
-          *reinterpret_cast<word_t*>(out + c) = w;
+        *reinterpret_cast<word_t*>(out + c) = w;
       } else {
         for (int e = 0; e < kVec && c + e < ldq; ++e)
           out[c + e] = static_cast<int8_t>(word[e / 4] >> (8 * (e % 4)));
@@ -170,15 +216,13 @@ __global__ __launch_bounds__(64 * (kWaves < 4 ? 4 : kWaves)) void quantize_rows_
     };
     if constexpr (kHeld) {
 #pragma unroll
-      for (int i = 0; i < kQuantEach / kVec; ++i) {
-        const int64_t c = i * kSpan + t * kVec;
-        if (c < ldq) put(c, f + i * kVec);
+      for (int i = 0; i < kVecs; ++i) {
+        const int c = i * kSpan + t * kVec;
+        if (c < ldq) put(c, held[i]);
       }
     }
-    for (int64_t c = (kHeld ? int64_t{kQuantEach} * kRow : 0) + t * kVec; c < ldq; c += kSpan) {
-      get(row, c, f);
-      put(c, f);
-    }
+    for (int64_t c = (kHeld ? int64_t{kQuantEach} * kRow : 0) + t * kVec; c < ldq; c += kSpan)
+      put(c, kHeld ? u32x4{0, 0, 0, 0} : get(row, static_cast<col_t>(c)));
   }
 }
 
