@@ -14,7 +14,7 @@
 // place where a running sum over the vocabulary passes a level: its neighbours'
 // borders are 1e-5 and less apart, so sums off by 1e-7 would give other ids for
 // the same numbers. The card's fp64 rate is that of its unpacked fp32, and the
-// exponential is about 18 such instructions a logit (exp2_64), so the pass over
+// exponential is about 17 such instructions a logit (exp2_64), so the pass over
 // the logits stays within about twice its memory time.
 //
 // Three launches. The rows are cut into slabs of 8192 logits, a workgroup each,
@@ -35,46 +35,42 @@
 namespace nmce {
 namespace {
 
-constexpr int kBlock = 256;
-constexpr int kWaves = kBlock / 64;
-constexpr int kEach = 32;                 // logits a thread holds
-constexpr int kSlab = kBlock * kEach;     // 8192
+constexpr int kSlab = 8192;               // logits of a workgroup
 constexpr int kStat = 4;                  // doubles of a slab's statistics
 constexpr double kLog2e64 = 1.4426950408889634;
-constexpr double kLn2 = 0.6931471805599453;
 constexpr float kInf = __builtin_huge_valf();
 
-// 2^z for z <= 0: the nearest integer apart, the Taylor series of e^(f ln 2) to
-// f^11 for |f| <= 1/2 (the first term left out is below 7e-15), and the exponent
-// put back. -inf (a masked logit's) never gets here; NaN stays NaN. z is held
-// above -4000 (where 2^z is 0) before n is taken off: a product fused into that
-// subtraction would leave the product's rounding, which is large where z is.
+// 2^z for z <= 0, -inf or NaN (which it stays). The nearest integer n is taken off
+// (adding 1.5 2^52 leaves it in the low bits), 2^f is the polynomial that equals it
+// at the ten Chebyshev points of [-1/2, 1/2] (1.9e-14 relative at most), and n goes
+// back into the exponent; below 2^-1022 the result is 0. (What the exponent's sum is
+// there does not matter, and a NaN's low bits are 0.)
 __device__ __forceinline__ double exp2_64(double z) {
-  z = z < -4000.0 ? -4000.0 : z;
-  const double n = rint(z);
-  const double f = z - n;
-  constexpr double l1 = kLn2, l2 = l1 * kLn2 / 2, l3 = l2 * kLn2 / 3, l4 = l3 * kLn2 / 4,
-                   l5 = l4 * kLn2 / 5, l6 = l5 * kLn2 / 6, l7 = l6 * kLn2 / 7,
-                   l8 = l7 * kLn2 / 8, l9 = l8 * kLn2 / 9, l10 = l9 * kLn2 / 10,
-                   l11 = l10 * kLn2 / 11;
-  double p = l11;
-  p = fma(p, f, l10);
-  p = fma(p, f, l9);
-  p = fma(p, f, l8);
-  p = fma(p, f, l7);
-  p = fma(p, f, l6);
-  p = fma(p, f, l5);
-  p = fma(p, f, l4);
-  p = fma(p, f, l3);
-  p = fma(p, f, l2);
-  p = fma(p, f, l1);
-  p = fma(p, f, 1.0);
-  return ldexp(p, static_cast<int>(n));
+  constexpr double kMagic = 6755399441055744.0;
+  const double s = z + kMagic;
+  const double f = z - (s - kMagic);
+  double p = 0x1.b6571de2f2351p-24;
+  p = fma(p, f, 0x1.63ef969a64d3cp-20);
+  p = fma(p, f, 0x1.ffcb76789860fp-17);
+  p = fma(p, f, 0x1.43088e257f341p-13);
+  p = fma(p, f, 0x1.5d87fe908f88ap-10);
+  p = fma(p, f, 0x1.3b2ab72b175eep-7);
+  p = fma(p, f, 0x1.c6b08d7044119p-5);
+  p = fma(p, f, 0x1.ebfbdff8149f2p-3);
+  p = fma(p, f, 0x1.62e42fefa39f7p-1);
+  p = fma(p, f, 0x1.000000000003dp+0);
+  const uint32_t hi = static_cast<uint32_t>(__double2hiint(p)) +
+                      (static_cast<uint32_t>(__double2loint(s)) << 20);
+  return z < -1022.0 ? 0.0 : __hiloint2double(static_cast<int>(hi), __double2loint(p));
 }
 
-// exp((x - m) / T) with c = log2(e) / T; a masked logit's is 0 whatever m is.
+// exp((x - m) / T) with c = log2(e) / T > 0; a masked logit's (-inf) is 0, for which
+// m has to be a number (finite_max).
 __device__ __forceinline__ double weight_of(float x, double m, double c) {
-  return x == -kInf ? 0.0 : exp2_64((static_cast<double>(x) - m) * c);
+  return exp2_64((static_cast<double>(x) - m) * c);
+}
+__device__ __forceinline__ double finite_max(float m) {
+  return m == -kInf ? 0.0 : static_cast<double>(m);
 }
 
 // A probability: its weight times the row's 1 / sum, rounded. Kept out of a fused
@@ -93,7 +89,8 @@ __device__ __forceinline__ double inverse_temperature(const nmce_verify_batch& a
                                                       bool* greedy) {
   const float t = a.temperature ? a.temperature[b] : a.temperature_all;
   *greedy = !(t > 0.0f);
-  return *greedy ? 1.0 : 1.0 / static_cast<double>(t);
+  // (An infinite one is merely very large: every finite logit weighs 1.)
+  return *greedy ? 1.0 : fmax(1.0 / static_cast<double>(t), 1e-300);
 }
 
 // A uniform number: outside [0, 1) the nearest inside, NaN 0.
@@ -114,21 +111,23 @@ __device__ __forceinline__ void load_vec(const T* p, float* f) {
   Elem<T>::unpack(v, f);
 }
 
-// A slab's logits from element c0 of the row; -inf past its end. kInOrder: a
-// thread's 32 are consecutive; otherwise its vectors lie a block apart.
-template <typename T, bool kInOrder>
+// A slab's logits from element c0 of the row, kSlab / kBlock a thread; -inf past its
+// end. kInOrder: a thread's are consecutive; otherwise its vectors lie a block apart.
+template <typename T, int kBlock, bool kInOrder>
 __device__ __forceinline__ int64_t place(int64_t c0, int i) {
+  constexpr int kEach = kSlab / kBlock;
   constexpr int kVec = Elem<T>::kPerVec;
   if constexpr (kInOrder) return c0 + threadIdx.x * kEach + i;
   return c0 + (static_cast<int64_t>(i / kVec) * kBlock + threadIdx.x) * kVec + i % kVec;
 }
-template <typename T, bool kInOrder>
+template <typename T, int kBlock, bool kInOrder>
 __device__ __forceinline__ void load_slab(const T* __restrict__ row, int64_t c0, int64_t v,
                                           float* f) {
   constexpr int kVec = Elem<T>::kPerVec;
+  constexpr int kEach = kSlab / kBlock;
 #pragma unroll
   for (int i = 0; i < kEach; i += kVec) {
-    const int64_t c = place<T, kInOrder>(c0, i);
+    const int64_t c = place<T, kBlock, kInOrder>(c0, i);
     if (c + kVec <= v) {
       load_vec(row + c, f + i);
     } else {
@@ -146,10 +145,12 @@ __device__ __forceinline__ double wave_add(double v) {
 // ---- 1: every slab's statistics ---------------------------------------------
 // Rows: the targets' (batch x (drafts + 1)), then the drafts' (batch x drafts).
 // stats[row][slab] = {maximum, sum of exp((x - maximum) / T), the drafted token's
-// logit (-inf where it is not in the slab), the lowest id of the maximum}.
-template <typename T>
+// logit (-inf where it is not in the slab), the lowest id of the maximum (of greedy
+// sequences)}.
+template <typename T, int kBlock>
 __global__ __launch_bounds__(kBlock) void verify_stats_kernel(nmce_verify_batch a, int64_t slabs,
                                                               double* __restrict__ stats) {
+  constexpr int kEach = kSlab / kBlock, kWaves = kBlock / 64;
   __shared__ float wave_m[kWaves];
   __shared__ double wave_s[kWaves];
   __shared__ int wave_i[kWaves];
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kBlock) void verify_stats_kernel(nmce_verify_batch 
                             i * a.draft_row_stride;
   const int64_t c0 = slab * kSlab;
   float f[kEach];
-  load_slab<T, false>(x, c0, a.vocab_local, f);
+  load_slab<T, kBlock, false>(x, c0, a.vocab_local, f);
   bool greedy;
   const double c = inverse_temperature(a, b, &greedy) * kLog2e64;
   float m = -kInf;
@@ -177,19 +178,19 @@ __global__ __launch_bounds__(kBlock) void verify_stats_kernel(nmce_verify_batch 
   __syncthreads();
   for (int w = 0; w < kWaves; ++w) m = fmaxf(m, wave_m[w]);
   double sum = 0.0;
-  int best = kSlab;
+  const double at_m = finite_max(m);
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    sum += weight_of(f[e], m, c);
-    if (f[e] == m) {
-      const int at = static_cast<int>(place<T, false>(0, e));
-      best = at < best ? at : best;
-    }
-  }
+  for (int e = 0; e < kEach; ++e) sum += weight_of(f[e], at_m, c);
   sum = wave_add(sum);
-  for (int s = 32; s > 0; s >>= 1) {
-    const int o = __shfl_xor(best, s);
-    best = o < best ? o : best;
+  int best = kSlab;
+  if (greedy) {
+#pragma unroll
+    for (int e = kEach - 1; e >= 0; --e)
+      if (f[e] == m) best = static_cast<int>(place<T, kBlock, false>(0, e));
+    for (int s = 32; s > 0; s >>= 1) {
+      const int o = __shfl_xor(best, s);
+      best = o < best ? o : best;
+    }
   }
   if (lane == 0) {
     wave_s[wave] = sum;
@@ -294,11 +295,12 @@ struct Weights {
   }
 };
 
-template <typename T>
+template <typename T, int kBlock>
 __global__ __launch_bounds__(kBlock) void verify_masses_kernel(
     nmce_verify_batch a, int64_t slabs, int ranks, const double* __restrict__ stats,
     Decision* __restrict__ decisions, double* __restrict__ masses, int64_t* __restrict__ tokens,
     int64_t* __restrict__ accepted, float* __restrict__ logprobs) {
+  constexpr int kEach = kSlab / kBlock, kWaves = kBlock / 64;
   constexpr int kAtOnce = kBlock / 16;
   __shared__ bool stands[kAtOnce];
   __shared__ Decision dec[kAtOnce];
@@ -376,10 +378,10 @@ __global__ __launch_bounds__(kBlock) void verify_masses_kernel(
     w.init(a, b, chosen, c);
     const int64_t c0 = slab * kSlab;
     float f[kEach];
-    load_slab<T, false>(w.x, c0, a.vocab_local, f);
+    load_slab<T, kBlock, false>(w.x, c0, a.vocab_local, f);
     if (w.rest) {
       float g[kEach];
-      load_slab<T, false>(w.y, c0, a.vocab_local, g);
+      load_slab<T, kBlock, false>(w.y, c0, a.vocab_local, g);
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         const double p = probability(weight_of(f[e], w.pm, c), w.pi);
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(kBlock) void verify_masses_kernel(
       for (int e = 0; e < kEach; ++e) {
         const double p = probability(weight_of(f[e], w.pm, c), w.pi);
         plain += p;
-        rest += place<T, false>(c0, e) == w.skip ? 0.0 : p;
+        rest += place<T, kBlock, false>(c0, e) == w.skip ? 0.0 : p;
       }
     }
   }
@@ -417,11 +419,12 @@ __global__ __launch_bounds__(kBlock) void verify_masses_kernel(
 // where it is this rank's, the id within: picked[b] = {id, log-probability}, or
 // {-1, -inf} on the other ranks. Without `picked` (one rank) the outputs
 // themselves are written.
-template <typename T>
+template <typename T, int kBlock>
 __global__ __launch_bounds__(kBlock) void verify_pick_kernel(
     nmce_verify_batch a, int64_t slabs, int ranks, int rank,
     const Decision* __restrict__ decisions, const double* __restrict__ masses,
     int64_t* __restrict__ tokens, float* __restrict__ logprobs, double* __restrict__ picked) {
+  constexpr int kEach = kSlab / kBlock, kWaves = kBlock / 64;
   __shared__ double part[kBlock];
   __shared__ double wave_sum[kWaves];
   __shared__ int last_s[kWaves];
@@ -494,20 +497,20 @@ __global__ __launch_bounds__(kBlock) void verify_pick_kernel(
   Weights<T> w;
   w.init(a, b, d, c);
   float f[kEach];
-  load_slab<T, true>(w.x, c0, a.vocab_local, f);
+  load_slab<T, kBlock, true>(w.x, c0, a.vocab_local, f);
   double wt[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) wt[e] = probability(weight_of(f[e], w.pm, c), w.pi);
   if (which == 0 && w.rest) {
     float g[kEach];
-    load_slab<T, true>(w.y, c0, a.vocab_local, g);
+    load_slab<T, kBlock, true>(w.y, c0, a.vocab_local, g);
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
       wt[e] = fmax(wt[e] - probability(weight_of(g[e], w.qm, c), w.qi), 0.0);
   } else if (which == 0) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e)
-      if (place<T, true>(c0, e) == w.skip) wt[e] = 0.0;
+      if (place<T, kBlock, true>(c0, e) == w.skip) wt[e] = 0.0;
   }
   // Sums before each thread's 32, and the last thread with any weight.
   double sum = 0.0;
@@ -560,10 +563,10 @@ __global__ __launch_bounds__(kBlock) void verify_pick_kernel(
 }
 
 // The ranks' picks, merged by their maximum, into the outputs.
-__global__ __launch_bounds__(kBlock) void verify_finish_kernel(
+__global__ __launch_bounds__(256) void verify_finish_kernel(
     const double* __restrict__ picked, const Decision* __restrict__ decisions, int64_t batch,
     int64_t drafts, int64_t* __restrict__ tokens, float* __restrict__ logprobs) {
-  const int64_t b = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+  const int64_t b = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (b >= batch) return;
   const double id = picked[2 * b];
   const int64_t o = b * (drafts + 1) + decisions[b].accepted;
@@ -595,6 +598,12 @@ int check_batch(const nmce_verify_batch* a) {
   return NMCE_OK;
 }
 
+// A slab a workgroup of 256 threads, 32 logits each; of 1024 and 8 where there are
+// too few workgroups to fill the chip (fewer than one a compute unit), which then
+// wait for one thread's chain of exponentials: verify_one's three kernels 8, 16
+// and 14 us with 256 threads.
+inline bool few(int64_t workgroups) { return workgroups <= 256; }
+
 int64_t rows_of(const nmce_verify_batch& a) {
   return a.batch * (a.drafts + 1) + (a.draft ? a.batch * a.drafts : 0);
 }
@@ -619,12 +628,16 @@ int nmce_verify_stats(const nmce_verify_batch* a, double* stats, void* stream) {
   if (a->batch == 0) return NMCE_OK;
   if (!stats) return NMCE_EINVAL_PTR;
   const int64_t slabs = slabs_of(a->vocab_local);
-  const dim3 grid(static_cast<unsigned>(rows_of(*a) * slabs)), block(kBlock);
+  const dim3 grid(static_cast<unsigned>(rows_of(*a) * slabs));
   hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool small = few(grid.x);
+  auto run = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, *a, slabs, stats);
+  };
   if (a->dtype == NMCE_F32)
-    hipLaunchKernelGGL(verify_stats_kernel<float>, grid, block, 0, s, *a, slabs, stats);
+    small ? run(verify_stats_kernel<float, 1024>, 1024) : run(verify_stats_kernel<float, 256>, 256);
   else
-    hipLaunchKernelGGL(verify_stats_kernel<uint16_t>, grid, block, 0, s, *a, slabs, stats);
+    small ? run(verify_stats_kernel<uint16_t, 1024>, 1024) : run(verify_stats_kernel<uint16_t, 256>, 256);
   return launch_status();
 }
 
@@ -639,15 +652,17 @@ int nmce_verify_masses(const nmce_verify_batch* a, const double* stats, int rank
       workspace_bytes < nmce_verify_workspace_bytes(a->batch))
     return NMCE_EINVAL_WORKSPACE;
   const int64_t slabs = slabs_of(a->vocab_local);
-  const dim3 grid(static_cast<unsigned>(a->batch * slabs)), block(kBlock);
+  const dim3 grid(static_cast<unsigned>(a->batch * slabs));
   hipStream_t s = static_cast<hipStream_t>(stream);
   Decision* dec = static_cast<Decision*>(workspace);
+  const bool small = few(grid.x);
+  auto run = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, *a, slabs, ranks, stats, dec, masses, tokens, accepted, logprobs);
+  };
   if (a->dtype == NMCE_F32)
-    hipLaunchKernelGGL(verify_masses_kernel<float>, grid, block, 0, s, *a, slabs, ranks, stats,
-                       dec, masses, tokens, accepted, logprobs);
+    small ? run(verify_masses_kernel<float, 1024>, 1024) : run(verify_masses_kernel<float, 256>, 256);
   else
-    hipLaunchKernelGGL(verify_masses_kernel<uint16_t>, grid, block, 0, s, *a, slabs, ranks, stats,
-                       dec, masses, tokens, accepted, logprobs);
+    small ? run(verify_masses_kernel<uint16_t, 1024>, 1024) : run(verify_masses_kernel<uint16_t, 256>, 256);
   return launch_status();
 }
 
@@ -662,15 +677,17 @@ int nmce_verify_pick(const nmce_verify_batch* a, const double* masses, int ranks
       workspace_bytes < nmce_verify_workspace_bytes(a->batch))
     return NMCE_EINVAL_WORKSPACE;
   const int64_t slabs = slabs_of(a->vocab_local);
-  const dim3 grid(static_cast<unsigned>(a->batch)), block(kBlock);
+  const dim3 grid(static_cast<unsigned>(a->batch));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Decision* dec = static_cast<const Decision*>(workspace);
+  const bool small = few(grid.x);
+  auto run = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, *a, slabs, ranks, rank, dec, masses, tokens, logprobs, picked);
+  };
   if (a->dtype == NMCE_F32)
-    hipLaunchKernelGGL(verify_pick_kernel<float>, grid, block, 0, s, *a, slabs, ranks, rank, dec,
-                       masses, tokens, logprobs, picked);
+    small ? run(verify_pick_kernel<float, 1024>, 1024) : run(verify_pick_kernel<float, 256>, 256);
   else
-    hipLaunchKernelGGL(verify_pick_kernel<uint16_t>, grid, block, 0, s, *a, slabs, ranks, rank,
-                       dec, masses, tokens, logprobs, picked);
+    small ? run(verify_pick_kernel<uint16_t, 1024>, 1024) : run(verify_pick_kernel<uint16_t, 256>, 256);
   return launch_status();
 }
 
@@ -682,7 +699,7 @@ int nmce_verify_finish(const double* picked, const void* workspace, int64_t work
   if (!picked || !tokens || !logprobs) return NMCE_EINVAL_PTR;
   if (!workspace || !aligned16(workspace) || workspace_bytes < nmce_verify_workspace_bytes(batch))
     return NMCE_EINVAL_WORKSPACE;
-  const dim3 grid(static_cast<unsigned>((batch + kBlock - 1) / kBlock)), block(kBlock);
+  const dim3 grid(static_cast<unsigned>((batch + 255) / 256)), block(256);
   hipLaunchKernelGGL(verify_finish_kernel, grid, block, 0, static_cast<hipStream_t>(stream),
                      picked, static_cast<const Decision*>(workspace), batch, drafts, tokens,
                      logprobs);
