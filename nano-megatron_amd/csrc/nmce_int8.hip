@@ -509,7 +509,8 @@ int launch_few(const LinearArgs& a, hipStream_t s) {
 
 template <typename O>
 int launch_linear(const LinearArgs& a, bool vec, hipStream_t s) {
-  if (a.n <= kFewTokens) {
+  // (A launch's threads, 512 for 128 vocabulary rows, have to fit 32 bits.)
+  if (a.n <= kFewTokens && a.v <= (int64_t{1} << 29)) {
     if (a.n <= 16) return launch_few<O, 1>(a, s);
     if (a.n <= 32) return launch_few<O, 2>(a, s);
     if (a.n <= 64) return launch_few<O, 4>(a, s);

@@ -249,6 +249,30 @@ def test_graph_replays():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_offsets_past_32_bits():
+    """A weight and an output of more than 2^31 elements each, and dW of more than
+    2^32 bytes: rows at both ends."""
+    import nmce
+    ctx = nmce.ParallelContext.single()
+    v, h, n = 66000, 33000, 66000
+    weight = torch.zeros(v, h, dtype=BF, device=DEV)
+    weight[0], weight[v // 2], weight[v - 1] = 1.0, 2.0, 3.0
+    weight.requires_grad_(True)
+    tokens = torch.full((n,), -1, dtype=torch.int64, device=DEV)
+    tokens[0], tokens[1], tokens[n - 2], tokens[n - 1] = v - 1, 0, v // 2, v - 1
+    out = nmce.vocab_parallel_embedding(tokens, weight, 0, v, ctx, validate=False)
+    rows = out.detach()[[0, 1, 2, n - 2, n - 1]]
+    assert torch.equal(rows, torch.tensor([3.0, 1, 0, 2, 3], device=DEV).to(BF)[:, None].expand(5, h))
+    assert not out.detach()[n // 2].any()
+    grad = torch.zeros(n, h, dtype=BF, device=DEV)
+    grad[0], grad[1], grad[n - 2], grad[n - 1] = 1.0, 4.0, 8.0, 2.0
+    dw, = torch.autograd.grad(out, weight, grad)
+    sums = dw.sum(dim=1, dtype=torch.float64)
+    want = torch.zeros(v, dtype=torch.float64, device=DEV)
+    want[0], want[v // 2], want[v - 1] = 4.0 * h, 8.0 * h, 3.0 * h
+    assert torch.equal(sums, want)
+
+
 def test_second_derivatives():
     """The weight's gradient is linear in the output's: its derivative is the
     lookup of the second gradient, and that one's the scatter again."""

@@ -196,6 +196,22 @@ def test_rows_that_are_not_finite(n):
     assert not y[1, keep].any() and torch.equal(y[2:, keep], clean[2:, keep])
 
 
+@pytest.mark.parametrize("n,v,k", [(8300, 260000, 16), (40, 1100000, 4096), (300, 1100000, 4096)])
+def test_offsets_past_32_bits(n, v, k):
+    """Logits of more than 2^31 elements; a weight of more than 2^32 bytes, by both
+    kernels: rows and columns at the ends and in the middle."""
+    import nmce
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(n, k, device=DEV, generator=g).to(BF)
+    wq = torch.randint(-127, 128, (v, k), device=DEV, generator=g, dtype=torch.int8)
+    ws = torch.rand(v, device=DEV, generator=g)
+    y = nmce.int8_linear(x, wq, ws)
+    for rows, cols in ((slice(0, 3), slice(0, 5)), (slice(n - 3, n), slice(v - 5, v)),
+                       (slice(n - 3, n), slice(0, 5)), (slice(n // 2, n // 2 + 3),
+                                                        slice(v // 2, v // 2 + 5))):
+        _check(y[rows, cols], x[rows], wq[cols], ws[cols])
+
+
 def test_int8_refusals():
     import nmce
     x = torch.randn(4, 32, device=DEV)

@@ -225,3 +225,26 @@ def test_verify_has_no_cpu_path():
         nmce.vocab_parallel_verify_drafts(
             torch.zeros(1, 2, 5), torch.zeros(1, 1, dtype=torch.int64), None, torch.zeros(1, 1),
             torch.zeros(1), 0, 5, nmce.ParallelContext.single())
+
+
+def test_int8_products_keep_their_wait_states(tmp_path):
+    """The 8-bit products run on the GEMM core, whose MFMAs are inline asm: in the
+    generated code no VALU instruction writes one's source within two wait states
+    before it, and none touches its result within 16 behind it (as for the bf16
+    products). The few tokens' kernel uses the builtin, which the compiler
+    schedules itself."""
+    import re
+    import subprocess
+
+    from _util import mfma_hazards
+    from nmce import _build
+    asm = tmp_path / "int8.s"
+    subprocess.run([_build.hipcc(), *_build.HIPCC_FLAGS, "-S", "--cuda-device-only",
+                    str(_build.CSRC_DIR / "nmce_int8.hip"), "-o", str(asm)], check=True,
+                   capture_output=True)
+    bodies = re.findall(r"^_Z\w*int8_linear_kernel\w*:(.*?)\.end_amdhsa_kernel", asm.read_text(),
+                        re.S | re.M)
+    assert len(bodies) == 3
+    for body in bodies:
+        mfmas, offenders = mfma_hazards(body)
+        assert mfmas >= 384 and not offenders, offenders[:5]
