@@ -645,7 +645,9 @@ __device__ __forceinline__ void store_f32_tile(const Acc& acc, char* lds, float*
 // operands. Against words of two rows, unscrambled on the way out, and cached
 // stores: K = 512 875 -> 1030 TFLOP/s, K = 1600 1166 -> 1247, K = 4096 1445 ->
 // 1459. Tiles that reach past M or N, and outputs that are not 16-byte
-// aligned, test every row and column.
+// aligned, test every row and column. kAny: those outputs leave 16 bytes at a time
+// all the same, at their element's alignment (rows of an odd width).
+template <bool kAny = false>
 __device__ __forceinline__ void store_bf16_tile(const Acc& acc, char* lds,
                                                 uint16_t* __restrict__ C, int64_t ldc, int64_t M,
                                                 int64_t N, int64_t m0, int64_t n0) {
@@ -693,6 +695,9 @@ __device__ __forceinline__ void store_bf16_tile(const Acc& acc, char* lds,
     uint16_t* dst = C + r * ldc + col;
     if (vec_ok && col + 8 <= N) {
       store_stream(reinterpret_cast<u32x4*>(dst), w);
+    } else if (kAny && col + 8 <= N) {
+      typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+      *reinterpret_cast<u32x4_any*>(dst) = u32x4_any{w.x, w.y, w.z, w.w};
     } else {
       const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
       for (int e = 0; e < 8 && col + e < N; ++e)

@@ -273,11 +273,18 @@ __global__ __launch_bounds__(kThreads, 1) void int8_linear_kernel(LinearArgs a) 
       for (int e = 0; e < 4; ++e)
         acc.c[i][j][e] = static_cast<float>(__float_as_int(acc.c[i][j][e])) * sx[i] * sw[e];
   }
-  if constexpr (std::is_same<O, float>::value)
-    store_f32_tile<1, kVec>(acc, lds, static_cast<float*>(a.out), nullptr, a.ldo, a.n, a.v, m0,
-                            n0);
-  else
-    store_bf16_tile(acc, lds, static_cast<uint16_t*>(a.out), a.ldo, a.n, a.v, m0, n0);
+  // Rows of any width and start: 16-byte stores need no more than their element's
+  // alignment here, so only a tile that reaches past the last column goes element by
+  // element.
+  if constexpr (std::is_same<O, float>::value) {
+    float* out = static_cast<float*>(a.out);
+    if (kVec && n0 + kBN <= a.v)
+      store_f32_tile<1, kVec>(acc, lds, out, nullptr, a.ldo, a.n, a.v, m0, n0);
+    else
+      store_f32_tile<1, false>(acc, lds, out, nullptr, a.ldo, a.n, a.v, m0, n0);
+  } else {
+    store_bf16_tile<true>(acc, lds, static_cast<uint16_t*>(a.out), a.ldo, a.n, a.v, m0, n0);
+  }
 }
 
 // ---- few tokens -------------------------------------------------------------
@@ -407,7 +414,6 @@ __global__ __launch_bounds__(64 * kFewWavesWg, 4) void int8_few_kernel(LinearArg
     if (k + d < steps) mul(s[d], d);
   // Four consecutive logits a lane.
   O* out = static_cast<O*>(a.out);
-  const bool vec = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(O) - 1)) == 0;
   const int64_t v = v0 + 4 * g;
   if (v >= a.v) return;
   float sw[4];
@@ -422,12 +428,14 @@ __global__ __launch_bounds__(64 * kFewWavesWg, 4) void int8_few_kernel(LinearArg
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = static_cast<float>(acc[t][e]) * sx * sw[e];
     O* dst = out + tok * a.ldo + v;
-    if (vec && v + 4 <= a.v) {
+    if (v + 4 <= a.v) {  // at the element's alignment
       if constexpr (std::is_same<O, float>::value) {
-        *reinterpret_cast<u32x4*>(dst) = Elem<float>::pack(y);
+        typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+        *reinterpret_cast<f32x4_any*>(dst) = f32x4_any{y[0], y[1], y[2], y[3]};
       } else {
-        typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
-        *reinterpret_cast<u32x2v*>(dst) = u32x2v{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+        typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+        *reinterpret_cast<u32x2_any*>(dst) =
+            u32x2_any{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
       }
     } else {
       for (int e = 0; e < 4 && v + e < a.v; ++e) Elem<O>::store1(dst + e, y[e]);
@@ -586,12 +594,9 @@ int nmce_int8_linear(const void* x, int dtype, int64_t n_rows, int64_t columns, 
   a.ldw = ldw;
   a.ldo = ldo;
   a.w_chunks = (columns + 15) / 16;
-  // store_bf16_tile tests its own alignment; store_f32_tile's conditions for
-  // 16-byte stores.
+  // store_f32_tile addresses a pass's rows with 32 bits.
   if (out_dtype == NMCE_BF16) return launch_linear<uint16_t>(a, true, s);
-  const bool vec = vocab_local % 4 == 0 && ldo % 4 == 0 && aligned16(out) &&
-                   ldo * 4 * 512 < (int64_t{1} << 32);
-  return launch_linear<float>(a, vec, s);
+  return launch_linear<float>(a, ldo * 4 * 512 < (int64_t{1} << 32), s);
 }
 
 }  // extern "C"
