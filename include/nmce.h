@@ -6,6 +6,9 @@
  *   nano_megatron/cross_entropy.py:16-85  (_VocabParallelCrossEntropy and
  *                                           vocab_parallel_cross_entropy)
  *   nano_megatron/model.py:169-192         (ParallelLMHead, fused variant)
+ *   nano_megatron/tp_layers.py:91-132      (VocabParallelEmbedding's lookup)
+ * and adds what serving with those weights needs beside it: 8-bit products for
+ * the logits, and the verification of drafted tokens.
  *
  * Conventions shared by every entry point:
  *   - All tensor pointers are device memory owned by the caller. Unless an
@@ -576,6 +579,7 @@ int nmce_int8_linear(const void* x, int dtype, int64_t n_rows, int64_t columns, 
  * vocab_local] with the given strides (elements; the vocabulary's is 1),
  * aligned to their elements; draft_tokens and accept_u [batch, drafts] and
  * sample_u [batch] contiguous; temperature [batch], or NULL: temperature_all.
+ * batch x (2 drafts + 1) x slabs (nmce_verify_slabs) is at most 2^23.
  */
 typedef struct nmce_verify_batch {
   const void* target;
