@@ -93,6 +93,9 @@ def vocab_parallel_embedding(
     """
     out_dtype = weight.dtype if out_dtype is None else out_dtype
     _check_embedding(tokens, weight, vocab_start, vocab_end, out_dtype)
+    if sequence_parallel and tokens.dim() < 2:
+        raise ValueError("nmce: sequence-parallel tokens must be [batch, seq], got "
+                         f"{tuple(tokens.shape)}")
     pending = None
     if validate:
         pending = launch_target_check(tokens, ctx.tp_size * (vocab_end - vocab_start))

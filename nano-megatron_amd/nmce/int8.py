@@ -29,6 +29,7 @@ from .parallel import divide
 
 # The product's rows of 8-bit weights lie a multiple of this many bytes apart.
 _ROW_ALIGN = 16
+_MAX_STRIDE = 1 << 23  # and at most this many
 # Sums of this many products of two 8-bit integers fit 32 bits.
 MAX_COLUMNS = 131072
 
@@ -74,7 +75,7 @@ def _weight_rows(weight: torch.Tensor) -> tuple[torch.Tensor, int]:
     ld = weight.stride(0) if v > 1 else -(-k // _ROW_ALIGN) * _ROW_ALIGN
     whole = (v - 1) * ld + -(-k // _ROW_ALIGN) * _ROW_ALIGN
     held = weight.untyped_storage().nbytes() - weight.storage_offset()
-    if ((weight.stride(1) == 1 or k == 1) and ld >= k and ld % _ROW_ALIGN == 0
+    if ((weight.stride(1) == 1 or k == 1) and k <= ld < _MAX_STRIDE and ld % _ROW_ALIGN == 0
             and weight.data_ptr() % _ROW_ALIGN == 0 and whole <= held):
         return weight, ld
     ld = -(-k // _ROW_ALIGN) * _ROW_ALIGN

@@ -86,9 +86,10 @@ def vocab_parallel_verify_drafts(
     ``draft_logits`` ``[B, K, V/tp]``, what they were drawn from at the same
     temperature, or None (copied drafts: ``q`` is one at the drafted token).
     ``accept_uniform`` ``[B, K]`` and ``sample_uniform`` ``[B]`` are fp32 in
-    ``[0, 1)``. ``temperature`` is a number or fp32 ``[B]``; 0 is greedy: a
-    draft stands where it is the largest logit (the lowest id of equal ones),
-    which is also the next token.
+    ``[0, 1)``. ``temperature`` is a number or fp32 ``[B]``; 0 is greedy (so is
+    what a tensor holds that is not above 0, NaN among it): a draft stands where
+    it is the largest logit (the lowest id of equal ones), which is also the next
+    token.
 
     ``tokens`` ``[B, K + 1]`` holds the drafts that stand, the next token, and -1
     behind it; ``accepted`` ``[B]`` how many stand; ``logprobs`` ``[B, K + 1]``

@@ -165,6 +165,9 @@ def test_ids_outside_the_vocabulary_are_refused():
         tokens = torch.tensor([2, bad, 5], device=DEV)
         with pytest.raises(ValueError, match="outside the model vocabulary"):
             nmce.vocab_parallel_embedding(tokens, weight, 0, 20, ctx)
+    with pytest.raises(ValueError, match=r"must be \[batch, seq\]"):
+        nmce.vocab_parallel_embedding(torch.zeros(4, dtype=torch.int64, device=DEV), weight, 0, 20,
+                                      ctx, sequence_parallel=True)
     two = nmce.ParallelContext(rank=0, world_size=2, tp_size=2, tp_rank=0, pp_size=1, pp_rank=0,
                                dp_size=1, dp_rank=0)
     with pytest.raises(ValueError, match="outside the model vocabulary"):

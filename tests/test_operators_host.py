@@ -168,6 +168,8 @@ def test_int8_weight_rows():
         assert (got is w) == same, (w.shape, w.stride())
         assert ld % 16 == 0 and ld >= w.shape[1]
         assert torch.equal(got[:, :w.shape[1]], w)
+    far = torch.zeros((1 << 23) + 48, dtype=torch.int8).as_strided((2, 48), (1 << 23, 1))
+    assert _weight_rows(far)[0] is not far and _weight_rows(far)[1] == 48
     # the last row ends with the storage, inside 16 bytes
     tight = torch.zeros(9 * 48 + 33, dtype=torch.int8).as_strided((10, 33), (48, 1))
     assert _weight_rows(tight)[0] is not tight

@@ -207,8 +207,9 @@ def test_masked_empty_and_broken_rows(dtype):
     x[21, 0, 0] = torch.finfo(dtype).max     # exp of everything else is 0
     x[22, 0] = torch.finfo(dtype).max
     heat = torch.tensor([1.0, 0.5])[torch.arange(24) % 2]
+    odd = torch.tensor([NAN, -1.0, INF, 2.0 ** -149])[torch.arange(24) % 4]
     for draft in (y, None):
-        for t in (1.0, 0.0, heat, 1e-30, INF):
+        for t in (1.0, 0.0, heat, 1e-30, INF, odd):
             _check(x, tokens, draft, au, su, t)
 
 
