@@ -16,7 +16,7 @@ fixed order, without atomics on values, so the same inputs give the same bits
 at every run, however often an id is repeated.
 
 The autograd node is C++ (``_nmce_autograd``): with a node in Python a training
-step of 512 tokens took 128 us, the host's, where it takes 54.
+step of 512 tokens took 128 us, the host's, where it takes 53.
 
 There is no CPU path.
 """

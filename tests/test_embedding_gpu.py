@@ -80,6 +80,7 @@ CASES = [
     (16384, 72, 128256, 0, BF, BF, "text"),
     (14336, 64, 32000, 0, BF, BF, "same"),
     (14337, 64, 32000, 5, BF, BF, "wide"),
+    (16385, 40, 50257, 0, BF, F32, "text"),    # one more than one workgroup sorts
     (20011, 24, 262143, 0, F32, F32, "any"),   # 18 bits of key
     (20011, 24, 262144, 0, F32, F32, "text"),  # 19: three passes
     (131072, 16, 97, 0, BF, F32, "any"),       # hundreds of chunks an id
