@@ -205,9 +205,10 @@ __global__ __launch_bounds__(kBlock) void verify_stats_kernel(nmce_verify_batch 
     float xd = -kInf;
     if (i < a.drafts) {
       const int64_t d = a.draft_tokens[b * a.drafts + i];
-      const int64_t at = d - a.vocab_start;
-      if (is_id(d, a) && at >= c0 && at < c0 + kSlab && at < a.vocab_local)
-        xd = Elem<T>::load1(x + at);
+      if (is_id(d, a)) {
+        const int64_t at = d - a.vocab_start;
+        if (at >= c0 && at < c0 + kSlab && at < a.vocab_local) xd = Elem<T>::load1(x + at);
+      }
     }
     double* o = stats + blockIdx.x * static_cast<int64_t>(kStat);
     o[0] = m;
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(kBlock) void verify_masses_kernel(
   const int slot = threadIdx.x >> 4, sub = threadIdx.x & 15;
   const bool first = slab == 0;
 
-  // 16 positions at a time until one does not stand.
+  // A position for every 16 threads at a time, until one does not stand.
   for (int64_t base = 0; base <= k; base += kAtOnce) {
     const int64_t i = base + slot;
     if (i <= k) {

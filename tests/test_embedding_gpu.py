@@ -85,6 +85,8 @@ CASES = [
     (20011, 24, 262144, 0, F32, F32, "text"),  # 19: three passes
     (131072, 16, 97, 0, BF, F32, "any"),       # hundreds of chunks an id
     (300000, 8, 1000, 0, F32, BF, "two"),      # tiles larger than the smallest
+    (70001, 9, 500, 0, F32, BF, "any"),        # eight rows a wave: an odd width,
+    (70003, 12, 300, 300, F32, F32, "wide"),   # and whole vectors with a rest
 ]
 
 
