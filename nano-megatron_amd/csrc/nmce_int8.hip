@@ -127,22 +127,21 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t top, uint16_t) {
   return lo > hi ? lo : hi;
 }
 
-// kWaves waves quantise a row: its largest magnitude, then the elements, which a
+// kRow threads quantise a row: its largest magnitude, then the elements, which a
 // thread holds in registers (32 of them; kHeld = false: longer rows, read twice). A
 // row with an infinity or a NaN gets the scale NaN and zeros, so its products are
-// NaN; a row of zeros gets the scale 0. One wave a row needs no barrier, and four
-// are faster for few rows. 50257 rows of 1600 bf16 take 47 us (5.2 TB/s), of fp32 73
-// (5.5); read twice an element at a time by a workgroup each, 136.
+// NaN; a row of zeros gets the scale 0. A wave or a part of one needs no barrier;
+// four waves are faster for few rows. 50257 rows of 1600 bf16 take 47 us (5.2 TB/s),
+// of fp32 73 (5.5); read twice an element at a time by a workgroup each, 136.
 constexpr int kQuantEach = 32;
 
-template <typename T, int kWaves, bool kHeld>
-__global__ __launch_bounds__(64 * (kWaves < 4 ? 4 : kWaves)) void quantize_rows_kernel(
+template <typename T, int kRow, bool kHeld>
+__global__ __launch_bounds__(kRow < 256 ? 256 : kRow) void quantize_rows_kernel(
     const T* __restrict__ x, int64_t n, int64_t k, int64_t ldx, int8_t* __restrict__ q,
     int64_t ldq, float* __restrict__ scale, bool whole_stores) {
   constexpr int kVec = Elem<T>::kPerVec;
-  constexpr int kBlock = 64 * (kWaves < 4 ? 4 : kWaves);
-  constexpr int kRow = 64 * kWaves;            // threads of a row
-  constexpr int kRowsAtOnce = kBlock / kRow;
+  constexpr int kWaves = kRow < 64 ? 1 : kRow / 64;
+  constexpr int kRowsAtOnce = (kRow < 256 ? 256 : kRow) / kRow;
   constexpr int kSpan = kRow * kVec;           // columns a round of vectors covers
   constexpr int kVecs = kQuantEach / kVec;
   // 16 bytes of elements at any element's alignment.
@@ -175,7 +174,7 @@ __global__ __launch_bounds__(64 * (kWaves < 4 ? 4 : kWaves)) void quantize_rows_
       for (int64_t c = t * kVec; c < k; c += kSpan) raise(top, get(row, c), T());
     }
     top = top_bits(top, T());
-    for (int s = 32; s > 0; s >>= 1) {
+    for (int s = (kRow < 64 ? kRow : 64) / 2; s > 0; s >>= 1) {
       const uint32_t o = __shfl_xor(top, s);
       top = o > top ? o : top;
     }
@@ -450,15 +449,15 @@ __global__ __launch_bounds__(64 * kFewWavesWg, 4) void int8_few_kernel(LinearArg
 inline bool dtype_ok(int d) { return d == NMCE_F32 || d == NMCE_BF16; }
 inline int64_t size_of(int d) { return d == NMCE_F32 ? 4 : 2; }
 
-template <typename T, int kWaves, bool kHeld>
+template <typename T, int kRow, bool kHeld>
 int launch_quantize_as(const void* x, int64_t n, int64_t k, int64_t ldx, int8_t* q, int64_t ldq,
                        float* scale, hipStream_t s) {
-  constexpr int kBlock = 64 * (kWaves < 4 ? 4 : kWaves), kRows = kBlock / (64 * kWaves);
+  constexpr int kBlock = kRow < 256 ? 256 : kRow, kRows = kBlock / kRow;
   const int64_t most = 1 << 21, want = (n + kRows - 1) / kRows;
   // A vector's bytes leave in one store where every row starts on such a boundary.
   constexpr int kVec = Elem<T>::kPerVec;
   const bool whole = reinterpret_cast<uintptr_t>(q) % kVec == 0 && ldq % kVec == 0;
-  hipLaunchKernelGGL((quantize_rows_kernel<T, kWaves, kHeld>),
+  hipLaunchKernelGGL((quantize_rows_kernel<T, kRow, kHeld>),
                      dim3(static_cast<unsigned>(want < most ? want : most)), dim3(kBlock), 0, s,
                      static_cast<const T*>(x), n, k, ldx, q, ldq, scale, whole);
   return launch_status();
@@ -467,15 +466,26 @@ int launch_quantize_as(const void* x, int64_t n, int64_t k, int64_t ldx, int8_t*
 template <typename T>
 int launch_quantize_of(const void* x, int64_t n, int64_t k, int64_t ldx, int8_t* q, int64_t ldq,
                        float* scale, hipStream_t s) {
-  // A wave a row where its registers hold the row and there are rows for two
-  // waves on every SIMD; else four, sixteen, or sixteen that read twice.
-  if (k <= 64 * kQuantEach && n >= 2048)
-    return launch_quantize_as<T, 1, true>(x, n, k, ldx, q, ldq, scale, s);
+  // A wave a row, or for short rows a part of one, where its registers hold the row
+  // and there are rows for two waves on every SIMD; else four, sixteen, or sixteen
+  // that read twice. The fewest threads that hold a row win: a wave's others would
+  // idle. 2^18 rows of 256 bf16 take 34 us with 8 threads a row, 44 with 16 and 171
+  // with 64; 2^17 of 512 33 with 16 and 81 with 64; 65536 of 1024 34 with 32 and 44
+  // with 64.
+  if (k <= 64 * kQuantEach && n >= 2048) {
+    if (k <= 8 * kQuantEach)
+      return launch_quantize_as<T, 8, true>(x, n, k, ldx, q, ldq, scale, s);
+    if (k <= 16 * kQuantEach)
+      return launch_quantize_as<T, 16, true>(x, n, k, ldx, q, ldq, scale, s);
+    if (k <= 32 * kQuantEach)
+      return launch_quantize_as<T, 32, true>(x, n, k, ldx, q, ldq, scale, s);
+    return launch_quantize_as<T, 64, true>(x, n, k, ldx, q, ldq, scale, s);
+  }
   if (k <= 256 * kQuantEach)
-    return launch_quantize_as<T, 4, true>(x, n, k, ldx, q, ldq, scale, s);
+    return launch_quantize_as<T, 256, true>(x, n, k, ldx, q, ldq, scale, s);
   if (k <= 1024 * kQuantEach)
-    return launch_quantize_as<T, 16, true>(x, n, k, ldx, q, ldq, scale, s);
-  return launch_quantize_as<T, 16, false>(x, n, k, ldx, q, ldq, scale, s);
+    return launch_quantize_as<T, 1024, true>(x, n, k, ldx, q, ldq, scale, s);
+  return launch_quantize_as<T, 1024, false>(x, n, k, ldx, q, ldq, scale, s);
 }
 
 int launch_quantize(const void* x, int dtype, int64_t n, int64_t k, int64_t ldx, int8_t* q,

@@ -48,7 +48,11 @@ def _rows(n, k, dtype, g, how):
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("n,k", [(1, 1), (3, 7), (5, 16), (33, 100), (4, 4096), (2, 8192),
-                                 (2, 8200), (7, 10007), (300, 520)])
+                                 (2, 8200), (7, 10007), (300, 520), (3, 40000), (2047, 130),
+                                 (2048, 1), (2050, 17), (2049, 127), (2051, 128), (2048, 129),
+                                 (2048, 255), (2049, 256), (2050, 257), (2048, 512),
+                                 (2053, 511), (2048, 513), (2055, 1000), (2048, 1024),
+                                 (2049, 1025), (2500, 1600), (2048, 2048), (2048, 2049)])
 @pytest.mark.parametrize("how", ["normal", "halves", "ends", "tiny", "huge", "zeros"])
 def test_quantize_rows(n, k, dtype, how):
     import nmce
