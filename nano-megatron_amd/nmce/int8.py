@@ -139,7 +139,8 @@ class Int8ParallelLMHead(torch.nn.Module):
     ``x``'s type (fp32 or bf16). ``load_weight(w)`` quantises a ``[V/tp,
     n_embd]`` weight (on a ROCm device); ``FusedParallelLMHead.quantized()``
     makes one of a trained head. The buffers ``weight_q`` (rows padded to 16
-    bytes) and ``weight_scale`` are what a checkpoint holds.
+    bytes) and ``weight_scale`` are what a checkpoint holds; a cast of the module
+    (``.to(torch.bfloat16)``, ``.half()``) leaves them int8 and fp32.
     """
 
     def __init__(self, config, ctx):
@@ -151,6 +152,17 @@ class Int8ParallelLMHead(torch.nn.Module):
         padded = -(-self.n_embd // _ROW_ALIGN) * _ROW_ALIGN
         self.register_buffer("weight_q", torch.zeros(per_partition, padded, dtype=torch.int8))
         self.register_buffer("weight_scale", torch.zeros(per_partition))
+
+    def _apply(self, fn, recurse=True):
+        # Casts are not for quantised buffers: what one changed goes back to its
+        # former bits, on the device that the call moved it to.
+        held = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, before in held.items():
+            after = self._buffers[name]
+            if after.dtype != before.dtype:
+                self._buffers[name] = before.to(after.device)
+        return self
 
     def vocab_range(self) -> tuple[int, int]:
         """This rank's global id range (model.py:242-245)."""

@@ -316,3 +316,17 @@ def test_head_of_a_trained_head():
             assert torch.equal(other(x), y)
         with pytest.raises(ValueError, match="is not this head's"):
             other.load_weight(head.weight[:, 1:])
+
+
+def test_head_of_a_model_that_is_cast():
+    """The serving head in a model cast to bf16 (and back) gives the logits it gave,
+    to the bit."""
+    import nmce
+    cfg = types.SimpleNamespace(vocab_size=300, n_embd=72, sequence_parallel=False)
+    torch.manual_seed(2)
+    head = nmce.FusedParallelLMHead(cfg, nmce.ParallelContext.single()).to(DEV).quantized()
+    x = torch.randn(2, 3, 72, device=DEV).to(BF)
+    want = head(x)
+    model = torch.nn.Sequential(head)
+    for dtype in (BF, torch.float16, F32):
+        assert torch.equal(model.to(dtype)(x), want)

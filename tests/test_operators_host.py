@@ -250,3 +250,30 @@ def test_int8_products_keep_their_wait_states(tmp_path):
     for body in bodies:
         mfmas, offenders = mfma_hazards(body)
         assert mfmas >= 384 and not offenders, offenders[:5]
+
+
+def test_int8_head_keeps_its_types_under_casts():
+    """A cast of the served model reaches its buffers too: the 8-bit rows and their
+    fp32 scales stay as they are, to the bit, and only move."""
+    import nmce
+    cfg = types.SimpleNamespace(vocab_size=40, n_embd=30)
+    head = nmce.Int8ParallelLMHead(cfg, nmce.ParallelContext.single())
+    g = torch.Generator().manual_seed(0)
+    head.weight_q.copy_(torch.randint(-127, 128, head.weight_q.shape, generator=g))
+    head.weight_scale.copy_(torch.rand(40, generator=g))
+    q, scale = head.weight_q.clone(), head.weight_scale.clone()
+    model = torch.nn.Sequential(torch.nn.Linear(4, 4), head)
+    for cast in (lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.bfloat16(),
+                 lambda m: m.double(), lambda m: m.type(torch.bfloat16), lambda m: m.float(),
+                 lambda m: m.to("cpu", torch.float16)):
+        cast(model)
+        for name, want in (("weight_q", q), ("weight_scale", scale)):
+            held = getattr(head, name)
+            assert held.dtype == want.dtype and torch.equal(held, want), name
+            assert model.state_dict()["1." + name] is not None
+    assert model[0].weight.dtype == torch.float16
+    # a move and a cast in one, and memory of its own
+    head.to("meta", torch.bfloat16)
+    assert head.weight_scale.is_meta and head.weight_scale.dtype == torch.float32
+    head.to_empty(device="cpu")
+    assert head.weight_q.dtype == torch.int8 and head.weight_scale.shape == (40,)
