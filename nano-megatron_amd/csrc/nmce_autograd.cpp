@@ -413,6 +413,20 @@ at::Tensor assumed_of(const at::Tensor& loss) {
   return saved[node->ctx_.saved_data.at("inplace").toBool() ? 2 : 4];
 }
 
+// A saved tensor as it came back, which saved-tensor hooks may have replaced: the
+// kernels read it at its address, so it has to be on the device, of the type and of
+// the shape that went in. (Strides are its own.)
+const at::Tensor& came_back(const at::Tensor& t, const at::Device& device, at::ScalarType type,
+                            at::IntArrayRef shape, const char* what) {
+  TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type &&
+                  t.sizes() == shape,
+              "nmce: saved-tensor hooks handed the backward other ", what, " than were saved: ",
+              type, " ", shape, " on ", device, " became ",
+              t.defined() ? c10::str(t.scalar_type(), " ", t.sizes(), " on ", t.device())
+                          : std::string("nothing"));
+  return t;
+}
+
 // ---- the embedding -----------------------------------------------------------
 // One shard's lookup (nmce_embedding_fwd) and the weight's dense gradient
 // (nmce_embedding_bwd). The gradient is linear in the output's, so its own
@@ -474,6 +488,17 @@ at::Tensor lookup_grad(const at::Tensor& grad, const at::Tensor& flat, int64_t v
 at::Tensor embedding(const at::Tensor& weight, const at::Tensor& tokens, int64_t vocab_start,
                      double scale, at::ScalarType out_type);
 
+// The ids of a node, saved by its forward and taken back by its backward.
+void save_ids(AutogradContext* ctx, const at::Tensor& tokens) {
+  ctx->saved_data["shape"] = tokens.sizes().vec();
+  ctx->save_for_backward({tokens});
+}
+
+at::Tensor saved_ids(AutogradContext* ctx, const at::Device& device) {
+  const at::Tensor ids = ctx->get_saved_variables()[0];
+  return came_back(ids, device, at::kLong, ctx->saved_data["shape"].toIntVector(), "token ids");
+}
+
 struct EmbeddingGrad : public torch::autograd::Function<EmbeddingGrad> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& grad,
                             const at::Tensor& tokens, int64_t v, int64_t vocab_start, double scale,
@@ -481,14 +506,14 @@ struct EmbeddingGrad : public torch::autograd::Function<EmbeddingGrad> {
     ctx->saved_data["start"] = vocab_start;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["type"] = grad.scalar_type();
-    ctx->save_for_backward({tokens});
+    save_ids(ctx, tokens);
     return lookup_grad(grad, tokens.reshape({-1}).contiguous(), v, vocab_start, scale,
                        weight_type);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(6);
-    out[0] = embedding(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["start"].toInt(),
-                       ctx->saved_data["scale"].toDouble(),
+    out[0] = embedding(grads[0], saved_ids(ctx, grads[0].device()),
+                       ctx->saved_data["start"].toInt(), ctx->saved_data["scale"].toDouble(),
                        ctx->saved_data["type"].toScalarType());
     return out;
   }
@@ -502,12 +527,12 @@ struct Embedding : public torch::autograd::Function<Embedding> {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["type"] = weight.scalar_type();
     ctx->saved_data["rows"] = weight.size(0);
-    ctx->save_for_backward({tokens});
+    save_ids(ctx, tokens);
     return lookup(weight, tokens.reshape({-1}).contiguous(), tokens.sizes(), vocab_start, scale,
                   out_type);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const at::Tensor tokens = ctx->get_saved_variables()[0];
+    const at::Tensor tokens = saved_ids(ctx, grads[0].device());
     const int64_t start = ctx->saved_data["start"].toInt(), v = ctx->saved_data["rows"].toInt();
     const double scale = ctx->saved_data["scale"].toDouble();
     const at::ScalarType type = ctx->saved_data["type"].toScalarType();

@@ -345,3 +345,53 @@ def test_tied_with_the_fused_head():
     want = rdw + w.grad.double().cpu()
     bound = mag * (terms + 1) * 2.0 ** -24 * 1.01 + (want.abs() + rdw.abs()) * 2.0 ** -23
     assert bool(((emb.weight.grad.double().cpu() - want).abs() <= bound).all())
+
+
+def _with_hooks(unpack):
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack)
+
+
+def test_saved_ids_through_hooks():
+    """Ids that saved-tensor hooks keep elsewhere (save_on_cpu) or hand back in other
+    strides give the same gradients, the second ones too."""
+    import nmce
+    ctx = nmce.ParallelContext.single()
+    g = torch.Generator().manual_seed(13)
+    weight = torch.randn(300, 40, generator=g).to(DEV).requires_grad_(True)
+    tokens = torch.randint(-5, 305, (9, 50), generator=g).to(DEV)
+    dy = torch.randn(9, 50, 40, generator=g).to(DEV).requires_grad_(True)
+    second = torch.randn(300, 40, generator=g).to(DEV)
+
+    def step():
+        out = nmce.vocab_parallel_embedding(tokens, weight, 0, 300, ctx, scale=2.0, validate=False)
+        dw, = torch.autograd.grad(out, weight, dy, create_graph=True)
+        return dw.detach(), torch.autograd.grad(dw, dy, second)[0]
+
+    want = step()
+    for hooks in (torch.autograd.graph.save_on_cpu(),
+                  _with_hooks(lambda t: t.t().contiguous().t())):
+        with hooks:
+            got = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("what", ["device", "type", "fewer", "more", "shape"])
+def test_other_ids_from_hooks_are_refused(what):
+    """Hooks that hand back something else than the ids that were saved: nothing is
+    launched on it, by the gradient and by the gradient's own backward."""
+    import nmce
+    ctx = nmce.ParallelContext.single()
+    weight = torch.randn(30, 16, device=DEV, requires_grad=True)
+    tokens = torch.arange(12, device=DEV).view(3, 4)
+    unpack = {"device": lambda t: t.cpu(), "type": lambda t: t.int(), "fewer": lambda t: t[:2],
+              "more": lambda t: torch.cat([t, t]), "shape": lambda t: t.view(4, 3)}[what]
+    with _with_hooks(unpack):
+        out = nmce.vocab_parallel_embedding(tokens, weight, 0, 30, ctx)
+    with pytest.raises(RuntimeError, match="nmce: saved-tensor hooks"):
+        out.sum().backward()
+    dy = torch.randn(3, 4, 16, device=DEV, requires_grad=True)
+    out = nmce.vocab_parallel_embedding(tokens, weight, 0, 30, ctx)
+    with _with_hooks(unpack):
+        dw, = torch.autograd.grad(out, weight, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="nmce: saved-tensor hooks"):
+        dw.sum().backward()
