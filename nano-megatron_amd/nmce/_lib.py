@@ -15,6 +15,7 @@ import pathlib
 import threading
 
 import torch  # noqa: F401  (must be imported before the HIP library is loaded)
+from torch.autograd import forward_ad as _forward_ad
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libnmce.so"
 
@@ -169,6 +170,20 @@ def dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.bfloat16:
         return NMCE_BF16
     raise TypeError(f"unsupported logits dtype {dtype}; expected float32 or bfloat16")
+
+
+def refuse_gradient(t: torch.Tensor, what: str, kernels: str) -> None:
+    """Kernels without a derivative take no tensor that one is wanted through:
+    one that requires grad while grad mode is on, or a forward-mode dual (which
+    no_grad leaves on), whose tangent would end there unseen."""
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise RuntimeError(f"nmce: {what} requires grad, but {kernels} no backward; call it under "
+                           "torch.no_grad() or detach it")
+    # (Outside of dual levels there are no tangents; to ask costs 0.6 us a tensor.)
+    if (getattr(_forward_ad, "_current_level", 0) >= 0
+            and _forward_ad.unpack_dual(t).tangent is not None):
+        raise RuntimeError(f"nmce: {what} has a forward-mode tangent, but {kernels} no "
+                           "derivative; unpack it first")
 
 
 # torch's raw-stream query (what its compiled kernels' launchers call): a

@@ -13,8 +13,8 @@ the weight once (:func:`quantize_rows`), the tokens within the call, and
 with the sum exact in 32-bit integers, the scales in fp32 and one rounding to
 the output's type. A token that holds an infinity or a NaN gives a row of NaN.
 
-There is no backward (the training head is ``FusedParallelLMHead``) and no CPU
-path.
+There is no derivative (the training head is ``FusedParallelLMHead``; tensors that
+one is wanted through are refused) and no CPU path.
 """
 
 from __future__ import annotations
@@ -40,9 +40,7 @@ def _check_rows(x: torch.Tensor, what: str) -> None:
     _lib.dtype_code(x.dtype)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"nmce: {what} must have columns, got {tuple(x.shape)}")
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise RuntimeError(f"nmce: {what} requires grad, but the 8-bit kernels have no backward; "
-                           "call them under torch.no_grad() or detach it")
+    _lib.refuse_gradient(x, what, "the 8-bit kernels have")
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -104,6 +102,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if weight.dtype != torch.int8 or weight_scale.dtype != torch.float32:
         raise TypeError(f"nmce: weight must be int8 and weight_scale float32, got {weight.dtype} "
                         f"and {weight_scale.dtype}")
+    _lib.refuse_gradient(weight_scale, "weight_scale", "the 8-bit kernels have")
     k = x.shape[-1]
     if weight.dim() != 2 or weight.shape[1] != k or weight.shape[0] == 0:
         raise ValueError(f"nmce: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not share "

@@ -60,10 +60,11 @@ def _check_verify(target, tokens, draft, accept_u, sample_u, vocab_start, vocab_
             raise TypeError(f"nmce: {name} must be {dtype}, got {t.dtype}")
         if tuple(t.shape) != shape:
             raise ValueError(f"nmce: {name} must be {shape}, got {tuple(t.shape)}")
-    if torch.is_grad_enabled() and (target.requires_grad
-                                    or (draft is not None and draft.requires_grad)):
-        raise RuntimeError("nmce: the logits require grad, but verification has no backward; call "
-                           "it under torch.no_grad() or detach them")
+    # (What the log-probabilities depend on smoothly, and the draft's logits.)
+    for name, t in (("target_logits", target), ("draft_logits", draft),
+                    ("temperature", temperature)):
+        if isinstance(t, torch.Tensor):
+            _lib.refuse_gradient(t, name, "verification has")
 
 
 def vocab_parallel_verify_drafts(

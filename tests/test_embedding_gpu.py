@@ -395,3 +395,17 @@ def test_other_ids_from_hooks_are_refused(what):
         dw, = torch.autograd.grad(out, weight, dy, create_graph=True)
     with pytest.raises(RuntimeError, match="nmce: saved-tensor hooks"):
         dw.sum().backward()
+
+
+def test_a_weight_with_a_tangent_is_refused():
+    """Forward-mode derivatives: refused, not dropped."""
+    from torch.autograd import forward_ad
+    import nmce
+    weight, tokens = torch.randn(30, 16, device=DEV), torch.arange(12, device=DEV)
+    with forward_ad.dual_level():
+        for leaf in (weight, weight.clone().requires_grad_(True)):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises((RuntimeError, NotImplementedError)):
+                    nmce.vocab_parallel_embedding(
+                        tokens, forward_ad.make_dual(leaf, torch.ones_like(weight)), 0, 30,
+                        nmce.ParallelContext.single())

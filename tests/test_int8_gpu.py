@@ -330,3 +330,22 @@ def test_head_of_a_model_that_is_cast():
     model = torch.nn.Sequential(head)
     for dtype in (BF, torch.float16, F32):
         assert torch.equal(model.to(dtype)(x), want)
+
+
+def test_tangents_and_scales_that_require_grad_are_refused():
+    """There is no derivative in either mode: none is dropped in silence."""
+    from torch.autograd import forward_ad
+    import nmce
+    x = torch.randn(4, 32, device=DEV)
+    wq, ws = nmce.quantize_rows(torch.randn(10, 32, device=DEV))
+    with pytest.raises(RuntimeError, match="nmce: weight_scale requires grad"):
+        nmce.int8_linear(x, wq, ws.clone().requires_grad_(True))
+    with forward_ad.dual_level(), torch.no_grad():
+        nmce.int8_linear(x, *nmce.quantize_rows(x))
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="nmce: x has a forward-mode tangent"):
+            nmce.quantize_rows(dual)
+        with pytest.raises(RuntimeError, match="nmce: x has a forward-mode tangent"):
+            nmce.int8_linear(dual, wq, ws)
+        with pytest.raises(RuntimeError, match="nmce: weight_scale has a forward-mode tangent"):
+            nmce.int8_linear(x, wq, forward_ad.make_dual(ws, torch.ones_like(ws)))

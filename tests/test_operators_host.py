@@ -277,3 +277,26 @@ def test_int8_head_keeps_its_types_under_casts():
     assert head.weight_scale.is_meta and head.weight_scale.dtype == torch.float32
     head.to_empty(device="cpu")
     assert head.weight_q.dtype == torch.int8 and head.weight_scale.shape == (40,)
+
+
+def test_tensors_that_want_a_derivative_are_refused():
+    """What the kernels without one ask of each of their tensors (no device needed)."""
+    from torch.autograd import forward_ad
+    from nmce import _lib as L
+    t = torch.randn(3)
+    L.refuse_gradient(t, "x", "they have")
+    leaf = torch.randn(3, requires_grad=True)
+    with pytest.raises(RuntimeError, match="nmce: x requires grad, but they have no backward"):
+        L.refuse_gradient(leaf, "x", "they have")
+    with torch.no_grad():
+        L.refuse_gradient(leaf, "x", "they have")
+    with forward_ad.dual_level():
+        L.refuse_gradient(t, "x", "they have")
+        dual = forward_ad.make_dual(t, torch.ones(3))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match="forward-mode tangent"):
+                L.refuse_gradient(dual, "x", "they have")
+        L.refuse_gradient(forward_ad.unpack_dual(dual).primal, "x", "they have")
+        with torch.inference_mode():  # where torch's own operators drop tangents
+            assert forward_ad.unpack_dual(dual * 2).tangent is None
+            L.refuse_gradient(dual, "x", "they have")

@@ -418,3 +418,20 @@ def test_a_serving_step(v):
         out, n, lp = nmce.vocab_parallel_verify_drafts(logits, tokens, None, *u, 0, v, ctx)
     want = _reference(logits, tokens, None, u[0], u[1], 1.0)
     assert torch.equal(out.cpu(), want[0]) and torch.equal(n.cpu(), want[1])
+
+
+def test_tensors_that_want_a_derivative_are_refused():
+    """The log-probabilities have none, in either mode: none is dropped in silence."""
+    from torch.autograd import forward_ad
+    g = torch.Generator().manual_seed(14)
+    x, tokens, y, au, su = (t.to(DEV) for t in _inputs(2, 3, 50, F32, g))
+    heat = torch.ones(2, device=DEV)
+    for i, name in enumerate(("target_logits", "draft_logits", "temperature")):
+        args = [x, y, heat]
+        args[i] = args[i].clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match=f"nmce: {name} requires grad"):
+            _run(args[0], tokens, args[1], au, su, args[2])
+        with forward_ad.dual_level(), torch.no_grad():
+            args[i] = forward_ad.make_dual(args[i].detach(), torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError, match=f"nmce: {name} has a forward-mode tangent"):
+                _run(args[0], tokens, args[1], au, su, args[2])
