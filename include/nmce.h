@@ -578,7 +578,8 @@ int nmce_int8_linear(const void* x, int dtype, int64_t n_rows, int64_t columns, 
  * Shapes: target [batch, drafts + 1, vocab_local], draft [batch, drafts,
  * vocab_local] with the given strides (elements; the vocabulary's is 1),
  * aligned to their elements; draft_tokens and accept_u [batch, drafts] and
- * sample_u [batch] contiguous; temperature [batch], or NULL: temperature_all.
+ * sample_u [batch] contiguous; temperature [batch], or NULL: temperature_all
+ * (64 bits wide, as all of the arithmetic is).
  * batch x (2 drafts + 1) x slabs (nmce_verify_slabs) is at most 2^23.
  */
 typedef struct nmce_verify_batch {
@@ -592,7 +593,7 @@ typedef struct nmce_verify_batch {
   int64_t draft_batch_stride, draft_row_stride;
   int64_t batch, drafts;
   int64_t vocab_local, vocab_start, vocab_total;
-  float temperature_all;
+  double temperature_all;
   int dtype;
 } nmce_verify_batch;
 

@@ -1057,7 +1057,7 @@ const char* nmce_status_string(int status) {
   }
 }
 
-int nmce_version(void) { return (1 << 16) | 1; }
+int nmce_version(void) { return (1 << 16) | 2; }
 
 int nmce_ce_fwd_stats(const void* logits, int dtype, int64_t n_rows, int64_t vocab_local,
                       int64_t ld, const int64_t* target, int64_t vocab_start, float* row_max,

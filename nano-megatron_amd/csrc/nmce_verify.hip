@@ -87,10 +87,11 @@ constexpr double kNothing = 1e-14;
 // log-probabilities are those of T = 1.
 __device__ __forceinline__ double inverse_temperature(const nmce_verify_batch& a, int64_t b,
                                                       bool* greedy) {
-  const float t = a.temperature ? a.temperature[b] : a.temperature_all;
-  *greedy = !(t > 0.0f);
-  // (An infinite one is merely very large: every finite logit weighs 1.)
-  return *greedy ? 1.0 : fmax(1.0 / static_cast<double>(t), 1e-300);
+  const double t = a.temperature ? static_cast<double>(a.temperature[b]) : a.temperature_all;
+  *greedy = !(t > 0.0);
+  // (An infinite one is merely very large: every finite logit weighs 1. At the
+  // smallest ones all below the largest weigh 0: two logits differ by 2^-149 or more.)
+  return *greedy ? 1.0 : fmin(fmax(1.0 / t, 1e-300), 1e300);
 }
 
 // A uniform number: outside [0, 1) the nearest inside, NaN 0.

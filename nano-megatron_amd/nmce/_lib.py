@@ -103,7 +103,7 @@ class VerifyBatch(ctypes.Structure):
                                              "draft_batch_stride", "draft_row_stride", "batch",
                                              "drafts", "vocab_local", "vocab_start",
                                              "vocab_total")]
-                + [("temperature_all", ctypes.c_float), ("dtype", _c_int)])
+                + [("temperature_all", ctypes.c_double), ("dtype", _c_int)])
 
 
 NMCE_LMHEAD_LAYOUT_FIELDS = 10

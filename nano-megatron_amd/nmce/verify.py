@@ -87,7 +87,7 @@ def vocab_parallel_verify_drafts(
     ``draft_logits`` ``[B, K, V/tp]``, what they were drawn from at the same
     temperature, or None (copied drafts: ``q`` is one at the drafted token).
     ``accept_uniform`` ``[B, K]`` and ``sample_uniform`` ``[B]`` are fp32 in
-    ``[0, 1)``. ``temperature`` is a number or fp32 ``[B]``; 0 is greedy (so is
+    ``[0, 1)``. ``temperature`` is a number (64 bits) or fp32 ``[B]``; 0 is greedy (so is
     what a tensor holds that is not above 0, NaN among it): a draft stands where
     it is the largest logit (the lowest id of equal ones), which is also the next
     token.

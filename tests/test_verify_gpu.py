@@ -435,3 +435,47 @@ def test_tensors_that_want_a_derivative_are_refused():
             args[i] = forward_ad.make_dual(args[i].detach(), torch.ones_like(args[i]))
             with pytest.raises(RuntimeError, match=f"nmce: {name} has a forward-mode tangent"):
                 _run(args[0], tokens, args[1], au, su, args[2])
+
+
+def test_a_number_as_temperature_keeps_its_bits():
+    """A Python number's temperature is 64 bits wide like the rest: uniform numbers
+    that lie between a border of p at 0.7 and the same border at fp32's 0.7, where the
+    two give neighbouring ids (each at least 1e-11 from both, 100 times what the
+    sums' rounding moves a border)."""
+    import nmce
+    g = torch.Generator().manual_seed(15)
+    v = 20000
+    x = torch.randn(v, generator=g) * 2.0
+    t = 0.7
+    near = torch.tensor(t, dtype=F32).double().item()
+    a, b = (torch.cumsum(torch.softmax(x.double() / s, -1), 0) for s in (t, near))
+    lo, hi = torch.minimum(a, b), torch.maximum(a, b)
+    u = ((lo + hi) / 2).float()
+    inside = (u.double() > lo + 1e-11) & (u.double() < hi - 1e-11)
+    u = u[inside]
+    assert u.numel() > 200
+    want, other = (torch.searchsorted(c, u.double(), right=True) for c in (a, b))
+    assert bool((want != other).all())
+    n = u.numel()
+
+    def draw(temperature):
+        return nmce.vocab_parallel_verify_drafts(
+            x.to(DEV).expand(n, 1, v), torch.zeros(n, 0, dtype=torch.int64, device=DEV), None,
+            torch.zeros(n, 0, device=DEV), u.to(DEV), 0, v, nmce.ParallelContext.single(),
+            temperature=temperature)[0][:, 0].cpu()
+
+    assert torch.equal(draw(t), want)
+    assert torch.equal(draw(torch.full((n,), t, device=DEV)), other)  # fp32 as given
+
+
+def test_temperatures_outside_of_fp32():
+    """Numbers that fp32 would take for 0 or infinity: above 0 is not greedy (equal
+    largest logits share), and the largest only levels."""
+    g = torch.Generator().manual_seed(16)
+    x, tokens, y, au, su = _inputs(6, 2, 9000, F32, g)
+    x[0, 0, [3, 8999]] = 40.0
+    x[1, :, 7] = x[1, :, 8500] = 50.0
+    x[2, 0, 1:] = -INF
+    for draft in (y, None):
+        for t in (5e-324, 1e-300, 1e-60, 1e39, 1e300):
+            _check(x, tokens, draft, au, su, t)
