@@ -31,7 +31,7 @@ from .cross_entropy import _launch
 from .mappings import _all_gather_rows, _use_host
 
 
-def _check_verify(target, tokens, draft, accept_u, sample_u, vocab_start, vocab_end,
+def _check_verify(target, tokens, draft, accept_u, sample_u, vocab_start, vocab_end, ctx,
                   temperature) -> None:
     if not target.is_cuda:
         raise RuntimeError("nmce: target_logits must be on a ROCm device (there is no CPU path)")
@@ -44,6 +44,11 @@ def _check_verify(target, tokens, draft, accept_u, sample_u, vocab_start, vocab_
     if vocab_end - vocab_start != v or vocab_start < 0:
         raise ValueError(f"nmce: logits hold {v} vocabulary entries but the shard "
                          f"[{vocab_start}, {vocab_end}) has {vocab_end - vocab_start}")
+    # The running sums go over the shards in the order of their ranks.
+    rank = ctx.tp_rank if ctx.tp_size > 1 else 0
+    if vocab_start != rank * v:
+        raise ValueError(f"nmce: the shard [{vocab_start}, {vocab_end}) is not rank {rank}'s of "
+                         f"the {ctx.tp_size * v} entries of {ctx.tp_size} shards")
     others = [("draft_tokens", tokens, (b, k), torch.int64),
               ("accept_uniform", accept_u, (b, k), torch.float32),
               ("sample_uniform", sample_u, (b,), torch.float32)]
@@ -102,14 +107,12 @@ def vocab_parallel_verify_drafts(
     that is no distribution (only -inf, or an infinity or NaN) refuses its
     token, and the next comes from ``p``; such a target row gives the next token
     -1. A number outside ``[0, 1)`` is taken as the nearest inside, NaN as 0.
-    Ranks of a tensor-parallel group must be given the same numbers and tokens.
+    Ranks of a tensor-parallel group must be given the same numbers and tokens, and
+    each the shard of its rank, ``vocab_start = tp_rank * V/tp``.
     """
     _check_verify(target_logits, draft_tokens, draft_logits, accept_uniform, sample_uniform,
-                  vocab_start, vocab_end, temperature)
+                  vocab_start, vocab_end, ctx, temperature)
     b, rows, v = target_logits.shape
-    if vocab_end > ctx.tp_size * v:
-        raise ValueError(f"nmce: the shard [{vocab_start}, {vocab_end}) is outside the "
-                         f"{ctx.tp_size * v} entries of {ctx.tp_size} shards")
     lib = _lib.load()
     dev = target_logits.device
     k = rows - 1

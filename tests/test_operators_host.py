@@ -300,3 +300,33 @@ def test_tensors_that_want_a_derivative_are_refused():
         with torch.inference_mode():  # where torch's own operators drop tangents
             assert forward_ad.unpack_dual(dual * 2).tangent is None
             L.refuse_gradient(dual, "x", "they have")
+
+
+def test_verify_refuses_another_ranks_shard():
+    """The shards' running sums are joined in the order of the ranks: a shard that is
+    not the rank's own would give other tokens (stand-ins that claim a GPU)."""
+    import dataclasses
+    import nmce
+    from nmce import verify
+
+    class Fake:
+        is_cuda, device, requires_grad, dtype = True, torch.device("cuda:0"), False, torch.float32
+
+        def __init__(self, *shape, dtype=torch.float32):
+            self.shape, self.dtype = torch.Size(shape), dtype
+
+        def dim(self):
+            return len(self.shape)
+
+    one = nmce.ParallelContext.single()
+    args = (Fake(2, 4, 50), Fake(2, 3, dtype=torch.int64), None, Fake(2, 3), Fake(2))
+    for tp, rank, start, ok in ((1, 0, 0, True), (1, 0, 50, False), (2, 0, 0, True),
+                                (2, 1, 50, True), (2, 1, 0, False), (2, 0, 50, False),
+                                (4, 2, 100, True), (4, 2, 101, False), (4, 2, 99, False),
+                                (4, 1, 100, False), (2, 1, 100, False)):
+        ctx = dataclasses.replace(one, tp_size=tp, tp_rank=rank)
+        if ok:
+            verify._check_verify(*args, start, start + 50, ctx, 1.0)
+        else:
+            with pytest.raises(ValueError, match="is not rank"):
+                verify._check_verify(*args, start, start + 50, ctx, 1.0)
