@@ -585,7 +585,7 @@ int check_batch(const nmce_verify_batch* a) {
   const int64_t most = (int64_t{1} << 31) - 1;
   if (a->batch < 0 || a->batch > most || a->drafts < 0 || a->drafts > most || a->vocab_local < 1 ||
       a->vocab_local > most || a->vocab_start < 0 || a->vocab_total > most ||
-      a->vocab_start + a->vocab_local > a->vocab_total)
+      a->vocab_total < a->vocab_local || a->vocab_start > a->vocab_total - a->vocab_local)
     return NMCE_EINVAL_SHAPE;
   // A launch's workgroups times their threads fit 32 bits.
   if ((2 * a->drafts + 1) * a->batch > (int64_t{1} << 23) ||

@@ -330,3 +330,14 @@ def test_verify_refuses_another_ranks_shard():
         else:
             with pytest.raises(ValueError, match="is not rank"):
                 verify._check_verify(*args, start, start + 50, ctx, 1.0)
+
+
+def test_verify_starts_that_would_overflow(lib):
+    """A start near 2^63 is refused as outside the vocabulary: its sum with the
+    shard's size is not formed."""
+    import ctypes
+    from nmce import _lib as L
+    p = 4096
+    for start in ((1 << 63) - 1, (1 << 63) - 9, 1 << 62, 1 << 31, 11):
+        b = L.VerifyBatch(p, None, p, p, p, None, 40, 10, 0, 0, 2, 3, 10, start, 20, 1.0, 0)
+        assert lib.nmce_verify_stats(ctypes.addressof(b), p, None) == -2, start
