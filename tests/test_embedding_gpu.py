@@ -409,3 +409,27 @@ def test_a_weight_with_a_tangent_is_refused():
                     nmce.vocab_parallel_embedding(
                         tokens, forward_ad.make_dual(leaf, torch.ones_like(weight)), 0, 30,
                         nmce.ParallelContext.single())
+
+
+@pytest.mark.parametrize("n,h", [(530001, 8), (1100003, 8), (1100003, 9)])
+@pytest.mark.parametrize("kind", ["lengths", "two", "any", "few"])
+def test_long_chunks(n, h, kind):
+    """Lists long enough that a wave adds 128 or 256 positions, 64 keys at a time, all
+    of the shard: runs of equal ids that end on both sides of every 64th place and of
+    the chunks' ends. Gradients are small integers, so every sum is exact."""
+    import nmce
+    g = torch.Generator().manual_seed(n + h)
+    v = {"lengths": 20000, "two": 2, "any": 50257, "few": 700}[kind]
+    if kind == "lengths":
+        runs = torch.tensor([63, 1, 64, 65, 127, 128, 129, 191, 193, 255, 256, 257, 1, 2, 511, 513])
+        ids = torch.arange(v).repeat_interleave(runs[torch.arange(v) % len(runs)])[:n]
+        ids = ids[torch.randperm(n, generator=g)]
+    else:
+        ids = torch.randint(0, v, (n,), generator=g)
+    grad = torch.randint(-3, 4, (n, h), generator=g)
+    weight = torch.zeros(v, h, device=DEV, requires_grad=True)
+    out = nmce.vocab_parallel_embedding(ids.to(DEV), weight, 0, v, nmce.ParallelContext.single(),
+                                        scale=0.5, validate=False)
+    dw, = torch.autograd.grad(out, weight, grad.float().to(DEV))
+    want = torch.zeros(v, h, dtype=torch.int64).index_add_(0, ids, grad)
+    assert torch.equal(dw.double().cpu() * 2.0, want.double())

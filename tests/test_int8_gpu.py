@@ -349,3 +349,55 @@ def test_tangents_and_scales_that_require_grad_are_refused():
             nmce.int8_linear(dual, wq, ws)
         with pytest.raises(RuntimeError, match="nmce: weight_scale has a forward-mode tangent"):
             nmce.int8_linear(x, wq, forward_ad.make_dual(ws, torch.ones_like(ws)))
+
+
+@pytest.mark.parametrize("copies", [1, 17])
+def test_every_bf16_quotient(copies):
+    """Every bf16 mantissa as the largest magnitude against every bf16 number from
+    2^-10 up to it: quotients as near to a half as they come (129 x 2^-15 under 1 gives
+    16383 / 32768), few rows and many."""
+    import nmce
+    top = 1.0 + torch.arange(128).float() / 128
+    steps = torch.arange(2 ** 7, 2 ** 8).float() / 2 ** 7
+    x = torch.cat([steps * 2.0 ** e for e in range(-10, 1)])
+    rows = torch.where(x[None] <= top[:, None], x[None], 0.0)
+    rows[:, ::3] *= -1.0
+    rows = torch.cat([rows, top[:, None]], 1).repeat(copies, 1)
+    assert torch.equal(rows.to(BF).float(), rows)
+    q, s = nmce.quantize_rows(rows.to(BF).to(DEV))
+    want, scale = _quotients(rows)
+    assert torch.equal(q.cpu().long(), want)
+    assert bool(((s.double().cpu() - scale).abs() <= scale * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("n", [40, 2100])
+def test_fp32_neighbours_of_halves(n):
+    """fp32 numbers next to (k + 1/2) top / 127 for every k: up to three steps off on
+    both sides, under random largest magnitudes of any exponent."""
+    import nmce
+    g = torch.Generator().manual_seed(17)
+    top = (1.0 + torch.rand(n, 1, generator=g)) * 2.0 ** torch.randint(-70, 70, (n, 1),
+                                                                       generator=g).float()
+    half = (torch.arange(127).double() + 0.5)[None] * top.double() / 127.0
+    bits = half.float().view(torch.int32)[:, :, None] + torch.arange(-3, 4, dtype=torch.int32)
+    x = torch.cat([bits.view(torch.float32).reshape(n, -1), top], 1)
+    x[:, ::2] *= -1.0
+    q, _ = nmce.quantize_rows(x.to(DEV))
+    want, _ = _quotients(x)
+    assert torch.equal(q.cpu().long(), want)
+
+
+def test_fp32_logits_of_vast_vocabularies():
+    """Rows of more than 2^21 fp32 logits, whose tiles leave element by element: the
+    bits that the same tokens give a hundred at a time, and the definition's."""
+    import nmce
+    n, v, k = 300, (1 << 21) + 5, 16
+    g = torch.Generator(device=DEV).manual_seed(18)
+    x = torch.randn(n, k, device=DEV, generator=g)
+    wq = torch.randint(-127, 128, (v, k), device=DEV, generator=g, dtype=torch.int8)
+    ws = torch.rand(v, device=DEV, generator=g)
+    y = nmce.int8_linear(x, wq, ws)
+    for r in range(0, n, 100):
+        assert torch.equal(y[r:r + 100], nmce.int8_linear(x[r:r + 100], wq, ws))
+    for cols in (slice(0, 9), slice(v // 2, v // 2 + 300), slice(v - 300, v)):
+        _check(y[:, cols], x, wq[cols], ws[cols])

@@ -479,3 +479,62 @@ def test_temperatures_outside_of_fp32():
     for draft in (y, None):
         for t in (5e-324, 1e-300, 1e-60, 1e39, 1e300):
             _check(x, tokens, draft, au, su, t)
+
+
+def _stops(b, k, v, g):
+    """Drafts that stand up to a place of each sequence's own: any of the ends of the
+    rounds in which positions are decided (16 or 64 at a time), or all of them."""
+    x = torch.randn(b, k + 1, v, generator=g) * 2.0
+    y = x[:, :k].clone()
+    tokens = y.argmax(-1)
+    su = torch.rand(b, generator=g)
+    places = [p for p in (0, 1, 14, 15, 16, 17, 31, 32, 33, 62, 63, 64, 65, 127, 128, 129, k - 1, k)
+              if p <= k]
+    at = torch.tensor(places)[torch.randint(0, len(places), (b,), generator=g)]
+    for s in range(min(b, len(places))):
+        at[s] = places[s]
+    return x, tokens, y, su, at
+
+
+@pytest.mark.parametrize("b,k", [(30, 63), (30, 64), (30, 65), (20, 130), (18, 200),   # 1024 threads
+                                 (300, 15), (300, 16), (300, 17), (300, 33), (260, 70)])  # 256
+def test_decisions_in_several_rounds(b, k):
+    """More drafts than positions are decided at once, in workgroups of 1024 threads
+    (64 of them) and, from 257 workgroups on, of 256 (16): stops at the ends of the
+    rounds and on both sides, refused by their number, by greedy choice, or padding."""
+    v = 60
+    g = torch.Generator().manual_seed(b + k)
+    x, tokens, y, su, at = _stops(b, k, v, g)
+    every = torch.arange(b)
+    stop = at < k
+    au = torch.zeros(b, k)
+    # Copied drafts: u = 0 stands, and the largest number below 1 is not below p.
+    refused = au.clone()
+    refused[every[stop], at[stop]] = 1.0 - 2.0 ** -24
+    assert _check(x, tokens, None, refused, su)[1].tolist() == at.tolist()
+    padded = tokens.clone()
+    padded[every[stop], at[stop]] = -1
+    for draft in (y, None):
+        assert _check(x, padded, draft, au, su)[1].tolist() == at.tolist()
+        assert _check(x, padded, draft, au, su, 0.0)[1].tolist() == at.tolist()
+    other = tokens.clone()
+    other[every[stop], at[stop]] = (other[every[stop], at[stop]] + 1) % v
+    assert _check(x, other, y, au, su, 0.0)[1].tolist() == at.tolist()
+    ruled = x.clone()  # the target rules the draft out; the draft model is sure of it
+    ruled[every[stop], at[stop], tokens[every[stop], at[stop]]] = -INF
+    assert _check(ruled, tokens, y, au, su)[1].tolist() == at.tolist()
+
+
+@pytest.mark.parametrize("drafts", ["model", "copied"])
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("b,k,v", [(32, 2, 65536), (33, 2, 65536),   # 256 and 264 slabs' masses
+                                   (40, 5, 60001), (257, 0, 9000),
+                                   (256, 1, 9001), (257, 1, 9001)])  # sequences that draw
+def test_both_workgroup_sizes(b, k, v, dtype, drafts):
+    """Both sides of the change from 1024 threads a workgroup to 256, in the masses
+    and in the draw, over several slabs: whole tokens, counts and log-probabilities."""
+    g = torch.Generator().manual_seed(b + k + v)
+    x, tokens, y, au, su = _inputs(b, k, v, dtype, g)
+    heat = torch.tensor([0.0, 0.3, 1.0, 4.0])[torch.arange(b) % 4]
+    for temperature in (heat, 1.0):
+        _check(x, tokens, None if drafts == "copied" else y, au, su, temperature)
