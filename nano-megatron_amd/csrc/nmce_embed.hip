@@ -677,8 +677,9 @@ template <typename W, typename O>
 int launch_fwd(const int64_t* tokens, int64_t n, const void* weight, int64_t vocab, int64_t h,
                int64_t ldw, int64_t start, float scale, void* out, int64_t ldo, bool vec,
                hipStream_t s) {
-  // Eight rows a wave where they still make eight waves for every SIMD.
-  const bool many = n * slabs_of(h) >= 8 * 4 * 8 * 256;
+  // Eight rows a wave where they still make eight waves for every SIMD, of which a
+  // compute unit has four.
+  const bool many = n * slabs_of(h) >= int64_t{8} * 8 * 4 * device_cus();
 #define NMCE_FWD(VEC, ROWS)                                                                      \
   launch_fwd_rows<W, O, VEC, ROWS>(tokens, n, weight, vocab, h, ldw, start, scale, out, ldo, s)
   if (vec) return many ? NMCE_FWD(true, 8) : NMCE_FWD(true, 1);

@@ -604,7 +604,7 @@ int check_batch(const nmce_verify_batch* a) {
 // workgroup for every compute unit, and one thread's chain of exponentials is the
 // time: one sequence of four drafts over 50257 fp32 takes 6, 12 and 8 us in the three
 // kernels, and 8, 16 and 14 with 256 threads.
-inline bool few(int64_t workgroups) { return workgroups <= 256; }
+inline bool few(int64_t workgroups) { return workgroups <= device_cus(); }
 
 int64_t rows_of(const nmce_verify_batch& a) {
   return a.batch * (a.drafts + 1) + (a.draft ? a.batch * a.drafts : 0);
