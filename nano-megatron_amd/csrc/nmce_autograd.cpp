@@ -57,6 +57,20 @@ hipStream_t stream_of(const at::Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
+// A saved tensor as it came back, which saved-tensor hooks may have replaced: the
+// kernels read it at its address, so it has to be on the device, of the type and of
+// the shape that went in. (Strides are its own.)
+const at::Tensor& came_back(const at::Tensor& t, const at::Device& device, at::ScalarType type,
+                            at::IntArrayRef shape, const char* what) {
+  TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type &&
+                  t.sizes() == shape,
+              "nmce: saved-tensor hooks handed the backward other ", what, " than were saved: ",
+              type, " ", shape, " on ", device, " became ",
+              t.defined() ? c10::str(t.scalar_type(), " ", t.sizes(), " on ", t.device())
+                          : std::string("nothing"));
+  return t;
+}
+
 // Optional per-launch timing: HIP event pairs recorded on the launch stream
 // around every launch of this file while enabled, read back by
 // take_timeline() (the benchmark's per-call times).
@@ -136,6 +150,8 @@ struct OnePassMean : public torch::autograd::Function<OnePassMean> {
     ctx->saved_data["vocab_start"] = vocab_start;
     ctx->saved_data["handed_out"] = false;
     ctx->saved_data["shape"] = logits.sizes().vec();
+    ctx->saved_data["rows"] = n;
+    ctx->saved_data["type"] = logits.scalar_type();
     if (inplace) {
       // The logits now hold the gradient: autograd nodes that saved them fail
       // their version check rather than read it.
@@ -158,16 +174,23 @@ struct OnePassMean : public torch::autograd::Function<OnePassMean> {
     const at::Tensor hint = ctx->saved_data["hint"].toTensor();
     const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
     const int64_t V = shape.back();
+    const int64_t n = ctx->saved_data["rows"].toInt();
+    const at::ScalarType type = ctx->saved_data["type"].toScalarType();
+    const at::Device device = grad_outputs[0].device();
     const variable_list saved = ctx->get_saved_variables();
     variable_list grads(6);
+    const size_t first = inplace ? 0 : 1;
+    const at::Tensor target =
+        came_back(saved[first], device, at::kLong, {n}, "targets").contiguous();
+    const at::Tensor row_stat =
+        came_back(saved[first + 1], device, at::kFloat, {2, n}, "row statistics").contiguous();
+    const at::Tensor& assumed = came_back(saved.back(), device, at::kFloat, {1}, "upstream value");
     if (inplace) {
       TORCH_CHECK(!ctx->saved_data["handed_out"].toBool(),
                   "nmce: a second backward through an in-place one-pass loss needs the logits, "
                   "which now hold the gradient; pass inplace=False to differentiate it twice");
-      const at::Tensor& target = saved[0];
-      const at::Tensor& assumed = saved[2];
       at::Tensor grad = ctx->saved_data["grad_buf"].toTensor();
-      const int64_t n = target.numel(), ld = ctx->saved_data["ld"].toInt();
+      const int64_t ld = ctx->saved_data["ld"].toInt();
       hipStream_t st = stream_of(grad);
       const bool ragged = is_ragged(grad, V, ld);
       timed(ragged ? "nmce_ce_grad_rescale_unless_ragged" : "nmce_ce_grad_rescale_unless", st, [&] {
@@ -181,12 +204,9 @@ struct OnePassMean : public torch::autograd::Function<OnePassMean> {
       return grads;
     }
     // Saved-tensor hooks may hand back copies of other strides.
-    const at::Tensor rows = V > 1 && saved[0].stride(1) != 1 ? saved[0].contiguous() : saved[0];
-    const at::Tensor& target = saved[1];
-    const at::Tensor& row_stat = saved[2];
-    const at::Tensor grad = saved[3].contiguous();
-    const at::Tensor& assumed = saved[4];
-    const int64_t n = rows.size(0);
+    const at::Tensor& held = came_back(saved[0], device, type, {n, V}, "logits");
+    const at::Tensor rows = V > 1 && held.stride(1) != 1 ? held.contiguous() : held;
+    const at::Tensor grad = came_back(saved[3], device, type, {n, V}, "gradient").contiguous();
     const int64_t ld = n > 1 ? rows.stride(0) : V;
     const int64_t vocab_start = ctx->saved_data["vocab_start"].toInt();
     const float gdiv = static_cast<float>(n > 1 ? n : 1);
@@ -411,20 +431,6 @@ at::Tensor assumed_of(const at::Tensor& loss) {
   TORCH_CHECK(node, "nmce: not a one-pass loss");
   const variable_list saved = node->ctx_.get_saved_variables();
   return saved[node->ctx_.saved_data.at("inplace").toBool() ? 2 : 4];
-}
-
-// A saved tensor as it came back, which saved-tensor hooks may have replaced: the
-// kernels read it at its address, so it has to be on the device, of the type and of
-// the shape that went in. (Strides are its own.)
-const at::Tensor& came_back(const at::Tensor& t, const at::Device& device, at::ScalarType type,
-                            at::IntArrayRef shape, const char* what) {
-  TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type &&
-                  t.sizes() == shape,
-              "nmce: saved-tensor hooks handed the backward other ", what, " than were saved: ",
-              type, " ", shape, " on ", device, " became ",
-              t.defined() ? c10::str(t.scalar_type(), " ", t.sizes(), " on ", t.device())
-                          : std::string("nothing"));
-  return t;
 }
 
 // ---- the embedding -----------------------------------------------------------

@@ -225,6 +225,26 @@ def _exchange_stats(local: torch.Tensor, group, world_size: int) -> torch.Tensor
     return gathered.to(local.device) if host else gathered
 
 
+def _save(ctx, *tensors) -> None:
+    """``ctx.save_for_backward``, with what :func:`_take` compares."""
+    ctx.save_for_backward(*tensors)
+    ctx.saved_as = [None if t is None else (t.device, t.dtype, t.shape) for t in tensors]
+
+
+def _take(ctx) -> tuple:
+    """The tensors of :func:`_save`, which saved-tensor hooks may have replaced: the
+    kernels read (and write) them at their address, so each has to be on the device,
+    of the type and of the shape that went in. Strides are its own."""
+    tensors = ctx.saved_tensors
+    for t, was in zip(tensors, ctx.saved_as):
+        if was is not None and (t.device, t.dtype, t.shape) != was:
+            raise RuntimeError(
+                "nmce: saved-tensor hooks handed the backward another tensor than was saved: "
+                f"{was[1]} {tuple(was[2])} on {was[0]} became {t.dtype} {tuple(t.shape)} on "
+                f"{t.device}")
+    return tensors
+
+
 def _resolve_inplace(logits: torch.Tensor, inplace, in_forward: bool = False) -> bool:
     """Whether the gradient goes into the logits' storage. ``inplace=None``:
     for a gradient written by the backward (two-pass path), in place iff the
@@ -283,7 +303,7 @@ def _ce_forward(ctx, logits, target, vocab_start, vocab_end, group, world_size, 
     ctx.vocab_start = vocab_start
     ctx.logits_shape = logits.shape
     # `rows` aliases `logits` unless a contiguous copy was made above.
-    ctx.save_for_backward(rows, tgt, row_stat, logits if ctx.inplace else None)
+    _save(ctx, rows, tgt, row_stat, logits if ctx.inplace else None)
     return loss
 
 
@@ -357,7 +377,8 @@ def _grad_operand(grad_output):
 def _ce_backward(ctx, go, gstride, gdiv):
     """Backward of one shard (cross_entropy.py:53-65) with the per-token
     gradient ``go[r * gstride] / gdiv``; returns the logits gradient."""
-    rows, tgt, row_stat, original = ctx.saved_tensors
+    rows, tgt, row_stat, original = _take(ctx)
+    tgt, row_stat = tgt.contiguous(), row_stat.contiguous()
     lib = _lib.load()
     n, V = rows.shape
     # Saved-tensor hooks may hand back copies of other strides, and the rows

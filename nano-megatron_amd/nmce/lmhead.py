@@ -49,8 +49,8 @@ from types import SimpleNamespace
 import torch
 
 from . import _lib
-from .cross_entropy import (_check_hint, _check_target, _exchange_stats, _launch, _site_hint,
-                            launch_target_check)
+from .cross_entropy import (_check_hint, _check_target, _exchange_stats, _launch, _save,
+                            _site_hint, _take, launch_target_check)
 from .mappings import (
     copy_to_tensor_parallel_region,
     gather_from_sequence_parallel_region,
@@ -257,7 +257,7 @@ class _LMHeadVocabParallelCrossEntropyMean(torch.autograd.Function):
                     *args, tgt.data_ptr(), vocab_start, chunk, c, out[1].data_ptr(),
                     out[2].data_ptr(), local[2].data_ptr(), assumed.data_ptr(), 0, float(n),
                     dx.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws.numel(), stream)
-        ctx.save_for_backward(x, w, tgt, out[1:], dx, dw, assumed)
+        _save(ctx, x, w, tgt, out[1:], dx, dw, assumed)
         return out[0].mean()
 
     @staticmethod
@@ -267,7 +267,7 @@ class _LMHeadVocabParallelCrossEntropyMean(torch.autograd.Function):
             return (torch.zeros(ctx.hidden_shape, dtype=torch.bfloat16, device=dev),
                     torch.zeros(ctx.weight_shape, dtype=torch.bfloat16, device=dev),
                     None, None, None, None, None, None, None)
-        x, w, tgt, row_stat, dx, dw, assumed = ctx.saved_tensors
+        x, w, tgt, row_stat, dx, dw, assumed = (t.contiguous() for t in _take(ctx))
         lib = _lib.load()
         go = grad_output.reshape(1)
         if go.dtype != torch.float32:
@@ -365,7 +365,7 @@ class _LMHeadVocabParallelCrossEntropy(torch.autograd.Function):
                 world_size, stride, n, loss.data_ptr(), row_stat[0].data_ptr(),
                 row_stat[1].data_ptr(), stream)
 
-        ctx.save_for_backward(x, w, tgt, row_stat)
+        _save(ctx, x, w, tgt, row_stat)
         return loss.view(target.shape)
 
     @staticmethod
@@ -375,7 +375,7 @@ class _LMHeadVocabParallelCrossEntropy(torch.autograd.Function):
             return (torch.zeros(ctx.hidden_shape, dtype=torch.bfloat16, device=dev),
                     torch.zeros(ctx.weight_shape, dtype=torch.bfloat16, device=dev),
                     None, None, None, None, None, None)
-        x, w, tgt, row_stat = ctx.saved_tensors
+        x, w, tgt, row_stat = (t.contiguous() for t in _take(ctx))
         lib = _lib.load()
         dev = x.device
         n, hp = x.shape
