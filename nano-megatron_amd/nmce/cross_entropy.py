@@ -228,21 +228,15 @@ def _exchange_stats(local: torch.Tensor, group, world_size: int) -> torch.Tensor
 def _save(ctx, *tensors) -> None:
     """``ctx.save_for_backward``, with what :func:`_take` compares."""
     ctx.save_for_backward(*tensors)
-    ctx.saved_as = [None if t is None else (t.device, t.dtype, t.shape) for t in tensors]
+    ctx.saved_as = _lib.autograd_ext().SavedAs(tensors)
 
 
-def _take(ctx) -> tuple:
-    """The tensors of :func:`_save`, which saved-tensor hooks may have replaced: the
-    kernels read (and write) them at their address, so each has to be on the device,
-    of the type and of the shape that went in. Strides are its own."""
+def _take(ctx) -> tuple[tuple, bool]:
+    """The tensors of :func:`_save`, and whether all are contiguous. Saved-tensor hooks
+    may have replaced them, and the kernels read (and write) them at their address:
+    each has to be on the device, of the type and of the shape that went in."""
     tensors = ctx.saved_tensors
-    for t, was in zip(tensors, ctx.saved_as):
-        if was is not None and (t.device, t.dtype, t.shape) != was:
-            raise RuntimeError(
-                "nmce: saved-tensor hooks handed the backward another tensor than was saved: "
-                f"{was[1]} {tuple(was[2])} on {was[0]} became {t.dtype} {tuple(t.shape)} on "
-                f"{t.device}")
-    return tensors
+    return tensors, ctx.saved_as.check(tensors)
 
 
 def _resolve_inplace(logits: torch.Tensor, inplace, in_forward: bool = False) -> bool:
@@ -377,8 +371,9 @@ def _grad_operand(grad_output):
 def _ce_backward(ctx, go, gstride, gdiv):
     """Backward of one shard (cross_entropy.py:53-65) with the per-token
     gradient ``go[r * gstride] / gdiv``; returns the logits gradient."""
-    rows, tgt, row_stat, original = _take(ctx)
-    tgt, row_stat = tgt.contiguous(), row_stat.contiguous()
+    (rows, tgt, row_stat, original), contiguous = _take(ctx)
+    if not contiguous:
+        tgt, row_stat = tgt.contiguous(), row_stat.contiguous()
     lib = _lib.load()
     n, V = rows.shape
     # Saved-tensor hooks may hand back copies of other strides, and the rows

@@ -267,7 +267,9 @@ class _LMHeadVocabParallelCrossEntropyMean(torch.autograd.Function):
             return (torch.zeros(ctx.hidden_shape, dtype=torch.bfloat16, device=dev),
                     torch.zeros(ctx.weight_shape, dtype=torch.bfloat16, device=dev),
                     None, None, None, None, None, None, None)
-        x, w, tgt, row_stat, dx, dw, assumed = (t.contiguous() for t in _take(ctx))
+        saved, contiguous = _take(ctx)
+        x, w, tgt, row_stat, dx, dw, assumed = saved if contiguous else [
+            t.contiguous() for t in saved]
         lib = _lib.load()
         go = grad_output.reshape(1)
         if go.dtype != torch.float32:
@@ -375,7 +377,8 @@ class _LMHeadVocabParallelCrossEntropy(torch.autograd.Function):
             return (torch.zeros(ctx.hidden_shape, dtype=torch.bfloat16, device=dev),
                     torch.zeros(ctx.weight_shape, dtype=torch.bfloat16, device=dev),
                     None, None, None, None, None, None)
-        x, w, tgt, row_stat = (t.contiguous() for t in _take(ctx))
+        saved, contiguous = _take(ctx)
+        x, w, tgt, row_stat = saved if contiguous else [t.contiguous() for t in saved]
         lib = _lib.load()
         dev = x.device
         n, hp = x.shape
