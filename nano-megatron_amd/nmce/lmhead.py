@@ -52,7 +52,7 @@ from . import _lib
 from .cross_entropy import (_check_hint, _check_target, _exchange_stats, _launch, _save,
                             _site_hint, _take, launch_target_check)
 from .mappings import (
-    copy_to_tensor_parallel_region,
+    copy_to_product,
     gather_from_sequence_parallel_region,
     gather_tokens_rank_major,
     targets_rank_major,
@@ -539,14 +539,14 @@ class FusedParallelLMHead(torch.nn.Module):
             if self.sequence_parallel:
                 x = gather_from_sequence_parallel_region(x, self.ctx)
             else:
-                x = copy_to_tensor_parallel_region(x, self.ctx)
+                x = copy_to_product(x, self.ctx)
             return x @ self.weight.t()
         start, end = self.vocab_range()
         if self.sequence_parallel:
             rows = gather_tokens_rank_major(x, self.ctx)
             target = targets_rank_major(labels, self.ctx.tp_size)
         else:
-            rows = copy_to_tensor_parallel_region(x, self.ctx)
+            rows = copy_to_product(x, self.ctx)
             target = labels
         dev = rows.device
         hint = self._hints.get(dev)

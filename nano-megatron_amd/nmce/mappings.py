@@ -37,15 +37,15 @@ def _use_host(t: torch.Tensor, group) -> bool:
     return t.device.type != "cpu" and dist.get_backend(group) == dist.Backend.GLOO
 
 
-def _all_reduce(t: torch.Tensor, group, world_size: int) -> torch.Tensor:
-    """Sum of ``t`` over the group (mappings.py:28-34)."""
+def _all_reduce(t: torch.Tensor, group, world_size: int, own: bool = False) -> torch.Tensor:
+    """Sum of ``t`` over the group (mappings.py:28-34); ``own``: in its storage."""
     if world_size == 1:
         return t
     if _use_host(t, group):
         h = t.cpu()
         dist.all_reduce(h, group=group)
         return h.to(t.device)
-    t = t.contiguous()
+    t = t.contiguous() if own else t.clone(memory_format=torch.contiguous_format)
     dist.all_reduce(t, group=group)
     return t
 
@@ -78,16 +78,19 @@ def _check_sequence_tensor(t: torch.Tensor) -> None:
 
 
 class _CopyToTensorParallelRegion(torch.autograd.Function):
-    """``f``: identity forward, all-reduce backward (mappings.py:83-94)."""
+    """``f``: identity forward, all-reduce backward (mappings.py:83-94). The incoming
+    gradient may be another node's too (a sum hands both of its inputs the same
+    tensor) or the caller's: it is copied first, unless ``own`` says that it is this
+    node's alone."""
 
     @staticmethod
-    def forward(ctx, x, group, world_size):
-        ctx.group, ctx.world_size = group, world_size
+    def forward(ctx, x, group, world_size, own=False):
+        ctx.group, ctx.world_size, ctx.own = group, world_size, own
         return x.view_as(x)
 
     @staticmethod
     def backward(ctx, grad):
-        return _all_reduce(grad, ctx.group, ctx.world_size), None, None
+        return _all_reduce(grad, ctx.group, ctx.world_size, ctx.own), None, None, None
 
 
 class _GatherFromSequenceParallelRegion(torch.autograd.Function):
@@ -143,7 +146,7 @@ class _ReduceFromTensorParallelRegion(torch.autograd.Function):
     def forward(ctx, x, group, world_size):
         if world_size == 1:
             return x.view_as(x)
-        return _all_reduce(x.clone(), group, world_size)
+        return _all_reduce(x, group, world_size)
 
     @staticmethod
     def backward(ctx, grad):
@@ -177,6 +180,12 @@ class _ReduceScatterToSequenceParallelRegion(torch.autograd.Function):
 def copy_to_tensor_parallel_region(x: torch.Tensor, ctx) -> torch.Tensor:
     """``f`` of mappings.py:83-94 for the group in ``ctx``."""
     return _CopyToTensorParallelRegion.apply(x, ctx.tp_group, ctx.tp_size)
+
+
+def copy_to_product(x: torch.Tensor, ctx) -> torch.Tensor:
+    """``f`` in front of one product and nothing else, whose backward makes the
+    gradient: it is reduced where it lies."""
+    return _CopyToTensorParallelRegion.apply(x, ctx.tp_group, ctx.tp_size, True)
 
 
 def gather_from_sequence_parallel_region(x: torch.Tensor, ctx) -> torch.Tensor:

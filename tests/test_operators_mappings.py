@@ -67,3 +67,41 @@ def test_one_rank_is_the_identity():
         assert torch.equal(g, torch.ones_like(x))
     with pytest.raises(ValueError, match="at least 2 dims"):
         nmce.reduce_scatter_to_sequence_parallel_region(torch.zeros(3), ctx)
+
+
+def _grad_worker(rank: int, world: int, port: int, out_dir: str) -> None:
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        import nmce
+        ctx = nmce.ParallelContext(rank=rank, world_size=world, tp_size=world, tp_rank=rank,
+                                   pp_size=1, pp_rank=0, dp_size=1, dp_rank=0)
+        x = torch.randn(3, 4, generator=torch.Generator().manual_seed(1)).requires_grad_(True)
+        u = torch.zeros(3, 4, requires_grad=True)
+        dy = torch.randn(3, 4, generator=torch.Generator().manual_seed(300 + rank))
+        kept = dy.clone()
+        y = nmce.copy_to_tensor_parallel_region(x, ctx)
+        first, = torch.autograd.grad(y, x, dy, retain_graph=True)
+        again, = torch.autograd.grad(y, x, dy)
+        assert torch.equal(dy, kept) and torch.equal(first, again)
+        # a sum hands the same gradient to both of its inputs
+        (nmce.copy_to_tensor_parallel_region(x, ctx) + u).backward(dy)
+        assert torch.equal(dy, kept)
+        np.savez(os.path.join(out_dir, f"rank{rank}.npz"), dy=kept.numpy(), first=first.numpy(),
+                 du=u.grad.numpy(), dx=x.grad.numpy())
+    finally:
+        dist.destroy_process_group()
+
+
+def test_the_copys_backward_leaves_the_incoming_gradient(tmp_path):
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    mp.start_processes(_grad_worker, args=(2, port, str(tmp_path)), nprocs=2, join=True,
+                       start_method="spawn")
+    ranks = [dict(np.load(tmp_path / f"rank{r}.npz")) for r in range(2)]
+    total = ranks[0]["dy"] + ranks[1]["dy"]
+    for res in ranks:
+        assert np.array_equal(res["first"], total) and np.array_equal(res["dx"], total)
+        assert np.array_equal(res["du"], res["dy"])
