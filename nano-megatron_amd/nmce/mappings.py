@@ -23,6 +23,10 @@ The embedding's rows, nonzero on one rank each, go the other way: ``g``
 (all-reduce forward, identity backward) or, under sequence parallelism, the
 reduce-scatter along the sequence, whose backward all-gathers.
 
+``f`` and ``g`` are each other's adjoints, and so are the gather and the
+reduce-scatter: a backward whose own derivative is wanted (``create_graph``) goes
+through the adjoint's Function, so second derivatives cross the ranks too.
+
 A gloo group gets host copies of device tensors: gloo collectives are only
 run on CPU tensors here.
 """
@@ -72,6 +76,11 @@ def _reduce_scatter_rows(t: torch.Tensor, group, world_size: int) -> torch.Tenso
     return out.to(t.device) if host else out
 
 
+def _differentiable(grad: torch.Tensor) -> bool:
+    """Whether a backward's own derivative is wanted (create_graph)."""
+    return torch.is_grad_enabled() and grad.requires_grad
+
+
 def _check_sequence_tensor(t: torch.Tensor) -> None:
     if t.dim() < 2:
         raise ValueError(f"sequence-parallel tensor needs at least 2 dims, got {tuple(t.shape)}")
@@ -90,6 +99,9 @@ class _CopyToTensorParallelRegion(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
+        if _differentiable(grad):
+            return (_ReduceFromTensorParallelRegion.apply(grad, ctx.group, ctx.world_size),
+                    None, None, None)
         return _all_reduce(grad, ctx.group, ctx.world_size, ctx.own), None, None, None
 
 
@@ -110,6 +122,9 @@ class _GatherFromSequenceParallelRegion(torch.autograd.Function):
     def backward(ctx, grad):
         if ctx.world_size == 1:
             return grad, None, None
+        if _differentiable(grad):
+            return (_ReduceScatterToSequenceParallelRegion.apply(grad, ctx.group, ctx.world_size),
+                    None, None)
         if grad.shape[1] % ctx.world_size:
             raise ValueError(f"sequence length {grad.shape[1]} is not divisible by TP size "
                              f"{ctx.world_size}")
@@ -144,12 +159,15 @@ class _ReduceFromTensorParallelRegion(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, group, world_size):
+        ctx.group, ctx.world_size = group, world_size
         if world_size == 1:
             return x.view_as(x)
         return _all_reduce(x, group, world_size)
 
     @staticmethod
     def backward(ctx, grad):
+        if _differentiable(grad) and ctx.world_size > 1:
+            return _CopyToTensorParallelRegion.apply(grad, ctx.group, ctx.world_size), None, None
         return grad, None, None
 
 
@@ -173,6 +191,9 @@ class _ReduceScatterToSequenceParallelRegion(torch.autograd.Function):
     def backward(ctx, grad):
         if ctx.world_size == 1:
             return grad, None, None
+        if _differentiable(grad):
+            return (_GatherFromSequenceParallelRegion.apply(grad, ctx.group, ctx.world_size),
+                    None, None)
         g = _all_gather_rows(grad.transpose(0, 1), ctx.group, ctx.world_size)
         return g.transpose(0, 1).contiguous(), None, None
 

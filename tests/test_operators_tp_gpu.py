@@ -143,3 +143,53 @@ def test_verification_ranks(ranks, whole, drafts):
             assert np.array_equal(res[f"{drafts}_{part}"], whole[f"{drafts}_{part}"])
         a, b = res[f"{drafts}_logprobs"], whole[f"{drafts}_logprobs"]
         assert np.all(np.abs(a - b) <= np.abs(b) * 2.0 ** -23 + 1e-12)
+
+
+def _second(rank, ctx, dev):
+    """The embedding's second derivatives on this rank's shard: d<dW, C> / d(dY)."""
+    import nmce
+    weight, tokens, grad, *_ = _inputs()
+    c = torch.randn(V, H, generator=torch.Generator().manual_seed(22))
+    per = V // ctx.tp_size
+    lo, hi = rank * per, (rank + 1) * per
+    res = {}
+    for sp in (False, True):
+        w = weight[lo:hi].to(dev).requires_grad_(True)
+        out = nmce.vocab_parallel_embedding(tokens.to(dev), w, lo, hi, ctx, scale=3.0,
+                                            sequence_parallel=sp)
+        part = S // ctx.tp_size
+        dy = grad[:, rank * part:(rank + 1) * part] if sp else grad
+        dy = dy.to(dev).requires_grad_(True)
+        dw, = torch.autograd.grad(out, w, dy, create_graph=True)
+        ddy, = torch.autograd.grad(dw, dy, c[lo:hi].to(dev))
+        res["sp" if sp else "tp"] = ddy.cpu().numpy()
+    return res
+
+
+def _second_worker(rank: int, world: int, port: int, out_dir: str) -> None:
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        torch.cuda.set_device(0)
+        import nmce
+        ctx = nmce.ParallelContext(rank=rank, world_size=world, tp_size=world, tp_rank=rank,
+                                   pp_size=1, pp_rank=0, dp_size=1, dp_rank=0)
+        np.savez(os.path.join(out_dir, f"rank{rank}.npz"),
+                 **_second(rank, ctx, torch.device("cuda:0")))
+        print(f"[rank {rank}] done", flush=True)
+    finally:
+        dist.destroy_process_group()
+
+
+def test_embeddings_second_derivatives_cross_the_ranks(tmp_path):
+    import nmce
+    world = 2
+    mp.start_processes(_second_worker, args=(world, _free_port(), str(tmp_path)), nprocs=world,
+                       join=True, start_method="spawn")
+    ranks = [dict(np.load(tmp_path / f"rank{r}.npz")) for r in range(world)]
+    whole = _second(0, nmce.ParallelContext.single(), torch.device("cuda:0"))
+    part = S // world
+    for r, res in enumerate(ranks):
+        assert np.array_equal(res["tp"], whole["tp"])
+        assert np.array_equal(res["sp"], whole["tp"][:, r * part:(r + 1) * part])
