@@ -155,7 +155,7 @@ class Int8ParallelLMHead(torch.nn.Module):
     def _apply(self, fn, recurse=True):
         # Casts are not for quantised buffers: what one changed goes back to its
         # former bits, on the device that the call moved it to.
-        held = dict(self._buffers)
+        held = {name: self._buffers[name] for name in ("weight_q", "weight_scale")}
         super()._apply(fn, recurse)
         for name, before in held.items():
             after = self._buffers[name]

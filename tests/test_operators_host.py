@@ -341,3 +341,12 @@ def test_verify_starts_that_would_overflow(lib):
     for start in ((1 << 63) - 1, (1 << 63) - 9, 1 << 62, 1 << 31, 11):
         b = L.VerifyBatch(p, None, p, p, p, None, 40, 10, 0, 0, 2, 3, 10, start, 20, 1.0, 0)
         assert lib.nmce_verify_stats(ctypes.addressof(b), p, None) == -2, start
+
+
+def test_a_cast_reaches_other_buffers_of_the_head():
+    import nmce
+    head = nmce.Int8ParallelLMHead(types.SimpleNamespace(vocab_size=8, n_embd=16),
+                                   nmce.ParallelContext.single())
+    head.register_buffer("mine", torch.ones(3))
+    head.to(torch.bfloat16)
+    assert head.mine.dtype == torch.bfloat16 and head.weight_scale.dtype == torch.float32
