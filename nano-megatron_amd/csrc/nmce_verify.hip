@@ -14,8 +14,9 @@
 // place where a running sum over the vocabulary passes a level: its neighbours'
 // borders are 1e-5 and less apart, so sums off by 1e-7 would give other ids for
 // the same numbers. The card's fp64 rate is that of its unpacked fp32; a logit costs
-// about 17 fp64 instructions and 10 others, whose issue bounds the pass over the
-// logits (64 x 11 rows of 128256 bf16 82 us, 2.2 TB/s, a third of the memory's rate).
+// 26 instructions, 16 of them fp64 sums and products, whose issue bounds the pass over
+// the logits (64 x 11 rows of 128256 bf16 82 us, 2.2 TB/s, a third of the memory's rate;
+// the VALU is busy 0.78 of the time).
 //
 // Three launches. The rows are cut into slabs of 8192 logits, a workgroup each,
 // which holds its slab in registers: (1) every slab's (maximum, sum of
