@@ -625,6 +625,51 @@ int nmce_verify_finish(const double* picked, const void* workspace, int64_t work
                        void* stream);
 
 /*
+ * Penalties, biases and masks on a vocabulary shard's logits, in one pass:
+ * out[b, i, :] from logits[b, i, :], i < rows (after the first i drafts). With
+ * count = how often an id is in output[b] and drafts[b][0 .. i - 1],
+ *   in prompt[b] or count > 0:  x <- x / r where x > 0, else x r
+ *   count > 0:                  x <- x - f count - p
+ *   then x + the id's biases in their order, and -inf unless it is allowed.
+ * What any of this touches is formed in 64 bits and rounded once; the rest is
+ * copied. Ids are global; one outside [0, vocab_total) stands for none.
+ *   - prompt [batch, n_prompt], output [batch, n_output], drafts [batch,
+ *     rows - 1], bias_ids and bias [batch, n_bias] with the given strides
+ *     between lists; repetition, frequency, presence [batch], or NULL: the
+ *     *_all value of each. r that is not a finite number above 0 is taken as 1.
+ *   - allowed: bit id % 32 of word id / 32, ceil(vocab_total / 32) words a row
+ *     at the given strides (in words), or NULL (all are).
+ *   - out may be logits (in place, the same strides): only touched and masked
+ *     elements are written. Otherwise the two must not overlap.
+ * n_bias at most NMCE_ADJUST_MAX_BIASES, n_output at most 2^29; batch x rows x
+ * ceil(vocab_local / 8192) at most 2^21.
+ */
+#define NMCE_ADJUST_MAX_BIASES 8192
+typedef struct nmce_adjust_batch {
+  const void* logits;
+  void* out;
+  const int64_t* prompt;
+  const int64_t* output;
+  const int64_t* drafts;
+  const int64_t* bias_ids;
+  const float* bias;
+  const uint32_t* allowed;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  int64_t logits_batch_stride, logits_row_stride;
+  int64_t out_batch_stride, out_row_stride;
+  int64_t prompt_stride, output_stride, drafts_stride, bias_ids_stride, bias_stride;
+  int64_t allowed_batch_stride, allowed_row_stride;
+  int64_t n_prompt, n_output, n_bias;
+  int64_t batch, rows;
+  int64_t vocab_local, vocab_start, vocab_total;
+  double repetition_all, frequency_all, presence_all;
+  int dtype;
+} nmce_adjust_batch;
+int nmce_adjust_logits(const nmce_adjust_batch* batch, void* stream);
+
+/*
  * The GEMM core of the fused path, exposed for testing and measurement (no
  * counterpart in the reference): c[i, j] = sum_l a[i, l] * b[j, l] for
  * i < m, j < n, l < k, with bf16 a [m, lda] and b [n, ldb], fp32

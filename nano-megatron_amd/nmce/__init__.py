@@ -19,6 +19,8 @@ Public API (mirrors nano_megatron/cross_entropy.py and parallel.py):
   of it (``FusedParallelLMHead.quantized()``).
 * ``vocab_parallel_verify_drafts(...)`` -- drafted tokens against the target's
   sharded logits, from given uniform numbers; with no drafts, sampling.
+* ``vocab_parallel_adjust_logits(...)`` -- penalties for repeated tokens, biases
+  and masks of allowed ids, on sharded logits.
 * ``copy_to_tensor_parallel_region`` / ``gather_from_sequence_parallel_region``
   / ``gather_tokens_rank_major`` -- the collectives on the LM head's input side
   (mappings.py:83-94, :109-120); ``reduce_from_tensor_parallel_region`` /
@@ -30,6 +32,7 @@ All loss compute runs in ``libnmce.so`` (hand-written HIP for gfx950) through th
 ABI in ``include/nmce.h``; there is no CPU or PyTorch fallback.
 """
 
+from .adjust import vocab_parallel_adjust_logits
 from .cross_entropy import (
     _VocabParallelCrossEntropy,
     validate_targets,
@@ -71,6 +74,7 @@ __all__ = [
     "reduce_scatter_to_sequence_parallel_region",
     "targets_rank_major",
     "validate_targets",
+    "vocab_parallel_adjust_logits",
     "vocab_parallel_cross_entropy",
     "vocab_parallel_embedding",
     "vocab_parallel_verify_drafts",

@@ -85,6 +85,7 @@ SIGNATURES: dict[str, tuple] = {
     "nmce_verify_masses": (_c_int, [_p, _p, _c_int, _p, _p, _p, _p, _p, _i64, _p]),
     "nmce_verify_pick": (_c_int, [_p, _p, _c_int, _c_int, _p, _i64, _p, _p, _p, _p]),
     "nmce_verify_finish": (_c_int, [_p, _p, _i64, _i64, _i64, _p, _p, _p]),
+    "nmce_adjust_logits": (_c_int, [_p, _p]),
     "nmce_gemm_nt_bf16": (_c_int, [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _c_int, _i64, _p]),
     "nmce_gemm_mn_bf16": (_c_int, [_c_int, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "nmce_lmhead_ce_bwd_layout": (_c_int, [_i64, _i64, _i64, _i64, _p]),
@@ -104,6 +105,24 @@ class VerifyBatch(ctypes.Structure):
                                              "drafts", "vocab_local", "vocab_start",
                                              "vocab_total")]
                 + [("temperature_all", ctypes.c_double), ("dtype", _c_int)])
+
+
+class AdjustBatch(ctypes.Structure):
+    """``nmce_adjust_batch`` of include/nmce.h."""
+
+    _fields_ = ([(name, _p) for name in ("logits", "out", "prompt", "output", "drafts", "bias_ids",
+                                         "bias", "allowed", "repetition", "frequency",
+                                         "presence")]
+                + [(name, _i64) for name in ("logits_batch_stride", "logits_row_stride",
+                                             "out_batch_stride", "out_row_stride",
+                                             "prompt_stride", "output_stride", "drafts_stride",
+                                             "bias_ids_stride", "bias_stride",
+                                             "allowed_batch_stride", "allowed_row_stride",
+                                             "n_prompt", "n_output", "n_bias", "batch", "rows",
+                                             "vocab_local", "vocab_start", "vocab_total")]
+                + [(name, ctypes.c_double) for name in ("repetition_all", "frequency_all",
+                                                        "presence_all")]
+                + [("dtype", _c_int)])
 
 
 NMCE_LMHEAD_LAYOUT_FIELDS = 10

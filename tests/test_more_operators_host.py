@@ -1,0 +1,126 @@
+"""What the adjusted logits, the top logits and their distillation refuse: no GPU needed."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from nmce import _lib as L
+    return L.load()
+
+
+class Fake:
+    """A stand-in that claims a GPU, for the checks behind the device's."""
+
+    def __init__(self, shape, dtype, device="cuda:0"):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype, torch.device(device)
+        self.is_cuda = self.device.type == "cuda"
+        self.requires_grad = False
+
+    def dim(self):
+        return len(self.shape)
+
+
+F32, BF, I64 = torch.float32, torch.bfloat16, torch.int64
+
+
+def _adjust_batch(**kw):
+    from nmce import _lib as L
+    p = 4096  # a fake, aligned device address; never dereferenced
+    a = L.AdjustBatch()
+    fields = dict(logits=p, out=2 * p, prompt=p, output=p, drafts=p, bias_ids=p, bias=p, allowed=p,
+                  logits_batch_stride=30, logits_row_stride=10, out_batch_stride=30,
+                  out_row_stride=10, prompt_stride=4, output_stride=4, drafts_stride=2,
+                  bias_ids_stride=4, bias_stride=4, allowed_batch_stride=3, allowed_row_stride=1,
+                  n_prompt=4, n_output=4, n_bias=4, batch=2, rows=3, vocab_local=10, vocab_start=0,
+                  vocab_total=10, repetition_all=1.0, dtype=0)
+    fields.update(kw)
+    for name, value in fields.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(dtype=2), -1), (dict(batch=-1), -2), (dict(rows=0), -2), (dict(vocab_local=0), -2),
+    (dict(vocab_start=-1), -2), (dict(vocab_start=1), -2), (dict(vocab_total=9), -2),
+    (dict(vocab_total=1 << 31), -2), (dict(n_prompt=-1), -2), (dict(n_output=-1), -2),
+    (dict(n_output=(1 << 29) + 1), -2), (dict(n_bias=-1), -2), (dict(n_bias=8193), -2),
+    (dict(batch=1 << 22), -2), (dict(rows=1 << 21), -2), (dict(logits=None), -4),
+    (dict(out=None), -4), (dict(prompt=None), -4), (dict(output=None), -4), (dict(drafts=None), -4),
+    (dict(bias_ids=None), -4), (dict(bias=None), -4), (dict(logits=4098), -3),
+    (dict(out=4097, dtype=1), -3), (dict(allowed=4098), -3),
+    (dict(out=4096, out_row_stride=11), -2), (dict(out=4096, out_batch_stride=31), -2),
+    (dict(batch=0, logits=None), 0)])
+def test_adjust_argument_errors_before_launch(lib, change, status):
+    a = _adjust_batch(**change)
+    assert lib.nmce_adjust_logits(ctypes.addressof(a), None) == status
+    assert lib.nmce_adjust_logits(None, None) == -4
+
+
+def test_adjust_refuses_shapes_and_types():
+    import nmce
+    from nmce import adjust
+    ctx = nmce.ParallelContext.single()
+    good = dict(logits=Fake((2, 3, 40), F32), vocab_start=0, vocab_end=40, ctx=ctx,
+                prompt=Fake((2, 9), I64), output=Fake((2, 0), I64), drafts=Fake((2, 2), I64),
+                penalties=(("repetition_penalty", 1.5), ("frequency_penalty", Fake((2,), F32)),
+                           ("presence_penalty", 0.0)),
+                bias_ids=Fake((2, 4), I64), bias_values=Fake((2, 4), F32),
+                allowed=Fake((2, 3, 2), torch.int32))
+
+    def check(**kw):
+        adjust._check_adjust(**{**good, **kw})
+
+    check()
+    check(prompt=None, output=None, bias_ids=None, bias_values=None, allowed=None)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        check(logits=Fake((2, 3, 40), F32, "cpu"))
+    with pytest.raises(TypeError, match="unsupported"):
+        check(logits=Fake((2, 3, 40), torch.float16))
+    for shape in ((2, 40), (2, 0, 40), (2, 3, 0), (1, 2, 3, 40)):
+        with pytest.raises(ValueError, match="must be"):
+            check(logits=Fake(shape, F32))
+    for start, end in ((0, 41), (1, 40), (-1, 39), (1, 41)):
+        with pytest.raises(ValueError, match="shard"):
+            check(vocab_start=start, vocab_end=end)
+    with pytest.raises(ValueError, match="draft_tokens"):
+        check(drafts=None)
+    with pytest.raises(ValueError, match="come together"):
+        check(bias_ids=None)
+    with pytest.raises(ValueError, match="come together"):
+        check(bias_values=None)
+    for name, shape, dtype in (("prompt", (3, 9), I64), ("prompt", (9,), I64),
+                               ("output", (2,), I64), ("drafts", (2, 3), I64),
+                               ("bias_values", (2, 5), F32), ("allowed", (2, 3, 1), torch.int32),
+                               ("allowed", (2, 1, 2), torch.int32)):
+        with pytest.raises(ValueError, match="must be"):
+            check(**{name: Fake(shape, dtype)})
+    for name, shape, dtype in (("prompt", (2, 9), torch.int32), ("output", (2, 1), F32),
+                               ("drafts", (2, 2), torch.int32), ("bias_ids", (2, 4), torch.int32),
+                               ("bias_values", (2, 4), BF), ("allowed", (2, 3, 2), I64)):
+        with pytest.raises(TypeError, match="must be"):
+            check(**{name: Fake(shape, dtype)})
+        with pytest.raises(RuntimeError, match="on cuda:1"):
+            check(**{name: Fake(shape, dtype, "cuda:1")})
+    with pytest.raises(ValueError, match="at most 8192"):
+        check(bias_ids=Fake((2, 8193), I64), bias_values=Fake((2, 8193), F32))
+    for name, value in (("repetition_penalty", 0.0), ("repetition_penalty", -1.0),
+                        ("repetition_penalty", float("nan")),
+                        ("frequency_penalty", float("inf")), ("presence_penalty", float("nan"))):
+        with pytest.raises(ValueError, match=name):
+            check(penalties=((name, value),))
+    with pytest.raises(ValueError, match="must be"):
+        check(penalties=(("frequency_penalty", Fake((3,), F32)),))
+    with pytest.raises(TypeError, match="must be"):
+        check(penalties=(("frequency_penalty", Fake((2,), torch.float64)),))
+
+
+def test_adjust_has_no_cpu_path():
+    import nmce
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nmce.vocab_parallel_adjust_logits(torch.zeros(1, 1, 8), 0, 8, nmce.ParallelContext.single())
