@@ -670,6 +670,28 @@ typedef struct nmce_adjust_batch {
 int nmce_adjust_logits(const nmce_adjust_batch* batch, void* stream);
 
 /*
+ * The k largest logits of each row of a vocabulary shard with their ids, in order
+ * (of equal ones the lowest id first; NaN above +inf; -0 as 0), and the row's
+ * log sum exp(x / temperature). k at most NMCE_TOP_MAX_K, n_rows at most 2^22.
+ *   - list NULL: the results. values [n_rows, k] in the logits' type, ids
+ *     [n_rows, k], log_normalizer [n_rows]; k is at most vocab_local.
+ *   - otherwise list [n_rows, k + 1]: this shard's part (fewer than k entries
+ *     where it has fewer columns), of which nmce_top_merge takes the ranks',
+ *     [ranks, n_rows, k + 1], to the results.
+ * logits [n_rows, ld] is aligned to its element. The workspace (16-byte aligned)
+ * belongs to this call until it is done on the stream.
+ */
+#define NMCE_TOP_MAX_K 512
+int64_t nmce_top_workspace_bytes(int64_t n_rows, int64_t vocab_local, int k);
+int nmce_top_logits(const void* logits, int dtype, int64_t n_rows, int64_t vocab_local, int64_t ld,
+                    int64_t vocab_start, int k, double temperature, int64_t* list, void* values,
+                    int64_t* ids, float* log_normalizer, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+int nmce_top_merge(const int64_t* lists, int ranks, int dtype, int64_t n_rows, int k,
+                   double temperature, void* values, int64_t* ids, float* log_normalizer,
+                   void* stream);
+
+/*
  * The GEMM core of the fused path, exposed for testing and measurement (no
  * counterpart in the reference): c[i, j] = sum_l a[i, l] * b[j, l] for
  * i < m, j < n, l < k, with bf16 a [m, lda] and b [n, ldb], fp32

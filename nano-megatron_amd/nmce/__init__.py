@@ -21,6 +21,8 @@ Public API (mirrors nano_megatron/cross_entropy.py and parallel.py):
   sharded logits, from given uniform numbers; with no drafts, sampling.
 * ``vocab_parallel_adjust_logits(...)`` -- penalties for repeated tokens, biases
   and masks of allowed ids, on sharded logits.
+* ``vocab_parallel_top_logits(...)`` -- the largest logits of each row, their ids
+  and the row's log-normaliser.
 * ``copy_to_tensor_parallel_region`` / ``gather_from_sequence_parallel_region``
   / ``gather_tokens_rank_major`` -- the collectives on the LM head's input side
   (mappings.py:83-94, :109-120); ``reduce_from_tensor_parallel_region`` /
@@ -54,6 +56,7 @@ from .mappings import (
     targets_rank_major,
 )
 from .parallel import ParallelContext, divide, vocab_range
+from .top import vocab_parallel_top_logits
 from .verify import vocab_parallel_verify_drafts
 
 __all__ = [
@@ -77,6 +80,7 @@ __all__ = [
     "vocab_parallel_adjust_logits",
     "vocab_parallel_cross_entropy",
     "vocab_parallel_embedding",
+    "vocab_parallel_top_logits",
     "vocab_parallel_verify_drafts",
     "vocab_range",
 ]

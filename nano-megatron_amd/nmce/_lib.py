@@ -86,6 +86,11 @@ SIGNATURES: dict[str, tuple] = {
     "nmce_verify_pick": (_c_int, [_p, _p, _c_int, _c_int, _p, _i64, _p, _p, _p, _p]),
     "nmce_verify_finish": (_c_int, [_p, _p, _i64, _i64, _i64, _p, _p, _p]),
     "nmce_adjust_logits": (_c_int, [_p, _p]),
+    "nmce_top_workspace_bytes": (_i64, [_i64, _i64, _c_int]),
+    "nmce_top_logits": (_c_int, [_p, _c_int, _i64, _i64, _i64, _i64, _c_int, ctypes.c_double, _p,
+                                 _p, _p, _p, _p, _i64, _p]),
+    "nmce_top_merge": (_c_int, [_p, _c_int, _c_int, _i64, _c_int, ctypes.c_double, _p, _p, _p,
+                                _p]),
     "nmce_gemm_nt_bf16": (_c_int, [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _c_int, _i64, _p]),
     "nmce_gemm_mn_bf16": (_c_int, [_c_int, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "nmce_lmhead_ce_bwd_layout": (_c_int, [_i64, _i64, _i64, _i64, _p]),

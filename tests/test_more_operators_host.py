@@ -124,3 +124,68 @@ def test_adjust_has_no_cpu_path():
     import nmce
     with pytest.raises(RuntimeError, match="no CPU path"):
         nmce.vocab_parallel_adjust_logits(torch.zeros(1, 1, 8), 0, 8, nmce.ParallelContext.single())
+
+
+def test_top_argument_errors_before_launch(lib):
+    p = 4096
+    size = lib.nmce_top_workspace_bytes
+    ws = size(4, 100, 10)
+    assert ws > 0 and size(0, 100, 10) >= 0
+    assert size(-1, 100, 10) == size((1 << 22) + 1, 100, 10) == size(4, 0, 10) == -1
+    assert size(4, 1 << 31, 10) == size(4, 100, 0) == size(4, 100, 513) == -1
+
+    def top(logits=p, dtype=0, n=4, v=100, ld=100, start=0, k=10, t=1.0, lists=None, values=p,
+            ids=p, norm=p, space=p, size_=ws):
+        return lib.nmce_top_logits(logits, dtype, n, v, ld, start, k, t, lists, values, ids, norm,
+                                   space, size_, None)
+
+    assert top(dtype=2) == -1
+    for bad in (dict(n=-1), dict(n=(1 << 22) + 1), dict(v=0), dict(v=1 << 31), dict(ld=99),
+                dict(start=-1), dict(start=(1 << 31) - 100), dict(k=0), dict(k=513), dict(k=101),
+                dict(t=0.0), dict(t=-1.0), dict(t=float("nan")), dict(t=float("inf"))):
+        assert top(**bad) == -2, bad
+    assert top(logits=p + 2) == top(logits=p + 1, dtype=1) == -3
+    for name in ("logits", "values", "ids", "norm"):
+        assert top(**{name: None}) == -4
+    assert top(space=None) == top(space=p + 8) == top(size_=ws - 1) == -6
+    assert top(n=0, logits=None) == 0
+    assert top(lists=p, k=101, values=None, ids=None, norm=None, size_=0) == -6
+    merge = lib.nmce_top_merge
+    assert merge(p, 2, 3, 4, 10, 1.0, p, p, p, None) == -1
+    assert merge(p, 2, 0, -1, 10, 1.0, p, p, p, None) == -2
+    assert merge(p, 2, 0, 4, 513, 1.0, p, p, p, None) == -2
+    assert merge(p, 0, 0, 4, 10, 1.0, p, p, p, None) == -5
+    assert merge(None, 2, 0, 4, 10, 1.0, p, p, p, None) == -4
+    assert merge(None, 2, 0, 0, 10, 1.0, None, p, p, None) == 0
+
+
+def test_top_refuses_shapes_and_types():
+    import nmce
+    from nmce import top
+    ctx = nmce.ParallelContext.single()
+
+    def check(logits=Fake((2, 40), F32), k=5, start=0, end=40, ctx=ctx, t=1.0):
+        top._check_top(logits, k, start, end, ctx, t)
+
+    check()
+    check(Fake((40,), BF))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        check(Fake((2, 40), F32, "cpu"))
+    with pytest.raises(TypeError, match="unsupported"):
+        check(Fake((2, 40), torch.float16))
+    for shape in ((), (2, 0)):
+        with pytest.raises(ValueError, match="must be"):
+            check(Fake(shape, F32), end=0)
+    for start, end in ((0, 41), (1, 41), (-1, 39)):
+        with pytest.raises(ValueError, match="shard"):
+            check(start=start, end=end)
+    for k in (0, -3, 41):
+        with pytest.raises(ValueError, match="k must be"):
+            check(k=k)
+    with pytest.raises(ValueError, match="k must be"):
+        check(Fake((2, 1000), F32), k=513, end=1000)
+    for t in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            check(t=t)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nmce.vocab_parallel_top_logits(torch.zeros(2, 8), 2, 0, 8, ctx)
