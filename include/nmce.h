@@ -692,6 +692,64 @@ int nmce_top_merge(const int64_t* lists, int ranks, int dtype, int64_t n_rows, i
                    void* stream);
 
 /*
+ * Distillation from a teacher's top logits. With q = softmax(z / T) of a student's
+ * row over the whole vocabulary and the teacher's p at its k listed ids,
+ *   p = exp(t / T - teacher_log_normalizer), r = max(1 - sum p, 0), or, with
+ *   teacher_log_normalizer NULL, p = softmax(t / T) over the list, r = 0:
+ *   loss = sum p (log p - log q) + r (log r - log s)
+ * where s is the sum of q outside the list (one class).
+ *   - An id outside [0, vocab_total) is padding. A row without any other (or,
+ *     with NULL, whose list holds only -inf) has no teacher: loss and gradient
+ *     0, whatever its logits are. An id that comes several times adds up its p.
+ *   - Where the student gives everything outside the list nothing (-inf), the
+ *     rest has no term. A student's row of only -inf, or with +inf or NaN: NaN.
+ * logits [n_rows, ld] of this shard, teacher_logits and teacher_ids [n_rows, k]
+ * at their own row strides, teacher_log_normalizer [n_rows]; aligned to their
+ * elements. k at most NMCE_DISTILL_MAX_K, n_rows at most 2^22, vocab_total below
+ * 2^31 - 1, temperature from 1e-6 to 1e6.
+ */
+#define NMCE_DISTILL_MAX_K 1024
+typedef struct nmce_distill_batch {
+  const void* logits;
+  const void* teacher_logits;
+  const int64_t* teacher_ids;
+  const float* teacher_log_normalizer;
+  int64_t ld, teacher_ld, ids_ld;
+  int64_t n_rows;
+  int64_t vocab_local, vocab_start, vocab_total;
+  double temperature;
+  int k;
+  int dtype, teacher_dtype;
+} nmce_distill_batch;
+
+/* What a forward leaves for its backward, in bytes (16-byte aligned). */
+int64_t nmce_distill_state_bytes(int64_t n_rows, int k);
+
+/*
+ * The forward in two steps: this shard's statistics, [n_rows, 5] doubles (with
+ * several ranks gather them to [ranks, n_rows, 5]), and the per-token fp32 loss
+ * from them, with what the backward needs, both in `state`.
+ */
+int nmce_distill_stats(const nmce_distill_batch* batch, void* state, int64_t state_bytes,
+                       double* stats, void* stream);
+int nmce_distill_combine(void* state, int64_t state_bytes, int64_t n_rows, int k,
+                         double temperature, const double* stats, int ranks, float* loss,
+                         void* stream);
+
+/*
+ * grad = d loss / d logits of each row times grad_output[row * gout_stride] /
+ * gout_div, over this shard; the state is the forward's. grad may be logits
+ * (ld_grad == ld), else the two must not overlap. With `assumed` (one float; the
+ * gradient is there for that upstream value) nothing is done where
+ * grad_output[0] equals it, and observed[0] gets grad_output[0].
+ */
+int nmce_distill_bwd(const void* logits, void* grad, int dtype, int64_t n_rows,
+                     int64_t vocab_local, int64_t ld, int64_t ld_grad, int k, double temperature,
+                     void* state, int64_t state_bytes, const float* grad_output,
+                     int64_t gout_stride, float gout_div, const float* assumed, float* observed,
+                     void* stream);
+
+/*
  * The GEMM core of the fused path, exposed for testing and measurement (no
  * counterpart in the reference): c[i, j] = sum_l a[i, l] * b[j, l] for
  * i < m, j < n, l < k, with bf16 a [m, lda] and b [n, ldb], fp32

@@ -110,24 +110,6 @@ __device__ __forceinline__ void lane_fold(float& m, float& a, const float* f) {
   else online_fold<K>(m, a, f);
 }
 
-// Byte offset of p from the previous 16-byte boundary, in elements of T.
-template <typename T>
-__device__ __forceinline__ int64_t head_elems(const T* p, int64_t v) {
-  const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u);
-  int64_t h = static_cast<int64_t>(((16u - mis) & 15u) / sizeof(T));
-  return h < v ? h : v;
-}
-
-// Column of the edge element that lane `tid` holds of a row whose 16-byte
-// body (nvec vectors) starts at column `head`: the elements before it, then
-// the ones past it; -1 for every other lane.
-template <int EPV>
-__device__ __forceinline__ int edge_column(int tid, int head, int nvec, int V) {
-  const int body_end = head + nvec * EPV;
-  if (tid < head) return tid;
-  return tid >= EPV && tid - EPV < V - body_end ? body_end + tid - EPV : -1;
-}
-
 // kFinal = false: per-shard statistics (out0 = row max, out1 = row exp-sum
 //                  minus one, out2 = raw target logit or 0 when the shard does
 //                  not own it).

@@ -71,6 +71,32 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // token's loss.)
 __device__ __forceinline__ float exp_shift(float x, float m) { return exp2_hw((x - m) * kLog2e); }
 
+constexpr double kLog2e64 = 1.4426950408889634;
+
+// 2^z for z <= 0, -inf or NaN (which it stays). The nearest integer n is taken off
+// (adding 1.5 2^52 leaves it in the low bits), 2^f is the polynomial that equals it
+// at the ten Chebyshev points of [-1/2, 1/2] (1.9e-14 relative at most), and n goes
+// back into the exponent; below 2^-1022 the result is 0. (What the exponent's sum is
+// there does not matter, and a NaN's low bits are 0.)
+__device__ __forceinline__ double exp2_64(double z) {
+  constexpr double kMagic = 6755399441055744.0;
+  const double s = z + kMagic;
+  const double f = z - (s - kMagic);
+  double p = 0x1.b6571de2f2351p-24;
+  p = fma(p, f, 0x1.63ef969a64d3cp-20);
+  p = fma(p, f, 0x1.ffcb76789860fp-17);
+  p = fma(p, f, 0x1.43088e257f341p-13);
+  p = fma(p, f, 0x1.5d87fe908f88ap-10);
+  p = fma(p, f, 0x1.3b2ab72b175eep-7);
+  p = fma(p, f, 0x1.c6b08d7044119p-5);
+  p = fma(p, f, 0x1.ebfbdff8149f2p-3);
+  p = fma(p, f, 0x1.62e42fefa39f7p-1);
+  p = fma(p, f, 0x1.000000000003dp+0);
+  const uint32_t hi = static_cast<uint32_t>(__double2hiint(p)) +
+                      (static_cast<uint32_t>(__double2loint(s)) << 20);
+  return z < -1022.0 ? 0.0 : __hiloint2double(static_cast<int>(hi), __double2loint(p));
+}
+
 // ---- row statistics as (max, sum - 1) --------------------------------------
 // A set of values x_j is summarised by m = max_j x_j and
 // t = sum_j exp(x_j - m) - 1: the maximum's own term, exactly 1, is left out.
@@ -200,6 +226,24 @@ __device__ __forceinline__ u32x4 load_stream(const u32x4* p) {
 }
 __device__ __forceinline__ void store_stream(u32x4* p, const u32x4& v) {
   __builtin_nontemporal_store(v, p);
+}
+
+// Byte offset of p from the previous 16-byte boundary, in elements of T.
+template <typename T>
+__device__ __forceinline__ int64_t head_elems(const T* p, int64_t v) {
+  const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u);
+  int64_t h = static_cast<int64_t>(((16u - mis) & 15u) / sizeof(T));
+  return h < v ? h : v;
+}
+
+// Column of the edge element that lane `tid` holds of a row whose 16-byte
+// body (nvec vectors) starts at column `head`: the elements before it, then
+// the ones past it; -1 for every other lane.
+template <int EPV>
+__device__ __forceinline__ int edge_column(int tid, int head, int nvec, int V) {
+  const int body_end = head + nvec * EPV;
+  if (tid < head) return tid;
+  return tid >= EPV && tid - EPV < V - body_end ? body_end + tid - EPV : -1;
 }
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));

@@ -38,32 +38,7 @@ namespace {
 
 constexpr int kSlab = 8192;               // logits of a workgroup
 constexpr int kStat = 4;                  // doubles of a slab's statistics
-constexpr double kLog2e64 = 1.4426950408889634;
 constexpr float kInf = __builtin_huge_valf();
-
-// 2^z for z <= 0, -inf or NaN (which it stays). The nearest integer n is taken off
-// (adding 1.5 2^52 leaves it in the low bits), 2^f is the polynomial that equals it
-// at the ten Chebyshev points of [-1/2, 1/2] (1.9e-14 relative at most), and n goes
-// back into the exponent; below 2^-1022 the result is 0. (What the exponent's sum is
-// there does not matter, and a NaN's low bits are 0.)
-__device__ __forceinline__ double exp2_64(double z) {
-  constexpr double kMagic = 6755399441055744.0;
-  const double s = z + kMagic;
-  const double f = z - (s - kMagic);
-  double p = 0x1.b6571de2f2351p-24;
-  p = fma(p, f, 0x1.63ef969a64d3cp-20);
-  p = fma(p, f, 0x1.ffcb76789860fp-17);
-  p = fma(p, f, 0x1.43088e257f341p-13);
-  p = fma(p, f, 0x1.5d87fe908f88ap-10);
-  p = fma(p, f, 0x1.3b2ab72b175eep-7);
-  p = fma(p, f, 0x1.c6b08d7044119p-5);
-  p = fma(p, f, 0x1.ebfbdff8149f2p-3);
-  p = fma(p, f, 0x1.62e42fefa39f7p-1);
-  p = fma(p, f, 0x1.000000000003dp+0);
-  const uint32_t hi = static_cast<uint32_t>(__double2hiint(p)) +
-                      (static_cast<uint32_t>(__double2loint(s)) << 20);
-  return z < -1022.0 ? 0.0 : __hiloint2double(static_cast<int>(hi), __double2loint(p));
-}
 
 // exp((x - m) / T) with c = log2(e) / T > 0; a masked logit's (-inf) is 0, for which
 // m has to be a number (finite_max).

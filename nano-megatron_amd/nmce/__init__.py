@@ -23,6 +23,8 @@ Public API (mirrors nano_megatron/cross_entropy.py and parallel.py):
   and masks of allowed ids, on sharded logits.
 * ``vocab_parallel_top_logits(...)`` -- the largest logits of each row, their ids
   and the row's log-normaliser.
+* ``vocab_parallel_distillation_loss(...)`` -- the divergence from a teacher's top
+  logits, with its gradient.
 * ``copy_to_tensor_parallel_region`` / ``gather_from_sequence_parallel_region``
   / ``gather_tokens_rank_major`` -- the collectives on the LM head's input side
   (mappings.py:83-94, :109-120); ``reduce_from_tensor_parallel_region`` /
@@ -40,6 +42,7 @@ from .cross_entropy import (
     validate_targets,
     vocab_parallel_cross_entropy,
 )
+from .distill import vocab_parallel_distillation_loss
 from .embedding import VocabParallelEmbedding, vocab_parallel_embedding
 from .int8 import Int8ParallelLMHead, int8_linear, quantize_rows
 from .lmhead import (
@@ -79,6 +82,7 @@ __all__ = [
     "validate_targets",
     "vocab_parallel_adjust_logits",
     "vocab_parallel_cross_entropy",
+    "vocab_parallel_distillation_loss",
     "vocab_parallel_embedding",
     "vocab_parallel_top_logits",
     "vocab_parallel_verify_drafts",

@@ -29,7 +29,8 @@ BUILD_DIR = PROJECT_DIR / "_build"
 LIB_PATH = PKG_DIR / "libnmce.so"
 
 SOURCES = ["nmce_ce.hip", "nmce_lmhead.hip", "nmce_embed.hip", "nmce_int8.hip",
-           "nmce_verify.hip", "nmce_adjust.hip", "nmce_top.hip"]
+           "nmce_verify.hip", "nmce_adjust.hip", "nmce_top.hip",
+           "nmce_distill.hip"]
 EXT_SOURCE = "nmce_autograd.cpp"
 EXT_NAME = "_nmce_autograd"
 EXT_PATH = PKG_DIR / (EXT_NAME + sysconfig.get_config_var("EXT_SUFFIX"))

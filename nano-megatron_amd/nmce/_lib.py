@@ -91,6 +91,12 @@ SIGNATURES: dict[str, tuple] = {
                                  _p, _p, _p, _p, _i64, _p]),
     "nmce_top_merge": (_c_int, [_p, _c_int, _c_int, _i64, _c_int, ctypes.c_double, _p, _p, _p,
                                 _p]),
+    "nmce_distill_state_bytes": (_i64, [_i64, _c_int]),
+    "nmce_distill_stats": (_c_int, [_p, _p, _i64, _p, _p]),
+    "nmce_distill_combine": (_c_int, [_p, _i64, _i64, _c_int, ctypes.c_double, _p, _c_int, _p,
+                                      _p]),
+    "nmce_distill_bwd": (_c_int, [_p, _p, _c_int, _i64, _i64, _i64, _i64, _c_int, ctypes.c_double,
+                                  _p, _i64, _p, _i64, ctypes.c_float, _p, _p, _p]),
     "nmce_gemm_nt_bf16": (_c_int, [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _c_int, _i64, _p]),
     "nmce_gemm_mn_bf16": (_c_int, [_c_int, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "nmce_lmhead_ce_bwd_layout": (_c_int, [_i64, _i64, _i64, _i64, _p]),
@@ -128,6 +134,17 @@ class AdjustBatch(ctypes.Structure):
                 + [(name, ctypes.c_double) for name in ("repetition_all", "frequency_all",
                                                         "presence_all")]
                 + [("dtype", _c_int)])
+
+
+class DistillBatch(ctypes.Structure):
+    """``nmce_distill_batch`` of include/nmce.h."""
+
+    _fields_ = ([(name, _p) for name in ("logits", "teacher_logits", "teacher_ids",
+                                         "teacher_log_normalizer")]
+                + [(name, _i64) for name in ("ld", "teacher_ld", "ids_ld", "n_rows",
+                                             "vocab_local", "vocab_start", "vocab_total")]
+                + [("temperature", ctypes.c_double)]
+                + [(name, _c_int) for name in ("k", "dtype", "teacher_dtype")])
 
 
 NMCE_LMHEAD_LAYOUT_FIELDS = 10

@@ -189,3 +189,127 @@ def test_top_refuses_shapes_and_types():
             check(t=t)
     with pytest.raises(RuntimeError, match="no CPU path"):
         nmce.vocab_parallel_top_logits(torch.zeros(2, 8), 2, 0, 8, ctx)
+
+
+def _distill_batch(**kw):
+    from nmce import _lib as L
+    p = 4096
+    a = L.DistillBatch()
+    fields = dict(logits=p, teacher_logits=p, teacher_ids=p, teacher_log_normalizer=p, ld=100,
+                  teacher_ld=8, ids_ld=8, n_rows=4, vocab_local=100, vocab_start=0,
+                  vocab_total=100, temperature=1.0, k=8, dtype=0, teacher_dtype=0)
+    fields.update(kw)
+    for name, value in fields.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(dtype=2), -1), (dict(teacher_dtype=-1), -1), (dict(n_rows=-1), -2),
+    (dict(n_rows=(1 << 22) + 1), -2), (dict(vocab_local=0), -2), (dict(vocab_start=-1), -2),
+    (dict(vocab_start=1), -2), (dict(vocab_total=99), -2), (dict(vocab_total=(1 << 31) - 1), -2),
+    (dict(ld=99), -2), (dict(k=0), -2), (dict(k=1025), -2), (dict(teacher_ld=-1), -2),
+    (dict(ids_ld=-1), -2), (dict(temperature=0.0), -2), (dict(temperature=1e-7), -2),
+    (dict(temperature=float("nan")), -2), (dict(temperature=1e7), -2), (dict(logits=None), -4),
+    (dict(teacher_logits=None), -4), (dict(teacher_ids=None), -4), (dict(logits=4098), -3),
+    (dict(logits=4097, dtype=1), -3), (dict(teacher_logits=4098), -3),
+    (dict(n_rows=0, logits=None), 0)])
+def test_distill_argument_errors_before_launch(lib, change, status):
+    p, size = 4096, lib.nmce_distill_state_bytes(4, 8)
+    a = _distill_batch(**change)
+    assert lib.nmce_distill_stats(ctypes.addressof(a), p, size, p, None) == status
+
+
+def test_distill_steps_refuse_before_launch(lib):
+    p, state = 4096, lib.nmce_distill_state_bytes
+    size = state(4, 8)
+    assert size > 0 and state(0, 8) >= 0
+    assert state(-1, 8) == state((1 << 22) + 1, 8) == state(4, 0) == state(4, 1025) == -1
+    good = _distill_batch()
+    stats = lib.nmce_distill_stats
+    assert stats(None, p, size, p, None) == -4
+    assert stats(ctypes.addressof(good), p, size, None, None) == -4
+    for space, bytes_ in ((None, size), (p + 8, size), (p, size - 1)):
+        assert stats(ctypes.addressof(good), space, bytes_, p, None) == -6
+    combine = lib.nmce_distill_combine
+    assert combine(p, size, -1, 8, 1.0, p, 1, p, None) == -2
+    assert combine(p, size, 4, 0, 1.0, p, 1, p, None) == -2
+    assert combine(p, size, 4, 8, 0.0, p, 1, p, None) == -2
+    assert combine(p, size, 4, 8, 1.0, p, 0, p, None) == -5
+    assert combine(p, size, 4, 8, 1.0, None, 1, p, None) == -4
+    assert combine(p, size, 4, 8, 1.0, p, 1, None, None) == -4
+    assert combine(p, size - 1, 4, 8, 1.0, p, 1, p, None) == -6
+    assert combine(None, 0, 0, 8, 1.0, None, 1, None, None) == 0
+
+    def bwd(x=p, g=2 * p, dtype=0, n=4, v=100, ld=100, ldg=100, k=8, t=1.0, space=p, bytes_=size,
+            go=p, stride=0, div=4.0):
+        return lib.nmce_distill_bwd(x, g, dtype, n, v, ld, ldg, k, t, space, bytes_, go, stride,
+                                    div, None, None, None)
+
+    assert bwd(dtype=3) == -1
+    for bad in (dict(n=-1), dict(v=0), dict(ld=99), dict(ldg=99), dict(k=0), dict(k=1025),
+                dict(stride=-1), dict(div=0.0), dict(div=float("nan")), dict(t=0.0),
+                dict(g=p, ldg=101)):
+        assert bwd(**bad) == -2, bad
+    assert bwd(x=None) == bwd(g=None) == bwd(go=None) == -4
+    assert bwd(x=p + 2) == bwd(g=p + 1, dtype=1) == -3
+    assert bwd(space=None) == bwd(space=p + 4) == bwd(bytes_=size - 1) == -6
+    assert bwd(n=0, x=None) == 0
+
+
+def test_distillation_refuses_shapes_and_types():
+    import nmce
+    from nmce import distill
+    ctx = nmce.ParallelContext.single()
+    good = dict(logits=Fake((2, 3, 40), F32), teacher_logits=Fake((2, 3, 5), BF),
+                teacher_ids=Fake((2, 3, 5), I64), normalizer=Fake((2, 3), F32), vocab_start=0,
+                vocab_end=40, ctx=ctx, temperature=1.0, reduction="mean")
+
+    def check(**kw):
+        distill._check_distillation(**{**good, **kw})
+
+    check()
+    check(normalizer=None, reduction="none", temperature=2)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        check(logits=Fake((2, 3, 40), F32, "cpu"))
+    with pytest.raises(TypeError, match="unsupported"):
+        check(logits=Fake((2, 3, 40), torch.float16))
+    with pytest.raises(ValueError, match="must be"):
+        check(logits=Fake((2, 3, 0), F32), vocab_end=0)
+    for start, end in ((0, 41), (1, 41), (-1, 39)):
+        with pytest.raises(ValueError, match="shard"):
+            check(vocab_start=start, vocab_end=end)
+    for shape in ((2, 3), (3, 2, 5), (6, 5), (5,)):
+        with pytest.raises(ValueError, match="not a list"):
+            check(teacher_logits=Fake(shape, F32))
+    for k in (0, 1025):
+        with pytest.raises(ValueError, match="1 to 1024"):
+            check(teacher_logits=Fake((2, 3, k), F32), teacher_ids=Fake((2, 3, k), I64))
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        check(teacher_logits=Fake((2, 3, 5), torch.float16))
+    with pytest.raises(TypeError, match="int64"):
+        check(teacher_ids=Fake((2, 3, 5), torch.int32))
+    with pytest.raises(ValueError, match="must be"):
+        check(teacher_ids=Fake((2, 3, 4), I64))
+    with pytest.raises(ValueError, match="must be"):
+        check(normalizer=Fake((2, 3, 1), F32))
+    with pytest.raises(TypeError, match="must be"):
+        check(normalizer=Fake((2, 3), BF))
+    for name, shape, dtype in (("teacher_logits", (2, 3, 5), F32), ("teacher_ids", (2, 3, 5), I64),
+                               ("normalizer", (2, 3), F32)):
+        with pytest.raises(RuntimeError, match="on cuda:1"):
+            check(**{name: Fake(shape, dtype, "cuda:1")})
+    for t in (0.0, -1.0, 1e-7, 1e7, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="temperature"):
+            check(temperature=t)
+    with pytest.raises(ValueError, match="reduction"):
+        check(reduction="sum")
+    teacher = Fake((2, 3, 5), F32)
+    teacher.requires_grad = True
+    with pytest.raises(RuntimeError, match="requires grad"):
+        check(teacher_logits=teacher)
+    with torch.no_grad():
+        check(teacher_logits=teacher)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        nmce.vocab_parallel_distillation_loss(torch.zeros(2, 8), torch.zeros(2, 3),
+                                              torch.zeros(2, 3, dtype=I64), 0, 8, ctx)
