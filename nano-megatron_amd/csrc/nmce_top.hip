@@ -28,6 +28,8 @@ constexpr int kBlock = 512;
 constexpr int kWaves = kBlock / 64;
 constexpr int kVecs = 4;      // 16-byte vectors of a thread's chunk
 constexpr int kNotes = 2048;  // keys noted at most; cut to k past half of them
+constexpr int kLeast = 4096;
+constexpr int kFew = 64;
 constexpr int kMaxK = NMCE_TOP_MAX_K;
 static_assert(2 * kMaxK <= kNotes && kMaxK <= kBlock && kMaxK <= 2 * kBlock, "");
 constexpr float kInf = __builtin_huge_valf();
@@ -70,11 +72,23 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 }
 __device__ __forceinline__ uint64_t wave_min_u64(uint64_t v) { return ~wave_max_u64(~v); }
 
-// One wave: a key that exactly k of n unique keys (n >= k) reach.
+// One wave: a key that exactly k of n unique keys (n >= k) reach. Up to 512 are held in
+// registers: 14 cycles a key and step, where LDS would answer each in a hundred.
 __device__ uint64_t kth_key(const uint64_t* list, int n, int k) {
+  constexpr int kHeld = 8;
   const int lane = threadIdx.x & 63;
+  uint64_t held[kHeld];
   uint64_t lo = ~uint64_t{0}, hi = 0;
-  for (int i = lane; i < n; i += 64) {
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = j * 64 + lane;
+    held[j] = i < n ? list[i] : 0;
+    if (i < n) {
+      lo = held[j] < lo ? held[j] : lo;
+      hi = held[j] > hi ? held[j] : hi;
+    }
+  }
+  for (int i = kHeld * 64 + lane; i < n; i += 64) {
     lo = list[i] < lo ? list[i] : lo;
     hi = list[i] > hi ? list[i] : hi;
   }
@@ -82,9 +96,11 @@ __device__ uint64_t kth_key(const uint64_t* list, int n, int k) {
   hi = wave_max_u64(hi) + 1;
   if (n == k) return lo;
   while (hi - lo > 1) {  // all reach lo, more than k of them; fewer reach hi
-    const uint64_t mid = lo + (hi - lo) / 2;
+    const uint64_t mid = lo + (hi - lo) / 2;  // (above lo, so a 0 does not reach it)
     int c = 0;
-    for (int i = 0; i < n; i += 64)
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) c += __popcll(__ballot(held[j] >= mid));
+    for (int i = kHeld * 64; i < n; i += 64)
       c += __popcll(__ballot(i + lane < n && list[i + lane] >= mid));
     if (c == k) return mid;
     if (c > k) lo = mid;
@@ -94,14 +110,15 @@ __device__ uint64_t kth_key(const uint64_t* list, int n, int k) {
 }
 
 // One wave: a rank that k or somewhat more of the maxima reach; 0 if fewer are there.
-__device__ uint32_t floor_rank(const uint32_t* maxima, int n, int k) {
+template <int kMaxima>
+__device__ uint32_t floor_rank(const uint32_t* maxima, int k) {
   const int lane = threadIdx.x & 63;
-  uint32_t r[2 * kBlock / 64];
+  uint32_t r[kMaxima / 64];
   uint32_t lo = 0xffffffffu, hi = 0;
   int here = 0;
 #pragma unroll
-  for (int i = 0; i < 2 * kBlock / 64; ++i) {
-    r[i] = i * 64 < n ? maxima[i * 64 + lane] : 0u;
+  for (int i = 0; i < kMaxima / 64; ++i) {
+    r[i] = maxima[i * 64 + lane];
     here += __popcll(__ballot(r[i] != 0));
     if (r[i] != 0) lo = r[i] < lo ? r[i] : lo;
     hi = r[i] > hi ? r[i] : hi;
@@ -117,7 +134,7 @@ __device__ uint32_t floor_rank(const uint32_t* maxima, int n, int k) {
     const uint32_t mid = lo + (hi - lo) / 2;
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < 2 * kBlock / 64; ++i) c += __popcll(__ballot(r[i] >= mid));
+    for (int i = 0; i < kMaxima / 64; ++i) c += __popcll(__ballot(r[i] >= mid));
     if (c >= k) {
       lo = mid;
       if (c <= enough) break;
@@ -128,11 +145,19 @@ __device__ uint32_t floor_rank(const uint32_t* maxima, int n, int k) {
   return lo;
 }
 
+// 16 bytes at any element's alignment (rows of odd widths start anywhere).
+__device__ __forceinline__ u32x4 load16(const void* p) {
+  u32x4 v;
+  memcpy(&v, p, 16);
+  return v;
+}
+
 struct Shared {
   uint64_t notes[kNotes];
   uint64_t kept[kMaxK];
   uint64_t key;    // what the k largest reach
   uint32_t floor;  // of the first chunk
+  float first;     // the largest logit
   int n, n_kept, counts[2];
   float wave_m[kWaves];
   double wave_s[kWaves];
@@ -153,59 +178,95 @@ __device__ void cut_notes(Shared& sh, int n, int k) {
   __syncthreads();
 }
 
-// Row blockIdx.x / slabs, columns [slab * width, + width) of it. lists[row][slab] gets k
-// entries in order and the pair (maximum, sum of exp((x - maximum) / T)).
+// The results of whole rows; norm null: lists are wanted.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void top_kernel(const T* __restrict__ x, int64_t ld,
-                                                     int64_t v, int64_t vocab_start, int64_t slabs,
-                                                     int64_t width, int k, int id_bits, float c,
-                                                     uint64_t* __restrict__ lists) {
+struct Out {
+  T* values;
+  int64_t* ids;
+  float* norm;
+};
+
+// log sum exp(x / T) from the maximum m, the sum over exp((x - m) / T) and the first of
+// the top logits, which is NaN where any is. +inf beside numbers is the sum.
+__device__ __forceinline__ float log_norm(float m, double s, float first, double c) {
+  return first != first ? first
+         : m == kInf    ? kInf
+                        : static_cast<float>(static_cast<double>(m) * c + log(s));
+}
+
+// Row blockIdx.x / slabs, columns [slab * width, + width) of it. lists[row][slab] gets k
+// entries in order and the pair (maximum, sum of exp((x - maximum) / T)); or, of whole
+// rows, `out` the results.
+// 64 registers: four workgroups share a compute unit, and while one looks for its floor or
+// its k-th key (a wave's work, the others wait) the rest read.
+template <typename T>
+__global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x, int64_t ld,
+                                                        int64_t v, int64_t vocab_start,
+                                                        int64_t slabs, int64_t width, int k,
+                                                        int id_bits, float c, double c64,
+                                                        uint64_t* __restrict__ lists,
+                                                        Out<T> results) {
   using E = Elem<T>;
   constexpr int EPV = E::kPerVec;
-  constexpr int kChunk = kBlock * kVecs * EPV;
+  constexpr uint32_t kChunk = kBlock * kVecs * EPV;
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / slabs, slab = blockIdx.x - row * slabs;
-  const T* xr = x + row * ld;
+  // Columns below are of the slab, from 0.
   const int64_t from = slab * width;
-  const int64_t end = from + width < v ? from + width : v;
+  const uint32_t end = static_cast<uint32_t>(v - from < width ? v - from : width);
+  const T* xr = x + row * ld + from;
+  const uint64_t last_id = (uint64_t{1} << id_bits) - 1 - static_cast<uint64_t>(from);
   const uint64_t id_mask = (uint64_t{1} << id_bits) - 1;
-  auto key_of = [&](float f, int64_t column) {
-    return static_cast<uint64_t>(Rank<T>::of(f)) << id_bits |
-           (id_mask - static_cast<uint64_t>(column));
+  auto key_of = [&](float f, uint32_t column) {
+    return static_cast<uint64_t>(Rank<T>::of(f)) << id_bits | (last_id - column);
   };
-  auto load_chunk = [&](int64_t base, u32x4* w) {
+  // The first column of the thread's vector i. (Opaque to the compiler, which would keep
+  // what it can compute from each of them in registers through the loop.)
+  auto column_of = [&](uint32_t base, int i) {
+    uint32_t t = base + static_cast<uint32_t>(tid * EPV);
+    asm volatile("" : "+v"(t));
+    return t + i * kBlock * EPV;
+  };
+  auto load_chunk = [&](uint32_t base, u32x4 (&w)[kVecs]) {
+    const uint32_t col = column_of(base, 0);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      if (col + i * kBlock * EPV + EPV <= end) w[i] = load16(xr + col + i * kBlock * EPV);
+    if (base + kChunk <= end) return;
+    // The vector that the row ends in, and none behind it.
+    constexpr uint32_t kNone = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int64_t col = base + (i * kBlock + tid) * EPV;
-      if (col + EPV <= end) {
-        memcpy(&w[i], xr + col, 16);
-      } else {
-        float f[EPV];
+      const uint32_t c0 = col + i * kBlock * EPV;
+      if (c0 + EPV > end) {
+        w[i] = u32x4{kNone, kNone, kNone, kNone};
+        if (c0 < end) {
+          float f[EPV];
 #pragma unroll
-        for (int e = 0; e < EPV; ++e) f[e] = col + e < end ? E::load1(xr + col + e) : -kInf;
-        w[i] = E::pack(f);
+          for (int e = 0; e < EPV; ++e) f[e] = c0 + e < end ? E::load1(xr + c0 + e) : -kInf;
+          w[i] = E::pack(f);
+        }
       }
     }
   };
   if (tid == 0) sh.n = 0;
   u32x4 cur[kVecs];
-  load_chunk(from, cur);
   float m = kNegHuge, s = 0.0f;
   float floor = 0.0f;
   int n = 0;  // notes
-  for (int64_t base = from; base < end; base += kChunk) {
-    u32x4 next[kVecs];
-    if (base + kChunk < end) load_chunk(base + kChunk, next);
-    if (base == from) {
+  for (uint32_t base = 0; base < end; base += kChunk) {
+    load_chunk(base, cur);
+    if (base == 0) {
       // The floor: from the maxima of a thread's even and odd vectors.
       uint32_t* maxima = reinterpret_cast<uint32_t*>(sh.notes);
+      uint32_t tops[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t top = 0;
 #pragma unroll
         for (int i = h; i < kVecs; i += 2) {
-          if (base + (i * kBlock + tid) * EPV < end) {
+          if (column_of(base, i) < end) {
             float f[EPV];
             E::unpack(cur[i], f);
             float q = -kInf;
@@ -215,11 +276,15 @@ __global__ __launch_bounds__(kBlock) void top_kernel(const T* __restrict__ x, in
             top = r > top ? r : top;
           }
         }
-        maxima[h * kBlock + tid] = top;
+        tops[h] = top;
       }
+      // One maximum a thread does for few.
+      const bool two = k > kFew;
+      maxima[tid] = two || tops[0] > tops[1] ? tops[0] : tops[1];
+      if (two) maxima[kBlock + tid] = tops[1];
       __syncthreads();
       if (wave == 0) {
-        const uint32_t r = floor_rank(maxima, 2 * kBlock, k);
+        const uint32_t r = two ? floor_rank<2 * kBlock>(maxima, k) : floor_rank<kBlock>(maxima, k);
         if (lane == 0) sh.floor = r;
       }
       __syncthreads();
@@ -228,10 +293,11 @@ __global__ __launch_bounds__(kBlock) void top_kernel(const T* __restrict__ x, in
       floor = r > Rank<T>::of(-kInf) ? Rank<T>::below(r) : __builtin_nanf("");
     }
     const int before = n;
-    if (base != from) __syncthreads();  // every thread has read the last chunk's count
+    if (base != 0) __syncthreads();  // every thread has read the last chunk's count
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-      const int64_t col = base + (i * kBlock + tid) * EPV;
+      if (base + i * kBlock * EPV >= end) break;  // (the same for all threads)
+      const uint32_t col = column_of(base, i);
       float f[EPV], e[EPV];
       E::unpack(cur[i], f);
       float q = f[0];
@@ -267,29 +333,28 @@ __global__ __launch_bounds__(kBlock) void top_kernel(const T* __restrict__ x, in
     n = sh.n;
     if (n > kNotes) {
       // More reach the floor than fit: the chunk's k largest keys alone, by bisection
-      // over the registers. (The notes from before are whole.)
-      auto keys_from = [&](uint64_t least) {
-        int count = 0;
+      // over its elements, read again. (The notes from before are whole.)
+      auto each_key = [&](auto&& use) {
 #pragma unroll 1
         for (int i = 0; i < kVecs; ++i) {
-          const int64_t col = base + (i * kBlock + tid) * EPV;
-          u32x4 w = cur[0];
+          const uint32_t col = column_of(base, i);
+          if (col + EPV <= end) {
+            float f[EPV];
+            E::unpack(load16(xr + col), f);
 #pragma unroll
-          for (int u = 1; u < kVecs; ++u) w = i == u ? cur[u] : w;
-          float f[EPV];
-          E::unpack(w, f);
-#pragma unroll
-          for (int j = 0; j < EPV; ++j)
-            count += col + j < end && key_of(f[j], col + j) >= least;
+            for (int j = 0; j < EPV; ++j) use(key_of(f[j], col + j));
+          } else {
+            for (uint32_t c = col; c < end; ++c) use(key_of(E::load1(xr + c), c));
+          }
         }
-        return count;
       };
       uint64_t lo = 0, hi = uint64_t{1} << (32 - Rank<T>::kShift + id_bits);
       if (tid == 0) sh.counts[0] = sh.counts[1] = 0;
       __syncthreads();
       for (int turn = 0; hi - lo > 1; turn ^= 1) {
         const uint64_t mid = lo + (hi - lo) / 2;
-        int count = keys_from(mid);
+        int count = 0;
+        each_key([&](uint64_t key) { count += key >= mid; });
         for (int d = 32; d > 0; d >>= 1) count += __shfl_xor(count, d);
         if (lane == 0) atomicAdd(&sh.counts[turn], count);
         __syncthreads();
@@ -305,24 +370,13 @@ __global__ __launch_bounds__(kBlock) void top_kernel(const T* __restrict__ x, in
       }
       if (tid == 0) sh.n = before;
       __syncthreads();
-#pragma unroll 1
-      for (int i = 0; i < kVecs; ++i) {
-        const int64_t col = base + (i * kBlock + tid) * EPV;
-        u32x4 w = cur[0];
-#pragma unroll
-        for (int u = 1; u < kVecs; ++u) w = i == u ? cur[u] : w;
-        float f[EPV];
-        E::unpack(w, f);
-#pragma unroll
-        for (int j = 0; j < EPV; ++j) {
-          const uint64_t key = key_of(f[j], col + j);
-          if (col + j < end && key >= lo) sh.notes[atomicAdd(&sh.n, 1)] = key;
-        }
-      }
+      each_key([&](uint64_t key) {
+        if (key >= lo) sh.notes[atomicAdd(&sh.n, 1)] = key;
+      });
       __syncthreads();
       n = sh.n;
     }
-    if (base == from && sh.floor != 0) floor = Rank<T>::value(sh.floor);
+    if (base == 0 && sh.floor != 0) floor = Rank<T>::value(sh.floor);
     if (n > kNotes / 2) {
       cut_notes(sh, n, k);
       for (int i = tid; i < k; i += kBlock) sh.notes[i] = sh.kept[i];
@@ -332,8 +386,6 @@ __global__ __launch_bounds__(kBlock) void top_kernel(const T* __restrict__ x, in
       floor = Rank<T>::value(static_cast<uint32_t>(sh.key >> id_bits));
       __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) cur[i] = next[i];
   }
 
   // The sum over the workgroup, in 64 bits.
@@ -356,37 +408,68 @@ __global__ __launch_bounds__(kBlock) void top_kernel(const T* __restrict__ x, in
     const uint64_t key = sh.kept[tid];
     int rank = 0;
     for (int i = 0; i < have; ++i) rank += sh.kept[i] > key;
-    const int64_t column = static_cast<int64_t>(id_mask - (key & id_mask));
-    const uint32_t r = static_cast<uint32_t>(key >> id_bits);
-    out[rank] = entry_of(Rank<T>::value(r), vocab_start + column);
+    const int64_t id = vocab_start + static_cast<int64_t>(id_mask - (key & id_mask));
+    const float f = Rank<T>::value(static_cast<uint32_t>(key >> id_bits));
+    if (results.norm) {
+      E::store1(results.values + row * k + rank, f);
+      results.ids[row * k + rank] = id;
+    } else {
+      out[rank] = entry_of(f, id);
+    }
+    if (rank == 0) sh.first = f;
   } else if (tid < k) {
     out[tid] = 0;
   }
+  __syncthreads();
   if (tid == 0) {
     total = 0.0;
     for (int w = 0; w < kWaves; ++w) total += sh.wave_s[w];
+    if (results.norm) {
+      results.norm[row] = log_norm(wm, total, sh.first, c64);
+      return;
+    }
     out[k] = static_cast<uint64_t>(__float_as_uint(wm)) << 32 |
              __float_as_uint(static_cast<float>(total));
   }
 }
 
+constexpr int kMergeBlock = 512;
+constexpr int kCounted = 1024;  // entries up to which a place is found by counting
+constexpr int kStageBytes = 64 * 1024;
+
 // One row's lists (entries of list l at lists + l * list_stride + row * row_stride), each
 // in order, as one: an entry's place is how many are above it, its own list's by its index
 // and the others' by bisection. Either the list again (merged) or the results.
 template <typename T>
-__global__ __launch_bounds__(256) void top_merge_kernel(
+__global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
     const uint64_t* __restrict__ lists, int64_t list_stride, int64_t row_stride, int n_lists,
-    int k, double c, uint64_t* __restrict__ merged, T* __restrict__ values,
+    int k, bool staged, double c, uint64_t* __restrict__ merged, T* __restrict__ values,
     int64_t* __restrict__ ids, float* __restrict__ norm) {
+  extern __shared__ uint64_t stage[];
   const int64_t row = blockIdx.x;
   const uint64_t* in = lists + row * row_stride;
   const int total = n_lists * k;
-  for (int i = threadIdx.x; i < total; i += 256) {
+  if (staged) {
+    for (int i = threadIdx.x; i < n_lists * (k + 1); i += kMergeBlock) {
+      const int l = i / (k + 1);
+      stage[i] = in[l * list_stride + (i - l * (k + 1))];
+    }
+    __syncthreads();
+    in = stage;
+    list_stride = k + 1;
+  }
+  for (int i = threadIdx.x; i < total; i += kMergeBlock) {
     const int l = i / k, j = i - l * k;
     const uint64_t key = in[l * list_stride + j];
     int rank = j;
     if (key == 0) continue;  // (fewer entries than k: the places behind are filled below)
-    for (int o = 0; o < n_lists && rank < k; ++o) {
+    if (staged && total <= kCounted) {
+      // Few entries are counted one by one: no read waits for another.
+      rank = 0;
+      for (int o = 0; o < n_lists * (k + 1); o += k + 1)
+#pragma unroll 4
+        for (int e = 0; e < k; ++e) rank += stage[o + e] > key;
+    } else for (int o = 0; o < n_lists && rank < k; ++o) {
       if (o == l) continue;
       const uint64_t* p = in + o * list_stride;
       int lo = 0, hi = k;  // entries before lo are above key, from hi on are not
@@ -446,13 +529,8 @@ __global__ __launch_bounds__(256) void top_merge_kernel(
         ids[row * k + i] = -1;
       }
     }
-    if (!merged && threadIdx.x == 0) {
-      // The first entry tells of a NaN; +inf beside numbers is the sum.
-      const float top = Rank<float>::value(static_cast<uint32_t>(first >> 32));
-      norm[row] = top != top ? top
-                  : top == kInf ? kInf
-                                : static_cast<float>(static_cast<double>(m) * c + log(s));
-    }
+    if (!merged && threadIdx.x == 0)
+      norm[row] = log_norm(m, s, Rank<float>::value(static_cast<uint32_t>(first >> 32)), c);
   }
 }
 
@@ -465,9 +543,16 @@ int id_bits_of(int64_t v) {
   return bits;
 }
 
-// Columns of a slab, and slabs of a row.
+// Columns of a slab: the whole row, or, where the rows do not fill the card, as few as
+// give a workgroup's place to every slab, but no fewer than kLeast (a workgroup's own
+// steps take as long as reading these) and 16 a wanted logit (so that the floor holds).
 int64_t width_of(int64_t n_rows, int64_t v, int k) {
-  return v;
+  const int64_t places = 4 * static_cast<int64_t>(device_cus());
+  const int64_t slabs = n_rows > 0 ? places / n_rows : 1;
+  if (slabs <= 1) return v;
+  int64_t width = round_up((v + slabs - 1) / slabs, 8);
+  width = width > kLeast ? width : kLeast;
+  return width > 16 * k ? width : 16 * k;
 }
 
 int check_rows(int dtype, int64_t n_rows, int64_t v, int k, double temperature) {
@@ -481,14 +566,18 @@ int check_rows(int dtype, int64_t n_rows, int64_t v, int k, double temperature) 
 int merge(const uint64_t* lists, int64_t list_stride, int64_t row_stride, int n_lists, int dtype,
           int64_t n_rows, int k, double c, uint64_t* merged, void* values, int64_t* ids,
           float* norm, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(n_rows)), block(256);
+  const dim3 grid(static_cast<unsigned>(n_rows)), block(kMergeBlock);
+  const int64_t bytes = static_cast<int64_t>(n_lists) * (k + 1) * 8;
+  const bool staged = bytes <= kStageBytes;
+  const unsigned lds = staged ? static_cast<unsigned>(bytes) : 0;
   if (dtype == NMCE_F32)
-    hipLaunchKernelGGL(top_merge_kernel<float>, grid, block, 0, s, lists, list_stride, row_stride,
-                       n_lists, k, c, merged, static_cast<float*>(values), ids, norm);
-  else
-    hipLaunchKernelGGL(top_merge_kernel<uint16_t>, grid, block, 0, s, lists, list_stride,
-                       row_stride, n_lists, k, c, merged, static_cast<uint16_t*>(values), ids,
+    hipLaunchKernelGGL(top_merge_kernel<float>, grid, block, lds, s, lists, list_stride,
+                       row_stride, n_lists, k, staged, c, merged, static_cast<float*>(values), ids,
                        norm);
+  else
+    hipLaunchKernelGGL(top_merge_kernel<uint16_t>, grid, block, lds, s, lists, list_stride,
+                       row_stride, n_lists, k, staged, c, merged, static_cast<uint16_t*>(values),
+                       ids, norm);
   return launch_status();
 }
 
@@ -527,19 +616,25 @@ int nmce_top_logits(const void* logits, int dtype, int64_t n_rows, int64_t vocab
   const dim3 grid(static_cast<unsigned>(n_rows * slabs)), block(kBlock);
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint64_t* lists = static_cast<uint64_t*>(workspace);
-  const float c = static_cast<float>(1.4426950408889634 * inverse(temperature));
+  const double c = inverse(temperature);
+  const float c2 = static_cast<float>(1.4426950408889634 * c);
   const int bits = id_bits_of(vocab_local);
+  const bool whole = slabs == 1 && !list;
+  uint64_t* part = list && slabs == 1 ? reinterpret_cast<uint64_t*>(list) : lists;
   if (dtype == NMCE_F32)
     hipLaunchKernelGGL(top_kernel<float>, grid, block, 0, s, static_cast<const float*>(logits), ld,
-                       vocab_local, vocab_start, slabs, width, k, bits, c, lists);
+                       vocab_local, vocab_start, slabs, width, k, bits, c2, c, part,
+                       Out<float>{static_cast<float*>(values), ids, whole ? log_normalizer : nullptr});
   else
     hipLaunchKernelGGL(top_kernel<uint16_t>, grid, block, 0, s,
                        static_cast<const uint16_t*>(logits), ld, vocab_local, vocab_start, slabs,
-                       width, k, bits, c, lists);
+                       width, k, bits, c2, c, part,
+                       Out<uint16_t>{static_cast<uint16_t*>(values), ids,
+                                     whole ? log_normalizer : nullptr});
   if (const int st = launch_status()) return st;
-  return merge(lists, k + 1, slabs * (k + 1), static_cast<int>(slabs), dtype, n_rows, k,
-               inverse(temperature), reinterpret_cast<uint64_t*>(list), values, ids, log_normalizer,
-               s);
+  if (slabs == 1) return NMCE_OK;
+  return merge(lists, k + 1, slabs * (k + 1), static_cast<int>(slabs), dtype, n_rows, k, c,
+               reinterpret_cast<uint64_t*>(list), values, ids, log_normalizer, s);
 }
 
 int nmce_top_merge(const int64_t* lists, int ranks, int dtype, int64_t n_rows, int k,
