@@ -250,11 +250,27 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
       }
     }
   };
+  // The next free note. (The address is opaque: known to be the same for all lanes, the
+  // compiler would count the lanes first, for 15 instructions more.)
+  auto take_place = [&]() {
+    auto* p = (__attribute__((address_space(3))) int*)&sh.n;
+    asm volatile("" : "+v"(p));
+    return __hip_atomic_fetch_add(p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  };
   if (tid == 0) sh.n = 0;
   u32x4 cur[kVecs];
   float m = kNegHuge, s = 0.0f;
   float floor = 0.0f;
-  int n = 0;  // notes
+  int n = 0;     // notes,
+  int keys = 0;  // the first of them as keys; the others as (value, column), in fewer steps
+  auto to_keys = [&](int first, int last) {
+    for (int i = first + tid; i < last; i += kBlock) {
+      const uint64_t note = sh.notes[i];
+      sh.notes[i] = key_of(__uint_as_float(static_cast<uint32_t>(note >> 32)),
+                           static_cast<uint32_t>(note));
+    }
+    __syncthreads();
+  };
   for (uint32_t base = 0; base < end; base += kChunk) {
     load_chunk(base, cur);
     if (base == 0) {
@@ -295,36 +311,45 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
     const int before = n;
     if (base != 0) __syncthreads();  // every thread has read the last chunk's count
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
+    for (int i = 0; i < kVecs; i += 2) {
       if (base + i * kBlock * EPV >= end) break;  // (the same for all threads)
-      const uint32_t col = column_of(base, i);
-      float f[EPV], e[EPV];
-      E::unpack(cur[i], f);
-      float q = f[0];
+      float q, sum;
+      {
+        float f[2 * EPV];
+        E::unpack(cur[i], f);
+        E::unpack(cur[i + 1], f + EPV);
+        q = f[0];
 #pragma unroll
-      for (int j = 1; j < EPV; ++j) q = fmaxf(q, f[j]);
-      const float nm = fmaxf(m, q);
+        for (int j = 1; j < 2 * EPV; ++j) q = fmaxf(q, f[j]);
+        const float nm = fmaxf(m, q);
 #pragma unroll
-      for (int j = 0; j < EPV; ++j) e[j] = exp2_hw((f[j] - nm) * c);
+        for (int j = 0; j < 2 * EPV; ++j) f[j] = exp2_hw((f[j] - nm) * c);
 #pragma unroll
-      for (int w = 1; w < EPV; w *= 2) {
+        for (int w = 1; w < 2 * EPV; w *= 2) {
 #pragma unroll
-        for (int j = 0; j + w < EPV; j += 2 * w) e[j] += e[j + w];
+          for (int j = 0; j + w < 2 * EPV; j += 2 * w) f[j] += f[j + w];
+        }
+        sum = f[0];
+        s = fmaf(s, exp2_hw((m - nm) * c), sum);
+        m = nm;
       }
-      s = fmaf(s, exp2_hw((m - nm) * c), e[0]);
-      m = nm;
-      // (A NaN among them shows in their sum.)
-      if (__any((!(q <= floor) || e[0] != e[0]) && col < end)) {
+      // (A NaN among them shows in their sum.) Few lanes have anything to note, and
+      // those one element mostly: each notes its own.
+      if (!(q <= floor) || sum != sum) {
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) {
-          const bool up = !(f[j] <= floor) && col + j < end;
-          const uint64_t who = __ballot(up);
-          if (who) {
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&sh.n, static_cast<int>(__popcll(who)));
-            at = __builtin_amdgcn_readfirstlane(at) +
-                 __popcll(who & ((uint64_t{1} << lane) - 1));
-            if (up && at < kNotes) sh.notes[at] = key_of(f[j], col + j);
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t col = column_of(base, i + h);
+          u32x4 w = cur[i + h];
+          asm volatile("" : "+v"(w));  // unpack again: the exponentials took the registers
+          float f[EPV];
+          E::unpack(w, f);
+#pragma unroll
+          for (int j = 0; j < EPV; ++j) {
+            if (!(f[j] <= floor) && col + j < end) {
+              const int at = take_place();
+              if (at < kNotes)
+                sh.notes[at] = static_cast<uint64_t>(__float_as_uint(f[j])) << 32 | (col + j);
+            }
           }
         }
       }
@@ -375,13 +400,16 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
       });
       __syncthreads();
       n = sh.n;
+      to_keys(keys, before);
+      keys = n;
     }
     if (base == 0 && sh.floor != 0) floor = Rank<T>::value(sh.floor);
     if (n > kNotes / 2) {
+      to_keys(keys, n);
       cut_notes(sh, n, k);
       for (int i = tid; i < k; i += kBlock) sh.notes[i] = sh.kept[i];
       if (tid == 0) sh.n = k;
-      n = k;
+      n = keys = k;
       // Later columns of the same value come behind: only what is above it counts.
       floor = Rank<T>::value(static_cast<uint32_t>(sh.key >> id_bits));
       __syncthreads();
@@ -397,6 +425,7 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
   for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
   if (lane == 0) sh.wave_s[wave] = total;
   const int have = n < k ? n : k;
+  to_keys(keys, n);
   if (n > k) {
     cut_notes(sh, n, k);
   } else {
