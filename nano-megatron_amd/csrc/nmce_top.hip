@@ -24,14 +24,25 @@
 namespace nmce {
 namespace {
 
-constexpr int kBlock = 512;
-constexpr int kWaves = kBlock / 64;
-constexpr int kVecs = 4;      // 16-byte vectors of a thread's chunk
-constexpr int kNotes = 2048;  // keys noted at most; cut to k past half of them
-constexpr int kLeast = 4096;
-constexpr int kFew = 64;
 constexpr int kMaxK = NMCE_TOP_MAX_K;
-static_assert(2 * kMaxK <= kNotes && kMaxK <= kBlock && kMaxK <= 2 * kBlock, "");
+constexpr int kVecs = 4;  // 16-byte vectors of a thread's chunk
+constexpr int kLeast = 4096;
+
+// A workgroup's shape: threads, the wanted logits it is for, places for notes (past half of
+// them they are cut) and for those a cut leaves, maxima a thread gives to the floor.
+struct Few {
+  static constexpr int kBlock = 256, kMost = 128, kNotes = 1024, kRoom = 160, kTops = 1;
+};
+struct Many {
+  static constexpr int kBlock = 512, kMost = kMaxK, kNotes = 2048, kRoom = kMaxK, kTops = 2;
+};
+
+// A cut looks for a key that k or somewhat more reach: the last steps of a bisection would
+// only tell neighbours apart, which putting them in order does anyway.
+__host__ __device__ constexpr int enough(int k, int room) {
+  return k + k / 8 + 8 < room ? k + k / 8 + 8 : room;
+}
+static_assert(enough(Few::kMost, 1 << 20) <= Few::kRoom, "");
 constexpr float kInf = __builtin_huge_valf();
 
 // An order of the logits as integers: NaN (any) above +inf, -0 as 0. bf16 takes 16 bits.
@@ -72,43 +83,6 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 }
 __device__ __forceinline__ uint64_t wave_min_u64(uint64_t v) { return ~wave_max_u64(~v); }
 
-// One wave: a key that exactly k of n unique keys (n >= k) reach. Up to 512 are held in
-// registers: 14 cycles a key and step, where LDS would answer each in a hundred.
-__device__ uint64_t kth_key(const uint64_t* list, int n, int k) {
-  constexpr int kHeld = 8;
-  const int lane = threadIdx.x & 63;
-  uint64_t held[kHeld];
-  uint64_t lo = ~uint64_t{0}, hi = 0;
-#pragma unroll
-  for (int j = 0; j < kHeld; ++j) {
-    const int i = j * 64 + lane;
-    held[j] = i < n ? list[i] : 0;
-    if (i < n) {
-      lo = held[j] < lo ? held[j] : lo;
-      hi = held[j] > hi ? held[j] : hi;
-    }
-  }
-  for (int i = kHeld * 64 + lane; i < n; i += 64) {
-    lo = list[i] < lo ? list[i] : lo;
-    hi = list[i] > hi ? list[i] : hi;
-  }
-  lo = wave_min_u64(lo);
-  hi = wave_max_u64(hi) + 1;
-  if (n == k) return lo;
-  while (hi - lo > 1) {  // all reach lo, more than k of them; fewer reach hi
-    const uint64_t mid = lo + (hi - lo) / 2;  // (above lo, so a 0 does not reach it)
-    int c = 0;
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) c += __popcll(__ballot(held[j] >= mid));
-    for (int i = kHeld * 64; i < n; i += 64)
-      c += __popcll(__ballot(i + lane < n && list[i + lane] >= mid));
-    if (c == k) return mid;
-    if (c > k) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // One wave: a rank that k or somewhat more of the maxima reach; 0 if fewer are there.
 template <int kMaxima>
 __device__ uint32_t floor_rank(const uint32_t* maxima, int k) {
@@ -145,37 +119,172 @@ __device__ uint32_t floor_rank(const uint32_t* maxima, int k) {
   return lo;
 }
 
-// 16 bytes at any element's alignment (rows of odd widths start anywhere).
+// 16 bytes at any element's alignment (rows of odd widths start anywhere), streamed: 4096 x
+// 128256 bf16 241 -> 215 us.
 __device__ __forceinline__ u32x4 load16(const void* p) {
-  u32x4 v;
-  memcpy(&v, p, 16);
-  return v;
+  typedef u32x4 anywhere __attribute__((aligned(2)));
+  return __builtin_nontemporal_load(static_cast<const anywhere*>(p));
 }
 
+template <typename Shape>
 struct Shared {
-  uint64_t notes[kNotes];
-  uint64_t kept[kMaxK];
-  uint64_t key;    // what the k largest reach
+  uint64_t notes[Shape::kNotes];
+  __align__(16) uint64_t kept[Shape::kRoom];
+  uint64_t wave_lo[Shape::kBlock / 64], wave_hi[Shape::kBlock / 64];
   uint32_t floor;  // of the first chunk
   float first;     // the largest logit
-  int n, n_kept, counts[2];
-  float wave_m[kWaves];
-  double wave_s[kWaves];
+  int n, n_kept, counts[3];
+  float wave_m[Shape::kBlock / 64];
+  double wave_s[Shape::kBlock / 64];
 };
 
-// All but the k largest notes go (k <= n); every thread calls it, behind a barrier.
-__device__ void cut_notes(Shared& sh, int n, int k) {
-  if (threadIdx.x < 64) {
-    const uint64_t key = kth_key(sh.notes, n, k);
-    if (threadIdx.x == 0) {
-      sh.key = key;
-      sh.n_kept = 0;
+// One wave: a key that k to `most` of n unique keys (n >= k) reach, by bisection over eight
+// of them a lane in registers, and what there is beyond 512 from LDS.
+__device__ uint64_t kth_key(const uint64_t* list, int n, int k, int most) {
+  constexpr int kHeld = 8;
+  const int lane = threadIdx.x & 63;
+  uint64_t held[kHeld];
+  uint64_t lo = ~uint64_t{0}, hi = 0;
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = j * 64 + lane;
+    held[j] = i < n ? list[i] : 0;
+    if (i < n) {
+      lo = held[j] < lo ? held[j] : lo;
+      hi = held[j] > hi ? held[j] : hi;
+    }
+  }
+  for (int i = kHeld * 64 + lane; i < n; i += 64) {
+    lo = list[i] < lo ? list[i] : lo;
+    hi = list[i] > hi ? list[i] : hi;
+  }
+  lo = wave_min_u64(lo);
+  hi = wave_max_u64(hi) + 1;
+  while (n > most && hi - lo > 1) {  // more than `most` reach lo, fewer than k reach hi
+    const uint64_t mid = lo + (hi - lo) / 2;  // (above lo, so a 0 does not reach it)
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) c += __popcll(__ballot(held[j] >= mid));
+    for (int i = kHeld * 64; i < n; i += 64)
+      c += __popcll(__ballot(i + lane < n && list[i + lane] >= mid));
+    if (c >= k) lo = mid;
+    if (c >= k && c <= most) break;
+    if (c < k) hi = mid;
+  }
+  return lo;
+}
+
+// The k largest of the n notes (k <= n, unique keys), and a few more, into kept; the key
+// that they reach is returned. Every thread calls it, behind a barrier. Few notes are one wave's work
+// while the others wait (and other workgroups read): 4096 x 128256 bf16, k 64: 207 us, by
+// all waves 220. More are held by all threads, four a thread, a barrier a step: 777 x 100277
+// fp32, k 500: 112 us, by one wave from LDS 137.
+template <typename Shape>
+__device__ uint64_t cut_notes(Shared<Shape>& sh, int n, int k) {
+  constexpr int kEach = Shape::kNotes / Shape::kBlock, kWaves = Shape::kBlock / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int most = enough(k, Shape::kRoom);
+  if (Shape::kNotes <= 1024 || n <= 512) {
+    if (wave == 0) {
+      const uint64_t key = kth_key(sh.notes, n, k, most);
+      if (lane == 0) {
+        sh.wave_lo[0] = key;
+        sh.n_kept = 0;
+      }
+    }
+    __syncthreads();
+    const uint64_t key = sh.wave_lo[0];
+    for (int i = tid; i < n; i += Shape::kBlock)
+      if (sh.notes[i] >= key) sh.kept[atomicAdd(&sh.n_kept, 1)] = sh.notes[i];
+    __syncthreads();
+    return key;
+  }
+  uint64_t held[kEach];
+  uint64_t lo = ~uint64_t{0}, hi = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = j * Shape::kBlock + tid;
+    held[j] = i < n ? sh.notes[i] : 0;
+    if (i < n) {
+      lo = held[j] < lo ? held[j] : lo;
+      hi = held[j] > hi ? held[j] : hi;
+    }
+  }
+  lo = wave_min_u64(lo);
+  hi = wave_max_u64(hi);
+  if (lane == 0) {
+    sh.wave_lo[wave] = lo;
+    sh.wave_hi[wave] = hi;
+  }
+  if (tid == 0) sh.counts[0] = sh.counts[1] = sh.counts[2] = sh.n_kept = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    lo = sh.wave_lo[w] < lo ? sh.wave_lo[w] : lo;
+    hi = sh.wave_hi[w] > hi ? sh.wave_hi[w] : hi;
+  }
+  ++hi;
+  // More than `most` reach lo, fewer than k reach hi.
+  for (int turn = 0; n > most && hi - lo > 1; turn = turn == 2 ? 0 : turn + 1) {
+    const uint64_t mid = lo + (hi - lo) / 2;  // (above lo, so a 0 does not reach it)
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) c += __popcll(__ballot(held[j] >= mid));
+    if (lane == 0) atomicAdd(&sh.counts[turn], c);
+    __syncthreads();
+    c = sh.counts[turn];
+    if (tid == 0) sh.counts[turn == 0 ? 2 : turn - 1] = 0;  // read by all before this barrier
+    if (c >= k) lo = mid;
+    if (c >= k && c <= most) break;
+    if (c < k) hi = mid;
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (j * Shape::kBlock + tid < n && held[j] >= lo)
+      sh.kept[atomicAdd(&sh.n_kept, 1)] = held[j];
+  __syncthreads();
+  return lo;
+}
+
+// The n <= kRoom keys in falling order, put(place, key) each. Every thread calls it, behind a
+// barrier. Few are counted among one another (8 cycles of LDS for two keys and a wave);
+// 256 and more are sorted, in pairs of growing distance: 500 keys 2 us, counted 7.
+template <int kThreads, int kRoom, typename Put>
+__device__ void in_order(uint64_t* keys, int n, Put&& put) {
+  const int tid = threadIdx.x;
+  if (kRoom <= 256 || n <= 160) {
+    const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(keys);
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t key = keys[i];
+      int place = 0;
+#pragma unroll 4
+      for (int j = 0; j < n / 2; ++j) {
+        const ulonglong2 two = pairs[j];
+        place += (two.x > key) + (two.y > key);
+      }
+      if (n & 1) place += keys[n - 1] > key;
+      put(place, key);
+    }
+    return;
+  }
+  int all = 256;
+  while (all < n) all *= 2;
+  for (int i = n + tid; i < all; i += kThreads) keys[i] = 0;
+  for (int size = 2; size <= all; size *= 2) {
+    for (int apart = size / 2; apart > 0; apart /= 2) {
+      __syncthreads();
+      for (int t = tid; t < all / 2; t += kThreads) {
+        const int i = 2 * t - (t & (apart - 1)), j = i + apart;
+        const uint64_t a = keys[i], b = keys[j];
+        if ((a < b) == ((i & size) == 0)) {
+          keys[i] = b;
+          keys[j] = a;
+        }
+      }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kBlock)
-    if (sh.notes[i] >= sh.key) sh.kept[atomicAdd(&sh.n_kept, 1)] = sh.notes[i];
-  __syncthreads();
+  for (int i = tid; i < n; i += kThreads) put(i, keys[i]);
 }
 
 // The results of whole rows; norm null: lists are wanted.
@@ -199,8 +308,8 @@ __device__ __forceinline__ float log_norm(float m, double s, float first, double
 // rows, `out` the results.
 // 64 registers: four workgroups share a compute unit, and while one looks for its floor or
 // its k-th key (a wave's work, the others wait) the rest read.
-template <typename T>
-__global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x, int64_t ld,
+template <typename T, typename Shape>
+__global__ __launch_bounds__(Shape::kBlock, 8) void top_kernel(const T* __restrict__ x, int64_t ld,
                                                         int64_t v, int64_t vocab_start,
                                                         int64_t slabs, int64_t width, int k,
                                                         int id_bits, float c, double c64,
@@ -208,8 +317,11 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
                                                         Out<T> results) {
   using E = Elem<T>;
   constexpr int EPV = E::kPerVec;
+  constexpr int kBlock = Shape::kBlock, kNotes = Shape::kNotes, kWaves = kBlock / 64;
+  static_assert(2 * Shape::kMost <= kNotes && Shape::kMost <= Shape::kTops * kBlock &&
+                Shape::kTops * kBlock * 4 <= kNotes * 8, "");
+  __shared__ Shared<Shape> sh;
   constexpr uint32_t kChunk = kBlock * kVecs * EPV;
-  __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / slabs, slab = blockIdx.x - row * slabs;
   // Columns below are of the slab, from 0.
@@ -228,27 +340,29 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
     asm volatile("" : "+v"(t));
     return t + i * kBlock * EPV;
   };
-  auto load_chunk = [&](uint32_t base, u32x4 (&w)[kVecs]) {
-    const uint32_t col = column_of(base, 0);
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-      if (col + i * kBlock * EPV + EPV <= end) w[i] = load16(xr + col + i * kBlock * EPV);
-    if (base + kChunk <= end) return;
-    // The vector that the row ends in, and none behind it.
+  // Vectors i and i + 1 of the chunk from `base`: the one that the row ends in by its
+  // elements, -inf behind it.
+  auto load_pair = [&](uint32_t base, int i, u32x4& w0, u32x4& w1) {
     constexpr uint32_t kNone = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const uint32_t c0 = col + i * kBlock * EPV;
-      if (c0 + EPV > end) {
-        w[i] = u32x4{kNone, kNone, kNone, kNone};
-        if (c0 < end) {
-          float f[EPV];
-#pragma unroll
-          for (int e = 0; e < EPV; ++e) f[e] = c0 + e < end ? E::load1(xr + c0 + e) : -kInf;
-          w[i] = E::pack(f);
-        }
-      }
+    const uint32_t col = column_of(base, i);
+    if (base + (i + 2) * kBlock * EPV <= end) {  // (the same for all threads)
+      w0 = load16(xr + col);
+      w1 = load16(xr + col + kBlock * EPV);
+      return;
     }
+    w0 = w1 = u32x4{kNone, kNone, kNone, kNone};
+    auto last = [&](uint32_t c0, u32x4& w) {
+      if (c0 + EPV <= end) {
+        w = load16(xr + c0);
+      } else if (c0 < end) {
+        float f[EPV];
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) f[e] = c0 + e < end ? E::load1(xr + c0 + e) : -kInf;
+        w = E::pack(f);
+      }
+    };
+    last(col, w0);
+    last(col + kBlock * EPV, w1);
   };
   // The next free note. (The address is opaque: known to be the same for all lanes, the
   // compiler would count the lanes first, for 15 instructions more.)
@@ -271,17 +385,17 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
     }
     __syncthreads();
   };
+#pragma unroll
+  for (int i = 0; i < kVecs; i += 2) load_pair(0, i, cur[i], cur[i + 1]);
   for (uint32_t base = 0; base < end; base += kChunk) {
-    load_chunk(base, cur);
     if (base == 0) {
       // The floor: from the maxima of a thread's even and odd vectors.
       uint32_t* maxima = reinterpret_cast<uint32_t*>(sh.notes);
-      uint32_t tops[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < Shape::kTops; ++h) {
         uint32_t top = 0;
 #pragma unroll
-        for (int i = h; i < kVecs; i += 2) {
+        for (int i = h; i < kVecs; i += Shape::kTops) {
           if (column_of(base, i) < end) {
             float f[EPV];
             E::unpack(cur[i], f);
@@ -292,15 +406,11 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
             top = r > top ? r : top;
           }
         }
-        tops[h] = top;
+        maxima[h * kBlock + tid] = top;
       }
-      // One maximum a thread does for few.
-      const bool two = k > kFew;
-      maxima[tid] = two || tops[0] > tops[1] ? tops[0] : tops[1];
-      if (two) maxima[kBlock + tid] = tops[1];
       __syncthreads();
       if (wave == 0) {
-        const uint32_t r = two ? floor_rank<2 * kBlock>(maxima, k) : floor_rank<kBlock>(maxima, k);
+        const uint32_t r = floor_rank<Shape::kTops * kBlock>(maxima, k);
         if (lane == 0) sh.floor = r;
       }
       __syncthreads();
@@ -353,6 +463,8 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
           }
         }
       }
+      // The next chunk's take their place, under way across the barriers.
+      if (base + kChunk < end) load_pair(base + kChunk, i, cur[i], cur[i + 1]);
     }
     __syncthreads();
     n = sh.n;
@@ -406,12 +518,12 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
     if (base == 0 && sh.floor != 0) floor = Rank<T>::value(sh.floor);
     if (n > kNotes / 2) {
       to_keys(keys, n);
-      cut_notes(sh, n, k);
-      for (int i = tid; i < k; i += kBlock) sh.notes[i] = sh.kept[i];
-      if (tid == 0) sh.n = k;
-      n = keys = k;
+      const uint64_t key = cut_notes(sh, n, k);
+      n = keys = sh.n_kept;
+      for (int i = tid; i < n; i += kBlock) sh.notes[i] = sh.kept[i];
+      if (tid == 0) sh.n = n;
       // Later columns of the same value come behind: only what is above it counts.
-      floor = Rank<T>::value(static_cast<uint32_t>(sh.key >> id_bits));
+      floor = Rank<T>::value(static_cast<uint32_t>(key >> id_bits));
       __syncthreads();
     }
   }
@@ -424,31 +536,29 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
   double total = static_cast<double>(s) * static_cast<double>(exp2_hw((m - wm) * c));
   for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d);
   if (lane == 0) sh.wave_s[wave] = total;
-  const int have = n < k ? n : k;
   to_keys(keys, n);
   if (n > k) {
     cut_notes(sh, n, k);
+    n = sh.n_kept;
   } else {
     for (int i = tid; i < n; i += kBlock) sh.kept[i] = sh.notes[i];
     __syncthreads();
   }
   uint64_t* out = lists + blockIdx.x * static_cast<int64_t>(k + 1);
-  if (tid < have) {
-    const uint64_t key = sh.kept[tid];
-    int rank = 0;
-    for (int i = 0; i < have; ++i) rank += sh.kept[i] > key;
+  in_order<kBlock, Shape::kRoom>(sh.kept, n, [&](int place, uint64_t key) {
+    if (place >= k) return;
     const int64_t id = vocab_start + static_cast<int64_t>(id_mask - (key & id_mask));
     const float f = Rank<T>::value(static_cast<uint32_t>(key >> id_bits));
     if (results.norm) {
-      E::store1(results.values + row * k + rank, f);
-      results.ids[row * k + rank] = id;
+      E::store1(results.values + row * k + place, f);
+      results.ids[row * k + place] = id;
     } else {
-      out[rank] = entry_of(f, id);
+      out[place] = entry_of(f, id);
     }
-    if (rank == 0) sh.first = f;
-  } else if (tid < k) {
-    out[tid] = 0;
-  }
+    if (place == 0) sh.first = f;
+  });
+  if (!results.norm)
+    for (int i = n + tid; i < k; i += kBlock) out[i] = 0;
   __syncthreads();
   if (tid == 0) {
     total = 0.0;
@@ -463,104 +573,127 @@ __global__ __launch_bounds__(kBlock, 8) void top_kernel(const T* __restrict__ x,
 }
 
 constexpr int kMergeBlock = 512;
-constexpr int kCounted = 1024;  // entries up to which a place is found by counting
-constexpr int kStageBytes = 64 * 1024;
+constexpr int kStaged = 7168;  // entries that a workgroup holds in LDS
 
-// One row's lists (entries of list l at lists + l * list_stride + row * row_stride), each
-// in order, as one: an entry's place is how many are above it, its own list's by its index
-// and the others' by bisection. Either the list again (merged) or the results.
+// One row's lists (entries of list l at lists + l * list_stride + row * row_stride, in
+// order) as one, either a list again (merged) or the results: the k-th entry by bisection
+// over all of them in LDS, then those that reach it in order. Lists of so many ranks that
+// LDS does not hold them: an entry's place is how many are above it, its own list's by its
+// index and the others' by bisection, from memory.
 template <typename T>
 __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
     const uint64_t* __restrict__ lists, int64_t list_stride, int64_t row_stride, int n_lists,
-    int k, bool staged, double c, uint64_t* __restrict__ merged, T* __restrict__ values,
+    int k, double c, uint64_t* __restrict__ merged, T* __restrict__ values,
     int64_t* __restrict__ ids, float* __restrict__ norm) {
-  extern __shared__ uint64_t stage[];
+  extern __shared__ __align__(16) uint64_t stage[];  // n_lists * k entries, or none
+  __shared__ __align__(16) uint64_t kept[kMaxK];
+  __shared__ int counts[3], n_kept, n_have;
+  __shared__ float first;
   const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   const uint64_t* in = lists + row * row_stride;
   const int total = n_lists * k;
+  const bool staged = total <= kStaged;
+  const int most = enough(k, kMaxK);
+  if (tid == 0) n_kept = n_have = counts[0] = counts[1] = counts[2] = 0;
+  auto put = [&](int rank, uint64_t key) {
+    if (rank >= k) return;
+    if (merged) {
+      merged[row * (k + 1) + rank] = key;
+      return;
+    }
+    const float f = Rank<float>::value(static_cast<uint32_t>(key >> 32));
+    Elem<T>::store1(values + row * k + rank, f);
+    ids[row * k + rank] = 0xffffffffu - static_cast<uint32_t>(key);
+    if (rank == 0) first = f;
+  };
   if (staged) {
-    for (int i = threadIdx.x; i < n_lists * (k + 1); i += kMergeBlock) {
-      const int l = i / (k + 1);
-      stage[i] = in[l * list_stride + (i - l * (k + 1))];
+    int have = 0;
+    for (int i = tid; i < total; i += kMergeBlock) {
+      const int l = i / k;
+      stage[i] = in[l * list_stride + (i - l * k)];
+      have += stage[i] != 0;
     }
     __syncthreads();
-    in = stage;
-    list_stride = k + 1;
-  }
-  for (int i = threadIdx.x; i < total; i += kMergeBlock) {
-    const int l = i / k, j = i - l * k;
-    const uint64_t key = in[l * list_stride + j];
-    int rank = j;
-    if (key == 0) continue;  // (fewer entries than k: the places behind are filled below)
-    if (staged && total <= kCounted) {
-      // Few entries are counted one by one: no read waits for another.
-      rank = 0;
-      for (int o = 0; o < n_lists * (k + 1); o += k + 1)
+    atomicAdd(&n_have, have);
+    // The wanted reach lo (the k of some list do), fewer than k reach hi.
+    uint64_t lo = 1, hi = 0;
+    for (int l = 0; l < n_lists; ++l) {
+      lo = stage[l * k + k - 1] > lo ? stage[l * k + k - 1] : lo;
+      hi = stage[l * k] > hi ? stage[l * k] : hi;
+    }
+    ++hi;
+    __syncthreads();
+    const int some = n_have;
+    for (int turn = 0; some > most && hi - lo > 1; turn = turn == 2 ? 0 : turn + 1) {
+      const uint64_t mid = lo + (hi - lo) / 2;
+      int n = 0;
 #pragma unroll 4
-        for (int e = 0; e < k; ++e) rank += stage[o + e] > key;
-    } else for (int o = 0; o < n_lists && rank < k; ++o) {
-      if (o == l) continue;
-      const uint64_t* p = in + o * list_stride;
-      int lo = 0, hi = k;  // entries before lo are above key, from hi on are not
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (p[mid] > key) lo = mid + 1;
-        else hi = mid;
-      }
-      rank += lo;
+      for (int i = tid; i < total; i += kMergeBlock) n += stage[i] >= mid;
+      for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
+      if (lane == 0) atomicAdd(&counts[turn], n);
+      __syncthreads();
+      n = counts[turn];
+      if (tid == 0) counts[turn == 0 ? 2 : turn - 1] = 0;  // read by all before this barrier
+      if (n >= k) lo = mid;
+      if (n >= k && n <= most) break;
+      if (n < k) hi = mid;
     }
-    if (rank < k) {
-      if (merged) {
-        merged[row * (k + 1) + rank] = key;
-      } else {
-        const float f = Rank<float>::value(static_cast<uint32_t>(key >> 32));
-        Elem<T>::store1(values + row * k + rank, f);
-        ids[row * k + rank] = 0xffffffffu - static_cast<uint32_t>(key);
-      }
-    }
-  }
-  if (threadIdx.x < 64) {
-    // (maximum, sum) over the lists, a lane each.
-    float m = kNegHuge;
-    int have = 0;
-    for (int l = threadIdx.x; l < n_lists; l += 64) {
-      m = fmaxf(m, __uint_as_float(static_cast<uint32_t>(in[l * list_stride + k] >> 32)));
-      for (int j = k; j > 0; --j)
-        if (in[l * list_stride + j - 1] != 0) {
-          have += j;
-          break;
+    for (int i = tid; i < total; i += kMergeBlock)
+      if (stage[i] >= lo) kept[atomicAdd(&n_kept, 1)] = stage[i];
+    __syncthreads();
+    in_order<kMergeBlock, kMaxK>(kept, n_kept, put);
+  } else {
+    __syncthreads();
+    for (int i = tid; i < total; i += kMergeBlock) {
+      const int l = i / k, j = i - l * k;
+      const uint64_t key = in[l * list_stride + j];
+      if (key == 0) continue;
+      atomicAdd(&n_have, 1);
+      int rank = j;
+      for (int o = 0; o < n_lists && rank < k; ++o) {
+        if (o == l) continue;
+        const uint64_t* p = in + o * list_stride;
+        int lo = 0, hi = k;  // entries before lo are above key, from hi on are not
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (p[mid] > key) lo = mid + 1;
+          else hi = mid;
         }
-    }
-    m = wave_max(m);
-    double s = 0.0;
-    for (int l = threadIdx.x; l < n_lists; l += 64) {
-      const uint64_t pair = in[l * list_stride + k];
-      const double lm = __uint_as_float(static_cast<uint32_t>(pair >> 32));
-      s += static_cast<double>(__uint_as_float(static_cast<uint32_t>(pair))) *
-           (lm == m ? 1.0 : exp((lm - static_cast<double>(m)) * c));
-    }
-    for (int d = 32; d > 0; d >>= 1) {
-      s += __shfl_xor(s, d);
-      have += __shfl_xor(have, d);
-    }
-    uint64_t first = 0;
-    for (int l = threadIdx.x; l < n_lists; l += 64)
-      first = in[l * list_stride] > first ? in[l * list_stride] : first;
-    first = wave_max_u64(first);
-    if (merged) {
-      for (int i = have + threadIdx.x; i < k; i += 64) merged[row * (k + 1) + i] = 0;
-      if (threadIdx.x == 0)
-        merged[row * (k + 1) + k] = static_cast<uint64_t>(__float_as_uint(m)) << 32 |
-                                    __float_as_uint(static_cast<float>(s));
-    } else {
-      for (int i = have + threadIdx.x; i < k; i += 64) {  // (more wanted than there are)
-        Elem<T>::store1(values + row * k + i, -kInf);
-        ids[row * k + i] = -1;
+        rank += lo;
       }
+      put(rank, key);
     }
-    if (!merged && threadIdx.x == 0)
-      norm[row] = log_norm(m, s, Rank<float>::value(static_cast<uint32_t>(first >> 32)), c);
   }
+  __syncthreads();
+  for (int i = n_have + tid; i < k; i += kMergeBlock) {  // (more wanted than there are)
+    if (merged) {
+      merged[row * (k + 1) + i] = 0;
+    } else {
+      Elem<T>::store1(values + row * k + i, -kInf);
+      ids[row * k + i] = -1;
+    }
+  }
+  if (tid >= 64) return;
+  // (maximum, sum) over the lists, a lane each.
+  float m = kNegHuge;
+  for (int l = lane; l < n_lists; l += 64)
+    m = fmaxf(m, __uint_as_float(static_cast<uint32_t>(in[l * list_stride + k] >> 32)));
+  m = wave_max(m);
+  double s = 0.0;
+  for (int l = lane; l < n_lists; l += 64) {
+    const uint64_t pair = in[l * list_stride + k];
+    const double lm = __uint_as_float(static_cast<uint32_t>(pair >> 32));
+    s += static_cast<double>(__uint_as_float(static_cast<uint32_t>(pair))) *
+         exp2_64((lm - static_cast<double>(m)) * (c * kLog2e64));
+  }
+  for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+  if (lane != 0) return;
+  if (merged)
+    merged[row * (k + 1) + k] = static_cast<uint64_t>(__float_as_uint(m)) << 32 |
+                                __float_as_uint(static_cast<float>(s));
+  else
+    norm[row] = log_norm(m, s, first, c);
 }
 
 // (A temperature past these is merely very high or very low.)
@@ -579,7 +712,8 @@ int64_t width_of(int64_t n_rows, int64_t v, int k) {
   const int64_t places = 4 * static_cast<int64_t>(device_cus());
   const int64_t slabs = n_rows > 0 ? places / n_rows : 1;
   if (slabs <= 1) return v;
-  int64_t width = round_up((v + slabs - 1) / slabs, 8);
+  const int64_t most = slabs < kStaged / k ? slabs : kStaged / k;
+  int64_t width = round_up((v + most - 1) / most, 8);
   width = width > kLeast ? width : kLeast;
   return width > 16 * k ? width : 16 * k;
 }
@@ -596,17 +730,15 @@ int merge(const uint64_t* lists, int64_t list_stride, int64_t row_stride, int n_
           int64_t n_rows, int k, double c, uint64_t* merged, void* values, int64_t* ids,
           float* norm, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(n_rows)), block(kMergeBlock);
-  const int64_t bytes = static_cast<int64_t>(n_lists) * (k + 1) * 8;
-  const bool staged = bytes <= kStageBytes;
-  const unsigned lds = staged ? static_cast<unsigned>(bytes) : 0;
+  const int64_t total = static_cast<int64_t>(n_lists) * k;
+  const unsigned lds = total <= kStaged ? static_cast<unsigned>(total * 8) : 0;
   if (dtype == NMCE_F32)
     hipLaunchKernelGGL(top_merge_kernel<float>, grid, block, lds, s, lists, list_stride,
-                       row_stride, n_lists, k, staged, c, merged, static_cast<float*>(values), ids,
-                       norm);
+                       row_stride, n_lists, k, c, merged, static_cast<float*>(values), ids, norm);
   else
     hipLaunchKernelGGL(top_merge_kernel<uint16_t>, grid, block, lds, s, lists, list_stride,
-                       row_stride, n_lists, k, staged, c, merged, static_cast<uint16_t*>(values),
-                       ids, norm);
+                       row_stride, n_lists, k, c, merged, static_cast<uint16_t*>(values), ids,
+                       norm);
   return launch_status();
 }
 
@@ -642,7 +774,7 @@ int nmce_top_logits(const void* logits, int dtype, int64_t n_rows, int64_t vocab
     return NMCE_EINVAL_WORKSPACE;
   const int64_t width = width_of(n_rows, vocab_local, k);
   const int64_t slabs = (vocab_local + width - 1) / width;
-  const dim3 grid(static_cast<unsigned>(n_rows * slabs)), block(kBlock);
+  const dim3 grid(static_cast<unsigned>(n_rows * slabs));
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint64_t* lists = static_cast<uint64_t*>(workspace);
   const double c = inverse(temperature);
@@ -650,16 +782,19 @@ int nmce_top_logits(const void* logits, int dtype, int64_t n_rows, int64_t vocab
   const int bits = id_bits_of(vocab_local);
   const bool whole = slabs == 1 && !list;
   uint64_t* part = list && slabs == 1 ? reinterpret_cast<uint64_t*>(list) : lists;
+  auto run = [&](auto element, auto shape) {
+    using T = decltype(element);
+    using Shape = decltype(shape);
+    hipLaunchKernelGGL((top_kernel<T, Shape>), grid, dim3(Shape::kBlock), 0, s,
+                       static_cast<const T*>(logits), ld, vocab_local, vocab_start, slabs, width, k,
+                       bits, c2, c, part,
+                       Out<T>{static_cast<T*>(values), ids, whole ? log_normalizer : nullptr});
+  };
+  const bool few = k <= Few::kMost;
   if (dtype == NMCE_F32)
-    hipLaunchKernelGGL(top_kernel<float>, grid, block, 0, s, static_cast<const float*>(logits), ld,
-                       vocab_local, vocab_start, slabs, width, k, bits, c2, c, part,
-                       Out<float>{static_cast<float*>(values), ids, whole ? log_normalizer : nullptr});
+    few ? run(float{}, Few{}) : run(float{}, Many{});
   else
-    hipLaunchKernelGGL(top_kernel<uint16_t>, grid, block, 0, s,
-                       static_cast<const uint16_t*>(logits), ld, vocab_local, vocab_start, slabs,
-                       width, k, bits, c2, c, part,
-                       Out<uint16_t>{static_cast<uint16_t*>(values), ids,
-                                     whole ? log_normalizer : nullptr});
+    few ? run(uint16_t{}, Few{}) : run(uint16_t{}, Many{});
   if (const int st = launch_status()) return st;
   if (slabs == 1) return NMCE_OK;
   return merge(lists, k + 1, slabs * (k + 1), static_cast<int>(slabs), dtype, n_rows, k, c,
