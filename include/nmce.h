@@ -737,6 +737,21 @@ int nmce_distill_combine(void* state, int64_t state_bytes, int64_t n_rows, int k
                          void* stream);
 
 /*
+ * One rank (ids from 0, no exchange), rows of at most NMCE_DISTILL_ONE_PASS_BYTES:
+ * the loss, the state and the gradient of its mean for the upstream value
+ * expected[0] (1 if that is zero, subnormal or not finite), which goes to
+ * assumed[0], in one read of the logits; mean[0] too unless it is NULL (at most
+ * NMCE_DISTILL_MEAN_ROWS rows). gout_div: the token count. Rows of grad lie
+ * against 16-byte boundaries as the logits' rows do; grad may be logits
+ * (ld_grad == ld).
+ */
+#define NMCE_DISTILL_ONE_PASS_BYTES 262144
+#define NMCE_DISTILL_MEAN_ROWS 16384
+int nmce_distill_fwd_bwd(const nmce_distill_batch* batch, void* grad, int64_t ld_grad, void* state,
+                         int64_t state_bytes, float* loss, float* mean, const float* expected,
+                         float* assumed, float gout_div, void* stream);
+
+/*
  * grad = d loss / d logits of each row times grad_output[row * gout_stride] /
  * gout_div, over this shard; the state is the forward's. grad may be logits
  * (ld_grad == ld), else the two must not overlap. With `assumed` (one float; the

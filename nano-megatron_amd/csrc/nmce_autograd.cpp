@@ -1,5 +1,5 @@
-// The drop-in loss's one-pass path at TP = 1, and the embedding lookup, as C++
-// autograd nodes.
+// The drop-in loss's one-pass path at TP = 1, the embedding lookup, and the
+// distillation loss at TP = 1, as C++ autograd nodes.
 //
 // Forward and backward of cross_entropy.py:16-65 followed by the wrapper's
 // .mean() (:85), for the rows the one-pass kernel takes: one launch of
@@ -18,6 +18,7 @@
 // hint; the target check of cross_entropy.py:79-81 runs here too
 // (one_pass_mean_checked).
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 #include <ATen/TensorUtils.h>
 #include <ATen/core/DimVector.h>
@@ -611,6 +612,274 @@ at::Tensor embedding_entry(const at::Tensor& weight, const at::Tensor& tokens,
   return embedding(weight, tokens, vocab_start, scale, f32_out ? at::kFloat : at::kBFloat16);
 }
 
+// ---- distillation from a teacher's top logits ------------------------------------------
+// On one rank. DistillMean: nmce_distill_fwd_bwd writes the loss, the mean and its
+// gradient for the assumed upstream value in one read of the logits, as OnePassMean does.
+// Distill: two passes, each token's loss or their mean.
+
+// A batch for the C entries, and the tensors that it points into.
+struct DistillArgs {
+  at::Tensor rows, teacher, ids, norm;
+  nmce_distill_batch batch{};
+
+  DistillArgs(const at::Tensor& logits, const at::Tensor& teacher_logits,
+              const at::Tensor& teacher_ids, const c10::optional<at::Tensor>& normalizer,
+              double temperature) {
+    const int64_t V = logits.size(-1);
+    int64_t ld, t_ld, ids_ld;
+    rows = rows_of(logits, &ld);
+    teacher = rows_of(teacher_logits, &t_ld);
+    ids = rows_of(teacher_ids, &ids_ld);
+    if (normalizer.has_value() && normalizer->defined())
+      norm = normalizer->reshape({-1}).contiguous();
+    batch.logits = rows.data_ptr();
+    batch.teacher_logits = teacher.data_ptr();
+    batch.teacher_ids = ids.data_ptr<int64_t>();
+    batch.teacher_log_normalizer = norm.defined() ? norm.data_ptr<float>() : nullptr;
+    batch.ld = ld;
+    batch.teacher_ld = t_ld;
+    batch.ids_ld = ids_ld;
+    batch.n_rows = rows.size(0);
+    batch.vocab_local = batch.vocab_total = V;
+    batch.temperature = temperature;
+    batch.k = static_cast<int>(teacher.size(1));
+    batch.dtype = dtype_code(rows);
+    batch.teacher_dtype = dtype_code(teacher);
+  }
+  at::Tensor state() const {
+    const int64_t bytes = nmce_distill_state_bytes(batch.n_rows, batch.k);
+    return at::empty({bytes > 16 ? bytes : 16}, rows.options().dtype(at::kByte));
+  }
+};
+
+// What a backward hands out: under create_graph it carries a node that raises when the
+// kernels, which have no second derivative, are differentiated again.
+at::Tensor once(const at::Tensor& grad) {
+  if (!at::GradMode::is_enabled()) return grad;
+  auto raise = std::make_shared<torch::autograd::DelayedError>(
+      "nmce: the distillation loss cannot be differentiated twice", 1);
+  return (*raise)({grad.detach().requires_grad_(true)})[0];
+}
+
+at::Tensor distill_grad(AutogradContext* ctx, const at::Tensor& rows, at::Tensor out,
+                        const at::Tensor& state, const at::Tensor& go, int64_t stride,
+                        const float* assumed, float* observed) {
+  const int64_t n = rows.size(0), V = rows.size(1);
+  hipStream_t st = stream_of(rows);
+  timed("nmce_distill_bwd", st, [&] {
+    return nmce_distill_bwd(rows.data_ptr(), out.data_ptr(), dtype_code(rows), n, V,
+                            n > 1 ? rows.stride(0) : V, n > 1 ? out.stride(0) : V,
+                            static_cast<int>(ctx->saved_data["k"].toInt()),
+                            ctx->saved_data["temperature"].toDouble(), state.data_ptr(),
+                            state.numel(), go.data_ptr<float>(), stride,
+                            static_cast<float>(ctx->saved_data["divisor"].toInt()), assumed,
+                            observed, st);
+  });
+  return out;
+}
+
+void save_distill(AutogradContext* ctx, const DistillArgs& a, const at::Tensor& logits,
+                  const at::Tensor& state, bool inplace, int64_t divisor) {
+  ctx->saved_data["inplace"] = inplace;
+  ctx->saved_data["k"] = static_cast<int64_t>(a.batch.k);
+  ctx->saved_data["temperature"] = a.batch.temperature;
+  ctx->saved_data["divisor"] = divisor;
+  ctx->saved_data["shape"] = logits.sizes().vec();
+  ctx->saved_data["rows"] = a.batch.n_rows;
+  ctx->saved_data["type"] = logits.scalar_type();
+  ctx->saved_data["state"] = state.numel();
+}
+
+struct DistillMean : public torch::autograd::Function<DistillMean> {
+  // logits viewable as rows that nmce_distill_fwd_bwd takes (the wrapper checked).
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits,
+                            const at::Tensor& teacher_logits, const at::Tensor& teacher_ids,
+                            const c10::optional<at::Tensor>& normalizer, const at::Tensor& hint,
+                            double temperature, bool inplace) {
+    const c10::DeviceGuard device_guard(logits.device());
+    const DistillArgs a(logits, teacher_logits, teacher_ids, normalizer, temperature);
+    const int64_t n = a.batch.n_rows, V = a.batch.vocab_local;
+    const at::Tensor state = a.state();
+    const auto f32 = a.rows.options().dtype(at::kFloat);
+    at::Tensor loss = at::empty({n}, f32), mean = at::empty({}, f32), assumed = at::empty({1}, f32);
+    at::Tensor grad = inplace ? a.rows : at::empty({n, V}, a.rows.options());
+    hipStream_t st = stream_of(a.rows);
+    const bool own_mean = n <= NMCE_DISTILL_MEAN_ROWS;
+    timed("nmce_distill_fwd_bwd", st, [&] {
+      return nmce_distill_fwd_bwd(&a.batch, grad.data_ptr(), inplace ? a.batch.ld : V,
+                                  state.data_ptr(), state.numel(), loss.data_ptr<float>(),
+                                  own_mean ? mean.data_ptr<float>() : nullptr,
+                                  hint.data_ptr<float>(), assumed.data_ptr<float>(),
+                                  static_cast<float>(n), st);
+    });
+    save_distill(ctx, a, logits, state, inplace, n);
+    ctx->saved_data["hint"] = hint;  // itself: the backward writes into it
+    ctx->saved_data["handed_out"] = false;
+    if (inplace) {
+      torch::autograd::impl::bump_version(logits);
+      ctx->saved_data["grad_buf"] = logits.detach();
+      ctx->saved_data["ld"] = a.batch.ld;
+      ctx->save_for_backward({assumed});
+    } else {
+      ctx->save_for_backward({a.rows, state, grad, assumed});
+    }
+    return own_mean ? mean : loss.mean();
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grad_outputs) {
+    const c10::DeviceGuard device_guard(grad_outputs[0].device());
+    const at::Tensor go = grad_outputs[0].detach().reshape({1}).to(at::kFloat).contiguous();
+    const at::Tensor hint = ctx->saved_data["hint"].toTensor();
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t V = shape.back(), n = ctx->saved_data["rows"].toInt();
+    const at::Device device = grad_outputs[0].device();
+    const at::ScalarType type = ctx->saved_data["type"].toScalarType();
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor& assumed = came_back(saved.back(), device, at::kFloat, {1}, "upstream value");
+    variable_list grads(7);
+    if (ctx->saved_data["inplace"].toBool()) {
+      TORCH_CHECK(!ctx->saved_data["handed_out"].toBool(),
+                  "nmce: a second backward through an in-place one-pass loss needs the logits, "
+                  "which now hold the gradient; pass inplace=False to differentiate it twice");
+      at::Tensor grad = ctx->saved_data["grad_buf"].toTensor();
+      const int64_t ld = ctx->saved_data["ld"].toInt();
+      hipStream_t st = stream_of(grad);
+      const bool ragged = is_ragged(grad, V, ld);
+      timed(ragged ? "nmce_ce_grad_rescale_unless_ragged" : "nmce_ce_grad_rescale_unless", st, [&] {
+        return (ragged ? nmce_ce_grad_rescale_unless_ragged : nmce_ce_grad_rescale_unless)(
+            grad.data_ptr(), dtype_code(grad), n, V, ld, go.data_ptr<float>(),
+            assumed.data_ptr<float>(), hint.data_ptr<float>(), st);
+      });
+      ctx->saved_data["handed_out"] = true;
+      ctx->saved_data["grad_buf"] = at::Tensor();
+      grads[0] = once(grad);
+      return grads;
+    }
+    // Saved-tensor hooks may hand back copies of other strides.
+    const at::Tensor& held = came_back(saved[0], device, type, {n, V}, "logits");
+    const at::Tensor rows = V > 1 && held.stride(1) != 1 ? held.contiguous() : held;
+    const at::Tensor state = came_back(saved[1], device, at::kByte,
+                                       {ctx->saved_data["state"].toInt()}, "state").contiguous();
+    if (ctx->saved_data["handed_out"].toBool()) {
+      // The first backward's buffer belongs to its consumers; a new one.
+      grads[0] = once(distill_grad(ctx, rows, at::empty({n, V}, rows.options()), state, go, 0,
+                                   nullptr, nullptr).view(shape));
+      return grads;
+    }
+    const at::Tensor grad = came_back(saved[2], device, type, {n, V}, "gradient").contiguous();
+    distill_grad(ctx, rows, grad, state, go, 0, assumed.data_ptr<float>(), hint.data_ptr<float>());
+    ctx->saved_data["handed_out"] = true;
+    grads[0] = once(grad.view(shape));
+    return grads;
+  }
+};
+
+struct Distill : public torch::autograd::Function<Distill> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits,
+                            const at::Tensor& teacher_logits, const at::Tensor& teacher_ids,
+                            const c10::optional<at::Tensor>& normalizer, double temperature,
+                            bool mean, bool inplace) {
+    const c10::DeviceGuard device_guard(logits.device());
+    const DistillArgs a(logits, teacher_logits, teacher_ids, normalizer, temperature);
+    const int64_t n = a.batch.n_rows;
+    const at::Tensor state = a.state();
+    at::Tensor loss = at::empty({n}, a.rows.options().dtype(at::kFloat));
+    at::Tensor stats = at::empty({n, 5}, a.rows.options().dtype(at::kDouble));
+    hipStream_t st = stream_of(a.rows);
+    timed("nmce_distill_stats", st, [&] {
+      return nmce_distill_stats(&a.batch, state.data_ptr(), state.numel(),
+                                stats.data_ptr<double>(), st);
+    });
+    timed("nmce_distill_combine", st, [&] {
+      return nmce_distill_combine(state.data_ptr(), state.numel(), n, a.batch.k, temperature,
+                                  stats.data_ptr<double>(), 1, loss.data_ptr<float>(), st);
+    });
+    // Rows that had to be copied are not the logits' storage.
+    inplace = inplace && a.rows.data_ptr() == logits.data_ptr();
+    save_distill(ctx, a, logits, state, inplace, mean && n > 1 ? n : 1);
+    ctx->saved_data["mean"] = mean;
+    if (inplace) ctx->save_for_backward({a.rows, state, logits});
+    else ctx->save_for_backward({a.rows, state});
+    return mean ? loss.mean() : loss.view(logits.sizes().slice(0, logits.dim() - 1));
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grad_outputs) {
+    const c10::DeviceGuard device_guard(grad_outputs[0].device());
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t V = shape.back(), n = ctx->saved_data["rows"].toInt();
+    const at::Device device = grad_outputs[0].device();
+    const at::ScalarType type = ctx->saved_data["type"].toScalarType();
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor& held = came_back(saved[0], device, type, {n, V}, "logits");
+    const at::Tensor rows = V > 1 && held.stride(1) != 1 ? held.contiguous() : held;
+    const at::Tensor state = came_back(saved[1], device, at::kByte,
+                                       {ctx->saved_data["state"].toInt()}, "state").contiguous();
+    // A broadcast upstream value (a sum's or the mean's) is read where it is.
+    at::Tensor go = grad_outputs[0].detach().to(at::kFloat);
+    int64_t stride = 0;
+    if (!ctx->saved_data["mean"].toBool()) {
+      for (int64_t d = 0; d < go.dim(); ++d) stride = go.stride(d) != 0 ? 1 : stride;
+      if (stride) go = go.reshape({-1}).contiguous();
+    }
+    variable_list grads(7);
+    const bool inplace = ctx->saved_data["inplace"].toBool();
+    at::Tensor original, out;
+    if (inplace) {
+      original = came_back(saved[2], device, type, shape, "logits");
+      int64_t ld;
+      out = rows_of(original, &ld);
+    } else {
+      out = at::empty({n, V}, rows.options());
+    }
+    distill_grad(ctx, rows, out, state, go, stride, nullptr, nullptr);
+    if (inplace && out.data_ptr() == original.data_ptr()) {
+      // The logits hold the gradient: readers that saved them fail their version check.
+      torch::autograd::impl::bump_version(original);
+      grads[0] = once(original.detach());
+    } else {
+      grads[0] = once(out.view(shape));
+    }
+    return grads;
+  }
+};
+
+// The entries from Python. They read device addresses: what would hand them other kinds of
+// tensors is refused here too (the wrapper has checked the rest).
+void check_distill(const at::Tensor& logits, const at::Tensor& teacher_logits,
+                   const at::Tensor& teacher_ids, const c10::optional<at::Tensor>& normalizer) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() > 0 && logits.size(-1) > 0 &&
+                  teacher_logits.device() == logits.device() &&
+                  teacher_ids.device() == logits.device() &&
+                  teacher_ids.scalar_type() == at::kLong && teacher_logits.dim() > 0 &&
+                  teacher_ids.sizes() == teacher_logits.sizes() &&
+                  teacher_ids.sizes().slice(0, teacher_ids.dim() - 1) ==
+                      logits.sizes().slice(0, logits.dim() - 1) &&
+                  (!normalizer.has_value() ||
+                   (normalizer->device() == logits.device() &&
+                    normalizer->scalar_type() == at::kFloat &&
+                    normalizer->sizes() == logits.sizes().slice(0, logits.dim() - 1))),
+              "nmce: the distillation loss takes logits [..., vocabulary], teacher logits and "
+              "int64 ids [..., listed] and fp32 normalisers [...] on one ROCm device (there is no "
+              "CPU path)");
+}
+
+at::Tensor distill_mean(const at::Tensor& logits, const at::Tensor& teacher_logits,
+                        const at::Tensor& teacher_ids,
+                        const c10::optional<at::Tensor>& normalizer, const at::Tensor& hint,
+                        double temperature, bool inplace) {
+  check_distill(logits, teacher_logits, teacher_ids, normalizer);
+  return DistillMean::apply(logits, teacher_logits, teacher_ids, normalizer, hint, temperature,
+                            inplace);
+}
+
+at::Tensor distill(const at::Tensor& logits, const at::Tensor& teacher_logits,
+                   const at::Tensor& teacher_ids, const c10::optional<at::Tensor>& normalizer,
+                   double temperature, bool mean, bool inplace) {
+  check_distill(logits, teacher_logits, teacher_ids, normalizer);
+  return Distill::apply(logits, teacher_logits, teacher_ids, normalizer, temperature, mean,
+                        inplace);
+}
+
 void set_timing(bool on) { g_timing = on; }
 
 // (name, milliseconds) of every launch timed since the last call, in launch
@@ -661,8 +930,8 @@ at::Tensor head_output(const at::Tensor& logits, const at::Tensor& anchor) {
 }  // namespace
 
 PYBIND11_MODULE(_nmce_autograd, m) {
-  m.doc() = "The one-pass loss at TP = 1 and the embedding as C++ autograd nodes over libnmce's "
-            "C ABI.";
+  m.doc() = "The one-pass loss at TP = 1, the embedding and the distillation loss at TP = 1 as C++ "
+            "autograd nodes over libnmce's C ABI.";
   m.def("one_pass_mean", &one_pass_mean, "mean one-pass loss (forward + backward in C++)");
   m.def("one_pass_mean_checked", &one_pass_mean_checked,
         "one_pass_mean after the target check; ValueError on a target outside the vocabulary");
@@ -678,6 +947,8 @@ PYBIND11_MODULE(_nmce_autograd, m) {
   m.def("assumed_of", &assumed_of, "the assumed upstream value saved by a one-pass loss");
   m.def("embedding", &embedding_entry,
         "a vocabulary shard's scaled lookup, with the weight's dense gradient");
+  m.def("distill_mean", &distill_mean, "mean one-pass distillation loss of one rank");
+  m.def("distill", &distill, "distillation losses of one rank, or their mean, in two passes");
   m.def("set_timing", &set_timing, "time every launch with HIP events while on");
   m.def("take_timeline", &take_timeline, "(name, ms) of the launches timed since the last call");
   m.def("head_output", &head_output,

@@ -28,6 +28,7 @@ namespace {
 
 constexpr int kMaxK = NMCE_DISTILL_MAX_K;
 constexpr int kStat = 5;  // doubles of a rank's statistics of a row
+constexpr int kBufNonTemporal = 2;
 constexpr float kInf = __builtin_huge_valf();
 
 // What the list's side of a row comes to.
@@ -51,6 +52,7 @@ struct Slope {
 struct State {
   Taught* rows;
   Slope* slopes;
+  float* sums;  // outside the list, as the slope's m has it (of the one-pass forward)
   int* column;  // [n][k] of this shard; -1: none, another rank's, or said before
   float* p;
   float* z;
@@ -65,6 +67,7 @@ __host__ __device__ inline State state_of(void* base, int64_t n, int64_t k) {
   };
   s.rows = reinterpret_cast<Taught*>(take(n * static_cast<int64_t>(sizeof(Taught))));
   s.slopes = reinterpret_cast<Slope*>(take(n * static_cast<int64_t>(sizeof(Slope))));
+  s.sums = reinterpret_cast<float*>(take(n * 4));
   s.column = reinterpret_cast<int*>(take(n * k * 4));
   s.p = reinterpret_cast<float*>(take(n * k * 4));
   s.z = reinterpret_cast<float*>(take(n * k * 4));
@@ -334,6 +337,32 @@ __global__ __launch_bounds__(256) void distill_combine_kernel(State st, int64_t 
   st.slopes[row] = slope;
 }
 
+// The losses of the one-pass forward, and in one workgroup their mean (a fixed order of
+// sums in 64 bits).
+constexpr int kLossBlock = 1024;
+__global__ __launch_bounds__(kLossBlock) void distill_loss_kernel(State st, int64_t n, double c,
+                                                                  float* __restrict__ loss,
+                                                                  float* __restrict__ mean) {
+  __shared__ double part[kLossBlock / 64];
+  double sum = 0.0;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kLossBlock + threadIdx.x; row < n;
+       row += static_cast<int64_t>(gridDim.x) * kLossBlock) {
+    const Taught t = st.rows[row];
+    Slope slope;
+    const double one = loss_and_slope(t, t.any ? st.slopes[row].m : 0.0, st.sums[row], t.top,
+                                      t.sum, t.dot, c, &slope);
+    loss[row] = static_cast<float>(one);
+    sum += static_cast<float>(one);
+  }
+  if (!mean) return;
+  sum = wave_add(sum);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < kLossBlock / 64; ++w) sum += part[w];
+  mean[0] = static_cast<float>(sum / static_cast<double>(n));
+}
+
 // ---- the backward ------------------------------------------------------------------------
 // A row a workgroup: the dense elements, then the list's over them.
 template <typename T>
@@ -386,6 +415,405 @@ __global__ __launch_bounds__(kBlock) void distill_bwd_kernel(
   }
 }
 
+// ---- forward and backward in one read -----------------------------------------------------
+// Whole-vocabulary rows (one rank) held by a workgroup of 1024 threads: in registers (kLo
+// vectors a thread; two workgroups a compute unit), or the rest in LDS (kHi vectors). The
+// listed elements are set to -inf where they are held, so that the fold sees what is
+// outside; each wave does that for its own elements, one listed id after another, and
+// writes their gradients over the row's, by the lanes that stored it. The gradient is
+// that of the mean for the upstream value usable_hint(expect[0]), which goes to assumed[0];
+// loss and slopes as from distill_combine_kernel, the slopes in fp32. Vectors, edges
+// (kRagged: rows of any width and alignment, the gradient's as the logits') and buffer
+// resources as in the cross entropy's one-pass kernels. g may be x.
+constexpr int kRowBlock = 1024;
+constexpr int kRowWaves = kRowBlock / 64;
+constexpr int kWideLo = 7, kWideHi = 9;
+constexpr int kWideLdsBytes = kWideHi * kRowBlock * 16;
+static_assert(kWideLdsBytes + 2 * kRowWaves * 8 <= 160 * 1024, "");
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+// Where a row's column is held: vector `slot` of thread `owner`, element e; slot -1: the
+// thread's edge element.
+struct Place {
+  int owner, slot, e;
+};
+template <int EPV>
+__device__ __forceinline__ Place place_of(int column, int head, int nvec) {
+  const int rel = column - head;
+  if (rel < 0) return {column, -1, 0};
+  if (rel >= nvec * EPV) return {EPV + rel - nvec * EPV, -1, 0};
+  const int vec = rel / EPV;
+  return {vec % kRowBlock, vec / kRowBlock, rel % EPV};
+}
+
+// Element e (the same for all lanes) of v to -inf where `on`.
+template <typename T>
+__device__ __forceinline__ void mask_out(u32x4& v, int e, bool on) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    if constexpr (sizeof(T) == 4) {
+      if (e == d) v[d] = on ? 0xff800000u : v[d];
+    } else {
+      if (e == 2 * d) v[d] = on ? (v[d] & 0xffff0000u) | 0xff80u : v[d];
+      if (e == 2 * d + 1) v[d] = on ? (v[d] & 0xffffu) | 0xff800000u : v[d];
+    }
+  }
+}
+
+// Fold K values into (m, sum of 2^((x - m) cl)).
+template <int K>
+__device__ __forceinline__ void fold(float& m, float& s, float* f, float cl) {
+  float q = f[0];
+#pragma unroll
+  for (int k = 1; k < K; ++k) q = fmaxf(q, f[k]);
+  const float nm = fmaxf(m, q);
+#pragma unroll
+  for (int k = 0; k < K; ++k) f[k] = exp2_hw((f[k] - nm) * cl);
+#pragma unroll
+  for (int w = 1; w < K; w *= 2) {
+#pragma unroll
+    for (int k = 0; k + w < K; k += 2 * w) f[k] += f[k + w];
+  }
+  s = fmaf(s, exp2_hw((m - nm) * cl), f[0]);
+  m = nm;
+}
+
+// (m, s) of the wave, in every lane.
+__device__ __forceinline__ void wave_merge(float& m, float& s, float cl) {
+  const float wm = wave_max(m);
+  s = wave_sum(s * exp2_hw((m - wm) * cl));
+  m = wm;
+}
+
+// loss_and_slope's slope in fp32, by every wave for itself.
+__device__ __forceinline__ Slope slope_of(const Taught& t, float m, float s, float cl) {
+  const float top = t.top, sum = static_cast<float>(t.sum), r = static_cast<float>(t.r);
+  const float all_m = fmaxf(m, top);
+  const float out = exp2_hw((m - all_m) * cl);
+  const float all = fmaf(s, out, sum * exp2_hw((top - all_m) * cl));
+  const bool rest = r > 0.0f && !(s == 0.0f);
+  const float b = (static_cast<float>(t.p) + (rest ? r : 0.0f)) / all;
+  Slope o{m, b * out - (rest ? r / s : 0.0f), all_m, b};
+  if (all == 0.0f || all != all || all_m == kInf) o.a = o.b = __builtin_nanf("");
+  if (!t.any) o = Slope{0.0f, 0.0f, 0.0f, -1.0f};
+  return o;
+}
+
+// The listed ids of a row that a wave's elements hold, 64 of the list at a time.
+template <typename T>
+struct Listed {
+  static constexpr int EPV = Elem<T>::kPerVec;
+  const int* column;
+  const float* p;
+  const float* z;
+  int k, lane, wave;
+  int first;  // the list's first 64, asked for early
+  float first_p, first_z;
+
+  __device__ __forceinline__ void ask(const State& st, int64_t row, int k_, int lane_, int wave_) {
+    column = st.column + row * k_;
+    p = st.p + row * k_;
+    z = st.z + row * k_;
+    k = k_;
+    lane = lane_;
+    wave = wave_;
+    first = lane < k ? column[lane] : -1;
+    first_p = lane < k ? p[lane] : 0.0f;
+    first_z = lane < k ? z[lane] : 0.0f;
+  }
+  // use(place, column, value of `each` in the lane that holds the id) for every id of the
+  // wave's; the arguments are the same in all lanes.
+  template <typename Each, typename Use>
+  __device__ __forceinline__ void visit(int head, int nvec, Each&& each, Use&& use) const {
+    for (int base = 0; base < k; base += 64) {
+      const int j = base + lane;
+      const int c = base == 0 ? first : j < k ? column[j] : -1;
+      const bool mine = c >= 0 && place_of<EPV>(c, head, nvec).owner >> 6 == wave;
+      uint64_t who = __ballot(mine);
+      if (who == 0) continue;
+      float value = 0.0f;
+      if (mine) value = base == 0 ? each(first_p, first_z) : each(p[j], z[j]);
+      for (; who; who &= who - 1) {
+        const int src = __builtin_ctzll(who);
+        const int at = __builtin_amdgcn_readlane(c, src);
+        use(place_of<EPV>(at, head, nvec), at,
+            __int_as_float(__builtin_amdgcn_readlane(__float_as_int(value), src)));
+      }
+    }
+  }
+};
+
+template <typename T, int kVec, bool kRagged>
+__global__ __launch_bounds__(kRowBlock, 8) void distill_row_kernel(
+    const T* x, T* g, int64_t n_rows, int64_t V, int64_t ld, int64_t ldg, int k, State st,
+    float cl, const float* __restrict__ expect_in, float* __restrict__ assumed, float gdiv) {
+  using E = Elem<T>;
+  constexpr int EPV = E::kPerVec;
+  __shared__ float sm_m[2][kRowWaves];
+  __shared__ float sm_s[2][kRowWaves];
+  const float expect = usable_hint(expect_in[0]);
+  if (blockIdx.x == 0 && threadIdx.x == 0) assumed[0] = expect;
+  const float up = expect / gdiv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int head = 0;
+  int nvec = static_cast<int>(V / EPV);
+  const int row_end = static_cast<int>(V * sizeof(T));
+  auto rsrc = [&](const T* base, int64_t r, int64_t stride) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + r * stride), 0, row_end,
+                                             0x00020000);
+  };
+  auto rsrc_k = [&](const T* base, int64_t r, int64_t stride, int i) {
+    const int rest = (nvec - i * kRowBlock) * 16;
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<T*>(base + r * stride + head + i * kRowBlock * EPV), 0, rest > 0 ? rest : 0,
+        0x00020000);
+  };
+  const uint32_t voff = static_cast<uint32_t>(tid) * 16u;
+  u32x4 cur[kVec];
+  int parity = 0;
+  for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x, parity ^= 1) {
+    if constexpr (kRagged) {
+      head = static_cast<int>(head_elems(x + row * ld, V));
+      nvec = (static_cast<int>(V) - head) / EPV;
+    }
+    Listed<T> listed;
+    listed.ask(st, row, k, lane, wave);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      cur[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_k(x, row, ld, i), voff, 0,
+                                                     kBufNonTemporal);
+    const int ec =
+        kRagged ? edge_column<EPV>(tid, head, nvec, static_cast<int>(V)) : -1;
+    float edge = 0.0f;
+    if constexpr (kRagged)
+      edge = E::buf_load1(rsrc(x, row, ld), ec >= 0 ? static_cast<uint32_t>(ec) * sizeof(T)
+                                                    : static_cast<uint32_t>(row_end));
+    const Taught t = st.rows[row];
+    listed.visit(head, nvec, [](float, float) { return 0.0f; },
+                 [&](const Place& at, int, float) {
+                   const bool on = lane == (at.owner & 63);
+#pragma unroll
+                   for (int i = 0; i < kVec; ++i)
+                     if (at.slot == i) mask_out<T>(cur[i], at.e, on);
+                   if (kRagged && at.slot < 0) edge = on ? -kInf : edge;
+                 });
+    float m = kNegHuge, s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      if (tid + i * kRowBlock < nvec) {
+        u32x4 w = cur[i];
+        asm volatile("" : "+v"(w));
+        float f[EPV];
+        E::unpack(w, f);
+        fold<EPV>(m, s, f, cl);
+      }
+    }
+    if (kRagged && ec >= 0) {
+      float f[1] = {edge};
+      fold<1>(m, s, f, cl);
+    }
+    wave_merge(m, s, cl);
+    if (lane == 0) {
+      sm_m[parity][wave] = m;
+      sm_s[parity][wave] = s;
+    }
+    __syncthreads();
+    m = lane < kRowWaves ? sm_m[parity][lane] : kNegHuge;
+    s = lane < kRowWaves ? sm_s[parity][lane] : 0.0f;
+    wave_merge(m, s, cl);
+    const Slope slope = slope_of(t, m, s, cl);
+    const float scale = slope.a * up;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      u32x4 out = {0u, 0u, 0u, 0u};
+      if (t.any && tid + i * kRowBlock < nvec) {
+        u32x4 w = cur[i];
+        asm volatile("" : "+v"(w));  // unpack again from the packed row
+        float f[EPV];
+        E::unpack(w, f);
+#pragma unroll
+        for (int e = 0; e < EPV; ++e) f[e] = exp2_hw((f[e] - slope.m) * cl) * scale;
+        out = E::pack(f);
+      }
+      buffer_store_b128<kBufNonTemporal>(out, rsrc_k(g, row, ldg, i), voff);
+    }
+    const auto rg = rsrc(g, row, ldg);
+    if constexpr (kRagged)
+      E::buf_store1(t.any ? exp2_hw((edge - slope.m) * cl) * scale : 0.0f, rg,
+                    ec >= 0 ? static_cast<uint32_t>(ec) * sizeof(T)
+                            : static_cast<uint32_t>(row_end));
+    listed.visit(head, nvec,
+                 [&](float p, float z) {
+                   return (exp2_hw((z - slope.top) * cl) * slope.b - p) * up;
+                 },
+                 [&](const Place& at, int column, float value) {
+                   E::buf_store1(value, rg, lane == (at.owner & 63)
+                                                ? static_cast<uint32_t>(column) * sizeof(T)
+                                                : static_cast<uint32_t>(row_end));
+                 });
+    if (tid == kRowBlock - 64) {
+      st.slopes[row] = slope;
+      st.sums[row] = s;
+    }
+  }
+}
+
+// Rows wider than 8 vectors a thread: vectors 0 .. 6 in registers and 7 .. 15 in LDS, the
+// next row's on their way while this one's gradient is written. Every wave fills, reads and
+// masks its own part of LDS, so only the statistics need a barrier.
+template <typename T, bool kRagged>
+__global__ __launch_bounds__(kRowBlock) void distill_wide_row_kernel(
+    const T* x, T* g, int64_t n_rows, int64_t V, int64_t ld, int64_t ldg, int k, State st,
+    float cl, const float* __restrict__ expect_in, float* __restrict__ assumed, float gdiv) {
+  using E = Elem<T>;
+  constexpr int EPV = E::kPerVec;
+  extern __shared__ __align__(16) char lds_dyn[];
+  u32x4* hi = reinterpret_cast<u32x4*>(lds_dyn);  // vector kWideLo + i of thread t: hi[i * kRowBlock + t]
+  __shared__ float sm_m[2][kRowWaves];
+  __shared__ float sm_s[2][kRowWaves];
+  const float expect = usable_hint(expect_in[0]);
+  if (blockIdx.x == 0 && threadIdx.x == 0) assumed[0] = expect;
+  const float up = expect / gdiv;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  struct Geom {
+    int head, nvec, cnt;
+  };
+  auto geom = [&](int64_t r) {
+    Geom q;
+    q.head = kRagged ? static_cast<int>(head_elems(x + r * ld, V)) : 0;
+    q.nvec = (static_cast<int>(V) - q.head) / EPV;
+    q.cnt = q.nvec > tid ? (q.nvec - tid + kRowBlock - 1) / kRowBlock : 0;
+    return q;
+  };
+  auto row_rsrc = [&](const T* base, const Geom& q) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + q.head), 0, q.nvec * 16,
+                                             0x00020000);
+  };
+  const uint32_t voff = static_cast<uint32_t>(tid) * 16u;
+  u32x4 cur[kWideLo], nxt[kWideLo];
+  auto load_lo = [&](int64_t r, const Geom& q, u32x4 (&v)[kWideLo]) {
+    const auto rs = row_rsrc(x + r * ld, q);
+#pragma unroll
+    for (int i = 0; i < kWideLo; ++i)
+      if (i < q.cnt)
+        v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, voff, i * kRowBlock * 16,
+                                                     kBufNonTemporal);
+  };
+  auto load_hi = [&](int64_t r, const Geom& q) {
+    const uint64_t addr = reinterpret_cast<uint64_t>(x + r * ld + q.head);
+    i32x4_t rs;
+    rs[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(addr & 0xffffffffu));
+    rs[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(addr >> 32));
+    rs[2] = q.nvec * 16;
+    rs[3] = 0x00020000;
+#pragma unroll
+    for (int i = 0; i < kWideHi; ++i)
+      if (kWideLo + i < q.cnt)
+        raw_buffer_load_lds(rs, (lds_void_t*)(hi + i * kRowBlock + wave * 64), 16,
+                            static_cast<int>(voff) + (kWideLo + i) * kRowBlock * 16, 0, 0, 0);
+  };
+  int64_t row = blockIdx.x;
+  Geom q{};
+  Listed<T> listed{};
+  if (row < n_rows) {
+    q = geom(row);
+    listed.ask(st, row, k, lane, wave);
+    load_lo(row, q, cur);
+    load_hi(row, q);
+  }
+  int parity = 0;
+  for (; row < n_rows; row += gridDim.x, parity ^= 1) {
+    const Taught t = st.rows[row];
+    const int ec =
+        kRagged ? edge_column<EPV>(tid, q.head, q.nvec, static_cast<int>(V)) : -1;
+    float edge = 0.0f;
+    if (kRagged && ec >= 0) edge = E::load1(x + row * ld + ec);
+    // The wave's part of the row has landed.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    listed.visit(q.head, q.nvec, [](float, float) { return 0.0f; },
+                 [&](const Place& at, int, float) {
+                   const bool on = lane == (at.owner & 63);
+#pragma unroll
+                   for (int i = 0; i < kWideLo; ++i)
+                     if (at.slot == i) mask_out<T>(cur[i], at.e, on);
+                   if (at.slot >= kWideLo && on)
+                     E::store1(reinterpret_cast<T*>(hi + (at.slot - kWideLo) * kRowBlock + tid) +
+                                   at.e, -kInf);
+                   if (kRagged && at.slot < 0) edge = on ? -kInf : edge;
+                 });
+    float m = kNegHuge, s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWideLo + kWideHi; ++i) {
+      if (i < q.cnt) {
+        u32x4 w = i < kWideLo ? cur[i < kWideLo ? i : 0] : hi[(i - kWideLo) * kRowBlock + tid];
+        asm volatile("" : "+v"(w));
+        float f[EPV];
+        E::unpack(w, f);
+        fold<EPV>(m, s, f, cl);
+      }
+    }
+    if (kRagged && ec >= 0) {
+      float f[1] = {edge};
+      fold<1>(m, s, f, cl);
+    }
+    const int64_t next = row + gridDim.x;
+    Geom qn = q;
+    Listed<T> then = listed;
+    if (next < n_rows) {
+      if constexpr (kRagged) qn = geom(next);
+      then.ask(st, next, k, lane, wave);
+      load_lo(next, qn, nxt);
+    }
+    wave_merge(m, s, cl);
+    if (lane == 0) {
+      sm_m[parity][wave] = m;
+      sm_s[parity][wave] = s;
+    }
+    __syncthreads();
+    m = lane < kRowWaves ? sm_m[parity][lane] : kNegHuge;
+    s = lane < kRowWaves ? sm_s[parity][lane] : 0.0f;
+    wave_merge(m, s, cl);
+    const Slope slope = slope_of(t, m, s, cl);
+    const float scale = slope.a * up;
+    const auto grs = row_rsrc(g + row * ldg, q);
+    auto write_grad = [&](u32x4 v, int i) {
+      float f[EPV];
+      E::unpack(v, f);
+#pragma unroll
+      for (int e = 0; e < EPV; ++e)
+        f[e] = t.any ? exp2_hw((f[e] - slope.m) * cl) * scale : 0.0f;
+      buffer_store_b128<kBufNonTemporal>(E::pack(f), grs, voff + i * kRowBlock * 16);
+    };
+#pragma unroll
+    for (int i = 0; i < kWideHi; ++i)
+      if (kWideLo + i < q.cnt) write_grad(hi[i * kRowBlock + tid], kWideLo + i);
+    // The wave has read its part of LDS: the next row's may come.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next < n_rows) load_hi(next, qn);
+#pragma unroll
+    for (int i = 0; i < kWideLo; ++i)
+      if (i < q.cnt) write_grad(cur[i], i);
+    T* gr = g + row * ldg;
+    if (kRagged && ec >= 0)
+      E::store1(gr + ec, t.any ? exp2_hw((edge - slope.m) * cl) * scale : 0.0f);
+    listed.visit(q.head, q.nvec,
+                 [&](float p, float z) {
+                   return (exp2_hw((z - slope.top) * cl) * slope.b - p) * up;
+                 },
+                 [&](const Place& at, int column, float value) {
+                   if (lane == (at.owner & 63)) E::store1(gr + column, value);
+                 });
+    if (tid == kRowBlock - 64) {
+      st.slopes[row] = slope;
+      st.sums[row] = s;
+    }
+    q = qn;
+    listed = then;
+#pragma unroll
+    for (int i = 0; i < kWideLo; ++i) cur[i] = nxt[i];
+  }
+}
+
 int check_batch(const nmce_distill_batch* a) {
   if (!a) return NMCE_EINVAL_PTR;
   if ((a->dtype != NMCE_F32 && a->dtype != NMCE_BF16) ||
@@ -431,6 +859,34 @@ int launch_list(const nmce_distill_batch& a, const State& st, hipStream_t s) {
   return launch_status();
 }
 
+template <typename T, bool kRagged>
+int launch_rows(const nmce_distill_batch& a, void* grad, int64_t ldg, const State& st,
+                const float* expect, float* assumed, float gdiv, hipStream_t s) {
+  const T* x = static_cast<const T*>(a.logits);
+  T* g = static_cast<T*>(grad);
+  const float cl = log2e_over(a.temperature);
+  const int64_t per_thread = (a.vocab_local / Elem<T>::kPerVec + kRowBlock - 1) / kRowBlock;
+  const dim3 block(kRowBlock);
+  auto run = [&](auto kernel, int per_cu, int lds) {
+    const int64_t most = static_cast<int64_t>(per_cu) * device_cus();
+    const dim3 grid(static_cast<unsigned>(per_cu == 0 || a.n_rows < most ? a.n_rows : most));
+    hipLaunchKernelGGL(kernel, grid, block, lds, s, x, g, a.n_rows, a.vocab_local, a.ld, ldg, a.k,
+                       st, cl, expect, assumed, gdiv);
+  };
+  if (per_thread > 8) {
+    static std::atomic<bool> lds_ok{false};
+    const int rc = allow_lds(reinterpret_cast<const void*>(&distill_wide_row_kernel<T, kRagged>),
+                             kWideLdsBytes, lds_ok);
+    if (rc) return rc;
+    run(distill_wide_row_kernel<T, kRagged>, 1, kWideLdsBytes);
+  } else if (per_thread > 4) {
+    run(distill_row_kernel<T, 8, kRagged>, 0, 0);
+  } else {
+    run(distill_row_kernel<T, 4, kRagged>, 0, 0);
+  }
+  return launch_status();
+}
+
 }  // namespace
 }  // namespace nmce
 
@@ -441,7 +897,7 @@ extern "C" {
 int64_t nmce_distill_state_bytes(int64_t n_rows, int k) {
   if (n_rows < 0 || n_rows > (int64_t{1} << 22) || k < 1 || k > kMaxK) return -1;
   return align256(n_rows * static_cast<int64_t>(sizeof(Taught))) +
-         align256(n_rows * static_cast<int64_t>(sizeof(Slope))) + 3 * align256(n_rows * k * 4);
+         align256(n_rows * static_cast<int64_t>(sizeof(Slope))) + align256(n_rows * 4) + 3 * align256(n_rows * k * 4);
 }
 
 int nmce_distill_stats(const nmce_distill_batch* a, void* state, int64_t state_bytes,
@@ -475,6 +931,44 @@ int nmce_distill_combine(void* state, int64_t state_bytes, int64_t n_rows, int k
   hipLaunchKernelGGL(distill_combine_kernel, dim3(static_cast<unsigned>((n_rows + 255) / 256)),
                      dim3(256), 0, static_cast<hipStream_t>(stream), state_of(state, n_rows, k),
                      n_rows, 1.0 / temperature, stats, ranks, loss);
+  return launch_status();
+}
+
+int nmce_distill_fwd_bwd(const nmce_distill_batch* a, void* grad, int64_t ld_grad, void* state,
+                         int64_t state_bytes, float* loss, float* mean, const float* expected,
+                         float* assumed, float gout_div, void* stream) {
+  if (const int rc = check_batch(a)) return rc;
+  const int64_t epv = a->dtype == NMCE_F32 ? 4 : 8;
+  const uintptr_t es = 16 / epv;
+  if (a->vocab_local > NMCE_DISTILL_ONE_PASS_BYTES / static_cast<int64_t>(es) ||
+      a->vocab_start != 0 || a->vocab_total != a->vocab_local || ld_grad < a->vocab_local ||
+      (grad == a->logits && ld_grad != a->ld) || !(gout_div > 0.0f))
+    return NMCE_EINVAL_SHAPE;
+  if (a->n_rows == 0) return NMCE_OK;
+  if (!grad || !loss || !expected || !assumed) return NMCE_EINVAL_PTR;
+  if (mean && a->n_rows > NMCE_DISTILL_MEAN_ROWS) return NMCE_EINVAL_SHAPE;
+  const uintptr_t px = reinterpret_cast<uintptr_t>(a->logits),
+                  pg = reinterpret_cast<uintptr_t>(grad);
+  // Rows of the gradient lie against 16-byte boundaries as the logits' do.
+  if (pg % es || (px - pg) % 16 || ((a->ld - ld_grad) * static_cast<int64_t>(es)) % 16)
+    return NMCE_EINVAL_ALIGN;
+  if (const int rc = check_state(state, state_bytes, a->n_rows, a->k)) return rc;
+  const State st = state_of(state, a->n_rows, a->k);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (const int rc = launch_list(*a, st, s)) return rc;
+  const float gdiv = gout_div * static_cast<float>(a->temperature);
+  const bool ragged = px % 16 || a->vocab_local % epv || a->ld % epv || ld_grad % epv;
+  int rc;
+  if (a->dtype == NMCE_F32)
+    rc = ragged ? launch_rows<float, true>(*a, grad, ld_grad, st, expected, assumed, gdiv, s)
+                : launch_rows<float, false>(*a, grad, ld_grad, st, expected, assumed, gdiv, s);
+  else
+    rc = ragged ? launch_rows<uint16_t, true>(*a, grad, ld_grad, st, expected, assumed, gdiv, s)
+                : launch_rows<uint16_t, false>(*a, grad, ld_grad, st, expected, assumed, gdiv, s);
+  if (rc) return rc;
+  const int64_t blocks = mean ? 1 : (a->n_rows + kLossBlock - 1) / kLossBlock;
+  hipLaunchKernelGGL(distill_loss_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kLossBlock), 0,
+                     s, st, a->n_rows, 1.0 / a->temperature, loss, mean);
   return launch_status();
 }
 

@@ -135,8 +135,15 @@ def _check(x, t, ids, norm=None, temperature=1.0):
     again = _loss(d, t, ids, norm, temperature)
     one, = torch.autograd.grad(again, d)
     _within(one, grad / n, (slack + 4 * STEP * grad.abs()) / n, x.dtype, "mean")
+    # Without a gradient, and by two passes: sums in another order, within the same bound.
+    slack_mean = float(loss_slack.mean()) + STEP * (abs(float(want)) + 4 * float(
+        loss.abs().mean()))
     with torch.no_grad():
-        assert torch.equal(_loss(d, t, ids, norm, temperature), mean)
+        other = _loss(d, t, ids, norm, temperature)
+    two = _loss(d, t, ids, norm, temperature, one_pass=False)
+    assert abs(float(other) - float(want)) <= slack_mean and torch.equal(two.detach(), other)
+    g, = torch.autograd.grad(two, d)
+    _within(g, grad / n, (slack + 4 * STEP * grad.abs()) / n, x.dtype, "two passes")
 
 
 def _inputs(n, v, k, dtype, g, teacher_dtype=F32, temperature=1.0, spread=2.0):

@@ -231,6 +231,26 @@ def test_distill_steps_refuse_before_launch(lib):
     assert stats(ctypes.addressof(good), p, size, None, None) == -4
     for space, bytes_ in ((None, size), (p + 8, size), (p, size - 1)):
         assert stats(ctypes.addressof(good), space, bytes_, p, None) == -6
+    def one(batch=good, g=2 * p, ldg=100, space=p, bytes_=size, loss=p, mean=p, expect=p, assumed=p,
+            div=4.0):
+        return lib.nmce_distill_fwd_bwd(ctypes.addressof(batch), g, ldg, space, bytes_, loss, mean,
+                                        expect, assumed, div, None)
+
+    rows = _distill_batch(n_rows=16385)
+    assert one(_distill_batch(dtype=5)) == -1
+    for bad in (dict(batch=_distill_batch(vocab_total=200)), dict(ldg=99), dict(div=0.0),
+                dict(batch=_distill_batch(vocab_start=100, vocab_total=200)),
+                dict(batch=_distill_batch(vocab_local=65537, vocab_total=65537, ld=65537),
+                     ldg=65537),
+                dict(batch=_distill_batch(dtype=1, vocab_local=131073, vocab_total=131073,
+                                          ld=131073), ldg=131073),
+                dict(g=p, ldg=104), dict(batch=rows, bytes_=state(16385, 8))):
+        assert one(**bad) == -2, bad
+    for name in ("g", "loss", "expect", "assumed"):
+        assert one(**{name: None}) == -4
+    assert one(g=2 * p + 2) == one(g=2 * p + 4) == one(ldg=101) == -3
+    assert one(space=None) == one(space=p + 8) == one(bytes_=size - 1) == -6
+    assert one(_distill_batch(n_rows=0), g=None) == 0
     combine = lib.nmce_distill_combine
     assert combine(p, size, -1, 8, 1.0, p, 1, p, None) == -2
     assert combine(p, size, 4, 0, 1.0, p, 1, p, None) == -2
@@ -310,6 +330,11 @@ def test_distillation_refuses_shapes_and_types():
         check(teacher_logits=teacher)
     with torch.no_grad():
         check(teacher_logits=teacher)
+    x, t, ids = torch.zeros(2, 8), torch.zeros(2, 3), torch.zeros(2, 3, dtype=I64)
     with pytest.raises(RuntimeError, match="no CPU path"):
-        nmce.vocab_parallel_distillation_loss(torch.zeros(2, 8), torch.zeros(2, 3),
-                                              torch.zeros(2, 3, dtype=I64), 0, 8, ctx)
+        nmce.vocab_parallel_distillation_loss(x, t, ids, 0, 8, ctx)
+    from nmce import _lib as L
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        L.autograd_ext().distill(x, t, ids, None, 1.0, True, False)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        L.autograd_ext().distill_mean(x, t, ids, None, torch.ones(1), 1.0, False)
