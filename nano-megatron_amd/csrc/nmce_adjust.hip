@@ -7,15 +7,12 @@
 //   count > 0:                       x <- x - f count - p
 //   then x + the id's biases (in their order), and -inf where it is not allowed.
 //
-// Few of a row's ids are touched (those of the lists), so the row goes by in two
-// steps: the dense one copies it under its mask, 16 bytes a load, and the sparse one
-// writes the touched elements over it, in 64 bits rounded once. What bounds a batch is
-// one read and one write of the logits; in place, without a mask, the lists.
-//
-// A workgroup holds one sequence's counts of a slab of the vocabulary in LDS, so a
-// list is read once by every slab (from the L2 after the first) and nothing of the
-// vocabulary's size is kept in memory. The counts are integers: their order does not
-// matter.
+// A workgroup holds one sequence's counts of a slab of the vocabulary in LDS, so a list is
+// read once by every slab (from the L2 after the first) and nothing of the vocabulary's size
+// is kept in memory; the counts are integers, whose order does not matter. Then the rows go
+// by, 16 bytes a load and under their mask; the few elements with a count are formed in 64
+// bits and rounded once, in the registers, before the store. What bounds a batch is one
+// read and one write of the logits; in place only vectors with something to change move.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -28,19 +25,11 @@ namespace nmce {
 namespace {
 
 constexpr int kSlab = 8192;               // ids of a workgroup: 32 KiB of counts
+constexpr int kBiases = 512;              // biases of a slab that are summed by id in LDS
 constexpr uint32_t kPrompt = 1u << 31;    // of a count: the id is in the prompt,
 constexpr uint32_t kBiased = 1u << 30;    // has a bias,
 constexpr uint32_t kTimes = kBiased - 1;  // and comes so often in output and drafts
 constexpr float kInf = __builtin_huge_valf();
-
-// The bits of kVec allowed ids from global id g on, the first in bit 0.
-template <int kVec>
-__device__ __forceinline__ uint32_t allowed_bits(const uint32_t* __restrict__ words, int64_t g,
-                                                 int64_t total) {
-  const int64_t last = g + kVec <= total ? g + kVec - 1 : total - 1;
-  const uint64_t lo = words[g >> 5], hi = words[last >> 5];
-  return static_cast<uint32_t>((lo | hi << 32) >> (g & 31));
-}
 
 // z to T, rounded once: to bf16 through an fp32 whose last bit is set where the
 // conversion cut something off (to odd), which a second rounding cannot take for a tie.
@@ -71,15 +60,47 @@ __device__ __forceinline__ double of_sequence(const float* each, double all, int
   return each ? static_cast<double>(each[b]) : all;
 }
 
+// 16 bytes at any element's alignment, streamed.
+typedef u32x4 anywhere __attribute__((aligned(2)));
+__device__ __forceinline__ u32x4 load16(const void* p) {
+  return __builtin_nontemporal_load(static_cast<const anywhere*>(p));
+}
+__device__ __forceinline__ void store16(void* p, const u32x4& v) {
+  __builtin_nontemporal_store(v, static_cast<anywhere*>(p));
+}
+
+// Element e of a vector, by its bits.
+template <typename T>
+__device__ __forceinline__ uint32_t element(const u32x4& v, int e) {
+  constexpr int kPer = 4 / sizeof(T);
+  const int d = e / kPer;
+  const uint32_t w = d < 2 ? (d == 0 ? v[0] : v[1]) : (d == 2 ? v[2] : v[3]);
+  return kPer == 1 ? w : w >> (e % kPer * 16) & 0xffffu;
+}
+template <typename T>
+__device__ __forceinline__ void set_element(u32x4& v, int e, uint32_t bits) {
+  constexpr int kPer = 4 / sizeof(T);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const uint32_t keep = kPer == 1 ? 0u : e % kPer ? 0x0000ffffu : 0xffff0000u;
+    if (e / kPer == d) v[d] = (v[d] & keep) | bits << (kPer == 1 ? 0 : e % kPer * 16);
+  }
+}
+
 // Part `part` of sequence b's rows, slab `slab` of the vocabulary.
 template <typename T, int kBlock, bool kInPlace>
-__global__ __launch_bounds__(kBlock) void adjust_kernel(nmce_adjust_batch a, int64_t slabs,
-                                                        int64_t parts, int64_t rows_each) {
-  constexpr int kVec = Elem<T>::kPerVec;
+__global__ __launch_bounds__(kBlock, 4) void adjust_kernel(
+    nmce_adjust_batch a, int64_t slabs, int64_t parts, int64_t rows_each) {
+  using E = Elem<T>;
+  constexpr int kVec = E::kPerVec;
   constexpr int kEach = kSlab / kBlock / kVec;  // vectors of a thread
+  constexpr uint32_t kAll = (1u << kVec) - 1;
+  static_assert(kEach >= 1, "");
   __shared__ __align__(16) uint32_t count[kSlab];
-  __shared__ uint16_t touched[kSlab];
-  __shared__ int n_touched, repeated;
+  // The slab's biases where an id comes twice: its place, and at its first entry the sum.
+  __shared__ uint16_t bias_place[kBiases];
+  __shared__ double bias_sum[kBiases];
+  __shared__ int biased, repeated, wave_n[kBlock / 64];
   const int tid = threadIdx.x;
   const int64_t bp = blockIdx.x / slabs, slab = blockIdx.x - bp * slabs;
   const int64_t b = bp / parts, part = bp - b * parts;
@@ -91,22 +112,47 @@ __global__ __launch_bounds__(kBlock) void adjust_kernel(nmce_adjust_batch a, int
   const int64_t g0 = a.vocab_start + c0;  // the slab's first global id
   const T* x = static_cast<const T*>(a.logits) + b * a.logits_batch_stride + c0;
   T* y = static_cast<T*>(a.out) + b * a.out_batch_stride + c0;
+  // The first column of the thread's vector k. (Opaque to the compiler, which would keep
+  // what it can compute from each of them in registers through the rows.)
+  auto column_of = [&](int k) {
+    int t = tid * kVec;
+    asm volatile("" : "+v"(t));
+    return t + k * kBlock * kVec;
+  };
 
   // The first row's vectors are on their way while the lists are counted.
   u32x4 v[kEach];
+  uint32_t lo[kEach], hi[kEach];  // the words with the vectors' mask bits
+  auto words_of = [&](int64_t row) {
+    return a.allowed ? a.allowed + b * a.allowed_batch_stride + row * a.allowed_row_stride
+                     : nullptr;
+  };
   auto load_row = [&](int64_t row) {
-    const T* p = x + row * a.logits_row_stride;
+    if (const uint32_t* words = words_of(row)) {
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int c = (k * kBlock + tid) * kVec;
-      if (c + kVec <= width) memcpy(&v[k], p + c, 16);
+      for (int k = 0; k < kEach; ++k) {
+        // (Past the vocabulary its last word again: no load waits for a condition.)
+        const int64_t g = g0 + column_of(k), end = a.vocab_total - 1;
+        lo[k] = words[(g < end ? g : end) >> 5];
+        hi[k] = words[(g + kVec - 1 < end ? g + kVec - 1 : end) >> 5];
+      }
+    }
+    if (kInPlace) return;
+    const T* p = x + row * a.logits_row_stride;
+    if (width == kSlab) {
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) v[k] = load16(p + column_of(k));
+    } else {
+#pragma unroll
+      for (int k = 0; k < kEach; ++k)
+        if (column_of(k) + kVec <= width) v[k] = load16(p + column_of(k));
     }
   };
-  if constexpr (!kInPlace) load_row(first);
+  load_row(first);
 
   for (int i = tid * 4; i < kSlab; i += kBlock * 4)
     *reinterpret_cast<u32x4*>(count + i) = u32x4{0u, 0u, 0u, 0u};
-  if (tid == 0) n_touched = repeated = 0;
+  if (tid == 0) biased = repeated = 0;
   __syncthreads();
 
   Penalties pen;
@@ -114,21 +160,33 @@ __global__ __launch_bounds__(kBlock) void adjust_kernel(nmce_adjust_batch a, int
   pen.f = of_sequence(a.frequency, a.frequency_all, b);
   pen.p = of_sequence(a.presence, a.presence_all, b);
   if (!(pen.r > 0.0 && pen.r < static_cast<double>(kInf))) pen.r = 1.0;
+  const bool counted = !pen.none();
   // An id's place in the slab, or kSlab and above.
   auto place = [&](int64_t id) {
     const uint64_t s = static_cast<uint64_t>(id) - static_cast<uint64_t>(g0);
     return s < static_cast<uint64_t>(width) ? static_cast<int>(s) : kSlab;
   };
-  auto note = [&](int s, uint32_t old) {
-    if (old == 0) touched[atomicAdd(&n_touched, 1)] = static_cast<uint16_t>(s);
-  };
+  // kAhead ids of a thread are on their way at once: the lists come from the L2, a
+  // microsecond away.
   auto count_list = [&](const int64_t* __restrict__ ids, int64_t n, bool prompt) {
-    for (int64_t j = tid; j < n; j += kBlock) {
-      const int s = place(ids[j]);
-      if (s < kSlab) note(s, prompt ? atomicOr(&count[s], kPrompt) : atomicAdd(&count[s], 1u));
+    constexpr int kAhead = 8;
+    for (int64_t j0 = tid; j0 < n; j0 += kBlock * kAhead) {
+      int64_t id[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        // (The last one again past the end: a load under a condition would be waited for
+        // before the next.)
+        const int64_t j = j0 + i * kBlock;
+        id[i] = ids[j < n ? j : n - 1];
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int s = place(id[i]);
+        if (s < kSlab && j0 + i * kBlock < n) prompt ? atomicOr(&count[s], kPrompt) : atomicAdd(&count[s], 1u);
+      }
     }
   };
-  if (!pen.none()) {
+  if (counted) {
     if (pen.r != 1.0) count_list(a.prompt + b * a.prompt_stride, a.n_prompt, true);
     count_list(a.output + b * a.output_stride, a.n_output, false);
     count_list(a.drafts + b * a.drafts_stride, first, false);
@@ -137,83 +195,165 @@ __global__ __launch_bounds__(kBlock) void adjust_kernel(nmce_adjust_batch a, int
   const float* bias = a.bias + b * a.bias_stride;
   for (int64_t j = tid; j < a.n_bias; j += kBlock) {
     const int s = place(bias_ids[j]);
-    if (s < kSlab && (atomicOr(&count[s], kBiased) & kBiased)) repeated = 1;
+    if (s < kSlab) {
+      biased = 1;
+      if (atomicOr(&count[s], kBiased) & kBiased) repeated = 1;
+    }
   }
   __syncthreads();
+  const bool some_biased = biased != 0;
+  int summed = 0;  // biases in LDS, by id
+  bool apart = repeated != 0;
+  if (apart) {
+    // The slab's entries in their order, then each id's at the first of them: 300 biases
+    // with a few ids twice, over 100277 fp32, 65 -> 36 us.
+    for (int64_t j0 = 0; j0 < a.n_bias; j0 += kBlock) {
+      const int64_t j = j0 + tid;
+      const int s = j < a.n_bias ? place(bias_ids[j]) : kSlab;
+      const uint64_t here = __ballot(s < kSlab);
+      if ((tid & 63) == 0) wave_n[tid >> 6] = __popcll(here);
+      __syncthreads();
+      int at = summed + __popcll(here & ((uint64_t{1} << (tid & 63)) - 1));
+      for (int w = 0; w < kBlock / 64; ++w) {
+        if (w < tid >> 6) at += wave_n[w];
+        summed += wave_n[w];
+      }
+      if (s < kSlab && at < kBiases) {
+        bias_place[at] = static_cast<uint16_t>(s);
+        bias_sum[at] = bias[j];
+      }
+      __syncthreads();
+    }
+    apart = summed > kBiases;  // too many: one by one, from memory
+    if (!apart) {
+      double sum[(kBiases + kBlock - 1) / kBlock];
+      bool mine[(kBiases + kBlock - 1) / kBlock];
+#pragma unroll
+      for (int r = 0; r < (kBiases + kBlock - 1) / kBlock; ++r) {
+        const int t = r * kBlock + tid;
+        mine[r] = t < summed;
+        sum[r] = 0.0;
+        if (!mine[r]) continue;
+        const uint16_t s = bias_place[t];
+        int before = 0;
+#pragma unroll 8
+        for (int i = 0; i < summed; ++i) {
+          const bool same = bias_place[i] == s;
+          before += same && i < t;
+          sum[r] += same && i >= t ? bias_sum[i] : 0.0;
+        }
+        mine[r] = before == 0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < (kBiases + kBlock - 1) / kBlock; ++r) {
+        const int t = r * kBlock + tid;
+        if (t < summed) {
+          if (!mine[r]) bias_place[t] = kSlab;
+          bias_sum[t] = sum[r];
+        }
+      }
+      __syncthreads();
+    }
+  }
+  const bool in_lds = repeated != 0 && !apart;
 
   for (int64_t row = first; row < last; ++row) {
     const T* xr = x + row * a.logits_row_stride;
     T* yr = y + row * a.out_row_stride;
-    const uint32_t* words =
-        a.allowed ? a.allowed + b * a.allowed_batch_stride + row * a.allowed_row_stride : nullptr;
+    const uint32_t* words = words_of(row);
     auto allowed = [&](int s) {
       return !words || (words[(g0 + s) >> 5] >> ((g0 + s) & 31) & 1u);
     };
-    if (!kInPlace || words) {
 #pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        const int c = (k * kBlock + tid) * kVec;
-        if (c + kVec > width) break;
-        constexpr uint32_t kAll = (1u << kVec) - 1;
-        const uint32_t bits = words ? allowed_bits<kVec>(words, g0 + c, a.vocab_total) & kAll
-                                    : kAll;
-        if (kInPlace) {
-          // All allowed: nothing to write; none: nothing to read.
-          if (bits == kAll) continue;
-          if (bits != 0) memcpy(&v[k], xr + c, 16);
-        }
-        if (bits != kAll) {
-          float f[kVec];
-          Elem<T>::unpack(v[k], f);
+    for (int k = 0; k < kEach; ++k) {
+      const int c = column_of(k);
+      if (c + kVec > width) break;
+      // The vector's allowed ids, the first in bit 0.
+      const uint64_t both = static_cast<uint64_t>(hi[k]) << 32 | lo[k];
+      const uint32_t bits =
+          words ? static_cast<uint32_t>(both >> ((g0 + c) & 31)) & kAll : kAll;
+      uint32_t touched = 0;  // counted and allowed
+      if (counted) {
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) f[e] = bits >> e & 1u ? f[e] : -kInf;
-          v[k] = Elem<T>::pack(f);
+        for (int e = 0; e < kVec; e += 4) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(count + c + e);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) touched |= (w[i] & (kPrompt | kTimes)) ? 1u << (e + i) : 0u;
         }
-        memcpy(yr + c, &v[k], 16);
+        touched &= bits;
       }
-      // The shard's last elements, of no whole vector.
-      const int c = width / kVec * kVec + tid;
-      if (c < width) {
-        if (!allowed(c)) Elem<T>::store1(yr + c, -kInf);
-        else if (!kInPlace) yr[c] = xr[c];
+      if (kInPlace) {
+        if (bits == kAll && touched == 0) continue;  // nothing to write
+        if (bits != 0) v[k] = load16(xr + c);
       }
-      // The dense stores have reached the memory before any thread of the workgroup
+      for (; touched; touched &= touched - 1) {  // (with a bias: formed by that, below)
+        const int e = __builtin_ctz(touched);
+        const uint32_t was = element<T>(v[k], e);
+        const float f = sizeof(T) == 4 ? __uint_as_float(was)
+                                       : bf16_to_f32(static_cast<uint16_t>(was));
+        T to;
+        const uint32_t word = count[c + e];
+        if (word & kBiased) continue;
+        store_rounded(&to, pen.on(static_cast<double>(f), word));
+        uint32_t is;
+        if constexpr (sizeof(T) == 4) is = __float_as_uint(to);
+        else is = to;
+        set_element<T>(v[k], e, is);
+      }
+      if (bits != kAll) {
+        float f[kVec];
+        E::unpack(v[k], f);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) f[e] = bits >> e & 1u ? f[e] : -kInf;
+        v[k] = E::pack(f);
+      }
+      store16(yr + c, v[k]);
+    }
+    // The shard's last elements, of no whole vector.
+    const int c = width / kVec * kVec + tid;
+    if (c < width) {
+      const uint32_t word = count[c];
+      if (!allowed(c)) E::store1(yr + c, -kInf);
+      else if (!(word & kBiased) && (word & (kPrompt | kTimes)))
+        store_rounded(yr + c, pen.on(static_cast<double>(E::load1(xr + c)), word));
+      else if (!kInPlace) yr[c] = xr[c];
+    }
+    if (row + 1 < last) load_row(row + 1);
+    if (some_biased) {
+      // The row's stores have reached the memory before any thread of the workgroup
       // stores an element over them.
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-    }
-    if (!kInPlace && row + 1 < last) load_row(row + 1);
-    auto put = [&](int s, uint32_t word, double add) {
-      if (!allowed(s)) return;
-      const double z = pen.on(static_cast<double>(Elem<T>::load1(xr + s)), word);
-      store_rounded(yr + s, z + add);
-    };
-    const int n = n_touched;
-    for (int t = tid; t < n; t += kBlock) {
-      const int s = touched[t];
-      const uint32_t word = count[s];
-      if (!(word & kBiased)) put(s, word, 0.0);
-    }
-    for (int64_t j = tid; j < a.n_bias; j += kBlock) {
-      const int64_t id = bias_ids[j];
-      const int s = place(id);
-      if (s >= kSlab) continue;
-      double add = bias[j];
-      if (repeated) {
-        // The first entry of an id adds all of them, in their order.
-        bool mine = true;
-        for (int64_t i = 0; i < j && mine; ++i) mine = bias_ids[i] != id;
-        if (!mine) continue;
-        for (int64_t i = j + 1; i < a.n_bias; ++i)
-          if (bias_ids[i] == id) add += static_cast<double>(bias[i]);
+      auto put = [&](int s, double add) {
+        if (s < kSlab && allowed(s))
+          store_rounded(yr + s, pen.on(static_cast<double>(E::load1(xr + s)), count[s]) + add);
+      };
+      if (in_lds) {
+        for (int t = tid; t < summed; t += kBlock) put(bias_place[t], bias_sum[t]);
+      } else {
+        for (int64_t j = tid; j < a.n_bias; j += kBlock) {
+          const int64_t id = bias_ids[j];
+          const int s = place(id);
+          if (s >= kSlab) continue;
+          double add = bias[j];
+          if (apart) {
+            // The first entry of an id adds all of them, in their order.
+            bool mine = true;
+            for (int64_t i = 0; i < j && mine; ++i) mine = bias_ids[i] != id;
+            if (!mine) continue;
+            for (int64_t i = j + 1; i < a.n_bias; ++i)
+              if (bias_ids[i] == id) add += static_cast<double>(bias[i]);
+          }
+          put(s, add);
+        }
       }
-      put(s, count[s], add);
     }
-    if (row + 1 < last && !pen.none()) {
+    if (row + 1 < last && counted) {
       __syncthreads();  // every thread is done with this row's counts
       if (tid == 0) {
         const int s = place(a.drafts[b * a.drafts_stride + row]);
-        if (s < kSlab) note(s, atomicAdd(&count[s], 1u));
+        if (s < kSlab) atomicAdd(&count[s], 1u);
       }
       __syncthreads();
     }
@@ -268,18 +408,30 @@ int nmce_adjust_logits(const nmce_adjust_batch* a, void* stream) {
   if (in_place && (a->logits_batch_stride != a->out_batch_stride ||
                    a->logits_row_stride != a->out_row_stride))
     return NMCE_EINVAL_SHAPE;
-  const int64_t parts = 1, rows_each = a->rows;
+  // A sequence's rows go to as many workgroups as fill the card's places, each of which
+  // counts the lists again: not many where those are longer than the rows.
+  const int64_t lists = a->n_prompt + a->n_output;
+  const int64_t places = (lists <= 8192 ? 8 : 2) * static_cast<int64_t>(device_cus());
+  const int64_t want = places / (a->batch * slabs);
+  const int64_t rows_each = want <= 1 ? a->rows : (a->rows + want - 1) / want;
+  const int64_t parts = (a->rows + rows_each - 1) / rows_each;
   const dim3 grid(static_cast<unsigned>(a->batch * parts * slabs));
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto run = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, g, slabs, parts, rows_each);
   };
+  // Where there is no workgroup for every compute unit, 1024 threads share a slab.
+  const bool few = static_cast<int64_t>(grid.x) <= device_cus();
   if (a->dtype == NMCE_F32)
-    in_place ? run(adjust_kernel<float, 256, true>, 256)
-             : run(adjust_kernel<float, 256, false>, 256);
+    in_place ? few ? run(adjust_kernel<float, 1024, true>, 1024)
+                   : run(adjust_kernel<float, 256, true>, 256)
+             : few ? run(adjust_kernel<float, 1024, false>, 1024)
+                   : run(adjust_kernel<float, 256, false>, 256);
   else
-    in_place ? run(adjust_kernel<uint16_t, 256, true>, 256)
-             : run(adjust_kernel<uint16_t, 256, false>, 256);
+    in_place ? few ? run(adjust_kernel<uint16_t, 1024, true>, 1024)
+                   : run(adjust_kernel<uint16_t, 256, true>, 256)
+             : few ? run(adjust_kernel<uint16_t, 1024, false>, 1024)
+                   : run(adjust_kernel<uint16_t, 256, false>, 256);
   return launch_status();
 }
 
