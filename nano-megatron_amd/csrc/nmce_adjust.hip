@@ -46,11 +46,16 @@ __device__ __forceinline__ void store_rounded(uint16_t* p, double z) {
 }
 
 struct Penalties {
-  double r, f, p;
+  double r, f, p, inv;  // inv: 1 / r
   __device__ __forceinline__ bool none() const { return r == 1.0 && f == 0.0 && p == 0.0; }
+  // x / r by the reciprocal and one correction (an infinite x has none to take).
+  __device__ __forceinline__ double quotient(double x) const {
+    const double q = x * inv, e = fma(-q, r, x);
+    return e == e ? fma(e, inv, q) : q;
+  }
   __device__ __forceinline__ double on(double x, uint32_t word) const {
     const uint32_t times = word & kTimes;
-    if ((word & (kPrompt | kTimes)) && r != 1.0) x = x > 0.0 ? x / r : x * r;
+    if ((word & (kPrompt | kTimes)) && r != 1.0) x = x > 0.0 ? quotient(x) : x * r;
     if (times) x = x - f * static_cast<double>(times) - p;
     return x;
   }
@@ -160,11 +165,12 @@ __global__ __launch_bounds__(kBlock, 4) void adjust_kernel(
   pen.f = of_sequence(a.frequency, a.frequency_all, b);
   pen.p = of_sequence(a.presence, a.presence_all, b);
   if (!(pen.r > 0.0 && pen.r < static_cast<double>(kInf))) pen.r = 1.0;
+  pen.inv = 1.0 / pen.r;
   const bool counted = !pen.none();
   // An id's place in the slab, or kSlab and above.
   auto place = [&](int64_t id) {
-    const uint64_t s = static_cast<uint64_t>(id) - static_cast<uint64_t>(g0);
-    return s < static_cast<uint64_t>(width) ? static_cast<int>(s) : kSlab;
+    const uint32_t s = static_cast<uint32_t>(id) - static_cast<uint32_t>(g0);
+    return id >> 32 == 0 && s < static_cast<uint32_t>(width) ? static_cast<int>(s) : kSlab;
   };
   // kAhead ids of a thread are on their way at once: the lists come from the L2, a
   // microsecond away.

@@ -1,5 +1,6 @@
 // The drop-in loss's one-pass path at TP = 1, the embedding lookup, and the
-// distillation loss at TP = 1, as C++ autograd nodes.
+// distillation loss at TP = 1, as C++ autograd nodes; and the calls of the adjusted and
+// the top logits.
 //
 // Forward and backward of cross_entropy.py:16-65 followed by the wrapper's
 // .mean() (:85), for the rows the one-pass kernel takes: one launch of
@@ -880,6 +881,125 @@ at::Tensor distill(const at::Tensor& logits, const at::Tensor& teacher_logits,
                         inplace);
 }
 
+// ---- logits on their way to a sampler ---------------------------------------------------
+// No nodes (they have no derivative), but one call from Python each: through ctypes, with
+// its outputs made there, a small call took 14 to 19 us on the host, and takes 6 to 9.
+
+// Lists [batch, n] of consecutive elements: their address, stride and length.
+struct Lists {
+  at::Tensor held;
+  const void* at = nullptr;
+  int64_t stride = 0, n = 0;
+  explicit Lists(const c10::optional<at::Tensor>& t) {
+    if (!t.has_value() || !t->defined() || t->numel() == 0) return;
+    held = t->size(1) > 1 && t->stride(1) != 1 ? t->contiguous() : *t;
+    at = held.data_ptr();
+    stride = held.stride(0);
+    n = held.size(1);
+  }
+};
+
+// (The wrapper has checked the arguments; what is no address on the device is refused here.)
+at::Tensor adjust(const at::Tensor& logits, const c10::optional<at::Tensor>& prompt,
+                  const c10::optional<at::Tensor>& output,
+                  const c10::optional<at::Tensor>& drafts,
+                  const std::vector<c10::optional<at::Tensor>>& penalties,
+                  const std::vector<double>& alike, const c10::optional<at::Tensor>& bias_ids,
+                  const c10::optional<at::Tensor>& bias,
+                  const c10::optional<at::Tensor>& allowed, int64_t vocab_start,
+                  int64_t vocab_total, bool inplace) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 3 && penalties.size() == 3 && alike.size() == 3,
+              "nmce: logits are adjusted as [batch, rows, vocabulary] on a ROCm device (there is "
+              "no CPU path)");
+  for (const auto* t : {&prompt, &output, &drafts, &bias_ids, &bias, &allowed, &penalties[0],
+                        &penalties[1], &penalties[2]})
+    TORCH_CHECK(!t->has_value() || (*t)->device() == logits.device(),
+                "nmce: lists, penalties and masks on another device than the logits");
+  const c10::DeviceGuard device_guard(logits.device());
+  const int64_t v = logits.size(2);
+  const at::Tensor x =
+      inplace || v == 1 || logits.stride(2) == 1 ? logits.detach() : logits.detach().contiguous();
+  at::Tensor out = inplace ? logits : at::empty(logits.sizes(), logits.options());
+  const Lists p(prompt), o(output), d(drafts), bi(bias_ids), bv(bias);
+  at::Tensor mask, each[3];
+  if (allowed.has_value())
+    mask = allowed->size(2) > 1 && allowed->stride(2) != 1 ? allowed->contiguous() : *allowed;
+  const float* values[3] = {nullptr, nullptr, nullptr};
+  for (int i = 0; i < 3; ++i) {
+    if (!penalties[i].has_value()) continue;
+    each[i] = penalties[i]->contiguous();
+    values[i] = each[i].data_ptr<float>();
+  }
+  nmce_adjust_batch a{};
+  a.logits = x.data_ptr();
+  a.out = out.data_ptr();
+  a.prompt = static_cast<const int64_t*>(p.at);
+  a.output = static_cast<const int64_t*>(o.at);
+  a.drafts = static_cast<const int64_t*>(d.at);
+  a.bias_ids = static_cast<const int64_t*>(bi.at);
+  a.bias = static_cast<const float*>(bv.at);
+  a.allowed = mask.defined() ? static_cast<const uint32_t*>(mask.data_ptr()) : nullptr;
+  a.repetition = values[0];
+  a.frequency = values[1];
+  a.presence = values[2];
+  a.logits_batch_stride = x.stride(0);
+  a.logits_row_stride = x.stride(1);
+  a.out_batch_stride = out.stride(0);
+  a.out_row_stride = out.stride(1);
+  a.prompt_stride = p.stride;
+  a.output_stride = o.stride;
+  a.drafts_stride = d.stride;
+  a.bias_ids_stride = bi.stride;
+  a.bias_stride = bv.stride;
+  a.allowed_batch_stride = mask.defined() ? mask.stride(0) : 0;
+  a.allowed_row_stride = mask.defined() ? mask.stride(1) : 0;
+  a.n_prompt = p.n;
+  a.n_output = o.n;
+  a.n_bias = bi.n;
+  a.batch = logits.size(0);
+  a.rows = logits.size(1);
+  a.vocab_local = v;
+  a.vocab_start = vocab_start;
+  a.vocab_total = vocab_total;
+  a.repetition_all = alike[0];
+  a.frequency_all = alike[1];
+  a.presence_all = alike[2];
+  a.dtype = dtype_code(x);
+  hipStream_t st = stream_of(x);
+  timed("nmce_adjust_logits", st, [&] { return nmce_adjust_logits(&a, st); });
+  // (Inference tensors have no version.)
+  if (inplace && !logits.is_inference()) torch::autograd::impl::bump_version(logits);
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> top(const at::Tensor& logits, int64_t k,
+                                                   double temperature) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() > 0,
+              "nmce: top logits are taken on a ROCm device (there is no CPU path)");
+  const c10::DeviceGuard device_guard(logits.device());
+  std::vector<int64_t> lead = logits.sizes().vec();
+  const int64_t v = lead.back();
+  lead.pop_back();
+  std::vector<int64_t> shape = lead;
+  shape.push_back(k);
+  at::Tensor values = at::empty(shape, logits.options());
+  at::Tensor ids = at::empty(shape, logits.options().dtype(at::kLong));
+  at::Tensor norm = at::empty(lead, logits.options().dtype(at::kFloat));
+  if (logits.numel() == 0) return {values, ids, norm};
+  int64_t ld;
+  const at::Tensor rows = rows_of(logits.detach(), &ld);
+  const int64_t n = rows.size(0);
+  const int64_t bytes = nmce_top_workspace_bytes(n, v, static_cast<int>(k));
+  at::Tensor ws = at::empty({bytes > 16 ? bytes : 16}, logits.options().dtype(at::kByte));
+  hipStream_t st = stream_of(rows);
+  timed("nmce_top_logits", st, [&] {
+    return nmce_top_logits(rows.data_ptr(), dtype_code(rows), n, v, ld, 0, static_cast<int>(k),
+                           temperature, nullptr, values.data_ptr(), ids.data_ptr<int64_t>(),
+                           norm.data_ptr<float>(), ws.data_ptr(), ws.numel(), st);
+  });
+  return {values, ids, norm};
+}
+
 void set_timing(bool on) { g_timing = on; }
 
 // (name, milliseconds) of every launch timed since the last call, in launch
@@ -949,6 +1069,8 @@ PYBIND11_MODULE(_nmce_autograd, m) {
         "a vocabulary shard's scaled lookup, with the weight's dense gradient");
   m.def("distill_mean", &distill_mean, "mean one-pass distillation loss of one rank");
   m.def("distill", &distill, "distillation losses of one rank, or their mean, in two passes");
+  m.def("adjust", &adjust, "penalties, biases and masks on logits, in one call");
+  m.def("top", &top, "a rank's top logits, their ids and the rows' log-normalisers");
   m.def("set_timing", &set_timing, "time every launch with HIP events while on");
   m.def("take_timeline", &take_timeline, "(name, ms) of the launches timed since the last call");
   m.def("head_output", &head_output,

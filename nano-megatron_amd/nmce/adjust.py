@@ -18,13 +18,11 @@ exchanged. There is no derivative and no CPU path.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
 from . import _lib
-from .cross_entropy import _launch
 
 MAX_BIASES = 8192  # of one sequence (NMCE_ADJUST_MAX_BIASES)
 
@@ -94,15 +92,6 @@ def _overlaps_itself(t: torch.Tensor) -> bool:
     return False
 
 
-def _lists(t: torch.Tensor | None) -> tuple[torch.Tensor | None, int, int]:
-    """``(t, address, stride)`` of lists ``[batch, n]`` of consecutive elements."""
-    if t is None or t.numel() == 0:
-        return None, 0, 0
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t, t.data_ptr(), t.stride(0)
-
-
 def vocab_parallel_adjust_logits(
     logits: torch.Tensor,
     vocab_start: int,
@@ -142,48 +131,17 @@ def vocab_parallel_adjust_logits(
                   (("repetition_penalty", repetition_penalty),
                    ("frequency_penalty", frequency_penalty),
                    ("presence_penalty", presence_penalty)), bias_ids, bias_values, allowed)
-    b, rows, v = logits.shape
-    lib = _lib.load()
-    dev = logits.device
+    v = logits.shape[2]
     if inplace:
         if v > 1 and logits.stride(2) != 1:
             raise ValueError("nmce: logits that are written in place must have a contiguous "
                              "vocabulary")
         if _overlaps_itself(logits):
             raise ValueError("nmce: logits that are written in place must not overlap themselves")
-        x = out = logits
-    else:
-        x = logits if logits.stride(2) == 1 or v == 1 else logits.contiguous()
-        out = torch.empty((b, rows, v), dtype=logits.dtype, device=dev)
-    if b == 0:
-        return out
-    prompt, prompt_at, prompt_ld = _lists(prompt_tokens)
-    output, output_at, output_ld = _lists(output_tokens)
-    drafts, drafts_at, drafts_ld = _lists(draft_tokens)
-    ids, ids_at, ids_ld = _lists(bias_ids)
-    values, values_at, values_ld = _lists(bias_values)
-    if allowed is not None and allowed.shape[2] > 1 and allowed.stride(2) != 1:
-        allowed = allowed.contiguous()
-    each, alike = [], []
-    for value in (repetition_penalty, frequency_penalty, presence_penalty):
-        held = value.contiguous() if isinstance(value, torch.Tensor) else None
-        each.append(held)
-        alike.append(0.0 if held is not None else float(value))
-    batch = _lib.AdjustBatch(
-        x.data_ptr(), out.data_ptr(), prompt_at, output_at, drafts_at, ids_at, values_at,
-        allowed.data_ptr() if allowed is not None else None,
-        *(t.data_ptr() if t is not None else None for t in each),
-        x.stride(0), x.stride(1), out.stride(0), out.stride(1),
-        prompt_ld, output_ld, drafts_ld, ids_ld, values_ld,
-        allowed.stride(0) if allowed is not None else 0,
-        allowed.stride(1) if allowed is not None else 0,
-        prompt.shape[1] if prompt is not None else 0,
-        output.shape[1] if output is not None else 0,
-        ids.shape[1] if ids is not None else 0,
-        b, rows, v, vocab_start, ctx.tp_size * v, *alike, _lib.dtype_code(x.dtype))
-    with torch.cuda.device(dev):
-        _launch("nmce_adjust_logits", lib.nmce_adjust_logits, ctypes.addressof(batch),
-                _lib.stream_handle(dev))
-    if inplace and not logits.is_inference():  # (inference tensors have no version)
-        torch.autograd.graph.increment_version(logits)
-    return out
+    penalties = (repetition_penalty, frequency_penalty, presence_penalty)
+    tensors = [isinstance(t, torch.Tensor) for t in penalties]
+    return _lib.autograd_ext().adjust(
+        logits, prompt_tokens, output_tokens, draft_tokens,
+        [t if is_tensor else None for t, is_tensor in zip(penalties, tensors)],
+        [0.0 if is_tensor else float(t) for t, is_tensor in zip(penalties, tensors)],
+        bias_ids, bias_values, allowed, vocab_start, ctx.tp_size * v, inplace)

@@ -62,9 +62,13 @@ def vocab_parallel_top_logits(
     and the normaliser -inf); -0 comes back as 0.
     """
     _check_top(logits, k, vocab_start, vocab_end, ctx, temperature)
+    temperature = float(temperature)
+    tp = ctx.tp_size
+    if tp == 1:
+        return _lib.autograd_ext().top(logits, k, temperature)
     lib = _lib.load()
     dev = logits.device
-    lead, v, tp = tuple(logits.shape[:-1]), logits.shape[-1], ctx.tp_size
+    lead, v = tuple(logits.shape[:-1]), logits.shape[-1]
     values = torch.empty(lead + (k,), dtype=logits.dtype, device=dev)
     ids = torch.empty(lead + (k,), dtype=torch.int64, device=dev)
     norm = torch.empty(lead, dtype=torch.float32, device=dev)
@@ -74,19 +78,13 @@ def vocab_parallel_top_logits(
     n = rows.shape[0]
     code = _lib.dtype_code(rows.dtype)
     ws = torch.empty(max(16, lib.nmce_top_workspace_bytes(n, v, k)), dtype=torch.uint8, device=dev)
-    out = values.data_ptr(), ids.data_ptr(), norm.data_ptr()
     with torch.cuda.device(dev):
         stream = _lib.stream_handle(dev)
-        if tp == 1:
-            _launch("nmce_top_logits", lib.nmce_top_logits, rows.data_ptr(), code, n, v, ld,
-                    vocab_start, k, float(temperature), None, *out, ws.data_ptr(), ws.numel(),
-                    stream)
-            return values, ids, norm
         part = torch.empty((1, n, k + 1), dtype=torch.int64, device=dev)
         _launch("nmce_top_logits", lib.nmce_top_logits, rows.data_ptr(), code, n, v, ld,
-                vocab_start, k, float(temperature), part.data_ptr(), None, None, None,
-                ws.data_ptr(), ws.numel(), stream)
+                vocab_start, k, temperature, part.data_ptr(), None, None, None, ws.data_ptr(),
+                ws.numel(), stream)
         parts = _all_gather_rows(part, ctx.tp_group, tp)
         _launch("nmce_top_merge", lib.nmce_top_merge, parts.data_ptr(), tp, code, n, k,
-                float(temperature), *out, stream)
+                temperature, values.data_ptr(), ids.data_ptr(), norm.data_ptr(), stream)
     return values, ids, norm
