@@ -74,6 +74,33 @@ __host__ __device__ inline State state_of(void* base, int64_t n, int64_t k) {
   return s;
 }
 
+// 16 bytes at any element's alignment, streamed.
+typedef u32x4 anywhere __attribute__((aligned(2)));
+__device__ __forceinline__ u32x4 load16(const void* p) {
+  return __builtin_nontemporal_load(static_cast<const anywhere*>(p));
+}
+__device__ __forceinline__ void store16(void* p, const u32x4& v) {
+  __builtin_nontemporal_store(v, static_cast<anywhere*>(p));
+}
+
+// Fold K values into (m, sum of 2^((x - m) cl)).
+template <int K>
+__device__ __forceinline__ void fold(float& m, float& s, float* f, float cl) {
+  float q = f[0];
+#pragma unroll
+  for (int k = 1; k < K; ++k) q = fmaxf(q, f[k]);
+  const float nm = fmaxf(m, q);
+#pragma unroll
+  for (int k = 0; k < K; ++k) f[k] = exp2_hw((f[k] - nm) * cl);
+#pragma unroll
+  for (int w = 1; w < K; w *= 2) {
+#pragma unroll
+    for (int k = 0; k + w < K; k += 2 * w) f[k] += f[k + w];
+  }
+  s = fmaf(s, exp2_hw((m - nm) * cl), f[0]);
+  m = nm;
+}
+
 __device__ __forceinline__ double wave_add(double v) {
   for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
   return v;
@@ -226,35 +253,32 @@ __global__ __launch_bounds__(kBlock) void distill_stats_kernel(nmce_distill_batc
       if (at >= 0 && at < width) atomicOr(&bits[at >> 5], 1u << (at & 31));
     }
     __syncthreads();
-    for (int i = tid * EPV; i < width; i += kBlock * EPV) {
+    auto take = [&](int i, const u32x4& v) {
       float f[EPV];
-      if (i + EPV <= width) {
-        u32x4 v;
-        memcpy(&v, x + c0 + i, 16);
-        E::unpack(v, f);
-      } else {
-#pragma unroll
-        for (int e = 0; e < EPV; ++e) f[e] = i + e < width ? E::load1(x + c0 + i + e) : -kInf;
-      }
+      E::unpack(v, f);
       const uint32_t on = bits[i >> 5] >> (i & 31) & ((1u << EPV) - 1);
       if (on) {
 #pragma unroll
         for (int e = 0; e < EPV; ++e) f[e] = on >> e & 1u ? -kInf : f[e];
       }
-      float q = f[0];
-#pragma unroll
-      for (int e = 1; e < EPV; ++e) q = fmaxf(q, f[e]);
-      const float nm = fmaxf(m, q);
-      float y[EPV];
-#pragma unroll
-      for (int e = 0; e < EPV; ++e) y[e] = exp2_hw((f[e] - nm) * cl);
-#pragma unroll
-      for (int w = 1; w < EPV; w *= 2) {
-#pragma unroll
-        for (int e = 0; e + w < EPV; e += 2 * w) y[e] += y[e + w];
+      fold<EPV>(m, s, f, cl);
+    };
+    // Two vectors on their way at a time.
+    int i = tid * EPV;
+    for (; i + kBlock * EPV + EPV <= width; i += 2 * kBlock * EPV) {
+      const u32x4 v0 = load16(x + c0 + i), v1 = load16(x + c0 + i + kBlock * EPV);
+      take(i, v0);
+      take(i + kBlock * EPV, v1);
+    }
+    for (; i < width; i += kBlock * EPV) {
+      if (i + EPV <= width) {
+        take(i, load16(x + c0 + i));
+      } else {
+        for (int j = i; j < width; ++j) {
+          float f[1] = {bits[j >> 5] >> (j & 31) & 1u ? -kInf : E::load1(x + c0 + j)};
+          fold<1>(m, s, f, cl);
+        }
       }
-      s = fmaf(s, exp2_hw((m - nm) * cl), y[0]);
-      m = nm;
     }
     __syncthreads();
   }
@@ -337,31 +361,44 @@ __global__ __launch_bounds__(256) void distill_combine_kernel(State st, int64_t 
   st.slopes[row] = slope;
 }
 
-// The losses of the one-pass forward, and in one workgroup their mean (a fixed order of
-// sums in 64 bits).
+// The losses of the one-pass forward, and their mean where one workgroup has all rows; of
+// more, distill_mean_kernel's (8192 rows: 25 us in one workgroup, 5 and 4 in the two).
+// Sums in a fixed order, in 64 bits.
 constexpr int kLossBlock = 1024;
+constexpr int kLossRows = 64;  // of a workgroup, where there are several
+__device__ __forceinline__ void store_mean(double sum, int64_t n, float* __restrict__ mean) {
+  __shared__ double part[kLossBlock / 64];
+  sum = wave_add(sum);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < static_cast<int>(blockDim.x >> 6); ++w) sum += part[w];
+  mean[0] = static_cast<float>(sum / static_cast<double>(n));
+}
 __global__ __launch_bounds__(kLossBlock) void distill_loss_kernel(State st, int64_t n, double c,
                                                                   float* __restrict__ loss,
                                                                   float* __restrict__ mean) {
-  __shared__ double part[kLossBlock / 64];
   double sum = 0.0;
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * kLossBlock + threadIdx.x; row < n;
-       row += static_cast<int64_t>(gridDim.x) * kLossBlock) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (row < n) {
     const Taught t = st.rows[row];
     Slope slope;
     const double one = loss_and_slope(t, t.any ? st.slopes[row].m : 0.0, st.sums[row], t.top,
                                       t.sum, t.dot, c, &slope);
     loss[row] = static_cast<float>(one);
-    sum += static_cast<float>(one);
+    sum = static_cast<float>(one);
   }
-  if (!mean) return;
-  sum = wave_add(sum);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int w = 1; w < kLossBlock / 64; ++w) sum += part[w];
-  mean[0] = static_cast<float>(sum / static_cast<double>(n));
+  if (mean) store_mean(sum, n, mean);
 }
+__global__ __launch_bounds__(kLossBlock) void distill_mean_kernel(const float* __restrict__ loss,
+                                                                  int64_t n,
+                                                                  float* __restrict__ mean) {
+  double sum = 0.0;
+  for (int64_t row = threadIdx.x; row < n; row += kLossBlock) sum += loss[row];
+  store_mean(sum, n, mean);
+}
+
+constexpr int kBwdAhead = 4;  // vectors of a thread on their way
 
 // ---- the backward ------------------------------------------------------------------------
 // A row a workgroup: the dense elements, then the list's over them.
@@ -385,20 +422,28 @@ __global__ __launch_bounds__(kBlock) void distill_bwd_kernel(
     const float scale = s.a * up;
     const T* xr = x + row * ld;
     T* gr = g + row * ldg;
-    for (int64_t i = tid * EPV; i < v; i += kBlock * EPV) {
-      float f[EPV], y[EPV];
-      if (i + EPV <= v) {
-        u32x4 w;
-        memcpy(&w, xr + i, 16);
-        E::unpack(w, f);
+    auto slope_at = [&](float f) { return taught ? exp2_hw((f - s.m) * cl) * scale : 0.0f; };
+    auto put = [&](int64_t i, const u32x4& w) {
+      float f[EPV];
+      E::unpack(w, f);
 #pragma unroll
-        for (int e = 0; e < EPV; ++e) y[e] = taught ? exp2_hw((f[e] - s.m) * cl) * scale : 0.0f;
-        w = E::pack(y);
-        memcpy(gr + i, &w, 16);
+      for (int e = 0; e < EPV; ++e) f[e] = slope_at(f[e]);
+      store16(gr + i, E::pack(f));
+    };
+    constexpr int kStep = kBlock * EPV;
+    int64_t i = tid * EPV;
+    for (; i + (kBwdAhead - 1) * kStep + EPV <= v; i += kBwdAhead * kStep) {
+      u32x4 w[kBwdAhead];
+#pragma unroll
+      for (int u = 0; u < kBwdAhead; ++u) w[u] = load16(xr + i + u * kStep);
+#pragma unroll
+      for (int u = 0; u < kBwdAhead; ++u) put(i + u * kStep, w[u]);
+    }
+    for (; i < v; i += kStep) {
+      if (i + EPV <= v) {
+        put(i, load16(xr + i));
       } else {
-        for (int e = 0; i + e < v; ++e)
-          E::store1(gr + i + e,
-                    taught ? exp2_hw((E::load1(xr + i + e) - s.m) * cl) * scale : 0.0f);
+        for (int64_t j = i; j < v; ++j) E::store1(gr + j, slope_at(E::load1(xr + j)));
       }
     }
     // The dense stores have reached the memory before an element is stored over them.
@@ -458,24 +503,6 @@ __device__ __forceinline__ void mask_out(u32x4& v, int e, bool on) {
       if (e == 2 * d + 1) v[d] = on ? (v[d] & 0xffffu) | 0xff800000u : v[d];
     }
   }
-}
-
-// Fold K values into (m, sum of 2^((x - m) cl)).
-template <int K>
-__device__ __forceinline__ void fold(float& m, float& s, float* f, float cl) {
-  float q = f[0];
-#pragma unroll
-  for (int k = 1; k < K; ++k) q = fmaxf(q, f[k]);
-  const float nm = fmaxf(m, q);
-#pragma unroll
-  for (int k = 0; k < K; ++k) f[k] = exp2_hw((f[k] - nm) * cl);
-#pragma unroll
-  for (int w = 1; w < K; w *= 2) {
-#pragma unroll
-    for (int k = 0; k + w < K; k += 2 * w) f[k] += f[k + w];
-  }
-  s = fmaf(s, exp2_hw((m - nm) * cl), f[0]);
-  m = nm;
 }
 
 // (m, s) of the wave, in every lane.
@@ -966,9 +993,16 @@ int nmce_distill_fwd_bwd(const nmce_distill_batch* a, void* grad, int64_t ld_gra
     rc = ragged ? launch_rows<uint16_t, true>(*a, grad, ld_grad, st, expected, assumed, gdiv, s)
                 : launch_rows<uint16_t, false>(*a, grad, ld_grad, st, expected, assumed, gdiv, s);
   if (rc) return rc;
-  const int64_t blocks = mean ? 1 : (a->n_rows + kLossBlock - 1) / kLossBlock;
-  hipLaunchKernelGGL(distill_loss_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kLossBlock), 0,
-                     s, st, a->n_rows, 1.0 / a->temperature, loss, mean);
+  const bool one = a->n_rows <= kLossBlock && mean;
+  const int threads = one ? static_cast<int>(round_up(a->n_rows, 64)) : kLossRows;
+  const dim3 blocks(static_cast<unsigned>((a->n_rows + threads - 1) / threads));
+  hipLaunchKernelGGL(distill_loss_kernel, blocks, dim3(threads), 0, s, st, a->n_rows,
+                     1.0 / a->temperature, loss, one ? mean : nullptr);
+  if (mean && !one) {
+    if (const int rc2 = launch_status()) return rc2;
+    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(kLossBlock), 0, s, loss, a->n_rows,
+                       mean);
+  }
   return launch_status();
 }
 
