@@ -105,17 +105,20 @@ __device__ __forceinline__ double wave_add(double v) {
   for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
   return v;
 }
-__device__ __forceinline__ float wave_maxf(float v) {
-  for (int s = 32; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor(v, s));
-  return v;
+// exp(lp) of a log-probability (far above 0, as from a normaliser that is none, infinite).
+__device__ __forceinline__ double probability(double lp) {
+  return lp > 700.0 ? static_cast<double>(kInf) : exp2_64(lp * kLog2e64);
 }
 
 // ---- the list's side ------------------------------------------------------------
 constexpr int kListWaves = 4;
 
-template <typename T, typename TT>
+// kWhole: no normaliser, the teacher's distribution is over the list. The student's sum is
+// in fp32 terms, as the one outside the list is.
+template <typename T, typename TT, bool kWhole>
 __global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(nmce_distill_batch a,
-                                                                       int table, State st) {
+                                                                       int table, float cl,
+                                                                       State st) {
   extern __shared__ int tables[];  // `table` slots a wave: ids noted, 0 for none
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kListWaves + wave;
@@ -127,6 +130,10 @@ __global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(nmce_dist
   const double c = 1.0 / a.temperature;
   const int64_t base = row * a.k;
   auto held = [&](int64_t id) { return id >= 0 && id < a.vocab_total; };
+  auto column_of = [&](int64_t id) {
+    const int64_t at = id - a.vocab_start;
+    return held(id) && at >= 0 && at < a.vocab_local ? static_cast<int>(at) : -1;
+  };
 
   for (int i = lane; i < table; i += 64) seen[i] = 0;
   __builtin_amdgcn_wave_barrier();
@@ -134,12 +141,14 @@ __global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(nmce_dist
   bool any = false, again = false;
   for (int j = lane; j < a.k; j += 64) {
     const int64_t id = ids[j];
+    const int at = column_of(id);
+    const float zj = at >= 0 ? Elem<T>::load1(x + at) : -kInf;
+    st.z[base + j] = zj;
+    top = fmaxf(top, zj);
     if (!held(id)) continue;
     any = true;
     const float tj = Elem<TT>::load1(t + j);
     top_t = tj > top_t || tj != tj ? tj : top_t;
-    const int64_t at = id - a.vocab_start;
-    if (at >= 0 && at < a.vocab_local) top = fmaxf(top, Elem<T>::load1(x + at));
     // Whether another place names the id: the table holds each once.
     const int mark = static_cast<int>(id) + 1;
     uint32_t h = static_cast<uint32_t>(mark) * 2654435761u >> 7;
@@ -154,56 +163,72 @@ __global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(nmce_dist
   }
   any = __any(any);
   again = __any(again);
-  for (int s = 32; s > 0; s >>= 1) {
-    const float o = __shfl_xor(top_t, s);
-    top_t = o > top_t || o != o ? o : top_t;
+  top = wave_max(fmaxf(top, kNegHuge));
+  double norm = 0.0;
+  if constexpr (kWhole) {
+    for (int s = 32; s > 0; s >>= 1) {
+      const float o = __shfl_xor(top_t, s);
+      top_t = o > top_t || o != o ? o : top_t;
+    }
+    if (top_t == -kInf) any = false;  // no distribution
+    if (any) {
+      double sum = 0.0;
+      for (int j = lane; j < a.k; j += 64)
+        if (held(ids[j]))
+          sum += exp2_64((static_cast<double>(Elem<TT>::load1(t + j)) - top_t) * (c * kLog2e64));
+      norm = static_cast<double>(top_t) * c + log(wave_add(sum));
+    }
+  } else {
+    norm = static_cast<double>(a.teacher_log_normalizer[row]);
   }
-  top = wave_maxf(top);
-  const bool whole = a.teacher_log_normalizer == nullptr;
-  if (whole && top_t == -kInf) any = false;  // no distribution
-  double norm = whole ? 0.0 : static_cast<double>(a.teacher_log_normalizer[row]);
-  if (whole && any) {
-    double sum = 0.0;
-    for (int j = lane; j < a.k; j += 64)
-      if (held(ids[j]))
-        sum += exp2_64((static_cast<double>(Elem<TT>::load1(t + j)) - top_t) * (c * kLog2e64));
-    norm = static_cast<double>(top_t) * c + log(wave_add(sum));
-  }
+  // (The table is done with; of a list that names an id twice p and ids come there.)
+  float* held_p = reinterpret_cast<float*>(seen);
+  int* held_at = seen + a.k;
   double p_all = 0.0, h = 0.0, dot = 0.0, sum = 0.0;
   for (int j = lane; j < a.k; j += 64) {
     const int64_t id = ids[j];
-    int column = -1;
-    float pj = 0.0f, zj = 0.0f;
+    const int at = any ? column_of(id) : -1;
+    double p = 0.0;
     if (any && held(id)) {
       const double lp = static_cast<double>(Elem<TT>::load1(t + j)) * c - norm;
-      const double p = lp > 700.0 ? exp(lp) : exp2_64(lp * kLog2e64);
+      p = probability(lp);
       p_all += p;
-      if (p > 0.0 || p != p) h += p * lp;
-      const int64_t at = id - a.vocab_start;
-      if (at >= 0 && at < a.vocab_local) {
-        zj = Elem<T>::load1(x + at);
-        if (p > 0.0 || p != p) dot += p * (static_cast<double>(zj) * c);
-        bool first = true;
-        double p_id = p;
-        if (again) {
-          for (int i = 0; i < j && first; ++i) first = ids[i] != id;
-          if (first)
-            for (int i = j + 1; i < a.k; ++i)
-              if (ids[i] == id) {
-                const double l = static_cast<double>(Elem<TT>::load1(t + i)) * c - norm;
-                p_id += l > 700.0 ? exp(l) : exp2_64(l * kLog2e64);
-              }
-        }
-        if (first) {
-          column = static_cast<int>(at);
-          pj = static_cast<float>(p_id);
-          sum += zj == top ? 1.0 : exp2_64((static_cast<double>(zj) - top) * (c * kLog2e64));
-        }
+      const bool some = p > 0.0 || p != p;
+      if (some) h += p * lp;
+      if (at >= 0) {
+        const float zj = st.z[base + j];  // (the lane's own store)
+        if (some) dot += p * (static_cast<double>(zj) * c);
+        sum += exp2_hw((zj - top) * cl);
       }
     }
-    st.column[base + j] = column;
-    st.p[base + j] = pj;
-    st.z[base + j] = zj;
+    st.column[base + j] = at;
+    st.p[base + j] = static_cast<float>(p);
+    if (again) {
+      held_p[j] = static_cast<float>(p);
+      held_at[j] = at;
+    }
+  }
+  if (again) {
+    // An id's first place takes all of its p, in their order; the others are none.
+    __builtin_amdgcn_wave_barrier();
+    for (int j = lane; j < a.k; j += 64) {
+      const int at = held_at[j];
+      if (at < 0) continue;
+      int before = 0;
+      double p = 0.0;
+#pragma unroll 8
+      for (int i = 0; i < a.k; ++i) {
+        const bool same = held_at[i] == at;
+        before += same && i < j;
+        p += same && i >= j ? held_p[i] : 0.0f;
+      }
+      if (before == 0) {
+        st.p[base + j] = static_cast<float>(p);
+      } else {
+        st.column[base + j] = -1;
+        sum -= exp2_hw((Elem<T>::load1(x + at) - top) * cl);  // counted at the first
+      }
+    }
   }
   p_all = wave_add(p_all);
   h = wave_add(h);
@@ -211,13 +236,12 @@ __global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(nmce_dist
   sum = wave_add(sum);
   if (lane == 0) {
     Taught o;
-    o.r = whole || !any ? 0.0 : fmax(1.0 - p_all, 0.0);
+    o.r = kWhole || !any ? 0.0 : fmax(1.0 - p_all, 0.0);
     o.p = p_all;
     o.h = h;
     o.dot = dot;
-    // (Nothing above -inf there weighs nothing.)
-    o.sum = top == -kInf && sum == sum ? 0.0 : sum;
-    o.top = fmaxf(top, kNegHuge);
+    o.sum = sum;
+    o.top = top;
     o.any = any;
     st.rows[row] = o;
   }
@@ -841,6 +865,56 @@ __global__ __launch_bounds__(kRowBlock) void distill_wide_row_kernel(
   }
 }
 
+// The dense elements of rows on the 16-byte grid, a few vectors a workgroup wherever they
+// are (4096 x 151936 bf16 492 -> 390 us: many small workgroups keep more of the memory
+// busy), and the list's over them in a launch of their own.
+constexpr int kFlatBlock = 128, kFlatAhead = 2;
+template <typename T>
+__global__ __launch_bounds__(kFlatBlock) void distill_flat_kernel(
+    const T* x, T* g, uint32_t n_vec, uint32_t per_row, int64_t ld, int64_t ldg,
+    const Slope* __restrict__ slopes, float cl, const float* __restrict__ gout, int64_t gstride,
+    float gdiv) {
+  using E = Elem<T>;
+  constexpr int EPV = E::kPerVec;
+  const uint32_t base = blockIdx.x * static_cast<uint32_t>(kFlatBlock * kFlatAhead) + threadIdx.x;
+  u32x4 v[kFlatAhead];
+  uint32_t rows[kFlatAhead], cols[kFlatAhead];
+#pragma unroll
+  for (int u = 0; u < kFlatAhead; ++u) {
+    const uint32_t f = base + u * kFlatBlock;
+    rows[u] = f / per_row;
+    cols[u] = (f - rows[u] * per_row) * EPV;
+    if (f < n_vec)
+      v[u] = load_stream(reinterpret_cast<const u32x4*>(x + rows[u] * ld + cols[u]));
+  }
+#pragma unroll
+  for (int u = 0; u < kFlatAhead; ++u) {
+    if (base + u * kFlatBlock >= n_vec) continue;
+    const Slope s = slopes[rows[u]];
+    const float scale = s.a * (gout[rows[u] * gstride] / gdiv);
+    float f[EPV];
+    E::unpack(v[u], f);
+#pragma unroll
+    for (int e = 0; e < EPV; ++e)
+      f[e] = s.b < 0.0f ? 0.0f : exp2_hw((f[e] - s.m) * cl) * scale;
+    store_stream(reinterpret_cast<u32x4*>(g + rows[u] * ldg + cols[u]), E::pack(f));
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void distill_listed_kernel(
+    T* g, int64_t count, int64_t ldg, int k, State st, float cl, const float* __restrict__ gout,
+    int64_t gstride, float gdiv) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= count) return;
+  const int at = st.column[i];
+  if (at < 0) return;
+  const int64_t row = i / k;
+  const Slope s = st.slopes[row];
+  const float up = gout[row * gstride] / gdiv;
+  Elem<T>::store1(g + row * ldg + at, (exp2_hw((st.z[i] - s.top) * cl) * s.b - st.p[i]) * up);
+}
+
 int check_batch(const nmce_distill_batch* a) {
   if (!a) return NMCE_EINVAL_PTR;
   if ((a->dtype != NMCE_F32 && a->dtype != NMCE_BF16) ||
@@ -875,14 +949,22 @@ int launch_list(const nmce_distill_batch& a, const State& st, hipStream_t s) {
   while (table < 2 * a.k) table *= 2;
   const dim3 grid(static_cast<unsigned>((a.n_rows + kListWaves - 1) / kListWaves)),
       block(kListWaves * 64);
-  auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, block, kListWaves * table * 4, s, a, table, st);
+  auto run = [&](auto element, auto teacher) {
+    using T = decltype(element);
+    using TT = decltype(teacher);
+    const float cl = log2e_over(a.temperature);
+    const int lds = kListWaves * table * 4;
+    if (a.teacher_log_normalizer)
+      hipLaunchKernelGGL((distill_list_kernel<T, TT, false>), grid, block, lds, s, a, table, cl,
+                         st);
+    else
+      hipLaunchKernelGGL((distill_list_kernel<T, TT, true>), grid, block, lds, s, a, table, cl, st);
   };
   const bool f = a.dtype == NMCE_F32, tf = a.teacher_dtype == NMCE_F32;
   if (f)
-    tf ? run(distill_list_kernel<float, float>) : run(distill_list_kernel<float, uint16_t>);
+    tf ? run(float{}, float{}) : run(float{}, uint16_t{});
   else
-    tf ? run(distill_list_kernel<uint16_t, float>) : run(distill_list_kernel<uint16_t, uint16_t>);
+    tf ? run(uint16_t{}, float{}) : run(uint16_t{}, uint16_t{});
   return launch_status();
 }
 
@@ -1025,11 +1107,31 @@ int nmce_distill_bwd(const void* logits, void* grad, int dtype, int64_t n_rows,
   const State st = state_of(state, n_rows, k);
   const float cl = log2e_over(temperature);
   const float gdiv = gout_div * static_cast<float>(temperature);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t epv = 16 / static_cast<int64_t>(es), per_row = vocab_local / epv;
+  if (!assumed && vocab_local % epv == 0 && ld % epv == 0 && ld_grad % epv == 0 &&
+      aligned16(logits) && aligned16(grad) && n_rows * per_row < (int64_t{1} << 31)) {
+    const uint32_t n_vec = static_cast<uint32_t>(n_rows * per_row);
+    constexpr int kEach = kFlatBlock * kFlatAhead;
+    auto run = [&](auto element) {
+      using T = decltype(element);
+      hipLaunchKernelGGL(distill_flat_kernel<T>, dim3((n_vec + kEach - 1) / kEach),
+                         dim3(kFlatBlock), 0, s, static_cast<const T*>(logits),
+                         static_cast<T*>(grad), n_vec, static_cast<uint32_t>(per_row), ld, ld_grad,
+                         st.slopes, cl, grad_output, gout_stride, gdiv);
+      if (const int rc = launch_status()) return rc;
+      hipLaunchKernelGGL(distill_listed_kernel<T>,
+                         dim3(static_cast<unsigned>((n_rows * k + 255) / 256)), dim3(256), 0, s,
+                         static_cast<T*>(grad), n_rows * k, ld_grad, k, st, cl, grad_output,
+                         gout_stride, gdiv);
+      return launch_status();
+    };
+    return dtype == NMCE_F32 ? run(float{}) : run(uint16_t{});
+  }
   // After a one-pass forward the upstream value is usually the assumed one: a small
   // grid that walks the rows then ends at once.
   const int64_t most = assumed ? 2 * device_cus() : n_rows;
   const dim3 grid(static_cast<unsigned>(n_rows < most ? n_rows : most)), block(kBlock);
-  hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == NMCE_F32)
     hipLaunchKernelGGL(distill_bwd_kernel<float>, grid, block, 0, s,
                        static_cast<const float*>(logits), static_cast<float*>(grad), n_rows,
