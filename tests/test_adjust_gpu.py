@@ -153,6 +153,24 @@ def test_against_the_definition(b, k, v, prompt, output, bias, dtype, mask):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_long_lists_of_several_rows(dtype, inplace):
+    """Lists longer than a slab: a workgroup takes several rows, whose counts grow, with
+    fewer and with more places than are listed, and biases on counted ids."""
+    g = torch.Generator().manual_seed(20)
+    b, k, v = 16, 5, 50257
+    x, kw = _inputs(b, k, v, dtype, g, 9000, 400, 30, True)
+    kw["bias_ids"][:, :10] = kw["prompt"][:, :10]
+    kw["bias_ids"][:, 10:13] = kw["drafts"][:, :3]
+    kw["prompt"][3:] %= 300  # few ids, often
+    kw["prompt"][1] = torch.randperm(v, generator=g)[:9000]
+    kw["drafts"][:, 1] = torch.arange(b) * 3100 + 11
+    kw["drafts"][:, 3] = kw["drafts"][:, 1]
+    want = _reference(x, **kw)
+    _compare(_run(x.to(DEV), inplace, **kw), x, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
 def test_every_part_alone_and_numbers_for_tensors(dtype):
     g = torch.Generator().manual_seed(5)
     x, kw = _inputs(4, 2, 9001, dtype, g, 200, 90, 10, True)
