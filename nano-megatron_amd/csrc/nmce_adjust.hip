@@ -421,8 +421,8 @@ int check_batch(const nmce_adjust_batch* a) {
     return NMCE_EINVAL_SHAPE;
   const int64_t slabs = (a->vocab_local + kSlab - 1) / kSlab;
   // A launch's workgroups times their threads fit 32 bits.
-  if (a->batch > (int64_t{1} << 21) || a->batch * a->rows > (int64_t{1} << 21) ||
-      a->batch * a->rows * slabs > (int64_t{1} << 21))
+  if (a->batch > (int64_t{1} << 23) || a->batch * a->rows > (int64_t{1} << 23) ||
+      a->batch * a->rows * slabs > (int64_t{1} << 23))
     return NMCE_EINVAL_SHAPE;
   if (a->batch == 0) return NMCE_OK;
   if (!a->logits || !a->out || (a->n_prompt > 0 && !a->prompt) ||

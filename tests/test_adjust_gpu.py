@@ -170,6 +170,18 @@ def test_long_lists_of_several_rows(dtype, inplace):
     _compare(_run(x.to(DEV), inplace, **kw), x, want)
 
 
+@pytest.mark.parametrize("times", [16381, 16382, 16383, 16384, 70000])
+def test_an_id_thousands_of_times(times):
+    """At both sides of what a count of 16 bits holds, beside a neighbour that has none."""
+    x = torch.randn(2, 2, 500)
+    output = torch.full((2, times), 41)
+    output[1, ::2] = 40
+    kw = dict(prompt=torch.tensor([[41, 43], [42, 40]]), output=output, r=1.5, f=0.25, p=-0.5,
+              drafts=torch.tensor([[41], [40]]), bias_ids=torch.tensor([[41, 42], [39, 40]]),
+              bias=torch.randn(2, 2))
+    _check(x, **kw)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_every_part_alone_and_numbers_for_tensors(dtype):
     g = torch.Generator().manual_seed(5)
