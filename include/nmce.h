@@ -642,7 +642,7 @@ int nmce_verify_finish(const double* picked, const void* workspace, int64_t work
  *   - out may be logits (in place, the same strides): only touched and masked
  *     elements are written. Otherwise the two must not overlap.
  * n_bias at most NMCE_ADJUST_MAX_BIASES, n_output at most 2^29; batch x rows x
- * ceil(vocab_local / 8192) at most 2^21.
+ * ceil(vocab_local / 8192) at most 2^23.
  */
 #define NMCE_ADJUST_MAX_BIASES 8192
 typedef struct nmce_adjust_batch {
@@ -698,9 +698,10 @@ int nmce_top_merge(const int64_t* lists, int ranks, int dtype, int64_t n_rows, i
  *   teacher_log_normalizer NULL, p = softmax(t / T) over the list, r = 0:
  *   loss = sum p (log p - log q) + r (log r - log s)
  * where s is the sum of q outside the list (one class).
- *   - An id outside [0, vocab_total) is padding. A row without any other (or,
- *     with NULL, whose list holds only -inf) has no teacher: loss and gradient
- *     0, whatever its logits are. An id that comes several times adds up its p.
+ *   - An id outside [0, vocab_total) is padding. A row without any other, or
+ *     whose normaliser is -inf (with NULL, whose list holds only -inf), has no
+ *     teacher: loss and gradient 0, whatever its logits are. An id that comes
+ *     several times adds up its p.
  *   - Where the student gives everything outside the list nothing (-inf), the
  *     rest has no term. A student's row of only -inf, or with +inf or NaN: NaN.
  * logits [n_rows, ld] of this shard, teacher_logits and teacher_ids [n_rows, k]
@@ -728,25 +729,24 @@ int64_t nmce_distill_state_bytes(int64_t n_rows, int k);
 /*
  * The forward in two steps: this shard's statistics, [n_rows, 5] doubles (with
  * several ranks gather them to [ranks, n_rows, 5]), and the per-token fp32 loss
- * from them, with what the backward needs, both in `state`.
+ * from them, with what the backward needs, both in `state`; the losses' mean in
+ * mean[0] unless it is NULL.
  */
 int nmce_distill_stats(const nmce_distill_batch* batch, void* state, int64_t state_bytes,
                        double* stats, void* stream);
 int nmce_distill_combine(void* state, int64_t state_bytes, int64_t n_rows, int k,
                          double temperature, const double* stats, int ranks, float* loss,
-                         void* stream);
+                         float* mean, void* stream);
 
 /*
  * One rank (ids from 0, no exchange), rows of at most NMCE_DISTILL_ONE_PASS_BYTES:
  * the loss, the state and the gradient of its mean for the upstream value
  * expected[0] (1 if that is zero, subnormal or not finite), which goes to
- * assumed[0], in one read of the logits; mean[0] too unless it is NULL (at most
- * NMCE_DISTILL_MEAN_ROWS rows). gout_div: the token count. Rows of grad lie
- * against 16-byte boundaries as the logits' rows do; grad may be logits
- * (ld_grad == ld).
+ * assumed[0], in one read of the logits; mean[0] too unless it is NULL.
+ * gout_div: the token count. Rows of grad lie against 16-byte boundaries as the
+ * logits' rows do; grad may be logits (ld_grad == ld).
  */
 #define NMCE_DISTILL_ONE_PASS_BYTES 262144
-#define NMCE_DISTILL_MEAN_ROWS 16384
 int nmce_distill_fwd_bwd(const nmce_distill_batch* batch, void* grad, int64_t ld_grad, void* state,
                          int64_t state_bytes, float* loss, float* mean, const float* expected,
                          float* assumed, float gout_div, void* stream);

@@ -703,15 +703,15 @@ struct DistillMean : public torch::autograd::Function<DistillMean> {
     const at::Tensor state = a.state();
     const auto f32 = a.rows.options().dtype(at::kFloat);
     at::Tensor loss = at::empty({n}, f32), mean = at::empty({}, f32), assumed = at::empty({1}, f32);
+    // Rows that had to be copied (of an expanded tensor) are not the logits' storage.
+    inplace = inplace && a.rows.data_ptr() == logits.data_ptr();
     at::Tensor grad = inplace ? a.rows : at::empty({n, V}, a.rows.options());
     hipStream_t st = stream_of(a.rows);
-    const bool own_mean = n <= NMCE_DISTILL_MEAN_ROWS;
     timed("nmce_distill_fwd_bwd", st, [&] {
       return nmce_distill_fwd_bwd(&a.batch, grad.data_ptr(), inplace ? a.batch.ld : V,
                                   state.data_ptr(), state.numel(), loss.data_ptr<float>(),
-                                  own_mean ? mean.data_ptr<float>() : nullptr,
-                                  hint.data_ptr<float>(), assumed.data_ptr<float>(),
-                                  static_cast<float>(n), st);
+                                  mean.data_ptr<float>(), hint.data_ptr<float>(),
+                                  assumed.data_ptr<float>(), static_cast<float>(n), st);
     });
     save_distill(ctx, a, logits, state, inplace, n);
     ctx->saved_data["hint"] = hint;  // itself: the backward writes into it
@@ -724,7 +724,7 @@ struct DistillMean : public torch::autograd::Function<DistillMean> {
     } else {
       ctx->save_for_backward({a.rows, state, grad, assumed});
     }
-    return own_mean ? mean : loss.mean();
+    return mean;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grad_outputs) {
@@ -786,6 +786,7 @@ struct Distill : public torch::autograd::Function<Distill> {
     const at::Tensor state = a.state();
     at::Tensor loss = at::empty({n}, a.rows.options().dtype(at::kFloat));
     at::Tensor stats = at::empty({n, 5}, a.rows.options().dtype(at::kDouble));
+    at::Tensor result = mean && n > 0 ? at::empty({}, loss.options()) : at::Tensor();
     hipStream_t st = stream_of(a.rows);
     timed("nmce_distill_stats", st, [&] {
       return nmce_distill_stats(&a.batch, state.data_ptr(), state.numel(),
@@ -793,7 +794,8 @@ struct Distill : public torch::autograd::Function<Distill> {
     });
     timed("nmce_distill_combine", st, [&] {
       return nmce_distill_combine(state.data_ptr(), state.numel(), n, a.batch.k, temperature,
-                                  stats.data_ptr<double>(), 1, loss.data_ptr<float>(), st);
+                                  stats.data_ptr<double>(), 1, loss.data_ptr<float>(),
+                                  result.defined() ? result.data_ptr<float>() : nullptr, st);
     });
     // Rows that had to be copied are not the logits' storage.
     inplace = inplace && a.rows.data_ptr() == logits.data_ptr();
@@ -801,7 +803,8 @@ struct Distill : public torch::autograd::Function<Distill> {
     ctx->saved_data["mean"] = mean;
     if (inplace) ctx->save_for_backward({a.rows, state, logits});
     else ctx->save_for_backward({a.rows, state});
-    return mean ? loss.mean() : loss.view(logits.sizes().slice(0, logits.dim() - 1));
+    if (mean) return result.defined() ? result : loss.mean();  // (of no tokens: NaN)
+    return loss.view(logits.sizes().slice(0, logits.dim() - 1));
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grad_outputs) {
@@ -883,7 +886,7 @@ at::Tensor distill(const at::Tensor& logits, const at::Tensor& teacher_logits,
 
 // ---- logits on their way to a sampler ---------------------------------------------------
 // No nodes (they have no derivative), but one call from Python each: through ctypes, with
-// its outputs made there, a small call took 14 to 19 us on the host, and takes 6 to 9.
+// its outputs made there, a small call took 19 (adjust) and 16 us (top) on the host, and takes 11 and 7.
 
 // Lists [batch, n] of consecutive elements: their address, stride and length.
 struct Lists {

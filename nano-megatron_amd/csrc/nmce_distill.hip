@@ -115,11 +115,14 @@ constexpr int kListWaves = 4;
 
 // kWhole: no normaliser, the teacher's distribution is over the list. The student's sum is
 // in fp32 terms, as the one outside the list is.
+// `assumed` (of a one-pass forward, else NULL) takes the upstream value to assume: the row
+// kernels read it there, since another stream's backward may change the hint under them.
 template <typename T, typename TT, bool kWhole>
-__global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(nmce_distill_batch a,
-                                                                       int table, float cl,
-                                                                       State st) {
+__global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(
+    nmce_distill_batch a, int table, float cl, State st, const float* __restrict__ expect,
+    float* __restrict__ assumed) {
   extern __shared__ int tables[];  // `table` slots a wave: ids noted, 0 for none
+  if (assumed && blockIdx.x == 0 && threadIdx.x == 0) assumed[0] = usable_hint(expect[0]);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kListWaves + wave;
   if (row >= a.n_rows) return;  // (waves are on their own: no barrier below)
@@ -180,6 +183,7 @@ __global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(nmce_dist
     }
   } else {
     norm = static_cast<double>(a.teacher_log_normalizer[row]);
+    if (norm == -static_cast<double>(kInf)) any = false;  // (a teacher's row of only -inf)
   }
   // (The table is done with; of a list that names an id twice p and ids come there.)
   float* held_p = reinterpret_cast<float*>(seen);
@@ -339,8 +343,8 @@ __device__ __forceinline__ void merge(double& m, double& s, double o, double u, 
 
 // From the merged statistics of a row: outside the list (m, s), on it (top, sum), and
 // sum p z / T. A student's row of only -inf, or with a +inf or NaN, has no distribution:
-// NaN. Where it gives
-// the rest nothing (nothing outside above -inf) the rest has no class and no term.
+// NaN. Where it gives the rest nothing (nothing outside above -inf) the rest has no class
+// and no term.
 __device__ __forceinline__ double loss_and_slope(const Taught& t, double m, double s, double top,
                                                  double sum, double dot, double c, Slope* slope) {
   if (!t.any) {
@@ -417,8 +421,18 @@ __global__ __launch_bounds__(kLossBlock) void distill_loss_kernel(State st, int6
 __global__ __launch_bounds__(kLossBlock) void distill_mean_kernel(const float* __restrict__ loss,
                                                                   int64_t n,
                                                                   float* __restrict__ mean) {
+  constexpr int kAhead = 8;
   double sum = 0.0;
-  for (int64_t row = threadIdx.x; row < n; row += kLossBlock) sum += loss[row];
+  for (int64_t row = threadIdx.x; row < n; row += kAhead * kLossBlock) {
+    float one[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t at = row + i * kLossBlock;
+      one[i] = loss[at < n ? at : n - 1];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) sum += row + i * kLossBlock < n ? one[i] : 0.0f;
+  }
   store_mean(sum, n, mean);
 }
 
@@ -490,7 +504,7 @@ __global__ __launch_bounds__(kBlock) void distill_bwd_kernel(
 // listed elements are set to -inf where they are held, so that the fold sees what is
 // outside; each wave does that for its own elements, one listed id after another, and
 // writes their gradients over the row's, by the lanes that stored it. The gradient is
-// that of the mean for the upstream value usable_hint(expect[0]), which goes to assumed[0];
+// that of the mean for the upstream value assumed[0] (the list kernel's);
 // loss and slopes as from distill_combine_kernel, the slopes in fp32. Vectors, edges
 // (kRagged: rows of any width and alignment, the gradient's as the logits') and buffer
 // resources as in the cross entropy's one-pass kernels. g may be x.
@@ -597,14 +611,12 @@ struct Listed {
 template <typename T, int kVec, bool kRagged>
 __global__ __launch_bounds__(kRowBlock, 8) void distill_row_kernel(
     const T* x, T* g, int64_t n_rows, int64_t V, int64_t ld, int64_t ldg, int k, State st,
-    float cl, const float* __restrict__ expect_in, float* __restrict__ assumed, float gdiv) {
+    float cl, const float* __restrict__ assumed, float gdiv) {
   using E = Elem<T>;
   constexpr int EPV = E::kPerVec;
   __shared__ float sm_m[2][kRowWaves];
   __shared__ float sm_s[2][kRowWaves];
-  const float expect = usable_hint(expect_in[0]);
-  if (blockIdx.x == 0 && threadIdx.x == 0) assumed[0] = expect;
-  const float up = expect / gdiv;
+  const float up = assumed[0] / gdiv;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int head = 0;
   int nvec = static_cast<int>(V / EPV);
@@ -715,16 +727,14 @@ __global__ __launch_bounds__(kRowBlock, 8) void distill_row_kernel(
 template <typename T, bool kRagged>
 __global__ __launch_bounds__(kRowBlock) void distill_wide_row_kernel(
     const T* x, T* g, int64_t n_rows, int64_t V, int64_t ld, int64_t ldg, int k, State st,
-    float cl, const float* __restrict__ expect_in, float* __restrict__ assumed, float gdiv) {
+    float cl, const float* __restrict__ assumed, float gdiv) {
   using E = Elem<T>;
   constexpr int EPV = E::kPerVec;
   extern __shared__ __align__(16) char lds_dyn[];
   u32x4* hi = reinterpret_cast<u32x4*>(lds_dyn);  // vector kWideLo + i of thread t: hi[i * kRowBlock + t]
   __shared__ float sm_m[2][kRowWaves];
   __shared__ float sm_s[2][kRowWaves];
-  const float expect = usable_hint(expect_in[0]);
-  if (blockIdx.x == 0 && threadIdx.x == 0) assumed[0] = expect;
-  const float up = expect / gdiv;
+  const float up = assumed[0] / gdiv;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   struct Geom {
     int head, nvec, cnt;
@@ -944,7 +954,13 @@ int check_state(const void* state, int64_t bytes, int64_t n, int k) {
 // exp((x - m) / T) = 2^((x - m) * this).
 float log2e_over(double temperature) { return static_cast<float>(kLog2e64 / temperature); }
 
-int launch_list(const nmce_distill_batch& a, const State& st, hipStream_t s) {
+int launch_mean(const float* loss, int64_t n, float* mean, hipStream_t s) {
+  hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(kLossBlock), 0, s, loss, n, mean);
+  return launch_status();
+}
+
+int launch_list(const nmce_distill_batch& a, const State& st, const float* expect, float* assumed,
+                hipStream_t s) {
   int table = 64;
   while (table < 2 * a.k) table *= 2;
   const dim3 grid(static_cast<unsigned>((a.n_rows + kListWaves - 1) / kListWaves)),
@@ -955,10 +971,11 @@ int launch_list(const nmce_distill_batch& a, const State& st, hipStream_t s) {
     const float cl = log2e_over(a.temperature);
     const int lds = kListWaves * table * 4;
     if (a.teacher_log_normalizer)
-      hipLaunchKernelGGL((distill_list_kernel<T, TT, false>), grid, block, lds, s, a, table, cl,
-                         st);
+      hipLaunchKernelGGL((distill_list_kernel<T, TT, false>), grid, block, lds, s, a, table, cl, st,
+                         expect, assumed);
     else
-      hipLaunchKernelGGL((distill_list_kernel<T, TT, true>), grid, block, lds, s, a, table, cl, st);
+      hipLaunchKernelGGL((distill_list_kernel<T, TT, true>), grid, block, lds, s, a, table, cl, st,
+                         expect, assumed);
   };
   const bool f = a.dtype == NMCE_F32, tf = a.teacher_dtype == NMCE_F32;
   if (f)
@@ -970,17 +987,19 @@ int launch_list(const nmce_distill_batch& a, const State& st, hipStream_t s) {
 
 template <typename T, bool kRagged>
 int launch_rows(const nmce_distill_batch& a, void* grad, int64_t ldg, const State& st,
-                const float* expect, float* assumed, float gdiv, hipStream_t s) {
+                const float* assumed, float gdiv, hipStream_t s) {
   const T* x = static_cast<const T*>(a.logits);
   T* g = static_cast<T*>(grad);
   const float cl = log2e_over(a.temperature);
   const int64_t per_thread = (a.vocab_local / Elem<T>::kPerVec + kRowBlock - 1) / kRowBlock;
   const dim3 block(kRowBlock);
   auto run = [&](auto kernel, int per_cu, int lds) {
-    const int64_t most = static_cast<int64_t>(per_cu) * device_cus();
-    const dim3 grid(static_cast<unsigned>(per_cu == 0 || a.n_rows < most ? a.n_rows : most));
+    // (Where a workgroup takes one row: a launch's threads fit 32 bits.)
+    const int64_t most =
+        per_cu ? static_cast<int64_t>(per_cu) * device_cus() : int64_t{1} << 21;
+    const dim3 grid(static_cast<unsigned>(a.n_rows < most ? a.n_rows : most));
     hipLaunchKernelGGL(kernel, grid, block, lds, s, x, g, a.n_rows, a.vocab_local, a.ld, ldg, a.k,
-                       st, cl, expect, assumed, gdiv);
+                       st, cl, assumed, gdiv);
   };
   if (per_thread > 8) {
     static std::atomic<bool> lds_ok{false};
@@ -1006,7 +1025,8 @@ extern "C" {
 int64_t nmce_distill_state_bytes(int64_t n_rows, int k) {
   if (n_rows < 0 || n_rows > (int64_t{1} << 22) || k < 1 || k > kMaxK) return -1;
   return align256(n_rows * static_cast<int64_t>(sizeof(Taught))) +
-         align256(n_rows * static_cast<int64_t>(sizeof(Slope))) + align256(n_rows * 4) + 3 * align256(n_rows * k * 4);
+         align256(n_rows * static_cast<int64_t>(sizeof(Slope))) + align256(n_rows * 4) +
+         3 * align256(n_rows * k * 4);
 }
 
 int nmce_distill_stats(const nmce_distill_batch* a, void* state, int64_t state_bytes,
@@ -1017,7 +1037,7 @@ int nmce_distill_stats(const nmce_distill_batch* a, void* state, int64_t state_b
   if (const int rc = check_state(state, state_bytes, a->n_rows, a->k)) return rc;
   const State st = state_of(state, a->n_rows, a->k);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (const int rc = launch_list(*a, st, s)) return rc;
+  if (const int rc = launch_list(*a, st, nullptr, nullptr, s)) return rc;
   const dim3 grid(static_cast<unsigned>(a->n_rows)), block(kBlock);
   const float cl = log2e_over(a->temperature);
   if (a->dtype == NMCE_F32)
@@ -1029,7 +1049,7 @@ int nmce_distill_stats(const nmce_distill_batch* a, void* state, int64_t state_b
 
 int nmce_distill_combine(void* state, int64_t state_bytes, int64_t n_rows, int k,
                          double temperature, const double* stats, int ranks, float* loss,
-                         void* stream) {
+                         float* mean, void* stream) {
   if (n_rows < 0 || n_rows > (int64_t{1} << 22) || k < 1 || k > kMaxK ||
       !(temperature >= 1e-6 && temperature <= 1e6))
     return NMCE_EINVAL_SHAPE;
@@ -1040,7 +1060,8 @@ int nmce_distill_combine(void* state, int64_t state_bytes, int64_t n_rows, int k
   hipLaunchKernelGGL(distill_combine_kernel, dim3(static_cast<unsigned>((n_rows + 255) / 256)),
                      dim3(256), 0, static_cast<hipStream_t>(stream), state_of(state, n_rows, k),
                      n_rows, 1.0 / temperature, stats, ranks, loss);
-  return launch_status();
+  if (const int rc = launch_status()) return rc;
+  return mean ? launch_mean(loss, n_rows, mean, static_cast<hipStream_t>(stream)) : NMCE_OK;
 }
 
 int nmce_distill_fwd_bwd(const nmce_distill_batch* a, void* grad, int64_t ld_grad, void* state,
@@ -1055,7 +1076,6 @@ int nmce_distill_fwd_bwd(const nmce_distill_batch* a, void* grad, int64_t ld_gra
     return NMCE_EINVAL_SHAPE;
   if (a->n_rows == 0) return NMCE_OK;
   if (!grad || !loss || !expected || !assumed) return NMCE_EINVAL_PTR;
-  if (mean && a->n_rows > NMCE_DISTILL_MEAN_ROWS) return NMCE_EINVAL_SHAPE;
   const uintptr_t px = reinterpret_cast<uintptr_t>(a->logits),
                   pg = reinterpret_cast<uintptr_t>(grad);
   // Rows of the gradient lie against 16-byte boundaries as the logits' do.
@@ -1064,28 +1084,24 @@ int nmce_distill_fwd_bwd(const nmce_distill_batch* a, void* grad, int64_t ld_gra
   if (const int rc = check_state(state, state_bytes, a->n_rows, a->k)) return rc;
   const State st = state_of(state, a->n_rows, a->k);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (const int rc = launch_list(*a, st, s)) return rc;
+  if (const int rc = launch_list(*a, st, expected, assumed, s)) return rc;
   const float gdiv = gout_div * static_cast<float>(a->temperature);
   const bool ragged = px % 16 || a->vocab_local % epv || a->ld % epv || ld_grad % epv;
   int rc;
   if (a->dtype == NMCE_F32)
-    rc = ragged ? launch_rows<float, true>(*a, grad, ld_grad, st, expected, assumed, gdiv, s)
-                : launch_rows<float, false>(*a, grad, ld_grad, st, expected, assumed, gdiv, s);
+    rc = ragged ? launch_rows<float, true>(*a, grad, ld_grad, st, assumed, gdiv, s)
+                : launch_rows<float, false>(*a, grad, ld_grad, st, assumed, gdiv, s);
   else
-    rc = ragged ? launch_rows<uint16_t, true>(*a, grad, ld_grad, st, expected, assumed, gdiv, s)
-                : launch_rows<uint16_t, false>(*a, grad, ld_grad, st, expected, assumed, gdiv, s);
+    rc = ragged ? launch_rows<uint16_t, true>(*a, grad, ld_grad, st, assumed, gdiv, s)
+                : launch_rows<uint16_t, false>(*a, grad, ld_grad, st, assumed, gdiv, s);
   if (rc) return rc;
   const bool one = a->n_rows <= kLossBlock && mean;
   const int threads = one ? static_cast<int>(round_up(a->n_rows, 64)) : kLossRows;
   const dim3 blocks(static_cast<unsigned>((a->n_rows + threads - 1) / threads));
   hipLaunchKernelGGL(distill_loss_kernel, blocks, dim3(threads), 0, s, st, a->n_rows,
                      1.0 / a->temperature, loss, one ? mean : nullptr);
-  if (mean && !one) {
-    if (const int rc2 = launch_status()) return rc2;
-    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(kLossBlock), 0, s, loss, a->n_rows,
-                       mean);
-  }
-  return launch_status();
+  if (const int rc2 = launch_status()) return rc2;
+  return mean && !one ? launch_mean(loss, a->n_rows, mean, s) : NMCE_OK;
 }
 
 int nmce_distill_bwd(const void* logits, void* grad, int dtype, int64_t n_rows,
@@ -1110,7 +1126,8 @@ int nmce_distill_bwd(const void* logits, void* grad, int dtype, int64_t n_rows,
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t epv = 16 / static_cast<int64_t>(es), per_row = vocab_local / epv;
   if (!assumed && vocab_local % epv == 0 && ld % epv == 0 && ld_grad % epv == 0 &&
-      aligned16(logits) && aligned16(grad) && n_rows * per_row < (int64_t{1} << 31)) {
+      aligned16(logits) && aligned16(grad) && n_rows * per_row < (int64_t{1} << 31) &&
+      n_rows * k < (int64_t{1} << 31)) {
     const uint32_t n_vec = static_cast<uint32_t>(n_rows * per_row);
     constexpr int kEach = kFlatBlock * kFlatAhead;
     auto run = [&](auto element) {

@@ -94,7 +94,7 @@ SIGNATURES: dict[str, tuple] = {
     "nmce_distill_state_bytes": (_i64, [_i64, _c_int]),
     "nmce_distill_stats": (_c_int, [_p, _p, _i64, _p, _p]),
     "nmce_distill_combine": (_c_int, [_p, _i64, _i64, _c_int, ctypes.c_double, _p, _c_int, _p,
-                                      _p]),
+                                      _p, _p]),
     "nmce_distill_fwd_bwd": (_c_int, [_p, _p, _i64, _p, _i64, _p, _p, _p, _p, ctypes.c_float,
                                       _p]),
     "nmce_distill_bwd": (_c_int, [_p, _p, _c_int, _i64, _i64, _i64, _i64, _c_int, ctypes.c_double,

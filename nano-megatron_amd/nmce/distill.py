@@ -108,6 +108,7 @@ class _VocabParallelDistillation(torch.autograd.Function):
             rows, inplace = logits.contiguous().view(-1, v), False
         ld = rows.stride(0) if n > 1 else v
         loss = torch.empty((n,), dtype=torch.float32, device=dev)
+        result = torch.empty((), dtype=torch.float32, device=dev) if mean and n else None
         size = int(lib.nmce_distill_state_bytes(n, k))
         state = torch.empty(max(16, size), dtype=torch.uint8, device=dev)
         if n:
@@ -122,12 +123,14 @@ class _VocabParallelDistillation(torch.autograd.Function):
                     stats = _all_gather_rows(stats, group, world_size)
                 _launch("nmce_distill_combine", lib.nmce_distill_combine, state.data_ptr(),
                         state.numel(), n, k, temperature, stats.data_ptr(), world_size,
-                        loss.data_ptr(), stream)
+                        loss.data_ptr(), result.data_ptr() if mean else None, stream)
             del held
         ctx.inplace, ctx.k, ctx.temperature, ctx.mean = inplace, k, temperature, mean
         ctx.shape = logits.shape
         _save(ctx, rows, state, logits if inplace else None)
-        return loss.mean() if mean else loss.view(logits.shape[:-1])
+        if mean:
+            return result if n else loss.mean()  # (of no tokens: NaN)
+        return loss.view(logits.shape[:-1])
 
     @staticmethod
     @once_differentiable
@@ -190,8 +193,8 @@ def vocab_parallel_distillation_loss(
     ``[...]``. The usual factor ``temperature ** 2`` is the caller's.
 
     Shorter lists are padded with -1: an id outside the vocabulary stands for
-    nothing. A token without a teacher (nothing else in its list, or without the
-    normaliser only -inf) has loss and gradient 0, and counts in the mean. An id
+    nothing. A token without a teacher (nothing else in its list, a normaliser of -inf, or
+    without one only -inf) has loss and gradient 0, and counts in the mean. An id
     that comes several times adds up its probabilities. Where the student gives
     everything outside the list nothing (-inf), the rest has no term; a student's row
     of only -inf, or with a +inf or NaN, gives NaN.

@@ -416,6 +416,159 @@ def test_saved_tensor_hooks(reduction):
         run(lambda a: a, lambda a: a[:1] if a.dim() else a.double())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("v", [4000, 4001])
+def test_in_place_of_rows_that_share_memory(v, dtype):
+    """An expanded tensor's gradient does not fit its storage: it goes into a buffer."""
+    g = torch.Generator().manual_seed(15)
+    x, t, ids, norm = _inputs(4, v, 6, dtype, g)
+    leaf = x[:1].to(DEV).requires_grad_(True)
+    for one_pass in (True, False):
+        for up in (1.0, 0.5, 0.5, 1.0):  # (assumed or not)
+            got = []
+            for inplace in (True, False):
+                y = (leaf * 1.0).expand(4, v)
+                y.retain_grad()
+                loss = _loss(y, t, ids, norm, inplace=inplace, one_pass=one_pass)
+                (loss * up).backward()
+                got.append(y.grad)
+            assert torch.equal(y, leaf.expand(4, v)) and torch.equal(*got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_a_teacher_whose_row_was_masked(dtype):
+    """What the top logits of a row of only -inf are: no teacher."""
+    import nmce
+    ctx = nmce.ParallelContext.single()
+    g = torch.Generator().manual_seed(16)
+    teacher = torch.randn(5, 300, generator=g)
+    teacher[2] = -INF
+    t, ids, norm = nmce.vocab_parallel_top_logits(teacher.to(DEV), 8, 0, 300, ctx)
+    assert float(norm[2]) == -INF
+    x = torch.randn(5, 300, generator=g).to(dtype)
+    d = x.to(DEV).requires_grad_(True)
+    rest = torch.tensor([0, 1, 3, 4])
+    for reduction in ("none", "mean"):
+        loss = _loss(d, t, ids, norm, reduction=reduction)
+        grad, = torch.autograd.grad(loss.sum(), d)
+        assert not bool(grad[2].any()) and bool(torch.isfinite(loss).all())
+        if reduction == "none":
+            assert float(loss.detach()[2]) == 0.0
+            want, slack, _, _ = _reference(x[rest], t.cpu()[rest], ids.cpu()[rest],
+                                           norm.cpu()[rest], 1.0)
+            _within(loss.detach()[rest.to(DEV)], want, slack, F32, "loss")
+
+
+@pytest.mark.parametrize("n", [1023, 1025, 9000, 70000])
+def test_means_of_many_tokens(n):
+    """In the loss's own workgroup, and of as many rows as there are, in a captured graph too:
+    a sum in 64 bits of fp32 losses, rounded once."""
+    g = torch.Generator().manual_seed(n)
+    v = 40
+    x, t, ids, norm = (a.to(DEV) for a in _inputs(n, v, 3, F32, g))
+    d = x.clone().requires_grad_(True)
+
+    def run():
+        one = _loss(d, t, ids, norm)
+        two = _loss(d, t, ids, norm, one_pass=False)
+        return one, two, torch.autograd.grad(one, d)[0], torch.autograd.grad(two, d)[0]
+
+    def check(out):
+        each = _loss(d, t, ids, norm, reduction="none").detach().double()
+        one, two, g1, g2 = (o.detach().double() for o in out)
+        # The one-pass losses are sums in another order. Of 40 logits the mean distance from
+        # the largest is at most 2, so _reference's slacks are at most |loss| + 60 and 64 steps.
+        size = 2 * STEP * (float(each.abs().mean()) + 60)
+        assert abs(float(two - each.mean())) <= STEP * abs(float(each.mean())) + 1e-12
+        assert abs(float(one - each.mean())) <= size
+        assert bool(((g1 - g2).abs() <= 2 * STEP * 64 / n).all())
+
+    check(run())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for seed in range(3):
+        with torch.no_grad():
+            d.copy_(torch.randn(n, v, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out)
+
+
+def test_an_upstream_hint_and_its_miss():
+    g = torch.Generator().manual_seed(17)
+    x, t, ids, norm = _inputs(6, 5000, 7, F32, g)
+    leaf = x.to(DEV).requires_grad_(True)
+    want, = torch.autograd.grad(_loss(leaf, t, ids, norm, one_pass=False), leaf)
+    for inplace in (False, True):
+        hint = torch.ones(1, device=DEV)
+        for start, up in ((1.0, 1.0), (1.0, 4.0), (4.0, 4.0), (math.inf, 2.0), (0.0, 2.0),
+                          (math.nan, -0.5), (2.0, 0.0)):
+            hint.fill_(start)
+            y = leaf * 1.0
+            loss = _loss(y, t, ids, norm, upstream_hint=hint, inplace=inplace)
+            got, = torch.autograd.grad(loss, leaf, torch.tensor(up, device=DEV))
+            assert float(hint) == up
+            # (_reference's slack: at most 128 steps where 3 x the mean distance from the
+            # largest of 5000 logits, two sums and their elements come together; two sides)
+            bound = 2 * 128 * STEP * abs(up) / 6 + 4 * STEP * (want * up).abs()
+            assert bool(((got - want * up).abs() <= bound).all()), (inplace, start, up)
+
+
+def test_threads_on_streams_of_their_own():
+    """Two callers at once, of one call site, under different upstream values."""
+    import threading
+    g = torch.Generator().manual_seed(18)
+    data = [_inputs(64, 30000, 20, BF, g) for _ in range(2)]
+    data = [tuple(a.to(DEV) for a in d) for d in data]
+    ups = (1.0, 8.0)
+
+    def grad_of(i, one_pass):
+        x, t, ids, norm = data[i]
+        d = x.detach().requires_grad_(True)
+        loss = _loss(d, t, ids, norm, one_pass=one_pass)
+        return torch.autograd.grad(loss, d, torch.tensor(ups[i], device=DEV))[0]
+
+    # A value that the forward assumed and one written again: the same formula.
+    want = [grad_of(i, True) for i in range(2)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(12):
+                got = grad_of(i, True)
+                ok = (got.float() - want[i].float()).abs() <= 2.0 ** -7 * want[i].float().abs() + \
+                    1e-6 * ups[i] / 64
+                if not bool(ok.all()):
+                    wrong.append(i)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_long_lists_of_few_ids(tail):
+    """1024 entries of one id, of two in turn, and each of 512 twice."""
+    g = torch.Generator().manual_seed(19)
+    x = torch.randn(3, 2000, generator=g)
+    t = torch.randn(3, 1024, generator=g)
+    j = torch.arange(1024)
+    ids = torch.stack([torch.full((1024,), 1999), j % 2 * 7, j % 512])
+    _check(x, t, ids, torch.logsumexp(t.double(), 1).float() + 0.25 if tail else None)
+
+
 def test_the_same_bits_at_every_run():
     g = torch.Generator().manual_seed(14)
     x, t, ids, norm = _inputs(20, 60000, 100, BF, g)

@@ -50,7 +50,7 @@ def _adjust_batch(**kw):
     (dict(vocab_start=-1), -2), (dict(vocab_start=1), -2), (dict(vocab_total=9), -2),
     (dict(vocab_total=1 << 31), -2), (dict(n_prompt=-1), -2), (dict(n_output=-1), -2),
     (dict(n_output=(1 << 29) + 1), -2), (dict(n_bias=-1), -2), (dict(n_bias=8193), -2),
-    (dict(batch=1 << 22), -2), (dict(rows=1 << 21), -2), (dict(logits=None), -4),
+    (dict(batch=1 << 22), -2), (dict(rows=(1 << 22) + 1), -2), (dict(logits=None), -4),
     (dict(out=None), -4), (dict(prompt=None), -4), (dict(output=None), -4), (dict(drafts=None), -4),
     (dict(bias_ids=None), -4), (dict(bias=None), -4), (dict(logits=4098), -3),
     (dict(out=4097, dtype=1), -3), (dict(allowed=4098), -3),
@@ -236,7 +236,6 @@ def test_distill_steps_refuse_before_launch(lib):
         return lib.nmce_distill_fwd_bwd(ctypes.addressof(batch), g, ldg, space, bytes_, loss, mean,
                                         expect, assumed, div, None)
 
-    rows = _distill_batch(n_rows=16385)
     assert one(_distill_batch(dtype=5)) == -1
     for bad in (dict(batch=_distill_batch(vocab_total=200)), dict(ldg=99), dict(div=0.0),
                 dict(batch=_distill_batch(vocab_start=100, vocab_total=200)),
@@ -244,7 +243,7 @@ def test_distill_steps_refuse_before_launch(lib):
                      ldg=65537),
                 dict(batch=_distill_batch(dtype=1, vocab_local=131073, vocab_total=131073,
                                           ld=131073), ldg=131073),
-                dict(g=p, ldg=104), dict(batch=rows, bytes_=state(16385, 8))):
+                dict(g=p, ldg=104), dict(batch=_distill_batch(n_rows=(1 << 22) + 1))):
         assert one(**bad) == -2, bad
     for name in ("g", "loss", "expect", "assumed"):
         assert one(**{name: None}) == -4
@@ -252,14 +251,14 @@ def test_distill_steps_refuse_before_launch(lib):
     assert one(space=None) == one(space=p + 8) == one(bytes_=size - 1) == -6
     assert one(_distill_batch(n_rows=0), g=None) == 0
     combine = lib.nmce_distill_combine
-    assert combine(p, size, -1, 8, 1.0, p, 1, p, None) == -2
-    assert combine(p, size, 4, 0, 1.0, p, 1, p, None) == -2
-    assert combine(p, size, 4, 8, 0.0, p, 1, p, None) == -2
-    assert combine(p, size, 4, 8, 1.0, p, 0, p, None) == -5
-    assert combine(p, size, 4, 8, 1.0, None, 1, p, None) == -4
-    assert combine(p, size, 4, 8, 1.0, p, 1, None, None) == -4
-    assert combine(p, size - 1, 4, 8, 1.0, p, 1, p, None) == -6
-    assert combine(None, 0, 0, 8, 1.0, None, 1, None, None) == 0
+    assert combine(p, size, -1, 8, 1.0, p, 1, p, p, None) == -2
+    assert combine(p, size, 4, 0, 1.0, p, 1, p, p, None) == -2
+    assert combine(p, size, 4, 8, 0.0, p, 1, p, p, None) == -2
+    assert combine(p, size, 4, 8, 1.0, p, 0, p, p, None) == -5
+    assert combine(p, size, 4, 8, 1.0, None, 1, p, p, None) == -4
+    assert combine(p, size, 4, 8, 1.0, p, 1, None, p, None) == -4
+    assert combine(p, size - 1, 4, 8, 1.0, p, 1, p, None, None) == -6
+    assert combine(None, 0, 0, 8, 1.0, None, 1, None, None, None) == 0
 
     def bwd(x=p, g=2 * p, dtype=0, n=4, v=100, ld=100, ldg=100, k=8, t=1.0, space=p, bytes_=size,
             go=p, stride=0, div=4.0):

@@ -211,7 +211,8 @@ def test_captured_and_replayed():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
-@pytest.mark.parametrize("tp,per,k", [(2, 5, 9), (3, 1001, 40), (4, 20000, 512)])
+@pytest.mark.parametrize("tp,per,k", [(2, 5, 9), (3, 1001, 40), (4, 20000, 512), (14, 600, 512),
+                                      (15, 600, 512), (20, 3, 50), (72, 40, 100), (8, 9, 1)])
 def test_shards_merged(tp, per, k, dtype):
     """Each shard's list and their merge, as the ranks exchange them."""
     from nmce import _lib as L
