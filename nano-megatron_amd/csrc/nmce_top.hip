@@ -175,10 +175,10 @@ __device__ uint64_t kth_key(const uint64_t* list, int n, int k, int most) {
 }
 
 // The k largest of the n notes (k <= n, unique keys), and a few more, into kept; the key
-// that they reach is returned. Every thread calls it, behind a barrier. Few notes are one wave's work
-// while the others wait (and other workgroups read): 4096 x 128256 bf16, k 64: 207 us, by
-// all waves 220. More are held by all threads, four a thread, a barrier a step: 777 x 100277
-// fp32, k 500: 112 us, by one wave from LDS 137.
+// that they reach is returned. Every thread calls it, behind a barrier. Few notes are one
+// wave's work while the others wait (and other workgroups read): 4096 x 128256 bf16, k 64:
+// 207 us, by all waves 220. More are held by all threads, four a thread, a barrier a step:
+// 777 x 100277 fp32, k 500: 112 us, by one wave from LDS 137.
 template <typename Shape>
 __device__ uint64_t cut_notes(Shared<Shape>& sh, int n, int k) {
   constexpr int kEach = Shape::kNotes / Shape::kBlock, kWaves = Shape::kBlock / 64;
@@ -639,10 +639,13 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
       if (n >= k && n <= most) break;
       if (n < k) hi = mid;
     }
-    for (int i = tid; i < total; i += kMergeBlock)
-      if (stage[i] >= lo) kept[atomicAdd(&n_kept, 1)] = stage[i];
+    for (int i = tid; i < total; i += kMergeBlock) {
+      if (stage[i] < lo) continue;
+      const int at = atomicAdd(&n_kept, 1);
+      if (at < kMaxK) kept[at] = stage[i];  // (more: of lists that are not of different ids)
+    }
     __syncthreads();
-    in_order<kMergeBlock, kMaxK>(kept, n_kept, put);
+    in_order<kMergeBlock, kMaxK>(kept, n_kept < kMaxK ? n_kept : kMaxK, put);
   } else {
     __syncthreads();
     for (int i = tid; i < total; i += kMergeBlock) {
