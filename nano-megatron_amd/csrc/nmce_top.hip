@@ -577,9 +577,10 @@ constexpr int kStaged = 7168;  // entries that a workgroup holds in LDS
 
 // One row's lists (entries of list l at lists + l * list_stride + row * row_stride, in
 // order) as one, either a list again (merged) or the results: the k-th entry by bisection
-// over all of them in LDS, then those that reach it in order. Lists of so many ranks that
-// LDS does not hold them: an entry's place is how many are above it, its own list's by its
-// index and the others' by bisection, from memory.
+// over all of them in LDS, then those that reach it in order. Up to 1024 are one wave's work
+// (16 lists of 20: 6.2 us, by all waves, a barrier a step, 8.6), beside the last wave's
+// normaliser. Lists of so many ranks that LDS does not hold them: an entry's place is how
+// many are above it, its own list's by its index and the others' by bisection, from memory.
 template <typename T>
 __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
     const uint64_t* __restrict__ lists, int64_t list_stride, int64_t row_stride, int n_lists,
@@ -587,13 +588,12 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
     int64_t* __restrict__ ids, float* __restrict__ norm) {
   extern __shared__ __align__(16) uint64_t stage[];  // n_lists * k entries, or none
   __shared__ __align__(16) uint64_t kept[kMaxK];
+  __shared__ uint64_t reached;
   __shared__ int counts[3], n_kept, n_have;
-  __shared__ float first;
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint64_t* in = lists + row * row_stride;
   const int total = n_lists * k;
-  const bool staged = total <= kStaged;
   const int most = enough(k, kMaxK);
   if (tid == 0) n_kept = n_have = counts[0] = counts[1] = counts[2] = 0;
   auto put = [&](int rank, uint64_t key) {
@@ -602,12 +602,37 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
       merged[row * (k + 1) + rank] = key;
       return;
     }
-    const float f = Rank<float>::value(static_cast<uint32_t>(key >> 32));
-    Elem<T>::store1(values + row * k + rank, f);
+    Elem<T>::store1(values + row * k + rank,
+                    Rank<float>::value(static_cast<uint32_t>(key >> 32)));
     ids[row * k + rank] = 0xffffffffu - static_cast<uint32_t>(key);
-    if (rank == 0) first = f;
   };
-  if (staged) {
+  // (maximum, sum) over the lists and the largest entry, a lane each: the last wave's.
+  auto normaliser = [&]() {
+    uint64_t pair = lane < n_lists ? in[lane * list_stride + k] : 0;
+    uint64_t head = lane < n_lists ? in[lane * list_stride] : 0;
+    float m = lane < n_lists ? __uint_as_float(static_cast<uint32_t>(pair >> 32)) : kNegHuge;
+    for (int l = lane + 64; l < n_lists; l += 64) {
+      m = fmaxf(m, __uint_as_float(static_cast<uint32_t>(in[l * list_stride + k] >> 32)));
+      head = in[l * list_stride] > head ? in[l * list_stride] : head;
+    }
+    m = wave_max(m);
+    head = wave_max_u64(head);
+    double s = 0.0;
+    for (int l = lane; l < n_lists; l += 64) {
+      if (l > lane) pair = in[l * list_stride + k];
+      const double lm = __uint_as_float(static_cast<uint32_t>(pair >> 32));
+      s += static_cast<double>(__uint_as_float(static_cast<uint32_t>(pair))) *
+           exp2_64((lm - static_cast<double>(m)) * (c * kLog2e64));
+    }
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+    if (lane != 0) return;
+    if (merged)
+      merged[row * (k + 1) + k] = static_cast<uint64_t>(__float_as_uint(m)) << 32 |
+                                  __float_as_uint(static_cast<float>(s));
+    else
+      norm[row] = log_norm(m, s, Rank<float>::value(static_cast<uint32_t>(head >> 32)), c);
+  };
+  if (total <= kStaged) {
     int have = 0;
     for (int i = tid; i < total; i += kMergeBlock) {
       const int l = i / k;
@@ -615,29 +640,42 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
       have += stage[i] != 0;
     }
     __syncthreads();
-    atomicAdd(&n_have, have);
-    // The wanted reach lo (the k of some list do), fewer than k reach hi.
-    uint64_t lo = 1, hi = 0;
-    for (int l = 0; l < n_lists; ++l) {
-      lo = stage[l * k + k - 1] > lo ? stage[l * k + k - 1] : lo;
-      hi = stage[l * k] > hi ? stage[l * k] : hi;
-    }
-    ++hi;
+    if (have) atomicAdd(&n_have, have);
     __syncthreads();
     const int some = n_have;
-    for (int turn = 0; some > most && hi - lo > 1; turn = turn == 2 ? 0 : turn + 1) {
-      const uint64_t mid = lo + (hi - lo) / 2;
-      int n = 0;
-#pragma unroll 4
-      for (int i = tid; i < total; i += kMergeBlock) n += stage[i] >= mid;
-      for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
-      if (lane == 0) atomicAdd(&counts[turn], n);
+    uint64_t lo = 1;  // the wanted reach it
+    if (some > most && total <= 1024) {
+      if (wave == 0) {
+        lo = kth_key(stage, total, k, most);
+        if (lane == 0) reached = lo;
+      } else if (wave == kMergeBlock / 64 - 1) {
+        normaliser();
+      }
       __syncthreads();
-      n = counts[turn];
-      if (tid == 0) counts[turn == 0 ? 2 : turn - 1] = 0;  // read by all before this barrier
-      if (n >= k) lo = mid;
-      if (n >= k && n <= most) break;
-      if (n < k) hi = mid;
+      lo = reached;
+    } else {
+      // (The k of some list reach lo), fewer than k reach hi.
+      uint64_t hi = 0;
+      for (int l = 0; l < n_lists; ++l) {
+        lo = stage[l * k + k - 1] > lo ? stage[l * k + k - 1] : lo;
+        hi = stage[l * k] > hi ? stage[l * k] : hi;
+      }
+      ++hi;
+      for (int turn = 0; some > most && hi - lo > 1; turn = turn == 2 ? 0 : turn + 1) {
+        const uint64_t mid = lo + (hi - lo) / 2;
+        int n = 0;
+#pragma unroll 4
+        for (int i = tid; i < total; i += kMergeBlock) n += stage[i] >= mid;
+        for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
+        if (lane == 0) atomicAdd(&counts[turn], n);
+        __syncthreads();
+        n = counts[turn];
+        if (tid == 0) counts[turn == 0 ? 2 : turn - 1] = 0;  // read by all before this barrier
+        if (n >= k) lo = mid;
+        if (n >= k && n <= most) break;
+        if (n < k) hi = mid;
+      }
+      if (wave == kMergeBlock / 64 - 1) normaliser();
     }
     for (int i = tid; i < total; i += kMergeBlock) {
       if (stage[i] < lo) continue;
@@ -667,8 +705,9 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
       }
       put(rank, key);
     }
+    if (wave == kMergeBlock / 64 - 1) normaliser();
+    __syncthreads();
   }
-  __syncthreads();
   for (int i = n_have + tid; i < k; i += kMergeBlock) {  // (more wanted than there are)
     if (merged) {
       merged[row * (k + 1) + i] = 0;
@@ -677,26 +716,6 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
       ids[row * k + i] = -1;
     }
   }
-  if (tid >= 64) return;
-  // (maximum, sum) over the lists, a lane each.
-  float m = kNegHuge;
-  for (int l = lane; l < n_lists; l += 64)
-    m = fmaxf(m, __uint_as_float(static_cast<uint32_t>(in[l * list_stride + k] >> 32)));
-  m = wave_max(m);
-  double s = 0.0;
-  for (int l = lane; l < n_lists; l += 64) {
-    const uint64_t pair = in[l * list_stride + k];
-    const double lm = __uint_as_float(static_cast<uint32_t>(pair >> 32));
-    s += static_cast<double>(__uint_as_float(static_cast<uint32_t>(pair))) *
-         exp2_64((lm - static_cast<double>(m)) * (c * kLog2e64));
-  }
-  for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
-  if (lane != 0) return;
-  if (merged)
-    merged[row * (k + 1) + k] = static_cast<uint64_t>(__float_as_uint(m)) << 32 |
-                                __float_as_uint(static_cast<float>(s));
-  else
-    norm[row] = log_norm(m, s, first, c);
 }
 
 // (A temperature past these is merely very high or very low.)
