@@ -154,7 +154,11 @@ __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adj
   __shared__ double bias_sum[kBiases];
   __shared__ int repeated, wave_n[kBlock / 64];
   const int tid = threadIdx.x;
-  const int64_t bp = blockIdx.x / slabs, slab = blockIdx.x - bp * slabs;
+  // Neighbours in this order, which read the same lists, share an XCD and its L2 (workgroups go
+  // to the eight in turn): 8 rows with 139264 ids each 28 -> 25 us.
+  const uint32_t xcd = blockIdx.x % 8, eighth = gridDim.x / 8, over = gridDim.x % 8;
+  const int64_t turn = xcd * eighth + (xcd < over ? xcd : over) + blockIdx.x / 8;
+  const int64_t bp = turn / slabs, slab = turn - bp * slabs;
   const int64_t b = bp / parts, part = bp - b * parts;
   const int64_t first = part * rows_each;
   const int64_t last = first + rows_each < a.rows ? first + rows_each : a.rows;
