@@ -576,11 +576,13 @@ constexpr int kMergeBlock = 512;
 constexpr int kStaged = 7168;  // entries that a workgroup holds in LDS
 
 // One row's lists (entries of list l at lists + l * list_stride + row * row_stride, in
-// order) as one, either a list again (merged) or the results: the k-th entry by bisection
-// over all of them in LDS, then those that reach it in order. Up to 1024 are one wave's work
-// (16 lists of 20: 6.2 us, by all waves, a barrier a step, 8.6), beside the last wave's
-// normaliser. Lists of so many ranks that LDS does not hold them: an entry's place is how
-// many are above it, its own list's by its index and the others' by bisection, from memory.
+// order) as one, either a list again (merged) or the results. Staged in LDS, one wave finds
+// the k-th entry, then those that reach it are put in order. Up to 1024 are held by the wave
+// (16 lists of 20: 5.9 us; as below 7.6). Of more, a lane counts a list's entries that reach a
+// key, a search between those of the last two keys (16 rows of 14 lists of 500: 25 us; counted
+// by all waves among all entries 54). The last wave takes the normaliser meanwhile. Of more
+// lists, or than LDS holds, an entry's place is how many are above it, its own list's by its
+// index and the others' by bisection, from memory.
 template <typename T>
 __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
     const uint64_t* __restrict__ lists, int64_t list_stride, int64_t row_stride, int n_lists,
@@ -589,13 +591,13 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
   extern __shared__ __align__(16) uint64_t stage[];  // n_lists * k entries, or none
   __shared__ __align__(16) uint64_t kept[kMaxK];
   __shared__ uint64_t reached;
-  __shared__ int counts[3], n_kept, n_have;
+  __shared__ int n_kept, n_have;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint64_t* in = lists + row * row_stride;
   const int total = n_lists * k;
   const int most = enough(k, kMaxK);
-  if (tid == 0) n_kept = n_have = counts[0] = counts[1] = counts[2] = 0;
+  if (tid == 0) n_kept = n_have = 0;
   auto put = [&](int rank, uint64_t key) {
     if (rank >= k) return;
     if (merged) {
@@ -632,51 +634,77 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
     else
       norm[row] = log_norm(m, s, Rank<float>::value(static_cast<uint32_t>(head >> 32)), c);
   };
-  if (total <= kStaged) {
-    int have = 0;
-    for (int i = tid; i < total; i += kMergeBlock) {
-      const int l = i / k;
-      stage[i] = in[l * list_stride + (i - l * k)];
-      have += stage[i] != 0;
+  if (total <= kStaged && n_lists <= 64) {
+    constexpr int kAhead = 4;
+    for (int i0 = tid; i0 < total; i0 += kAhead * kMergeBlock) {
+      uint64_t e[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const int i = i0 + a * kMergeBlock < total ? i0 + a * kMergeBlock : total - 1;
+        const int l = i / k;
+        e[a] = in[l * list_stride + (i - l * k)];
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+        if (i0 + a * kMergeBlock < total) stage[i0 + a * kMergeBlock] = e[a];
     }
     __syncthreads();
-    if (have) atomicAdd(&n_have, have);
-    __syncthreads();
-    const int some = n_have;
-    uint64_t lo = 1;  // the wanted reach it
-    if (some > most && total <= 1024) {
-      if (wave == 0) {
-        lo = kth_key(stage, total, k, most);
-        if (lane == 0) reached = lo;
-      } else if (wave == kMergeBlock / 64 - 1) {
-        normaliser();
-      }
-      __syncthreads();
-      lo = reached;
-    } else {
-      // (The k of some list reach lo), fewer than k reach hi.
-      uint64_t hi = 0;
-      for (int l = 0; l < n_lists; ++l) {
-        lo = stage[l * k + k - 1] > lo ? stage[l * k + k - 1] : lo;
-        hi = stage[l * k] > hi ? stage[l * k] : hi;
-      }
-      ++hi;
-      for (int turn = 0; some > most && hi - lo > 1; turn = turn == 2 ? 0 : turn + 1) {
-        const uint64_t mid = lo + (hi - lo) / 2;
+    if (wave == 0) {
+      const uint64_t* own = stage + (lane < n_lists ? lane : 0) * k;
+      // How many of the list's entries, of which `a` do and those from b on do not, reach key.
+      auto reach = [&](uint64_t key, int a, int b) {
+        while (a < b) {
+          const int i = (a + b) / 2;
+          if (own[i] >= key) a = i + 1;
+          else b = i;
+        }
+        return a;
+      };
+      auto over_lists = [&](int v) {  // (of numbers up to kMaxK, a ballot a bit)
         int n = 0;
-#pragma unroll 4
-        for (int i = tid; i < total; i += kMergeBlock) n += stage[i] >= mid;
-        for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
-        if (lane == 0) atomicAdd(&counts[turn], n);
-        __syncthreads();
-        n = counts[turn];
-        if (tid == 0) counts[turn == 0 ? 2 : turn - 1] = 0;  // read by all before this barrier
-        if (n >= k) lo = mid;
-        if (n >= k && n <= most) break;
-        if (n < k) hi = mid;
+#pragma unroll
+        for (int bit = 0; kMaxK >> bit; ++bit) n += __popcll(__ballot(v >> bit & 1)) << bit;
+        return n;
+      };
+      // The k of some list reach lo (or, of short lists, all that there are).
+      uint64_t lo = wave_max_u64(lane < n_lists ? own[k - 1] : 0);
+      lo = lo > 0 ? lo : 1;
+      int a = 0, b = lane < n_lists ? reach(lo, 0, k) : 0;
+      const int all = over_lists(b);
+      // More than `most` reach lo, fewer than k some higher key: the middle one of the entries
+      // between in the list that has most of them is the next to count.
+      const bool small = total <= 1024;
+      if (small && all > most) lo = kth_key(stage, total, k, most);
+      for (int n = all; !small && n > most;) {
+        const uint64_t middle = a < b ? own[(a + b - 1) / 2] : 0;
+        const float widest =
+            wave_max(middle > lo ? static_cast<float>((b - a) * 64 + lane) : -1.0f);
+        if (widest < 0.0f) break;  // (of lists that are not of different ids)
+        const int from = __builtin_amdgcn_readfirstlane(static_cast<int>(widest)) & 63;
+        const uint64_t key =
+            static_cast<uint64_t>(static_cast<uint32_t>(
+                __builtin_amdgcn_readlane(static_cast<int>(middle >> 32), from)))
+                << 32 |
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(middle), from));
+        const int at = reach(key, a, b);
+        const int count = over_lists(at);
+        if (count >= k) {
+          lo = key;
+          b = at;
+          n = count;
+        } else {
+          a = at;
+        }
       }
-      if (wave == kMergeBlock / 64 - 1) normaliser();
+      if (lane == 0) {
+        reached = lo;
+        n_have = all;
+      }
+    } else if (wave == kMergeBlock / 64 - 1) {
+      normaliser();
     }
+    __syncthreads();
+    const uint64_t lo = reached;
     for (int i = tid; i < total; i += kMergeBlock) {
       if (stage[i] < lo) continue;
       const int at = atomicAdd(&n_kept, 1);
@@ -734,7 +762,8 @@ int64_t width_of(int64_t n_rows, int64_t v, int k) {
   const int64_t places = 4 * static_cast<int64_t>(device_cus());
   const int64_t slabs = n_rows > 0 ? places / n_rows : 1;
   if (slabs <= 1) return v;
-  const int64_t most = slabs < kStaged / k ? slabs : kStaged / k;
+  const int64_t merged = kStaged / k < 64 ? kStaged / k : 64;  // (from LDS)
+  const int64_t most = slabs < merged ? slabs : merged;
   int64_t width = round_up((v + most - 1) / most, 8);
   width = width > kLeast ? width : kLeast;
   return width > 16 * k ? width : 16 * k;
@@ -753,7 +782,7 @@ int merge(const uint64_t* lists, int64_t list_stride, int64_t row_stride, int n_
           float* norm, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(n_rows)), block(kMergeBlock);
   const int64_t total = static_cast<int64_t>(n_lists) * k;
-  const unsigned lds = total <= kStaged ? static_cast<unsigned>(total * 8) : 0;
+  const unsigned lds = total <= kStaged && n_lists <= 64 ? static_cast<unsigned>(total * 8) : 0;
   if (dtype == NMCE_F32)
     hipLaunchKernelGGL(top_merge_kernel<float>, grid, block, lds, s, lists, list_stride,
                        row_stride, n_lists, k, c, merged, static_cast<float*>(values), ids, norm);
