@@ -137,10 +137,10 @@ __device__ __forceinline__ void set_element(u32x4& v, int e, uint32_t bits) {
   }
 }
 
-// Part `part` of sequence b's rows, slab `slab` of the vocabulary.
+// Row `row` of sequence b, slab `slab` of the vocabulary.
 template <typename T, int kBlock, bool kInPlace, bool kNarrow>
 __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adjust_kernel(
-    nmce_adjust_batch a, int64_t slabs, int64_t parts, int64_t rows_each) {
+    nmce_adjust_batch a, int64_t slabs) {
   using E = Elem<T>;
   constexpr int kVec = E::kPerVec;
   constexpr int kEach = kSlab / kBlock / kVec;  // vectors of a thread
@@ -158,16 +158,17 @@ __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adj
   // to the eight in turn): 8 rows with 139264 ids each 28 -> 25 us.
   const uint32_t xcd = blockIdx.x % 8, eighth = gridDim.x / 8, over = gridDim.x % 8;
   const int64_t turn = xcd * eighth + (xcd < over ? xcd : over) + blockIdx.x / 8;
-  const int64_t bp = turn / slabs, slab = turn - bp * slabs;
-  const int64_t b = bp / parts, part = bp - b * parts;
-  const int64_t first = part * rows_each;
-  const int64_t last = first + rows_each < a.rows ? first + rows_each : a.rows;
+  const int64_t br = turn / slabs, slab = turn - br * slabs;
+  const int64_t b = br / a.rows, row = br - b * a.rows;
   const int64_t c0 = slab * kSlab;
   const int64_t left = a.vocab_local - c0;
   const int width = static_cast<int>(left < kSlab ? left : kSlab);
   const int64_t g0 = a.vocab_start + c0;  // the slab's first global id
-  const T* x = static_cast<const T*>(a.logits) + b * a.logits_batch_stride + c0;
-  T* y = static_cast<T*>(a.out) + b * a.out_batch_stride + c0;
+  const T* x = static_cast<const T*>(a.logits) + b * a.logits_batch_stride +
+               row * a.logits_row_stride + c0;
+  T* y = static_cast<T*>(a.out) + b * a.out_batch_stride + row * a.out_row_stride + c0;
+  const uint32_t* words =
+      a.allowed ? a.allowed + b * a.allowed_batch_stride + row * a.allowed_row_stride : nullptr;
   // The first column of the thread's vector k. (Opaque to the compiler, which would keep
   // what it can compute from each of them in registers through the rows.)
   auto column_of = [&](int k) {
@@ -176,35 +177,26 @@ __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adj
     return t + k * kBlock * kVec;
   };
 
-  // The first row's vectors are on their way while the lists are counted.
+  // The vectors and their masks are on their way while the lists are counted.
   u32x4 v[kEach];
   uint32_t lo[kEach], hi[kEach];  // the words with the vectors' mask bits
-  auto words_of = [&](int64_t row) {
-    return a.allowed ? a.allowed + b * a.allowed_batch_stride + row * a.allowed_row_stride
-                     : nullptr;
-  };
-  auto load_row = [&](int64_t row) {
-    if (const uint32_t* words = words_of(row)) {
+  if (words) {
 #pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        // (Past the vocabulary its last word again: no load waits for a condition.)
-        const int64_t g = g0 + column_of(k), end = a.vocab_total - 1;
-        lo[k] = words[(g < end ? g : end) >> 5];
-        hi[k] = words[(g + kVec - 1 < end ? g + kVec - 1 : end) >> 5];
-      }
+    for (int k = 0; k < kEach; ++k) {
+      // (Past the vocabulary its last word again: no load waits for a condition.)
+      const int64_t g = g0 + column_of(k), end = a.vocab_total - 1;
+      lo[k] = words[(g < end ? g : end) >> 5];
+      hi[k] = words[(g + kVec - 1 < end ? g + kVec - 1 : end) >> 5];
     }
-    if (kInPlace) return;
-    const T* p = x + row * a.logits_row_stride;
-    if (width == kSlab) {
+  }
+  if (!kInPlace && width == kSlab) {
 #pragma unroll
-      for (int k = 0; k < kEach; ++k) v[k] = load16(p + column_of(k));
-    } else {
+    for (int k = 0; k < kEach; ++k) v[k] = load16(x + column_of(k));
+  } else if (!kInPlace) {
 #pragma unroll
-      for (int k = 0; k < kEach; ++k)
-        if (column_of(k) + kVec <= width) v[k] = load16(p + column_of(k));
-    }
-  };
-  load_row(first);
+    for (int k = 0; k < kEach; ++k)
+      if (column_of(k) + kVec <= width) v[k] = load16(x + column_of(k));
+  }
 
   const int64_t* bias_ids = a.bias_ids + b * a.bias_ids_stride;
   const float* bias = a.bias + b * a.bias_stride;
@@ -282,7 +274,7 @@ __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adj
       __syncthreads();
     }
     count_list(a.output + b * a.output_stride, a.n_output, std::false_type{});
-    count_list(a.drafts + b * a.drafts_stride, first, std::false_type{});
+    count_list(a.drafts + b * a.drafts_stride, row, std::false_type{});
   }
   // The slab's biases in their order (the first of them were asked for at the start).
   int n_here = 0;
@@ -346,97 +338,83 @@ __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adj
     __syncthreads();
   }
 
-  for (int64_t row = first; row < last; ++row) {
-    const T* xr = x + row * a.logits_row_stride;
-    T* yr = y + row * a.out_row_stride;
-    const uint32_t* words = words_of(row);
-    auto allowed = [&](int s) {
-      return !words || (words[(g0 + s) >> 5] >> ((g0 + s) & 31) & 1u);
+  auto allowed = [&](int s) {
+    return !words || (words[(g0 + s) >> 5] >> ((g0 + s) & 31) & 1u);
+  };
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int c = column_of(k);
+    if (c + kVec > width) break;
+    // The vector's allowed ids, the first in bit 0.
+    const uint64_t both = static_cast<uint64_t>(hi[k]) << 32 | lo[k];
+    const uint32_t bits =
+        words ? static_cast<uint32_t>(both >> ((g0 + c) & 31)) & kAll : kAll;
+    // Those with a count, and allowed.
+    uint32_t touched = counted ? count.template some<kVec>(c) & bits : 0u;
+    if (kInPlace) {
+      if (bits == kAll && touched == 0) continue;  // nothing to write
+      if (bits != 0) v[k] = load16(x + c);
+    }
+    for (; touched; touched &= touched - 1) {  // (with a bias: formed by that, below)
+      const int e = __builtin_ctz(touched);
+      const uint32_t was = element<T>(v[k], e);
+      const float f = sizeof(T) == 4 ? __uint_as_float(was)
+                                     : bf16_to_f32(static_cast<uint16_t>(was));
+      T to;
+      const uint32_t word = count.at(c + e);
+      if (word & Count::kBiased) continue;
+      store_rounded(&to, pen.on(static_cast<double>(f), word, count));
+      uint32_t is;
+      if constexpr (sizeof(T) == 4) is = __float_as_uint(to);
+      else is = to;
+      set_element<T>(v[k], e, is);
+    }
+    if (bits != kAll) {
+      float f[kVec];
+      E::unpack(v[k], f);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) f[e] = bits >> e & 1u ? f[e] : -kInf;
+      v[k] = E::pack(f);
+    }
+    store16(y + c, v[k]);
+  }
+  // The shard's last elements, of no whole vector.
+  const int c = width / kVec * kVec + tid;
+  if (c < width) {
+    const uint32_t word = count.at(c);
+    if (!allowed(c)) E::store1(y + c, -kInf);
+    else if (!(word & Count::kBiased) && word)
+      store_rounded(y + c, pen.on(static_cast<double>(E::load1(x + c)), word, count));
+    else if (!kInPlace) y[c] = x[c];
+  }
+  if (n_here > 0) {
+    // The stores have reached the memory before any thread of the workgroup
+    // stores an element over them.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    auto put = [&](int s, double add) {
+      if (s < kSlab && allowed(s))
+        store_rounded(y + s, pen.on(static_cast<double>(E::load1(x + s)), count.at(s), count) +
+                                  add);
     };
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int c = column_of(k);
-      if (c + kVec > width) break;
-      // The vector's allowed ids, the first in bit 0.
-      const uint64_t both = static_cast<uint64_t>(hi[k]) << 32 | lo[k];
-      const uint32_t bits =
-          words ? static_cast<uint32_t>(both >> ((g0 + c) & 31)) & kAll : kAll;
-      // Those with a count, and allowed.
-      uint32_t touched = counted ? count.template some<kVec>(c) & bits : 0u;
-      if (kInPlace) {
-        if (bits == kAll && touched == 0) continue;  // nothing to write
-        if (bits != 0) v[k] = load16(xr + c);
-      }
-      for (; touched; touched &= touched - 1) {  // (with a bias: formed by that, below)
-        const int e = __builtin_ctz(touched);
-        const uint32_t was = element<T>(v[k], e);
-        const float f = sizeof(T) == 4 ? __uint_as_float(was)
-                                       : bf16_to_f32(static_cast<uint16_t>(was));
-        T to;
-        const uint32_t word = count.at(c + e);
-        if (word & Count::kBiased) continue;
-        store_rounded(&to, pen.on(static_cast<double>(f), word, count));
-        uint32_t is;
-        if constexpr (sizeof(T) == 4) is = __float_as_uint(to);
-        else is = to;
-        set_element<T>(v[k], e, is);
-      }
-      if (bits != kAll) {
-        float f[kVec];
-        E::unpack(v[k], f);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) f[e] = bits >> e & 1u ? f[e] : -kInf;
-        v[k] = E::pack(f);
-      }
-      store16(yr + c, v[k]);
-    }
-    // The shard's last elements, of no whole vector.
-    const int c = width / kVec * kVec + tid;
-    if (c < width) {
-      const uint32_t word = count.at(c);
-      if (!allowed(c)) E::store1(yr + c, -kInf);
-      else if (!(word & Count::kBiased) && word)
-        store_rounded(yr + c, pen.on(static_cast<double>(E::load1(xr + c)), word, count));
-      else if (!kInPlace) yr[c] = xr[c];
-    }
-    if (row + 1 < last) load_row(row + 1);
-    if (n_here > 0) {
-      // The row's stores have reached the memory before any thread of the workgroup
-      // stores an element over them.
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      auto put = [&](int s, double add) {
-        if (s < kSlab && allowed(s))
-          store_rounded(yr + s, pen.on(static_cast<double>(E::load1(xr + s)), count.at(s), count) +
-                                    add);
-      };
-      if (in_lds) {
-        for (int t = tid; t < n_here; t += kBlock) put(bias_place[t], bias_sum[t]);
-      } else {
-        for (int64_t j = tid; j < a.n_bias; j += kBlock) {
-          const int64_t id = bias_ids[j];
-          const int s = place(id);
-          if (s >= kSlab) continue;
-          double add = bias[j];
-          if (apart) {
-            // The first entry of an id adds all of them, in their order.
-            bool mine = true;
-            for (int64_t i = 0; i < j && mine; ++i) mine = bias_ids[i] != id;
-            if (!mine) continue;
-            for (int64_t i = j + 1; i < a.n_bias; ++i)
-              if (bias_ids[i] == id) add += static_cast<double>(bias[i]);
-          }
-          put(s, add);
+    if (in_lds) {
+      for (int t = tid; t < n_here; t += kBlock) put(bias_place[t], bias_sum[t]);
+    } else {
+      for (int64_t j = tid; j < a.n_bias; j += kBlock) {
+        const int64_t id = bias_ids[j];
+        const int s = place(id);
+        if (s >= kSlab) continue;
+        double add = bias[j];
+        if (apart) {
+          // The first entry of an id adds all of them, in their order.
+          bool mine = true;
+          for (int64_t i = 0; i < j && mine; ++i) mine = bias_ids[i] != id;
+          if (!mine) continue;
+          for (int64_t i = j + 1; i < a.n_bias; ++i)
+            if (bias_ids[i] == id) add += static_cast<double>(bias[i]);
         }
+        put(s, add);
       }
-    }
-    if (row + 1 < last && counted) {
-      __syncthreads();  // every thread is done with this row's counts
-      if (tid == 0) {
-        const int s = place(a.drafts[b * a.drafts_stride + row]);
-        if (s < kSlab) count.once_more(s);
-      }
-      __syncthreads();
     }
   }
 }
@@ -489,21 +467,19 @@ int nmce_adjust_logits(const nmce_adjust_batch* a, void* stream) {
   if (in_place && (a->logits_batch_stride != a->out_batch_stride ||
                    a->logits_row_stride != a->out_row_stride))
     return NMCE_EINVAL_SHAPE;
-  // A workgroup for every row (24 x 9 rows of 151936 bf16 with 1250 ids each: 38 us, by three
-  // rows 42, by nine 68), unless the lists, which each counts again, are longer than a slab.
-  const int64_t lists = a->n_prompt + a->n_output;
-  const int64_t want = 2 * static_cast<int64_t>(device_cus()) / (a->batch * slabs);
-  const int64_t rows_each = lists <= kSlab ? 1
-                            : want <= 1    ? a->rows
-                                           : (a->rows + want - 1) / want;
-  const int64_t parts = (a->rows + rows_each - 1) / rows_each;
-  const dim3 grid(static_cast<unsigned>(a->batch * parts * slabs));
+  // A workgroup for a slab of every row, drafts' too, which counts the lists again (24 x 9 rows
+  // of 151936 bf16: with 1250 ids 29 us, by nine rows each 62; with 64250 82 and 134).
+  const dim3 grid(static_cast<unsigned>(a->batch * a->rows * slabs));
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto run = [&](auto kernel, int threads) {
-    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, g, slabs, parts, rows_each);
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, g, slabs);
   };
-  // Where there is no workgroup for every compute unit, 1024 threads share a slab.
-  const bool few = static_cast<int64_t>(grid.x) <= device_cus();
+  // Where there is no workgroup for every compute unit, 1024 threads share a slab (8 rows with
+  // 139264 ids each: 25 us, by 256 threads 54; 64 rows of 128256, enough workgroups: 24 and 16);
+  // with lists longer than a slab, two (30 rows of 128256, 30250 ids: 17 us and 23; 450: 11
+  // and 10).
+  const int64_t lists = a->n_prompt + a->n_output;
+  const bool few = static_cast<int64_t>(grid.x) <= (lists > kSlab ? 2 : 1) * device_cus();
   const bool narrow = a->n_output + a->rows <= static_cast<int64_t>(Counts<true>::kTimes);
   auto pick = [&](auto element, auto in_place_, auto narrow_) {
     using T = decltype(element);
