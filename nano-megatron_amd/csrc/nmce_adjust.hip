@@ -14,7 +14,7 @@
 // bits and rounded once, in the registers, before the store. What bounds a batch is one
 // read and one write of the logits; in place only vectors with something to change move.
 // 24 x 9 rows of 151936 bf16, 1250 listed ids, masked: 29 us (4.7 TB/s with the masks; the
-// counts, a barrier before the first store, are what is left to 24); 64 x 1 of 128256: 15;
+// counts, before the first store, are what is left to 21); 64 x 1 of 128256: 15;
 // one of 50257 fp32: 6, a launch and three dependent reads; 8 of 100277 fp32 with 139264 ids
 // and 300 biases each: 24, of which the lists take 12 (a compute unit's 64 bytes a cycle from
 // its L2: 7) and the biases 8.

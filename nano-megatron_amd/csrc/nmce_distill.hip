@@ -506,15 +506,14 @@ __global__ __launch_bounds__(kBlock) void distill_bwd_kernel(
 // Whole-vocabulary rows (one rank) held by a workgroup of 1024 threads: in registers (up to 8
 // vectors a thread; two workgroups a compute unit), or 9 of up to 16 in LDS. Bounded by HBM
 // with a whole row between its read and its write: 2047 x 50257 bf16 87 us (4.8 TB/s), 8192 x
-// 128256 790 (5.3; a copy 5.6). A step of these takes 136 and 871 us, by two passes 170 and 1018.
-// The
-// listed elements are set to -inf where they are held, so that the fold sees what is
-// outside; each wave does that for its own elements, one listed id after another, and
-// writes their gradients over the row's, by the lanes that stored it. The gradient is
-// that of the mean for the upstream value assumed[0] (the list kernel's);
-// loss and slopes as from distill_combine_kernel, the slopes in fp32. Vectors, edges
-// (kRagged: rows of any width and alignment, the gradient's as the logits') and buffer
-// resources as in the cross entropy's one-pass kernels. g may be x.
+// 128256 790 (5.3; a streaming copy 6.5). A step of these takes 136 and 871 us, by two passes 170 and
+// 1018. The listed elements are set to -inf where they are held, so that the fold sees what is
+// outside; each wave does that for its own elements, one listed id after another, and writes
+// their gradients over the row's, by the lanes that stored it. The gradient is that of the mean
+// for the upstream value assumed[0] (the list kernel's); loss and slopes as from
+// distill_combine_kernel, the slopes in fp32. Vectors, edges (kRagged: rows of any width and
+// alignment, the gradient's as the logits') and buffer resources as in the cross entropy's
+// one-pass kernels. g may be x.
 constexpr int kRowBlock = 1024;
 constexpr int kRowWaves = kRowBlock / 64;
 constexpr int kWideLo = 7, kWideHi = 9;
