@@ -558,6 +558,48 @@ def test_threads_on_streams_of_their_own():
     assert not wrong
 
 
+@pytest.mark.parametrize("mean", [False, True])
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_the_ranks_node_is_the_single_one(dtype, inplace, mean):
+    """The node of several ranks, of one: the same kernels, storage and refusals."""
+    from nmce.distill import _VocabParallelDistillation as Node
+    g = torch.Generator().manual_seed(20)
+    n, v = 6, 3003
+    x, t, ids, norm = (a.to(DEV) for a in _inputs(n, v, 11, dtype, g))
+    up = torch.tensor(0.75, device=DEV) if mean else \
+        torch.linspace(-1.0, 2.0, n, device=DEV)
+    wide = torch.zeros(n, v + 5, dtype=dtype, device=DEV)
+    wide[:, :v] = x
+    for rows in (lambda y: y, lambda y: y.t().contiguous().t(), lambda y: y.view(2, 3, v)):
+        got = []
+        for node in (True, False):
+            leaf = wide.clone().requires_grad_(True)
+            y = rows((leaf * 1.0)[:, :v])
+            lead = y.shape[:-1]
+            args = [t.view(*lead, 11), ids.view(*lead, 11), norm.view(lead)]
+            if node:
+                loss = Node.apply(y, *args, 0, None, 1, 1.0, mean, inplace)
+            else:
+                loss = _loss(y, *args, reduction="mean" if mean else "none", inplace=inplace,
+                             one_pass=False)
+            grad, = torch.autograd.grad(loss, leaf, up.view(loss.shape), retain_graph=True)
+            got.append((loss.detach(), grad))
+            if inplace and y._version:  # the logits hold the gradient now
+                with pytest.raises(RuntimeError):
+                    torch.autograd.grad(loss, leaf, up.view(loss.shape))
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_means_of_nothing():
+    for one_pass in (True, False):
+        x = torch.empty(0, 50, device=DEV, requires_grad=True)
+        loss = _loss(x, torch.empty(0, 3), torch.empty(0, 3, dtype=torch.int64),
+                     one_pass=one_pass)
+        assert loss.shape == () and bool(torch.isnan(loss))
+        assert torch.autograd.grad(loss, x)[0].shape == (0, 50)
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_long_lists_of_few_ids(tail):
     """1024 entries of one id, of two in turn, and each of 512 twice."""
