@@ -107,6 +107,63 @@ def test_serving_step(whole):
             assert abs(whole["logprobs"][b, i] - float(logp[b, i, j])) <= 2.0 ** -20 * 20
 
 
+def test_two_captured_runs_at_once():
+    """A server's and a trainer's calls, captured twice with other inputs and upstream
+    values, and replayed on two streams at the same time: no memory is shared."""
+    import nmce
+    ctx = nmce.ParallelContext.single()
+    n, v, k = 24, 20000, 20
+    g = torch.Generator().manual_seed(32)
+    runs = []
+    for i, up in enumerate((1.0, 8.0)):
+        logits = (torch.randn(n, 1, v, generator=g) * 3).to(DEV, torch.bfloat16)
+        output = torch.randint(0, v, (n, 300), generator=g).to(DEV)
+        student = torch.randn(n, v, generator=g).to(DEV, torch.bfloat16).requires_grad_(True)
+        runs.append((logits, output, student, torch.tensor(up, device=DEV)))
+
+    def step(logits, output, student, up):
+        with torch.no_grad():
+            adjusted = nmce.vocab_parallel_adjust_logits(
+                logits, 0, v, ctx, output_tokens=output, repetition_penalty=1.3,
+                frequency_penalty=0.5, bias_ids=output[:, :7], bias_values=output[:, :7].float())
+            values, ids, norm = nmce.vocab_parallel_top_logits(adjusted[:, 0], k, 0, v, ctx)
+        loss = nmce.vocab_parallel_distillation_loss(student, values, ids, 0, v, ctx,
+                                                     teacher_log_normalizer=norm)
+        grad, = torch.autograd.grad(loss, student, up)
+        return adjusted, values, ids, norm, loss.detach(), grad
+
+    want = [tuple(t.clone() for t in step(*r)) for r in runs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for r in runs:
+            step(*r)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for r in runs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(*r))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(4):
+        for o in outs:
+            for t in o:
+                t.fill_(-1)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for o, w, r in zip(outs, want, runs):
+            assert all(torch.equal(a, b) for a, b in zip(o[:5], w[:5]))
+            # (Written for the assumed upstream value or again: a bf16 step of rounding.)
+            a, b = o[5].float(), w[5].float()
+            assert bool(((a - b).abs() <= 2.0 ** -7 * b.abs() + float(r[3]) / n * 2.0 ** -24).all())
+        step(*runs[turn % 2])  # eager work between
+
+
 def test_distilling_step(whole):
     """The step's loss and weight gradient against the same in 64 bits. The logits are
     fp32 products of 96 terms (sums off by 96 2^-24 of their terms' sizes, about 2^-24
