@@ -672,7 +672,8 @@ int nmce_adjust_logits(const nmce_adjust_batch* batch, void* stream);
 /*
  * The k largest logits of each row of a vocabulary shard with their ids, in order
  * (of equal ones the lowest id first; NaN above +inf; -0 as 0), and the row's
- * log sum exp(x / temperature). k at most NMCE_TOP_MAX_K, n_rows at most 2^22.
+ * log sum exp(x / temperature). k at most NMCE_TOP_MAX_K, n_rows at most 2^22,
+ * temperature from 1e-30 to 1e30.
  *   - list NULL: the results. values [n_rows, k] in the logits' type, ids
  *     [n_rows, k], log_normalizer [n_rows]; k is at most vocab_local.
  *   - otherwise list [n_rows, k + 1]: this shard's part (fewer than k entries

@@ -752,9 +752,6 @@ __global__ __launch_bounds__(kMergeBlock) void top_merge_kernel(
   }
 }
 
-// (A temperature past these is merely very high or very low.)
-double inverse(double temperature) { return fmin(fmax(1.0 / temperature, 1e-30), 1e30); }
-
 int id_bits_of(int64_t v) {
   int bits = 1;
   while ((int64_t{1} << bits) < v) ++bits;
@@ -780,7 +777,7 @@ int64_t width_of(int64_t n_rows, int64_t v, int k) {
 int check_rows(int dtype, int64_t n_rows, int64_t v, int k, double temperature) {
   if (dtype != NMCE_F32 && dtype != NMCE_BF16) return NMCE_EINVAL_DTYPE;
   if (n_rows < 0 || n_rows > (int64_t{1} << 22) || v < 1 || v >= (int64_t{1} << 31) || k < 1 ||
-      k > kMaxK || !(temperature > 0.0 && temperature < HUGE_VAL))
+      k > kMaxK || !(temperature >= 1e-30 && temperature <= 1e30))  // (its inverse in fp32)
     return NMCE_EINVAL_SHAPE;
   return NMCE_OK;
 }
@@ -836,7 +833,7 @@ int nmce_top_logits(const void* logits, int dtype, int64_t n_rows, int64_t vocab
   const dim3 grid(static_cast<unsigned>(n_rows * slabs));
   hipStream_t s = static_cast<hipStream_t>(stream);
   uint64_t* lists = static_cast<uint64_t*>(workspace);
-  const double c = inverse(temperature);
+  const double c = 1.0 / temperature;
   const float c2 = static_cast<float>(1.4426950408889634 * c);
   const int bits = id_bits_of(vocab_local);
   const bool whole = slabs == 1 && !list;
@@ -868,7 +865,7 @@ int nmce_top_merge(const int64_t* lists, int ranks, int dtype, int64_t n_rows, i
   if (n_rows == 0) return NMCE_OK;
   if (!lists || !values || !ids || !log_normalizer) return NMCE_EINVAL_PTR;
   return merge(reinterpret_cast<const uint64_t*>(lists), n_rows * (k + 1), k + 1, ranks, dtype,
-               n_rows, k, inverse(temperature), nullptr, values, ids, log_normalizer,
+               n_rows, k, 1.0 / temperature, nullptr, values, ids, log_normalizer,
                static_cast<hipStream_t>(stream));
 }
 

@@ -125,7 +125,8 @@ def vocab_parallel_adjust_logits(
     set. A masked element is ``-inf`` whatever it held; a row may have none left.
 
     ``inplace=True`` writes into ``logits`` and returns it: only the touched and
-    the masked elements are written. Its rows must not overlap.
+    the masked elements are written. Its rows must not overlap. A call takes up to 2^23
+    slabs: ``B (K + 1) ceil(V / tp / 8192)``.
     """
     _check_adjust(logits, vocab_start, vocab_end, ctx, prompt_tokens, output_tokens, draft_tokens,
                   (("repetition_penalty", repetition_penalty),

@@ -12,8 +12,6 @@ of them return the same. There is no derivative and no CPU path.
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib
@@ -38,8 +36,8 @@ def _check_top(logits, k, vocab_start, vocab_end, ctx, temperature) -> None:
     if not 1 <= k <= min(MAX_TOP, total):
         raise ValueError(f"nmce: k must be from 1 to {min(MAX_TOP, total)} (at most {MAX_TOP}, and "
                          f"the vocabulary's {total}), got {k}")
-    if not (0.0 < temperature < math.inf):
-        raise ValueError(f"nmce: temperature must be a finite number above 0, got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"nmce: temperature must be from 1e-30 to 1e30, got {temperature}")
     _lib.refuse_gradient(logits, "logits", "the top logits have")
 
 
@@ -57,7 +55,7 @@ def vocab_parallel_top_logits(
     ``values`` ``[..., k]`` are the ``k`` largest logits (at most 512) in falling
     order, in the logits' type; ``ids`` ``[..., k]`` their global ids, int64, of
     equal logits the lowest first; ``log_normalizer`` ``[...]`` is the fp32
-    ``log sum exp(x / temperature)``. NaN counts as larger than +inf and makes the
+    ``log sum exp(x / temperature)``, temperatures from 1e-30 to 1e30. NaN counts as larger than +inf and makes the
     normaliser NaN; -inf is a logit like others (a masked row gives its lowest ids
     and the normaliser -inf); -0 comes back as 0.
     """

@@ -142,7 +142,7 @@ def test_top_argument_errors_before_launch(lib):
     assert top(dtype=2) == -1
     for bad in (dict(n=-1), dict(n=(1 << 22) + 1), dict(v=0), dict(v=1 << 31), dict(ld=99),
                 dict(start=-1), dict(start=(1 << 31) - 100), dict(k=0), dict(k=513), dict(k=101),
-                dict(t=0.0), dict(t=-1.0), dict(t=float("nan")), dict(t=float("inf"))):
+                dict(t=0.0), dict(t=-1.0), dict(t=float("nan")), dict(t=1e31), dict(t=1e-31)):
         assert top(**bad) == -2, bad
     assert top(logits=p + 2) == top(logits=p + 1, dtype=1) == -3
     for name in ("logits", "values", "ids", "norm"):
@@ -184,7 +184,7 @@ def test_top_refuses_shapes_and_types():
             check(k=k)
     with pytest.raises(ValueError, match="k must be"):
         check(Fake((2, 1000), F32), k=513, end=1000)
-    for t in (0.0, -1.0, float("inf"), float("nan")):
+    for t in (0.0, -1.0, 1e-31, 1e31, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="temperature"):
             check(t=t)
     with pytest.raises(RuntimeError, match="no CPU path"):

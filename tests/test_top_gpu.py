@@ -124,6 +124,13 @@ def test_values_far_apart_and_extreme_temperatures():
     _check(x, 50)
     _check(x[1:2], 50, 100.0)
     _check(x[3:], 50, 0.01)
+    _check(x[:1], 50, 1e30)
+    _check(x[1:2], 50, 1e-30)
+    _check(x, 50, 1e30)
+    y = torch.full((1, 600), -INF)
+    y[0, 7:9] = 3e38  # (over the highest temperature 3e8)
+    _check(y, 5, 1e30)
+    _check(torch.zeros(1, 600), 5, 1e-30)
 
 
 def test_shapes_strides_and_empty():
