@@ -187,16 +187,18 @@ __global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(
     norm = static_cast<double>(a.teacher_log_normalizer[row]);
     if (norm == -static_cast<double>(kInf)) any = false;  // (a teacher's row of only -inf)
   }
-  // (The table is done with; of a list that names an id twice p and ids come there.)
-  float* held_p = reinterpret_cast<float*>(seen);
-  int* held_at = seen + a.k;
+  // (The table is done with; of a list that names an id twice its logits and ids come there.)
+  float* held_t = reinterpret_cast<float*>(seen);
+  int* held_id = seen + a.k;
   double p_all = 0.0, h = 0.0, dot = 0.0, sum = 0.0;
   for (int j = lane; j < a.k; j += 64) {
     const int64_t id = ids[j];
     const int at = any ? column_of(id) : -1;
     double p = 0.0;
+    float tj = 0.0f;
     if (any && held(id)) {
-      const double lp = static_cast<double>(Elem<TT>::load1(t + j)) * c - norm;
+      tj = Elem<TT>::load1(t + j);
+      const double lp = static_cast<double>(tj) * c - norm;
       p = probability(lp);
       p_all += p;
       const bool some = p > 0.0 || p != p;
@@ -210,30 +212,41 @@ __global__ __launch_bounds__(kListWaves * 64) void distill_list_kernel(
     st.column[base + j] = at;
     st.p[base + j] = static_cast<float>(p);
     if (again) {
-      held_p[j] = static_cast<float>(p);
-      held_at[j] = at;
+      held_t[j] = tj;
+      held_id[j] = any && held(id) ? static_cast<int>(id) : -1;
     }
   }
   if (again) {
-    // An id's first place takes all of its p, in their order; the others are none.
+    // An id's first place takes all of its p, in their order, for p log p too (of every id of
+    // the list, other shards' as well: all ranks have the same); the others are none.
     __builtin_amdgcn_wave_barrier();
+    h = 0.0;
     for (int j = lane; j < a.k; j += 64) {
-      const int at = held_at[j];
-      if (at < 0) continue;
-      int before = 0;
-      double p = 0.0;
+      const int id = held_id[j];
+      if (id < 0) continue;
+      const int at = column_of(id);
+      int before = 0, others = 0;
 #pragma unroll 8
       for (int i = 0; i < a.k; ++i) {
-        const bool same = held_at[i] == at;
+        const bool same = held_id[i] == id;
         before += same && i < j;
-        p += same && i >= j ? held_p[i] : 0.0f;
+        others += same && i > j;
       }
-      if (before == 0) {
-        st.p[base + j] = static_cast<float>(p);
-      } else {
+      if (before) {
         st.column[base + j] = -1;
-        sum -= exp2_hw((Elem<T>::load1(x + at) - top) * cl);  // counted at the first
+        if (at >= 0) sum -= exp2_hw((Elem<T>::load1(x + at) - top) * cl);  // counted at the first
+        continue;
       }
+      double lp = static_cast<double>(held_t[j]) * c - norm;
+      double p = probability(lp);
+      if (others) {
+        for (int i = j + 1; i < a.k; ++i)
+          if (held_id[i] == id)
+            p += probability(static_cast<double>(held_t[i]) * c - norm);
+        lp = log(p);
+        st.p[base + j] = static_cast<float>(p);
+      }
+      if (p > 0.0 || p != p) h += p * lp;
     }
   }
   p_all = wave_add(p_all);
