@@ -144,8 +144,9 @@ struct Shared {
   double wave_s[Shape::kBlock / 64];
 };
 
-// One wave: a key that k to `most` of n unique keys (n >= k) reach, by bisection over eight
-// of them a lane in registers, and what there is beyond 512 from LDS.
+// One wave: a key that k to `most` of n keys reach, by bisection over eight of them a lane in
+// registers, and what there is beyond 512 from LDS. The keys are unique but for zeros, which
+// are none and reach nothing; of the others there are k at least, and more than `most` if n is.
 __device__ uint64_t kth_key(const uint64_t* list, int n, int k, int most) {
   constexpr int kHeld = 8;
   const int lane = threadIdx.x & 63;
@@ -164,7 +165,10 @@ __device__ uint64_t kth_key(const uint64_t* list, int n, int k, int most) {
     lo = list[i] < lo ? list[i] : lo;
     hi = list[i] > hi ? list[i] : hi;
   }
+  // Above 0: past the largest entry there can be (a NaN's at id 0, all ones) hi is 2^64, held
+  // as 0, and hi - lo is right only where lo is not 0 too.
   lo = wave_min_u64(lo);
+  lo = lo > 0 ? lo : 1;
   hi = wave_max_u64(hi) + 1;
   while (n > most && hi - lo > 1) {  // more than `most` reach lo, fewer than k reach hi
     const uint64_t mid = lo + (hi - lo) / 2;  // (above lo, so a 0 does not reach it)
