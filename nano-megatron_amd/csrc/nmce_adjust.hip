@@ -97,10 +97,11 @@ struct Counts {
 struct Penalties {
   double r, f, p, inv;  // inv: 1 / r
   __device__ __forceinline__ bool none() const { return r == 1.0 && f == 0.0 && p == 0.0; }
-  // x / r by the reciprocal and one correction (an infinite x has none to take).
+  // x / r, x > 0, by the reciprocal and one correction (an infinite quotient, of an infinite x
+  // or of an r whose reciprocal or quotient passes 64 bits, has none to take).
   __device__ __forceinline__ double quotient(double x) const {
     const double q = x * inv, e = fma(-q, r, x);
-    return e == e ? fma(e, inv, q) : q;
+    return fabs(e) < static_cast<double>(kInf) ? fma(e, inv, q) : q;
   }
   template <typename Count>
   __device__ __forceinline__ double on(double x, uint32_t word, const Count&) const {
