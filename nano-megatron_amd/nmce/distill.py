@@ -227,7 +227,9 @@ def vocab_parallel_distillation_loss(
                  or _one_pass_ragged(logits, tp, inplace))):
         if upstream_hint is None:
             caller = sys._getframe(1)
-            hint = _site_hint(logits.device, (caller.f_code.co_filename, caller.f_lineno))
+            # (Named: a cross entropy on the same line may have another upstream value.)
+            hint = _site_hint(logits.device,
+                              (caller.f_code.co_filename, caller.f_lineno, "distillation"))
         else:
             _check_hint(upstream_hint, logits.device)
             hint = upstream_hint
