@@ -143,6 +143,23 @@ __device__ __forceinline__ void set_element(u32x4& v, int e, uint32_t bits) {
   }
 }
 
+// -inf for the elements that have no bit (the first's is bit 0). The others keep their bits,
+// which a signalling NaN does not in a conversion.
+template <typename T>
+__device__ __forceinline__ void mask_out(u32x4& v, uint32_t bits) {
+  // All ones where bit i is set.
+  auto spread = [&](int i) {
+    return static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - i)) >> 31);
+  };
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const uint32_t keep = sizeof(T) == 4 ? spread(d)
+                                         : (spread(2 * d) & 0xffffu) |
+                                               (spread(2 * d + 1) & 0xffff0000u);
+    v[d] = (v[d] & keep) | ((sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u) & ~keep);
+  }
+}
+
 // Row `row` of sequence b, slab `slab` of the vocabulary.
 template <typename T, int kBlock, bool kInPlace, bool kNarrow>
 __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adjust_kernel(
@@ -375,13 +392,7 @@ __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adj
       else is = to;
       set_element<T>(v[k], e, is);
     }
-    if (bits != kAll) {
-      float f[kVec];
-      E::unpack(v[k], f);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) f[e] = bits >> e & 1u ? f[e] : -kInf;
-      v[k] = E::pack(f);
-    }
+    if (bits != kAll) mask_out<T>(v[k], bits);
     store16(y + c, v[k]);
   }
   // The shard's last elements, of no whole vector.
