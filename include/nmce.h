@@ -642,7 +642,9 @@ int nmce_verify_finish(const double* picked, const void* workspace, int64_t work
  *   - out may be logits (in place, the same strides): only touched and masked
  *     elements are written. Otherwise the two must not overlap.
  * n_bias at most NMCE_ADJUST_MAX_BIASES, n_output at most 2^29; batch x rows x
- * ceil(vocab_local / 8192) at most 2^23.
+ * ceil(vocab_local / 8192) at most 2^23. More than 512 biases within 8192 neighbouring
+ * ids (counted from vocab_start), one of whose ids comes again, are searched in n_bias
+ * steps each: 2048 take 0.5 ms a row, 8192 7 ms, where different ids take 13 and 20 us.
  */
 #define NMCE_ADJUST_MAX_BIASES 8192
 typedef struct nmce_adjust_batch {

@@ -14,10 +14,10 @@
 // bits and rounded once, in the registers, before the store. What bounds a batch is one
 // read and one write of the logits; in place only vectors with something to change move.
 // 24 x 9 rows of 151936 bf16, 1250 listed ids, masked: 29 us (4.7 TB/s with the masks; the
-// counts, before the first store, are what is left to 21); 64 x 1 of 128256: 15;
-// one of 50257 fp32: 6, a launch and three dependent reads; 8 of 100277 fp32 with 139264 ids
-// and 300 biases each: 24, of which the lists take 12 (a compute unit's 64 bytes a cycle from
-// its L2: 7) and the biases 8.
+// counts, before the first store, are what is left to 21), in place 26; 64 x 1 of 128256: 16,
+// in place 16; one of 50257 fp32: 6, a launch and three dependent reads; 8 of 100277 fp32 with
+// 139264 ids and 300 biases each: 24, in place 25, of which the lists take 12 (a compute unit's
+// 64 bytes a cycle from its L2: 7) and the biases 8.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -423,7 +423,8 @@ __global__ __launch_bounds__(kBlock, kNarrow && sizeof(T) == 2 ? 6 : 4) void adj
         if (s >= kSlab) continue;
         double add = bias[j];
         if (apart) {
-          // The first entry of an id adds all of them, in their order.
+          // The first entry of an id adds all of them, in their order. (The whole list from
+          // memory for each entry: milliseconds, where one id of so many comes again.)
           bool mine = true;
           for (int64_t i = 0; i < j && mine; ++i) mine = bias_ids[i] != id;
           if (!mine) continue;

@@ -115,8 +115,9 @@ constexpr int kListWaves = 4;
 
 // kWhole: no normaliser, the teacher's distribution is over the list. The student's sum is
 // in fp32 terms, as the one outside the list is. Latency bounds it (ids, then the logits that
-// they name, then fp64 exponentials; waits 0.67 to 0.83 of the waves' time): 256 rows of 20
-// 6 us, 8192 of 64 20.
+// they name, then fp64 exponentials; waits 0.64 to 0.80 of the waves' time): 256 rows of 20
+// 6 us, 8192 of 64 21. A list that names an id twice is compared with itself, K^2 / 64 reads of
+// LDS a lane: a step of 4096 rows 839 -> 1625 us where each of K 1024 does, 604 -> 624 of 128.
 // `assumed` (of a one-pass forward, else NULL) takes the upstream value to assume: the row
 // kernels read it there, since another stream's backward may change the hint under them.
 template <typename T, typename TT, bool kWhole>
@@ -519,8 +520,9 @@ __global__ __launch_bounds__(kBlock) void distill_bwd_kernel(
 // Whole-vocabulary rows (one rank) held by a workgroup of 1024 threads: in registers (up to 8
 // vectors a thread; two workgroups a compute unit), or 9 of up to 16 in LDS. Bounded by HBM
 // with a whole row between its read and its write: 2047 x 50257 bf16 87 us (4.8 TB/s), 8192 x
-// 128256 790 (5.3; a streaming copy 6.5). A step of these takes 136 and 871 us, by two passes 170 and
-// 1018. The listed elements are set to -inf where they are held, so that the fold sees what is
+// 128256 790 (5.3; a streaming copy 6.5). A step of these takes 101 and 815 us, by two passes 152 and
+// 994, in place 101 and 841; one whose upstream value is not the assumed one 192 and 1571.
+// The listed elements are set to -inf where they are held, so that the fold sees what is
 // outside; each wave does that for its own elements, one listed id after another, and writes
 // their gradients over the row's, by the lanes that stored it. The gradient is that of the mean
 // for the upstream value assumed[0] (the list kernel's); loss and slopes as from

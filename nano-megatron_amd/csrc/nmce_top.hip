@@ -12,11 +12,12 @@
 // every run. A chunk of which more reach the floor than fit (a row of equal logits) is
 // first cut to its k largest keys by bisection.
 //
-// The exponentials' sum rides along. 4096 x 128256 bf16, k 64: 200 us (5.3 TB/s; the VALU is
-// busy for 0.86 of it, 12 instructions an element, half of them the exponentials' sum). 777 x
-// 100277 fp32, k 500: 103 (3.0 TB/s): the cuts take half of the instructions, and some compute
-// units have four rows where the mean is 3.04. A few rows take the latency of their steps:
-// read, floor, notes, order, and the merge's: one of 50257, k 20: 8 and 5 us.
+// The exponentials' sum rides along. 4096 x 128256 bf16, k 64: 204 us (5.2 TB/s; the VALU is
+// busy for 0.86 of it, 12 instructions an element, half of them the exponentials' sum; up to 260
+// from the 2nd to the 9th millisecond of such work after idling, with or without a profiler).
+// 777 x 100277 fp32, k 500: 103 (3.0 TB/s): the cuts take half of the instructions, and some
+// compute units have four rows where the mean is 3.04. A few rows take the latency of their
+// steps: read, floor, notes, order, and the merge's: one of 50257, k 20: 8 and 5 us.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -34,8 +35,8 @@ constexpr int kLeast = 4096;
 
 // A workgroup's shape: threads, the wanted logits it is for, places for notes (past half of
 // them they are cut) and for those a cut leaves, maxima a thread gives to the floor. At k 128
-// Few takes 33 us for 64 rows of 128256 bf16, Many 37; 88 and 98 for 4096 of 32000; 63 and 56
-// for 512 of 128256. At k 20, 64 rows of 128256: 24 and 28.
+// Few takes 28 us for 64 rows of 128256 bf16, Many 32; 85 and 95 for 4096 of 32000; 58 and 52
+// for 512 of 128256. At k 20, 64 rows of 128256: 17 and 21; one of 50257 fp32: 12 and 14.
 struct Few {
   static constexpr int kBlock = 256, kMost = 128, kNotes = 1024, kRoom = 160, kTops = 1;
 };
@@ -763,10 +764,12 @@ int id_bits_of(int64_t v) {
 }
 
 // Columns of a slab: the whole row, or, where the rows do not fill the card, as few as
-// give a workgroup's place to every slab (64 rows of 128256 bf16, k 20: 23.6 us a call; half
-// the places 24.8, twice 26), but no fewer than kLeast (a workgroup's own steps take as long
-// as reading these: one row of 50257 fp32, k 20: 18.3; of 8192 columns 20, of 2048 18) and 16
-// a wanted logit (so that the floor holds).
+// give a workgroup's place to every slab (64 rows of 128256 bf16, k 20: 17.0 us a call; half
+// the places 19.0, twice 20.4), but no fewer than kLeast (a workgroup's own steps take as long
+// as reading these: one row of 50257 fp32, k 20: 11.9; of 8192 columns 13.6, of 2048 12.7; eight
+// of 100277: 13.6, 15.2 and 18.5; bf16, whose chunk is 8192, would have a little of the wider
+// ones: 16 of 128256 16.1, 14.5 and 20.8, 64 of them 17.0, 16.6 and 16.9) and 16 a wanted logit
+// (so that the floor holds).
 int64_t width_of(int64_t n_rows, int64_t v, int k) {
   const int64_t places = 4 * static_cast<int64_t>(device_cus());
   const int64_t slabs = n_rows > 0 ? places / n_rows : 1;

@@ -120,7 +120,8 @@ def vocab_parallel_adjust_logits(
     is a number or fp32 ``[B]`` (a repetition penalty that is not a finite number
     above 0 leaves that sequence as 1 would). ``bias_values`` is fp32 ``[B, N]``, at
     most 8192 a sequence; an id that comes several times gets them all, added in
-    their order. ``allowed`` is int32 ``[B, K + 1, ceil(V / 32)]`` (any strides of
+    their order (the caller adds them up first where a sequence has more than 512 within
+    8192 neighbouring ids: there one such id costs milliseconds). ``allowed`` is int32 ``[B, K + 1, ceil(V / 32)]`` (any strides of
     the first two): id ``j`` is allowed where bit ``j % 32`` of word ``j // 32`` is
     set. A masked element is ``-inf`` whatever it held; a row may have none left.
 
